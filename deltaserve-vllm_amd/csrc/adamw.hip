@@ -1,0 +1,337 @@
+// Clip by group and AdamW over many tensors, moments in 8 or 32 bits.
+//
+//   g' = g·min(1, max_norm / (‖group‖ + 1e-6))
+//   m' = β1·m + (1 − β1)·g',  v' = β2·v + (1 − β2)·g'²
+//   w' = w − lr·wd·w − (lr / bc1)·m' / (sqrt(v') / sqrt(bc2) + ε),  bc_i = 1 − β_i^t
+//
+// 8 bits. Blocks of 256 elements share two fp32 scales: m = code·m_scale and
+// sqrt(v) = code·r_scale, codes e4m3 (3 mantissa bits, largest 448, smallest 2^-9).
+// The square root halves the exponents that v takes, so a block holds v over 11
+// decades. m moves by a tenth of the gradient a step and is rounded to nearest
+// (half a step, 2^-4 relative). sqrt(v) moves by at most 0.05 % a step, far below
+// half a step of 6 to 12 %: to nearest it would never fall, so it is rounded up or
+// down at random in proportion to where it lies, and the mean moves as it should. It
+// is never rounded to 0 from above, where m / (0 + ε) would leap. The step uses m' and
+// v' before they are rounded. Blocks whose largest magnitude is below 2^-100 are held as
+// zeros.
+//
+// A workgroup takes a chunk of 4096 elements, a wave 4 blocks, 16 lanes a block:
+// every load of 4 elements a lane covers whole 256-byte runs, and the block's
+// maxima are 4 DPP steps.
+#include <cmath>
+#include <type_traits>
+
+#include "feedback.h"
+
+namespace dsb {
+
+namespace {
+
+constexpr int kBlock = DSB_ADAM_BLOCK, kChunk = DSB_ADAM_CHUNK;
+constexpr float kTiny = 0x1p-100f;
+
+struct Hyper {
+  float b1, ob1, b2, ob2;  // β and 1 − β, each rounded once from 64 bits
+  float decay;             // 1 − lr·wd
+  float step_size, rbc2;   // lr / bc1, 1 / sqrt(bc2)
+  float eps;
+  unsigned key;
+};
+
+__host__ __device__ inline unsigned mix32(unsigned x) {
+  x ^= x >> 16;
+  x *= 0x6a09e667u;  // the first bits of sqrt(2) and sqrt(3)
+  x ^= x >> 15;
+  x *= 0xbb67ae85u;
+  return x ^ (x >> 16);
+}
+constexpr unsigned kGolden = 0x9e3779b9u;
+
+__host__ __device__ inline Hyper make_hyper(double lr, double beta1, double beta2, double eps,
+                                            double wd, int64_t step, unsigned seed) {
+  const double bc1 = -expm1((double)step * log(beta1)), bc2 = -expm1((double)step * log(beta2));
+  Hyper h;
+  h.b1 = (float)beta1;
+  h.ob1 = (float)(1.0 - beta1);
+  h.b2 = (float)beta2;
+  h.ob2 = (float)(1.0 - beta2);
+  h.decay = (float)(1.0 - lr * wd);
+  h.step_size = (float)(lr / bc1);
+  h.rbc2 = (float)(1.0 / sqrt(bc2));
+  h.eps = (float)eps;
+  h.key = mix32(seed + (unsigned)step * kGolden);
+  return h;
+}
+
+// 4 consecutive elements from e of a tensor of `numel`, as fp32; zeros past its end
+DSB_DEV f32x4 load4(const void* p, long e, long numel, bool bf, bool vec) {
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  if (vec && e + 4 <= numel) {
+    if (bf) {
+      const bf16x4 b = *reinterpret_cast<const bf16x4*>((const bf16*)p + e);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] = (float)b[i];
+    } else {
+      o = *reinterpret_cast<const f32x4*>((const float*)p + e);
+    }
+    return o;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (e + i < numel) o[i] = bf ? (float)((const bf16*)p)[e + i] : ((const float*)p)[e + i];
+  return o;
+}
+DSB_DEV void store4(void* p, long e, long numel, bool bf, bool vec, f32x4 v) {
+  if (vec && e + 4 <= numel) {
+    if (bf)
+      *reinterpret_cast<bf16x4*>((bf16*)p + e) =
+          bf16x4{(bf16)v[0], (bf16)v[1], (bf16)v[2], (bf16)v[3]};
+    else
+      *reinterpret_cast<f32x4*>((float*)p + e) = v;
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (e + i < numel) {
+      if (bf)
+        ((bf16*)p)[e + i] = (bf16)v[i];
+      else
+        ((float*)p)[e + i] = v[i];
+    }
+}
+DSB_DEV bool aligned4(const void* p, bool bf) {
+  return ((unsigned long)p & (bf ? 7 : 15)) == 0;
+}
+
+// The largest of the 16 lanes of a block, as unsigned bits (of magnitudes: NaN wins).
+DSB_DEV unsigned max16(unsigned x) {
+  auto step = [&](auto ctrl) {
+    const unsigned y =
+        __builtin_amdgcn_update_dpp(0, x, decltype(ctrl)::value, 0xf, 0xf, false);
+    x = max(x, y);
+  };
+  step(std::integral_constant<int, 0xB1>{});   // lanes 1 0 3 2 of each four
+  step(std::integral_constant<int, 0x4E>{});   // 2 3 0 1
+  step(std::integral_constant<int, 0x141>{});  // mirrored within 8
+  step(std::integral_constant<int, 0x140>{});  // within 16
+  return x;
+}
+DSB_DEV unsigned mag(float x) { return __builtin_bit_cast(unsigned, x) & 0x7fffffffu; }
+
+DSB_DEV unsigned pack4_e4m3(const float x[4]) {
+  unsigned r = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
+  return __builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], r, true);
+}
+DSB_DEV void unpack4_e4m3(unsigned c, float x[4]) {
+  const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8(c, false);
+  const f32x2 b = __builtin_amdgcn_cvt_pk_f32_fp8(c, true);
+  x[0] = a[0];
+  x[1] = a[1];
+  x[2] = b[0];
+  x[3] = b[1];
+}
+
+// x in [0, 448] onto the e4m3 grid, up with the chance (x − below) / step: 16 random
+// bits (their middle) added under the three mantissa bits, the rest cut off. Below
+// 2^-6 the grid's step stays 2^-9: 2^-6 is added first.
+DSB_DEV float round_random(float x, unsigned r16) {
+  const float off = x < 0x1p-6f ? 0x1p-6f : 0.f;
+  const unsigned y = __builtin_bit_cast(unsigned, x + off) + ((r16 << 4) | 8u);
+  const float q = __builtin_bit_cast(float, y & 0xfff00000u) - off;
+  return x > 0.f ? fmaxf(q, 0x1p-9f) : 0.f;
+}
+
+}  // namespace
+
+__global__ void adam_hyper_kernel(const float* lr_dev, const int64_t* step_dev, double lr,
+                                  int64_t step, double beta1, double beta2, double eps, double wd,
+                                  unsigned seed, Hyper* out) {
+  *out = make_hyper(lr_dev ? (double)*lr_dev : lr, beta1, beta2, eps, wd,
+                    step_dev ? *step_dev : step, seed);
+}
+
+// Σ g² of a chunk, in 64 bits (gradients of any finite size).
+__global__ __launch_bounds__(256) void adam_sumsq_kernel(const dsb_adam_tensor* __restrict__ T,
+                                                         const int2* __restrict__ chunks,
+                                                         double* __restrict__ partial) {
+  __shared__ double red[4];
+  const int2 ck = chunks[blockIdx.x];
+  const dsb_adam_tensor t = T[ck.x];
+  const bool bf = (t.dtypes >> 8) == DSB_DT_BF16, vec = aligned4(t.g, bf);
+  const long e0 = (long)ck.y * kChunk + 4 * threadIdx.x;
+  double s = 0.0;
+#pragma unroll
+  for (int k = 0; k < kChunk / 1024; ++k) {
+    const f32x4 g = load4(t.g, e0 + 1024 * k, t.numel, bf, vec);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s += (double)g[i] * (double)g[i];
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) partial[blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
+}
+
+// One block per group: its chunks' sums in a fixed order, the norm and the factor.
+__global__ __launch_bounds__(256) void adam_norm_kernel(const int* __restrict__ group_chunks,
+                                                        const double* __restrict__ partial,
+                                                        double max_norm, float* __restrict__ norms,
+                                                        float* __restrict__ coef) {
+  __shared__ double red[4];
+  const int c0 = group_chunks[blockIdx.x], c1 = group_chunks[blockIdx.x + 1];
+  double s = 0.0;
+  for (int c = c0 + threadIdx.x; c < c1; c += 256) s += partial[c];
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const double norm = sqrt((red[0] + red[1]) + (red[2] + red[3]));
+    const double c = max_norm / (norm + 1e-6);
+    norms[blockIdx.x] = (float)norm;
+    coef[blockIdx.x] = c > 1.0 ? 1.f : (float)c;  // NaN stays
+  }
+}
+
+template <int BITS>
+__global__ __launch_bounds__(256) void adam_kernel(const dsb_adam_tensor* __restrict__ T,
+                                                   const int2* __restrict__ chunks, Hyper hv,
+                                                   const Hyper* __restrict__ hp,
+                                                   const float* __restrict__ coef, void* mp,
+                                                   void* vp, float* __restrict__ m_scale,
+                                                   float* __restrict__ r_scale) {
+  const int2 ck = chunks[blockIdx.x];
+  const dsb_adam_tensor t = T[ck.x];
+  Hyper h = hv;
+  if (hp) h = *hp;
+  const int l16 = threadIdx.x & 15, qb = threadIdx.x >> 4;  // 16 blocks of 256 per chunk
+  const long tb = (long)ck.y * (kChunk / kBlock) + qb;      // block within the tensor
+  if (tb * kBlock >= t.numel) return;                       // the 16 lanes of a block together
+  const bool wbf = (t.dtypes & 255) == DSB_DT_BF16, gbf = (t.dtypes >> 8) == DSB_DT_BF16;
+  const bool wvec = aligned4(t.w, wbf), gvec = aligned4(t.g, gbf);
+  const float cf = coef ? coef[t.group] : 1.f;
+  const long b = t.block0 + tb, e0 = tb * kBlock + 4 * l16, s0 = b * kBlock + 4 * l16;
+  f32x4 g[4], w[4];
+  float m[4][4], r[4][4];
+  unsigned mc[4], rc[4];
+  float ms = 0.f, rs = 0.f;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) g[k] = load4(t.g, e0 + 64 * k, t.numel, gbf, gvec);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) w[k] = load4(t.w, e0 + 64 * k, t.numel, wbf, wvec);
+  if constexpr (BITS == 8) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      mc[k] = *reinterpret_cast<const unsigned*>((const uint8_t*)mp + s0 + 64 * k);
+      rc[k] = *reinterpret_cast<const unsigned*>((const uint8_t*)vp + s0 + 64 * k);
+    }
+    ms = m_scale[b];
+    rs = r_scale[b];
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      *reinterpret_cast<f32x4*>(m[k]) = *reinterpret_cast<const f32x4*>((const float*)mp + s0 + 64 * k);
+      *reinterpret_cast<f32x4*>(r[k]) = *reinterpret_cast<const f32x4*>((const float*)vp + s0 + 64 * k);
+    }
+  }
+  unsigned mtop = 0, rtop = 0;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if constexpr (BITS == 8) {
+      unpack4_e4m3(mc[k], m[k]);
+      unpack4_e4m3(rc[k], r[k]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float gi = g[k][i] * cf;
+      float v;
+      if constexpr (BITS == 8) {
+        const float ro = r[k][i] * rs;
+        v = h.b2 * (ro * ro) + h.ob2 * (gi * gi);
+        m[k][i] = h.b1 * (m[k][i] * ms) + h.ob1 * gi;
+        r[k][i] = __builtin_amdgcn_sqrtf(v);
+        mtop = max(mtop, mag(m[k][i]));
+        rtop = max(rtop, mag(r[k][i]));
+        w[k][i] = w[k][i] * h.decay -
+                  h.step_size * m[k][i] * __builtin_amdgcn_rcpf(r[k][i] * h.rbc2 + h.eps);
+      } else {
+        v = h.b2 * r[k][i] + h.ob2 * (gi * gi);
+        m[k][i] = h.b1 * m[k][i] + h.ob1 * gi;
+        r[k][i] = v;
+        w[k][i] = w[k][i] * h.decay -
+                  h.step_size * m[k][i] *
+                      __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v) * h.rbc2 + h.eps);
+      }
+    }
+    store4(t.w, e0 + 64 * k, t.numel, wbf, wvec, w[k]);
+    if constexpr (BITS == 32) {
+      *reinterpret_cast<f32x4*>((float*)mp + s0 + 64 * k) = *reinterpret_cast<f32x4*>(m[k]);
+      *reinterpret_cast<f32x4*>((float*)vp + s0 + 64 * k) = *reinterpret_cast<f32x4*>(r[k]);
+    }
+  }
+  if constexpr (BITS == 8) {
+    const float mt = __builtin_bit_cast(float, max16(mtop));
+    const float rt = __builtin_bit_cast(float, max16(rtop));
+    // not below kTiny (so NaN and infinity show in the scale)
+    const float im = mt < kTiny ? 0.f : 448.f * __builtin_amdgcn_rcpf(mt);
+    const float ir = rt < kTiny ? 0.f : 448.f * __builtin_amdgcn_rcpf(rt);
+    const unsigned key = mix32(h.key ^ mix32((unsigned)b));
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      float q[4], p[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        q[i] = fminf(fmaxf(m[k][i] * im, -448.f), 448.f);
+        p[i] = fminf(r[k][i] * ir, 448.f);
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const unsigned x = mix32(key + (unsigned)(32 * k + 2 * l16 + j) * kGolden);
+        p[2 * j] = round_random(p[2 * j], x & 0xffffu);
+        p[2 * j + 1] = round_random(p[2 * j + 1], x >> 16);
+      }
+      *reinterpret_cast<unsigned*>((uint8_t*)mp + s0 + 64 * k) = pack4_e4m3(q);
+      *reinterpret_cast<unsigned*>((uint8_t*)vp + s0 + 64 * k) = pack4_e4m3(p);
+    }
+    if (l16 == 0) {
+      m_scale[b] = mt < kTiny ? 0.f : mt * (1.f / 448.f);
+      r_scale[b] = rt < kTiny ? 0.f : rt * (1.f / 448.f);
+    }
+  }
+}
+
+int64_t adam_bytes(int nchunks, int ngroups) {
+  return 256 + ((int64_t)nchunks * 8 + 255) / 256 * 256 + ((int64_t)ngroups * 4 + 255) / 256 * 256;
+}
+
+hipError_t adam_step(const AdamArgs& a, void* work, hipStream_t s) {
+  Hyper* hp = (Hyper*)work;
+  double* partial = (double*)((char*)work + 256);
+  float* coef = (float*)((char*)partial + ((int64_t)a.nchunks * 8 + 255) / 256 * 256);
+  const bool dev = a.lr_dev || a.step_dev, clip = a.max_norm >= 0;
+  Hyper hv{};
+  if (dev)
+    hipLaunchKernelGGL(adam_hyper_kernel, dim3(1), dim3(1), 0, s, a.lr_dev, a.step_dev, a.lr, a.step,
+                       a.beta1, a.beta2, a.eps, a.wd, a.seed, hp);
+  else
+    hv = make_hyper(a.lr, a.beta1, a.beta2, a.eps, a.wd, a.step, a.seed);
+  if (clip) {
+    if (a.nchunks > 0)
+      hipLaunchKernelGGL(adam_sumsq_kernel, dim3(a.nchunks), dim3(256), 0, s, a.tensors, a.chunks,
+                         partial);
+    hipLaunchKernelGGL(adam_norm_kernel, dim3(a.ngroups), dim3(256), 0, s, a.group_chunks, partial,
+                       a.max_norm, a.norms, coef);
+  }
+  if (a.nchunks > 0) {
+    if (a.bits == 8)
+      hipLaunchKernelGGL(adam_kernel<8>, dim3(a.nchunks), dim3(256), 0, s, a.tensors, a.chunks, hv,
+                         dev ? hp : nullptr, clip ? coef : nullptr, a.m, a.v, a.m_scale, a.r_scale);
+    else
+      hipLaunchKernelGGL(adam_kernel<32>, dim3(a.nchunks), dim3(256), 0, s, a.tensors, a.chunks, hv,
+                         dev ? hp : nullptr, clip ? coef : nullptr, a.m, a.v, a.m_scale, a.r_scale);
+  }
+  return hipGetLastError();
+}
+
+}  // namespace dsb

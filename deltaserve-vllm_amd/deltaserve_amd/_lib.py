@@ -25,6 +25,10 @@ PROJS = ("q", "k", "v", "o", "gate", "up", "down")
 PROJ_INDEX = {p: i for i, p in enumerate(PROJS)}
 FLAG_GRAPH, FLAG_NO_CLIP, FLAG_KTIMING, FLAG_SERIAL_LAYERS = 1, 2, 4, 8
 DT_BF16, DT_F16, DT_F32 = 0, 1, 2
+PREF_KINDS = {"sigmoid": 0, "hinge": 1, "ipo": 2}
+KL_KINDS = {"k3": 0, "k2": 1}
+REDUCTIONS = {"token": 0, "sequence": 1, "sum": 2}
+ADAM_BLOCK, ADAM_CHUNK = 256, 4096
 
 
 class DsbDesc(Structure):
@@ -73,6 +77,16 @@ class DsbDualPass(Structure):
 
 class DsbCycleInfo(Structure):
     _fields_ = [("gpu_ms", c_float), ("graph", c_int32), ("n_valid", c_int32)]
+
+
+class DsbPackPlan(Structure):
+    _fields_ = [(k, c_void_p) for k in ("tiles", "seq_tile", "starts", "chunk_seq")] + [
+        (k, c_int32) for k in ("ntiles", "nseq", "n", "npred", "nonempty")]
+
+
+class DsbAdamTensor(Structure):
+    _fields_ = [("w", c_void_p), ("g", c_void_p), ("numel", c_int64), ("block0", c_int64),
+                ("group", c_int32), ("dtypes", c_int32)]
 
 
 # name -> (restype, argtypes)
@@ -158,6 +172,29 @@ _SIGS = {
                                   POINTER(c_void_p), POINTER(c_int32), POINTER(c_int32),
                                   c_int, c_int, c_float, c_float, c_float, c_float, c_float,
                                   c_int64, c_float, c_int, c_void_p]),
+    "dsb_op_logprob_workspace": (c_int, [c_int, c_int, c_int, c_int, POINTER(c_int64)]),
+    "dsb_op_token_logprobs": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int, c_int, c_int,
+                                      c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
+    "dsb_op_token_logprobs_bwd": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int, c_int,
+                                          c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int64,
+                                          c_int, c_void_p, c_int64, c_void_p]),
+    "dsb_plan_sizes": (c_int, [POINTER(c_int32), c_int, POINTER(DsbPackPlan), POINTER(c_int64)]),
+    "dsb_plan_fill": (c_int, [POINTER(c_int32), POINTER(DsbPackPlan), c_void_p, c_void_p]),
+    "dsb_op_next_token_labels": (c_int, [c_void_p, c_void_p, POINTER(DsbPackPlan), c_void_p,
+                                         c_void_p, c_void_p]),
+    "dsb_op_loss_workspace": (c_int, [POINTER(DsbPackPlan), POINTER(c_int64)]),
+    "dsb_op_preference_loss": (c_int, [c_void_p, c_void_p, c_void_p, POINTER(DsbPackPlan), c_int,
+                                       c_double, c_double, c_double, c_int, c_double, c_void_p,
+                                       c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
+    "dsb_op_policy_loss": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p,
+                                   POINTER(DsbPackPlan), c_double, c_double, c_double, c_int, c_int,
+                                   c_double, c_double, c_void_p, c_void_p, c_void_p, c_int64,
+                                   c_void_p]),
+    "dsb_op_adam_workspace": (c_int, [c_int, c_int, POINTER(c_int64)]),
+    "dsb_op_adam_step": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p,
+                                 c_void_p, c_void_p, c_int, c_double, c_double, c_double, c_double,
+                                 c_double, c_double, c_int64, c_uint32, c_void_p, c_void_p, c_void_p,
+                                 c_void_p, c_int64, c_void_p]),
 }
 
 EXPORTED = tuple(_SIGS)

@@ -9,9 +9,11 @@ nothing here falls back to a PyTorch implementation.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
-from ctypes import byref, c_float, c_int, c_int32, c_void_p
+from ctypes import byref, c_float, c_int, c_int32, c_int64, c_void_p
 
+import numpy as np
 import torch
 
 from . import _lib as L
@@ -313,3 +315,323 @@ def clip_adamw_(ws, gs, ms, vs, groups, lr, step, beta1=0.9, beta2=0.999, eps=1e
                                        k, max(groups) + 1, float(lr), float(beta1), float(beta2),
                                        float(eps), float(wd), int(step), float(max_norm),
                                        int(clip), _stream()), what="dsb_op_clip_adamw")
+
+
+# ---------------------------------------------------------------- training from feedback
+#
+# These ops only enqueue on the current stream of their tensors' device (which need not be
+# the current device): no synchronisation, scratch memory from torch's caching allocator, so
+# they can be captured into a graph. The reference has no counterpart of them.
+
+_HERE = contextlib.nullcontext()
+
+
+def _on(what, *ts):
+    """A context in which the device that holds all tensors (None: left out) is the current one."""
+    dev = None
+    for t in ts:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise ValueError(f"{what}: takes CUDA (HIP) tensors")
+        if dev is not None and t.device != dev:
+            raise ValueError(f"{what}: the tensors are on different devices")
+        dev = t.device
+    return _HERE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
+def _vec(what, name, t, n, *dtypes):
+    """A contiguous vector of n elements of one of the dtypes."""
+    if t.dtype not in dtypes or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+        raise ValueError(f"{what}: {name} must be a contiguous vector of {n} elements of "
+                         f"{' or '.join(str(d) for d in dtypes)}")
+
+
+def _work(nbytes, device):
+    return torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=device)
+
+
+class PackPlan:
+    """Sequences packed row after row: their tables on the device, built once per packing by
+    :func:`pack_plan` and read by the losses. ``n`` rows, ``nseq`` sequences."""
+
+    __slots__ = ("n", "nseq", "device", "c", "tables", "loss_bytes")
+
+    def __init__(self, seq_lens, device):
+        lib = L.load()
+        lens = np.ascontiguousarray(seq_lens, dtype=np.int64).reshape(-1)
+        if lens.size and (lens.min() < 0 or lens.max() > 0x7fffffff):
+            raise ValueError("pack_plan: lengths must lie in [0, 2^31)")
+        lens = lens.astype(np.int32)
+        p = lens.ctypes.data_as(ctypes.POINTER(c_int32))
+        c, elems, nbytes = L.DsbPackPlan(), c_int64(), c_int64()
+        L.check(lib.dsb_plan_sizes(p, lens.size, byref(c), byref(elems)), what="dsb_plan_sizes")
+        self.device = torch.device(device)
+        if self.device.type != "cuda":
+            raise ValueError("pack_plan: the plan's device must be CUDA (HIP)")
+        host = torch.empty(max(elems.value, 4), dtype=torch.int32)
+        self.tables = torch.empty(host.shape, dtype=torch.int32, device=self.device)
+        self.device = self.tables.device
+        L.check(lib.dsb_plan_fill(p, byref(c), _p(host), _p(self.tables)), what="dsb_plan_fill")
+        self.tables.copy_(host)
+        L.check(lib.dsb_op_loss_workspace(byref(c), byref(nbytes)), what="dsb_op_loss_workspace")
+        self.c, self.n, self.nseq, self.loss_bytes = c, c.n, c.nseq, nbytes.value
+
+
+def pack_plan(seq_lens, device="cuda"):
+    """The :class:`PackPlan` of packed sequences of these lengths (zeros allowed)."""
+    return PackPlan(seq_lens, device)
+
+
+def _mask(what, mask, n):
+    if mask is not None:
+        _vec(what, "mask", mask, n, torch.bool, torch.uint8)
+
+
+def next_token_labels(ids, plan, mask=None):
+    """(labels int64 [n], rows bool [n]) of packed token ids [n] int64: the label of a row is its
+    sequence's next token, -1 where there is none or ``mask`` (by token: the tokens to score) is
+    not set there; ``rows`` marks the rows with a label."""
+    what = "next_token_labels"
+    _vec(what, "ids", ids, plan.n, torch.int64)
+    _mask(what, mask, plan.n)
+    with _on(what, ids, mask, plan.tables):
+        labels = torch.empty_like(ids)
+        rows = torch.empty(plan.n, dtype=torch.bool, device=ids.device)
+        L.check(L.load().dsb_op_next_token_labels(_p(ids), _p(mask), byref(plan.c), _p(labels),
+                                                  _p(rows), _stream()),
+                what="dsb_op_next_token_labels")
+    return labels, rows
+
+
+def _head_args(what, normed, lm_w, labels):
+    if normed.dtype != BF16 or lm_w.dtype != BF16 or normed.dim() != 2 or lm_w.dim() != 2:
+        raise ValueError(f"{what}: normed and lm_w must be bf16 matrices")
+    n, D = normed.shape
+    if lm_w.shape[1] != D or not lm_w.is_contiguous():
+        raise ValueError(f"{what}: lm_w must be a contiguous [V, {D}]")
+    if n and D > 1 and normed.stride(1) != 1:
+        raise ValueError(f"{what}: normed's last dimension must be contiguous")
+    _vec(what, "labels", labels, n, torch.int64)
+    # the row stride of a single row is any number
+    return n, D, lm_w.shape[0], normed.stride(0) if n > 1 else D
+
+
+def _logprob_work(n, D, V, backward, device):
+    nbytes = c_int64()
+    L.check(L.load().dsb_op_logprob_workspace(n, D, V, backward, byref(nbytes)),
+            what="dsb_op_logprob_workspace")
+    return _work(nbytes.value, device), max(nbytes.value, 256)
+
+
+def token_logprobs(normed, lm_w, labels):
+    """Log probabilities of labels through the LM head: normed bf16 [n, D] (final-norm rows, row
+    stride a multiple of 8), lm_w bf16 [V, D], labels int64 [n], a negative one unscored. Returns
+    fp32 (logp [n] = log softmax(normed·lm_wᵀ)[label], other [n] = the log-sum-exp of the other
+    words' logits, which :func:`token_logprobs_backward` takes); 0 on unscored rows, NaN where a
+    label is past the vocabulary. Only scored rows cost a product."""
+    what = "token_logprobs"
+    n, D, V, ld = _head_args(what, normed, lm_w, labels)
+    with _on(what, normed, lm_w, labels):
+        logp = torch.empty(n, dtype=torch.float32, device=normed.device)
+        other = torch.empty_like(logp)
+        work, nbytes = _logprob_work(n, D, V, 0, normed.device)
+        L.check(L.load().dsb_op_token_logprobs(_p(normed), ld, _p(lm_w), _p(labels), n, D, V,
+                                               _p(logp), _p(other), _p(work), nbytes, _stream()),
+                what="dsb_op_token_logprobs")
+    return logp, other
+
+
+def token_logprobs_backward(normed, lm_w, labels, logp, other, dlogp, out_dtype=BF16):
+    """The rows' gradient [n, D] (bf16 or fp32) of Σ dlogp·logp, from the forward's logp and other;
+    zeros on unscored rows and where dlogp is 0, which cost no product."""
+    what = "token_logprobs_backward"
+    n, D, V, ld = _head_args(what, normed, lm_w, labels)
+    for name, t in (("logp", logp), ("other", other), ("dlogp", dlogp)):
+        _vec(what, name, t, n, torch.float32)
+    if out_dtype not in (BF16, torch.float32):
+        raise ValueError(f"{what}: out_dtype is bfloat16 or float32")
+    with _on(what, normed, lm_w, labels, logp, other, dlogp):
+        dH = torch.empty(n, D, dtype=out_dtype, device=normed.device)
+        work, nbytes = _logprob_work(n, D, V, 1, normed.device)
+        L.check(L.load().dsb_op_token_logprobs_bwd(
+            _p(normed), ld, _p(lm_w), _p(labels), n, D, V, _p(logp), _p(other), _p(dlogp), _p(dH), D,
+            int(out_dtype == torch.float32), _p(work), nbytes, _stream()),
+            what="dsb_op_token_logprobs_bwd")
+    return dH
+
+
+def preference_loss(logp, ref_logp, plan, mask=None, kind="sigmoid", beta=0.1, label_smoothing=0.0,
+                    margin=0.0, average=False, grad_scale=1.0):
+    """Preference loss over pairs and its gradient: sequence 2i of the plan is preferred to 2i + 1.
+
+    logp, ref_logp (or None: 0): fp32 [n] log probabilities by row; mask (bool or uint8 [n]): the
+    scored rows, by default every row but the last of its sequence. With s = Σ (logp − ref_logp)
+    over a sequence's scored rows (their mean with ``average``) and z = beta·(s_2i − s_2i+1) −
+    margin, ``kind`` is "sigmoid" −(1 − ε)·log σ(z) − ε·log σ(−z) with ε ``label_smoothing``,
+    "hinge" max(0, 1 − z) or "ipo" (s_2i − s_2i+1 − 1/(2·beta))². Returns fp32 (loss, the mean over
+    pairs; rewards [nseq] = beta·s; dlogp [n] = grad_scale·dloss/dlogp)."""
+    what = "preference_loss"
+    if kind not in L.PREF_KINDS:
+        raise ValueError(f"{what}: kind is one of {', '.join(L.PREF_KINDS)}")
+    _vec(what, "logp", logp, plan.n, torch.float32)
+    if ref_logp is not None:
+        _vec(what, "ref_logp", ref_logp, plan.n, torch.float32)
+    _mask(what, mask, plan.n)
+    with _on(what, logp, ref_logp, mask, plan.tables):
+        dlogp = torch.empty_like(logp)
+        out = torch.empty(1 + plan.nseq, dtype=torch.float32, device=logp.device)
+        work = _work(plan.loss_bytes, logp.device)
+        L.check(L.load().dsb_op_preference_loss(
+            _p(logp), _p(ref_logp), _p(mask), byref(plan.c), L.PREF_KINDS[kind], beta,
+            label_smoothing, margin, int(average), grad_scale, _p(out),
+            c_void_p(out.data_ptr() + 4), _p(dlogp), _p(work), work.numel(), _stream()),
+            what="dsb_op_preference_loss")
+    return out[0], out[1:], dlogp
+
+
+def policy_loss(logp, old_logp, adv, plan, mask=None, ref_logp=None, clip_low=0.2, clip_high=0.2,
+                kl_coef=0.0, kl="k3", reduction="token", divisor=1.0, grad_scale=1.0):
+    """Clipped policy loss with a KL term, and its gradient.
+
+    logp, old_logp, ref_logp (or None): fp32 [n] by row; adv: fp32 advantages by row [n] or by
+    sequence [nseq] (n = nseq: by row); mask as in :func:`preference_loss`. With ρ = exp(logp −
+    old_logp) a scored row's policy term is −min(ρ·A, clamp(ρ, 1 − clip_low, 1 + clip_high)·A), its
+    KL term with u = ref_logp − logp is e^u − 1 − u ("k3") or u²/2 ("k2"). ``reduction``: "token"
+    (mean over scored rows), "sequence" (mean over the sequences that have some, of their rows'
+    mean) or "sum" (sum / divisor). Returns fp32 (loss = policy + kl_coef·kl; stats [3] = policy, kl,
+    the share of scored rows whose ratio is clipped; dlogp [n] = grad_scale·dloss/dlogp). Without
+    scored rows all are 0. As the formula has it, an infinite ratio with an advantage of 0 gives
+    NaN."""
+    what = "policy_loss"
+    if kl not in L.KL_KINDS:
+        raise ValueError(f"{what}: kl is one of {', '.join(L.KL_KINDS)}")
+    if reduction not in L.REDUCTIONS:
+        raise ValueError(f"{what}: reduction is one of {', '.join(L.REDUCTIONS)}")
+    _vec(what, "logp", logp, plan.n, torch.float32)
+    _vec(what, "old_logp", old_logp, plan.n, torch.float32)
+    if ref_logp is not None:
+        _vec(what, "ref_logp", ref_logp, plan.n, torch.float32)
+    by_row = adv.dim() == 1 and adv.shape[0] == plan.n
+    _vec(what, "adv", adv, plan.n if by_row else plan.nseq, torch.float32)
+    _mask(what, mask, plan.n)
+    with _on(what, logp, old_logp, adv, ref_logp, mask, plan.tables):
+        dlogp = torch.empty_like(logp)
+        out = torch.empty(4, dtype=torch.float32, device=logp.device)
+        work = _work(plan.loss_bytes, logp.device)
+        L.check(L.load().dsb_op_policy_loss(
+            _p(logp), _p(old_logp), _p(ref_logp), _p(adv), int(by_row), _p(mask), byref(plan.c),
+            clip_low, clip_high, kl_coef, L.KL_KINDS[kl], L.REDUCTIONS[reduction], divisor,
+            grad_scale, _p(out), _p(dlogp), _p(work), work.numel(), _stream()),
+            what="dsb_op_policy_loss")
+    return out[0], out[1:], dlogp
+
+
+class AdamW:
+    """AdamW over many tensors in one launch, with gradient clipping by group and moments in 8 or
+    32 bits (:func:`clip_adamw_` keeps fp32 moments of the caller's).
+
+    ws, gs: weights and their gradient buffers, fp32 or bf16 each, contiguous, on one device, no
+    two weights overlapping; they are bound: each step reads the gradients from, and writes the
+    weights to, the memory that these tensors had here (which is kept alive). groups:
+    non-decreasing group numbers from 0 (default: one group).
+
+    The moments start at zero, in blocks of 256 elements, each tensor from a block of its own.
+    :meth:`state` names them: ``m`` and ``v`` fp32 with bits=32; with bits=8 ``m`` and ``r`` in
+    float8_e4m3fn with a scale per block, ``m_scale`` and ``r_scale`` fp32: the first moment is
+    m·m_scale, the second (r·r_scale)². They may be saved and copied back."""
+
+    def __init__(self, ws, gs, bits=8, groups=None):
+        what = "AdamW"
+        ws, gs = list(ws), list(gs)
+        groups = [0] * len(ws) if groups is None else [int(g) for g in groups]
+        if bits not in (8, 32):
+            raise ValueError(f"{what}: bits is 8 or 32")
+        if not ws or len(gs) != len(ws) or len(groups) != len(ws):
+            raise ValueError(f"{what}: takes as many gradients and groups as weights, at least one")
+        if groups[0] < 0 or any(b < a for a, b in zip(groups, groups[1:])):
+            raise ValueError(f"{what}: groups must be non-decreasing, from 0")
+        code = {BF16: L.DT_BF16, torch.float32: L.DT_F32}
+        for w, g in zip(ws, gs):
+            if w.dtype not in code or g.dtype not in code:
+                raise ValueError(f"{what}: weights and gradients are fp32 or bf16")
+            if w.shape != g.shape or not w.is_contiguous() or not g.is_contiguous():
+                raise ValueError(f"{what}: a weight and its gradient are contiguous, of one shape")
+        span = sorted((w.data_ptr(), w.data_ptr() + w.numel() * w.element_size()) for w in ws
+                      if w.numel())
+        if any(b[0] < a[1] for a, b in zip(span, span[1:])):
+            raise ValueError(f"{what}: two weights overlap in memory")
+        with _on(what, *ws, *gs):
+            self.device, self.bits, self.ngroups = ws[0].device, bits, groups[-1] + 1
+            numel = np.array([w.numel() for w in ws], dtype=np.int64)
+            blocks = -(-numel // L.ADAM_BLOCK)
+            chunks = -(-numel // L.ADAM_CHUNK)
+            block0 = np.cumsum(blocks) - blocks
+            self.nblocks, self.nchunks = int(blocks.sum()), int(chunks.sum())
+            if self.nchunks > 0x7fffffff:
+                raise ValueError(f"{what}: too many elements")
+            rec = (L.DsbAdamTensor * len(ws))(*[
+                L.DsbAdamTensor(w.data_ptr(), g.data_ptr(), int(numel[i]), int(block0[i]), groups[i],
+                                code[w.dtype] + 256 * code[g.dtype])
+                for i, (w, g) in enumerate(zip(ws, gs))])
+            first = np.cumsum(chunks) - chunks
+            tensor = np.repeat(np.arange(len(ws)), chunks)
+            table = np.stack([tensor, np.arange(self.nchunks) - first[tensor]], 1).astype(np.int32)
+            per = np.bincount(np.array(groups), weights=chunks, minlength=self.ngroups)
+            ends = np.concatenate([[0], np.cumsum(per)]).astype(np.int32)
+
+            def dev(a):
+                raw = np.frombuffer(bytes(a), dtype=np.uint8).copy()
+                return torch.from_numpy(raw).to(self.device) if raw.size else _work(0, self.device)
+
+            self._tensors, self._chunks, self._ends = dev(rec), dev(table), dev(ends)
+            self._kept = [t.untyped_storage() for t in (*ws, *gs)]
+            nbytes = c_int64()
+            L.check(L.load().dsb_op_adam_workspace(self.nchunks, self.ngroups, byref(nbytes)),
+                    what="dsb_op_adam_workspace")
+            self._bytes = nbytes.value
+            n = self.nblocks * L.ADAM_BLOCK
+            zeros = lambda k, dt: torch.zeros(k, dtype=dt, device=self.device)  # noqa: E731
+            if bits == 8:
+                f8 = torch.float8_e4m3fn
+                self._state = {"m": zeros(n, torch.uint8).view(f8),
+                               "m_scale": zeros(self.nblocks, torch.float32),
+                               "r": zeros(n, torch.uint8).view(f8),
+                               "r_scale": zeros(self.nblocks, torch.float32)}
+            else:
+                self._state = {"m": zeros(n, torch.float32), "v": zeros(n, torch.float32)}
+
+    def state(self):
+        """The moments by name (the optimizer's own tensors)."""
+        return dict(self._state)
+
+    def step(self, lr, step, beta1=0.9, beta2=0.999, eps=1e-8, wd=0.0, max_norm=None, seed=0):
+        """One step, the step-th (from 1), in place on the weights and the moments. max_norm: clip
+        each group's gradient to this norm (the gradients stay as they are) and return the norms
+        before the clip, fp32 [ngroups]; None: no clip, returns None. 8-bit second moments are
+        rounded at random by ``seed`` and step, the same way for the same two. For a step that is
+        captured into a graph, lr (fp32) and step (int64) may be one-element tensors on the device,
+        read when it runs; numbers are baked in. A NaN or infinite gradient reaches the weights that
+        it reaches in the formula, and with 8 bits its block's moments."""
+        what = "AdamW.step"
+        lr_t = lr if isinstance(lr, torch.Tensor) else None
+        step_t = step if isinstance(step, torch.Tensor) else None
+        for name, t, dt in (("lr", lr_t, torch.float32), ("step", step_t, torch.int64)):
+            if t is not None and (t.numel() != 1 or t.dtype != dt):
+                raise ValueError(f"{what}: a {name} tensor holds one element of {dt}")
+        if max_norm is not None and not max_norm >= 0:
+            raise ValueError(f"{what}: max_norm must not be negative")
+        s = self._state
+        with _on(what, self._tensors, lr_t, step_t):
+            norms = None
+            if max_norm is not None:
+                norms = torch.empty(self.ngroups, dtype=torch.float32, device=self.device)
+            work = _work(self._bytes, self.device)
+            L.check(L.load().dsb_op_adam_step(
+                _p(self._tensors), _p(self._chunks), self.nchunks, _p(self._ends), self.ngroups,
+                _p(s["m"]), _p(s["r" if self.bits == 8 else "v"]), _p(s.get("m_scale")),
+                _p(s.get("r_scale")), self.bits, 0.0 if lr_t is not None else lr, beta1, beta2, eps,
+                wd, -1.0 if max_norm is None else max_norm, 0 if step_t is not None else step,
+                seed & 0xffffffff, _p(lr_t), _p(step_t), _p(norms), _p(work), work.numel(),
+                _stream()), what="dsb_op_adam_step")
+        return norms

@@ -382,6 +382,125 @@ int dsb_op_clip_adamw(float* const* w, float* const* g, float* const* m, float* 
                       float lr, float beta1, float beta2, float eps, float wd, int64_t step,
                       float max_norm, int do_clip, void* stream);
 
+/* ---- training from feedback: stream-ordered ops that only enqueue
+ *
+ * No counterpart in the reference, whose backward trains on next-token
+ * cross-entropy alone. They allocate nothing and do not synchronise, so they
+ * can be captured into a graph and replayed; `work` is device scratch of at
+ * least the bytes that the matching *_workspace call gives, 256-byte aligned,
+ * and belongs to the call until its work on `stream` is done. The stream's
+ * device has to be the current one. */
+
+/* Log probabilities of labels: row t of normed [n, D] (bf16, row stride ldh)
+ * against the LM head lm_w [V, D], labels int64 [n]; a negative label leaves the
+ * row unscored, one >= V gives NaN. logp[t] = log softmax(h·Wᵀ)[label] and
+ * other[t] = log Σ_{v ≠ label} exp(h·W_v), fp32 [n], 0 on unscored rows. D and
+ * ldh multiples of 8, V at least 2. */
+int dsb_op_logprob_workspace(int n, int D, int V, int backward, int64_t* bytes);
+int dsb_op_token_logprobs(const void* normed, int64_t ldh, const void* lm_w, const int64_t* labels,
+                          int n, int D, int V, float* logp, float* other, void* work,
+                          int64_t work_bytes, void* stream);
+/* The gradient of Σ_t dlogp[t]·logp[t] with respect to the rows, given the
+ * forward's logp and other: dH [n, D] bf16 or (out_f32) fp32, row stride lddh (a
+ * multiple of 8). Unscored rows and rows with dlogp = 0 get zeros and cost no
+ * product. */
+int dsb_op_token_logprobs_bwd(const void* normed, int64_t ldh, const void* lm_w,
+                              const int64_t* labels, int n, int D, int V, const float* logp,
+                              const float* other, const float* dlogp, void* dH, int64_t lddh,
+                              int out_f32, void* work, int64_t work_bytes, void* stream);
+
+/* A packing of nseq sequences over n rows on the device, built once per packing
+ * by dsb_plan_sizes and dsb_plan_fill (host) and copied there: int32 tables, each
+ * 16-byte aligned. tiles: (first row, end row, sequence, 0) of every run of at most
+ * DSB_TILE_ROWS rows of a sequence; seq_tile [nseq + 1]: a sequence's first tile;
+ * starts [nseq + 1]: its first row; chunk_seq [ceil(n / DSB_CHUNK_ROWS) + 1]: the
+ * sequence that holds row DSB_CHUNK_ROWS·c (the last entry: nseq − 1). npred:
+ * rows that are not the last of their sequence; nonempty: sequences with one. */
+enum { DSB_TILE_ROWS = 4096, DSB_CHUNK_ROWS = 4096 };
+typedef struct dsb_pack_plan {
+  const int32_t* tiles;
+  const int32_t* seq_tile;
+  const int32_t* starts;
+  const int32_t* chunk_seq;
+  int32_t ntiles, nseq, n, npred, nonempty;
+} dsb_pack_plan;
+/* Host only. seq_lens int32 [nseq], each >= 0, their sum below 2^31: the counts of
+ * the plan (its pointers untouched) and the int32 elements of all four tables. */
+int dsb_plan_sizes(const int32_t* seq_lens, int nseq, dsb_pack_plan* plan, int64_t* elems);
+/* Host only. Fills `tables` (host memory of `elems` int32) and the plan's pointers,
+ * as offsets from `device_base`, where the caller copies it. */
+int dsb_plan_fill(const int32_t* seq_lens, dsb_pack_plan* plan, int32_t* tables,
+                  const void* device_base);
+
+/* labels[t] = ids[t + 1] where row t has a next token in its sequence and mask[t + 1]
+ * (uint8 by token; null: all) is set, else −1; rows[t] (uint8) = labels[t] >= 0. */
+int dsb_op_next_token_labels(const int64_t* ids, const uint8_t* mask, const dsb_pack_plan* plan,
+                             int64_t* labels, uint8_t* rows, void* stream);
+
+int dsb_op_loss_workspace(const dsb_pack_plan* plan, int64_t* bytes);
+/* Preference loss over pairs: sequences 2i (preferred) and 2i + 1 of the plan.
+ * s_y = Σ over the scored rows of y of (logp − ref) (its mean with `average`; 0 where
+ * none is scored), z = beta·(s_2i − s_2i+1) − margin,
+ *   DSB_PREF_SIGMOID: (1 − smooth)·softplus(−z) + smooth·softplus(z)
+ *   DSB_PREF_HINGE:   max(0, 1 − z)
+ *   DSB_PREF_IPO:     (s_2i − s_2i+1 − 1/(2·beta))²
+ * and loss = the mean over pairs. Scored rows: mask [n] (uint8) or, null, every row
+ * but the last of its sequence; what lies in the others is not used. ref null: 0.
+ * Writes loss (fp32 scalar), rewards [nseq] = beta·s and dlogp [n] = grad_scale ·
+ * dloss/dlogp (0 on unscored rows). */
+enum { DSB_PREF_SIGMOID = 0, DSB_PREF_HINGE = 1, DSB_PREF_IPO = 2 };
+int dsb_op_preference_loss(const float* logp, const float* ref, const uint8_t* mask,
+                           const dsb_pack_plan* plan, int kind, double beta, double smooth,
+                           double margin, int average, double grad_scale, float* loss,
+                           float* rewards, float* dlogp, void* work, int64_t work_bytes,
+                           void* stream);
+/* Clipped policy loss: with ρ = exp(logp − old) and the row's advantage A,
+ *   policy = −min(ρ·A, clamp(ρ, 1 − clip_low, 1 + clip_high)·A)
+ *   kl (ref given): DSB_KL_K3 e^u − 1 − u, DSB_KL_K2 u²/2, u = ref − logp
+ * reduced over the scored rows (as above) by DSB_REDUCE_TOKEN (mean over rows),
+ * _SEQUENCE (mean over the sequences with scored rows of their rows' mean) or _SUM
+ * (sum / divisor). adv is fp32 [n] (adv_rows) or [nseq]. Writes out[4] = {policy +
+ * kl_coef·kl, policy, kl, share of scored rows whose ratio is clipped} and dlogp [n] =
+ * grad_scale · d out[0] / dlogp. */
+enum { DSB_KL_K3 = 0, DSB_KL_K2 = 1 };
+enum { DSB_REDUCE_TOKEN = 0, DSB_REDUCE_SEQUENCE = 1, DSB_REDUCE_SUM = 2 };
+int dsb_op_policy_loss(const float* logp, const float* old_logp, const float* ref,
+                       const float* adv, int adv_rows, const uint8_t* mask,
+                       const dsb_pack_plan* plan, double clip_low, double clip_high,
+                       double kl_coef, int kl, int reduction, double divisor, double grad_scale,
+                       float* out, float* dlogp, void* work, int64_t work_bytes, void* stream);
+
+/* One tensor of an AdamW step. w and g: element type by dtypes (DSB_DT_BF16 or
+ * DSB_DT_F32, w + 256·g), aligned to their type. block0: its first block of
+ * DSB_ADAM_BLOCK elements in the moments (a tensor starts on a block). */
+enum { DSB_ADAM_BLOCK = 256, DSB_ADAM_CHUNK = 4096 };
+typedef struct dsb_adam_tensor {
+  void* w;
+  const void* g;
+  int64_t numel;
+  int64_t block0;
+  int32_t group;
+  int32_t dtypes;
+} dsb_adam_tensor;
+/* Clip by group and AdamW over many tensors (the arithmetic of dsb_op_clip_adamw; the
+ * gradients are left as they are). tensors, chunks ((tensor, chunk of it) int32 pairs,
+ * chunks of DSB_ADAM_CHUNK elements, in order of the tensors' groups) and group_chunks
+ * [ngroups + 1] (first chunk of each group) live on the device.
+ * bits 32: m and v fp32 by block. bits 8: m holds e4m3 codes of m / m_scale and v those
+ * of sqrt(v) / r_scale, scales fp32 by block, the block's largest magnitude / 448; m is
+ * rounded to nearest, sqrt(v) up or down at random in proportion (a function of seed, step,
+ * block and element) and never down to 0 from above it. The step itself uses the moments
+ * before they are rounded. max_norm < 0: no clip, norms unused; else norms [ngroups]
+ * gets each group's gradient norm. lr_dev / step_dev: when set, the learning rate (fp32)
+ * and the step count (int64) are read on the device, for a captured step. */
+int dsb_op_adam_workspace(int nchunks, int ngroups, int64_t* bytes);
+int dsb_op_adam_step(const dsb_adam_tensor* tensors, const int32_t* chunks, int nchunks,
+                     const int32_t* group_chunks, int ngroups, void* m, void* v, float* m_scale,
+                     float* r_scale, int bits, double lr, double beta1, double beta2, double eps,
+                     double weight_decay, double max_norm, int64_t step, uint32_t seed,
+                     const float* lr_dev, const int64_t* step_dev, float* norms, void* work,
+                     int64_t work_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
