@@ -92,12 +92,51 @@ struct GemmProblem {
   // K1 load as zeros (the LM head's last vocabulary chunk runs K to a
   // multiple of 8 past the vocabulary)
   int kb_rows = 0;
+  // Tiles counted and dealt to the XCDs over the live rows (M_dev) instead of
+  // M: of a batch of which an unknown part is live, whole XCDs would
+  // otherwise hold no live tile. The grid is one-dimensional, live_grid
+  // blocks. With `part`, K is split on the device by the live tiles, over
+  // live_split(...) <= live_ks slices (those of a product of live_k, the same
+  // for every chunk of a longer K) whose partials lie live rows · N apart and
+  // take at most live_elems floats.
+  int live = 0;
+  int live_k = 0;
+  int live_ks = 1;
+  long live_elems = 0;
 };
 
-DSB_DEV void tile_map(int bid, int nbm, int nbn, int& pm, int& pn) {
-  const int total = nbm * nbn;
-  int lid = bid;
-  if ((total & 7) == 0) lid = (bid & 7) * (total >> 3) + (bid >> 3);
+// Slices of K that `tiles` output tiles of nk K tiles are split over so that
+// the device's 256 CUs are evenly loaded: the least number of K steps on the
+// busiest one, a block's epilogue (an fp32 tile stored while the others store
+// theirs) counting as `epi` steps. `most`: as many as their partials have room
+// for.
+__host__ __device__ inline int live_slices(int tiles, int nk, int most, int epi) {
+  int best = 1, least = 0x7fffffff;
+  for (int ks = 1; ks <= most; ++ks) {
+    const int steps = (tiles * ks + 255) / 256 * ((nk + ks - 1) / ks + epi);
+    if (steps < least) {
+      least = steps;
+      best = ks;
+    }
+  }
+  return best;
+}
+constexpr int kLiveEpi = 16;
+// The slices of a product of `rows` live rows.
+__host__ __device__ inline int live_split(int rows, int N, int K, int BM, int BN, int live_ks,
+                                          long live_elems) {
+  const int tiles = (rows + BM - 1) / BM * ((N + BN - 1) / BN);
+  const long fit = live_elems / ((long)max(rows, 1) * N);
+  return live_slices(tiles, (K + 63) / 64, (int)min((long)live_ks, max(fit, 1L)), kLiveEpi);
+}
+// Block `bid`'s place among `total` dealt to the 8 XCDs in contiguous runs
+// (blocks start round-robin over them).
+DSB_DEV int xcd_run(int bid, int total) {
+  const int x = bid & 7, q = total >> 3, r = total & 7;
+  return x * q + min(x, r) + (bid >> 3);
+}
+
+DSB_DEV void tile_order(int lid, int nbm, int nbn, int& pm, int& pn) {
   // 4 M-blocks per group (each XCD's 32 concurrent tiles span 4 M × 8 N
   // blocks): measured best of 2, 4, 6, 8, 16 on the C3 cycle
   constexpr int GM = 4;
@@ -108,6 +147,12 @@ DSB_DEV void tile_map(int bid, int nbm, int nbn, int& pm, int& pn) {
   const int r = lid - gid * per_group;
   pm = first_m + r % gsz;
   pn = r / gsz;
+}
+DSB_DEV void tile_map(int bid, int nbm, int nbn, int& pm, int& pn) {
+  const int total = nbm * nbn;
+  int lid = bid;
+  if ((total & 7) == 0) lid = (bid & 7) * (total >> 3) + (bid >> 3);
+  tile_order(lid, nbm, nbn, pm, pn);
 }
 
 // acc += A-fragment × B-fragment with the accumulator tied to its four AGPRs.
@@ -368,9 +413,19 @@ __attribute__((amdgpu_waves_per_eu(WM* WN / 4, WM* WN / 4))) void gemm_nt_kernel
 
   int M = p.M;
   if (p.M_dev) M = min(M, *p.M_dev);
-  const int nbm = (p.M + BM - 1) / BM, nbn = (p.N + BN - 1) / BN;
-  int pm, pn;
-  tile_map(blockIdx.x + p.tile0, nbm, nbn, pm, pn);
+  const int nbm = ((p.live ? M : p.M) + BM - 1) / BM, nbn = (p.N + BN - 1) / BN;
+  int pm, pn, slice = blockIdx.y, slices = gridDim.y;
+  if (p.live) {
+    if (M <= 0) return;
+    slices = p.part ? live_split(M, p.N, p.live_k, BM, BN, p.live_ks, p.live_elems) : 1;
+    const int tiles = nbm * nbn;
+    if ((int)blockIdx.x >= tiles * slices) return;
+    const int at = xcd_run(blockIdx.x, tiles * slices);
+    slice = at / tiles;
+    tile_order(at - slice * tiles, nbm, nbn, pm, pn);
+  } else {
+    tile_map(blockIdx.x + p.tile0, nbm, nbn, pm, pn);
+  }
   const int m0 = pm * BM, n0 = pn * BN;
   if (m0 >= M) return;
 
@@ -381,8 +436,8 @@ __attribute__((amdgpu_waves_per_eu(WM* WN / 4, WM* WN / 4))) void gemm_nt_kernel
   const int nk2 = p.K2 > 0 ? (p.K2 + BK - 1) / BK : 0;
   const int nk = nk1 + nk2;
   // this block's K tiles (all of them unless K is split over the grid's y)
-  const int kc = (nk + (int)gridDim.y - 1) / (int)gridDim.y;
-  const int kt0 = min(nk, (int)blockIdx.y * kc), kt1 = min(nk, kt0 + kc);
+  const int kc = (nk + slices - 1) / slices;
+  const int kt0 = min(nk, slice * kc), kt1 = min(nk, kt0 + kc);
 
   // Loader geometry: lane fills slot (lane & 7) of row (lane >> 3) of its
   // 8-row block; block b = wave + j·NW starts at row 8b, whose bit 3 is the
@@ -744,8 +799,8 @@ __attribute__((amdgpu_waves_per_eu(WM* WN / 4, WM* WN / 4))) void gemm_nt_kernel
 
   if constexpr (SplitPart<Epi>::enabled) {
     if (p.part) {
-      const typename SplitPart<Epi>::type ep{p.part + (long)blockIdx.y * p.M * p.N, (long)p.N,
-                                             p.N, p.part_acc, p.part_scale};
+      const typename SplitPart<Epi>::type ep{p.part + (long)slice * (p.live ? M : p.M) * p.N,
+                                             (long)p.N, p.N, p.part_acc, p.part_scale};
       ep.template run<FM, FN, WM, WN>(acc, m0 + wm * TM, n0 + wn * TN, M, lane, wave,
                                       (void*)smem);
       return;
@@ -1145,11 +1200,28 @@ __global__ __launch_bounds__(256) void gemm_split_reduce_kernel(GemmProblem p, i
   epi.apply8(m, n, v);
 }
 
+// Blocks of a live launch: the most tiles · slices over 1 .. M live rows.
+inline long live_grid(const GemmProblem& p, int BM, int BN) {
+  const int nbn = (p.N + BN - 1) / BN;
+  long most = 0;
+  for (int rows = 1; rows <= p.M; rows += BM) {
+    // the slices fall with the rows while their tiles stay the same
+    const long tiles = (long)((rows + BM - 1) / BM) * nbn;
+    int ks = 1;
+    if (p.part) {
+      const long fit = p.live_elems / ((long)rows * p.N);
+      ks = (int)std::min((long)p.live_ks, std::max(fit, 1L));
+    }
+    most = std::max(most, tiles * ks);
+  }
+  return most;
+}
+
 template <int BM, int BN, int WM, int WN, int NA = 2, int NB = 3, class Epi>
 hipError_t launch_gemm_cfg(const GemmProblem& p, const Epi& e, hipStream_t s, int ks = 1) {
   const int nbm = (p.M + BM - 1) / BM, nbn = (p.N + BN - 1) / BN;
   if (nbm == 0 || nbn == 0) return hipSuccess;
-  const dim3 grid(nbm * nbn, ks);
+  const dim3 grid(p.live ? (unsigned)live_grid(p, BM, BN) : (unsigned)(nbm * nbn), ks);
   if (p.b_kn)
     hipLaunchKernelGGL((gemm_nt_kernel<BM, BN, WM, WN, Epi, true, NA, NB>), grid, dim3(WM * WN * 64), 0,
                        s, p, e);

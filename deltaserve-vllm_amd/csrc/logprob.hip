@@ -24,6 +24,10 @@ namespace {
 // (a logit more than about 40 over the label's) the run takes its own maximum.
 constexpr float kRunLimit = 0x1p57f;
 
+// Probabilities held at a time (1 GiB of bf16), and the most K slices of the dH product.
+constexpr long kProbElems = 1L << 29;
+constexpr int kMaxSlices = 8;
+
 struct LPStat {
   float ref, sum;  // Σ exp(logit − ref) over a run, the label left out
 };
@@ -177,12 +181,12 @@ constexpr int lp_run(int cfg) {
   return cfg == GEMM_BIG ? 128 : cfg == GEMM_NARROW || cfg == GEMM_SKINNY ? 32 : 64;
 }
 
-// The forward product's tile: by cost over the whole vocabulary, nothing stored.
-int lp_cfg(int n, int D, int V) {
+// The logits products' tile: by cost, `ob` bytes stored per logit.
+int lp_cfg(int n, int D, int V, double ob) {
   int best = GEMM_BIG;
   double bt = 0;
   for (int cfg = 0; cfg < kGemmCfgs; ++cfg) {
-    const double c = gemm_cost(n, V, D, 0.0, cfg, 1);
+    const double c = gemm_cost(n, V, D, ob, cfg, 1);
     if (bt == 0 || c < bt) {
       bt = c;
       best = cfg;
@@ -203,6 +207,43 @@ struct Carve {
   }
 };
 
+// The backward's products: `vchunk` columns of the vocabulary at a time (a multiple of
+// 256), the tile of the logits product and the width of its runs, and the tile and most K
+// slices of the dH product.
+struct LPPlan {
+  int vchunk, prob_cfg, run, runs, dh_cfg, dh_bm, dh_bn, dh_ks;
+  long part_elems;
+};
+LPPlan lp_plan(int n, int D, int V) {
+  LPPlan q{};
+  const long vr = ((long)V + 255) / 256 * 256;
+  const long units = (vr * n + kProbElems - 1) / kProbElems;
+  q.vchunk = (int)((vr / 256 + units - 1) / units * 256);
+  q.prob_cfg = lp_cfg(n, D, q.vchunk, 2.0);
+  q.run = lp_run(q.prob_cfg);
+  q.runs = (V + q.run - 1) / q.run;
+  // accumulators of all slices: three times the rows, and up to eight slices
+  q.dh_ks = kMaxSlices;
+  q.part_elems = (n > 2048 ? 3L : (long)kMaxSlices) * n * D;
+  double bt = 0;
+  for (int cfg = 0; cfg < kGemmCfgs; ++cfg) {
+    const GemmTile t = gemm_tile(cfg);
+    const int ks = live_split(n, D, q.vchunk, t.bm, t.bn, q.dh_ks, q.part_elems);
+    const long blocks = (long)((n + t.bm - 1) / t.bm) * ((D + t.bn - 1) / t.bn) * ks;
+    const double steps = ((q.vchunk + 63) / 64 + ks - 1) / ks;
+    const double c = std::max(std::ceil((double)blocks / kGemmCus) * steps * t.step,
+                              2.0 * q.vchunk * ((double)n + D) / 6.8e6) +
+                     4.0 * ks * n * D / 3.9e6;
+    if (bt == 0 || c < bt) {
+      bt = c;
+      q.dh_cfg = cfg;
+      q.dh_bm = t.bm;
+      q.dh_bn = t.bn;
+    }
+  }
+  return q;
+}
+
 struct LPWork {
   int* count;   // scored rows
   int* rows;    // [n] their rows in order
@@ -212,8 +253,11 @@ struct LPWork {
   float* tgt;
   bf16* X;      // [n, D] the scored rows
   LPStat* stats;
-  float* rsum;
-  HeadArgs head;
+  // backward
+  float* rsum;   // [n, runs]
+  bf16* P;       // [n, vchunk]
+  float* part;   // the dH product's accumulators
+  LPPlan plan;
 };
 
 LPWork lp_layout(int n, int D, int V, bool backward, void* base, size_t* bytes) {
@@ -228,27 +272,13 @@ LPWork lp_layout(int n, int D, int V, bool backward, void* base, size_t* bytes) 
   w.tgt = c.take<float>(N);
   w.X = c.take<bf16>(N * D);
   if (!backward) {
-    const int run = lp_run(lp_cfg(n, D, V));
+    const int run = lp_run(lp_cfg(n, D, V, 0.0));
     w.stats = c.take<LPStat>(N * ((V + run - 1) / run));
   } else {
-    HeadArgs& a = w.head;
-    a.n = n;
-    a.D = D;
-    a.V = V;
-    a.vchunk = std::min(16384, (V + 255) / 256 * 256);
-    a.vchunk *= head_group(n, V, a.vchunk);
-    head_plan(a, -1, true);
-    w.rsum = c.take<float>(N * a.ntn);
-    a.dlog = c.take<bf16>(N * a.vchunk);
-    a.dH = c.take<float>(N * D);
-    if (a.dh_ks > 1) a.part = c.take<float>((size_t)head_part_elems(a));
-    if (a.dh_ks == 1 && a.dh_cfg == GEMM_BIG) {
-      int tail = 0;
-      a.ncu = kGemmCus;
-      const int kt = gemm_tail_split(n, D, a.vchunk, a.ncu, &tail);
-      a.tail_elems = kt > 1 ? (long)kt * tail * 65536 : 0;
-      if (a.tail_elems > 0) a.tail_part = c.take<float>((size_t)a.tail_elems);
-    }
+    w.plan = lp_plan(n, D, V);
+    w.rsum = c.take<float>(N * w.plan.runs);
+    w.P = c.take<bf16>(N * w.plan.vchunk);
+    w.part = c.take<float>((size_t)w.plan.part_elems);
   }
   *bytes = c.at;
   return w;
@@ -376,26 +406,28 @@ __global__ __launch_bounds__(256) void lp_finish_kernel(LPWork w, int cap, int r
 // bf16 holds them (their common rounding falls out), acc the sum of the K slices'
 // accumulators; zeros for rows left out, NaN for a label past V. The row is rounded
 // once, to the output's type.
-__global__ __launch_bounds__(256) void lp_dh_kernel(HeadArgs a, int n, const int* place, int ks,
-                                                    const float* __restrict__ rsum,
-                                                    const float* __restrict__ logp,
+__global__ __launch_bounds__(256) void lp_dh_kernel(const bf16* __restrict__ W, int n, int D,
+                                                    LPWork a, const float* __restrict__ logp,
                                                     const float* __restrict__ g, void* out,
                                                     long ldo, bool f32) {
   const int r = blockIdx.x * 4 + (threadIdx.x >> 6), l = threadIdx.x & 63;
   if (r >= n) return;
-  const int m = place[r];
+  const int m = a.place[r], M = *a.count;
+  const LPPlan& q = a.plan;
   float f = m == -2 ? NAN : 0.f, R = 0.f;
-  const bf16* w = a.W;
-  const float* src = a.dH;
+  const bf16* w = W;
+  const float* src = a.part;
+  int ks = 1;
   if (m >= 0) {
-    for (int j = l; j < a.ntn; j += 64) R += rsum[(long)m * a.ntn + j];
+    for (int j = l; j < q.runs; j += 64) R += a.rsum[(long)m * q.runs + j];
     R = wave_sum(R);
     f = -expm1f(logp[r]) * g[r] / R;
-    w += (long)a.labels[m] * a.D;
-    src = (ks > 1 ? a.part : a.dH) + (long)m * a.D;
+    w += (long)a.labels[m] * D;
+    src += (long)m * D;
+    ks = live_split(M, D, q.vchunk, q.dh_bm, q.dh_bn, q.dh_ks, q.part_elems);
   }
-  const long plane = (long)a.n * a.D;
-  for (int k = l; k < a.D / 8; k += 64) {
+  const long plane = (long)M * D;
+  for (int k = l; k < D / 8; k += 64) {
     float o[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) o[e] = f;
@@ -446,8 +478,9 @@ hipError_t token_logprobs(const bf16* normed, long ldh, const bf16* W, const int
   hipLaunchKernelGGL(lp_gather_kernel, dim3((n + 3) / 4), dim3(256), 0, s, normed, ldh, W, labels, D,
                      (const float*)nullptr, w);
   LPCK(hipGetLastError());
-  const int cfg = lp_cfg(n, D, V), run = lp_run(cfg);
+  const int cfg = lp_cfg(n, D, V, 0.0), run = lp_run(cfg);
   GemmProblem p{w.X, (long)D, W, (long)D, nullptr, 0, nullptr, 0, n, V, D, 0, w.count};
+  p.live = 1;
   LPCK(launch_gemm(p, EpiLogProb{w.stats, n, V, w.ref, w.labels, w.tgt}, s, cfg));
   hipLaunchKernelGGL(lp_finish_kernel, dim3((n + 15) / 16), dim3(256), 0, s, w, n,
                      (V + run - 1) / run, logp, other);
@@ -465,23 +498,30 @@ hipError_t token_logprobs_bwd(const bf16* normed, long ldh, const bf16* W, const
   hipLaunchKernelGGL(lp_gather_kernel, dim3((n + 3) / 4), dim3(256), 0, s, normed, ldh, W, labels, D,
                      other, w);
   LPCK(hipGetLastError());
-  HeadArgs& a = w.head;
-  a.normed = w.X;
-  a.ldh = D;
-  a.W = W;
-  a.labels = w.labels;
-  a.n_dev = w.count;
-  for (int c0 = 0; c0 < V; c0 += a.vchunk) {
-    const int Vc = std::min(a.vchunk, V - c0);
-    const GemmProblem p{w.X, (long)D, W + (long)c0 * D, (long)D, nullptr, 0, nullptr, 0,
-                        n,   Vc,      D,                0,       w.count};
-    const EpiProb epi{w.rsum, a.ntn, a.dlog, (long)a.vchunk, c0, Vc, (Vc + 7) / 8 * 8, w.ref,
-                      w.labels};
-    LPCK(launch_gemm(p, epi, s, a.ce_cfg));
-    LPCK(head_chunk_dh(a, c0, s));
+  const LPPlan& q = w.plan;
+  for (int c0 = 0; c0 < V; c0 += q.vchunk) {
+    const int Vc = std::min(q.vchunk, V - c0), Nc8 = (Vc + 7) / 8 * 8;
+    GemmProblem p{w.X, (long)D, W + (long)c0 * D, (long)D, nullptr, 0, nullptr, 0,
+                  n,   Vc,      D,                0,       w.count};
+    p.live = 1;
+    LPCK(launch_gemm(p,
+                     EpiProb{w.rsum, q.runs, w.P, (long)q.vchunk, c0, Vc, Nc8, w.ref, w.labels}, s,
+                     q.prob_cfg));
+    // the head read in place as the [K, N] operand; each slice adds up its own partial
+    GemmProblem h{w.P, (long)q.vchunk, W + (long)c0 * D, (long)D, nullptr, 0, nullptr, 0,
+                  n,   D,              Nc8,              0,       w.count};
+    h.b_kn = 1;
+    h.kb_rows = Vc;
+    h.part = w.part;
+    h.part_acc = c0 > 0 ? 1 : 0;
+    h.live = 1;
+    h.live_k = q.vchunk;
+    h.live_ks = q.dh_ks;
+    h.live_elems = q.part_elems;
+    LPCK(launch_gemm(h, EpiF32{w.part, (long)D, D, 0}, s, q.dh_cfg));
   }
-  hipLaunchKernelGGL(lp_dh_kernel, dim3((n + 3) / 4), dim3(256), 0, s, a, n, w.place, a.dh_ks, w.rsum,
-                     logp, dlogp, dH, lddh, out_f32);
+  hipLaunchKernelGGL(lp_dh_kernel, dim3((n + 3) / 4), dim3(256), 0, s, W, n, D, w, logp, dlogp, dH,
+                     lddh, out_f32);
   return hipGetLastError();
 }
 
