@@ -24,9 +24,19 @@ namespace {
 // (a logit more than about 40 over the label's) the run takes its own maximum.
 constexpr float kRunLimit = 0x1p57f;
 
-// Probabilities held at a time (1 GiB of bf16), and the most K slices of the dH product.
+// Probabilities held at a time: 1 GiB of bf16. Fewer chunks have fewer half-filled last
+// rounds of tiles and read and write the dH accumulators less often.
 constexpr long kProbElems = 1L << 29;
-constexpr int kMaxSlices = 8;
+// and at most this many columns: 256 rows of them stay within 32-bit byte offsets
+constexpr long kMaxChunk = 1L << 21;
+// Every product takes 256 × 256 tiles, also over few rows, where the head streams once:
+// at 16 to 2428 scored rows of the configured widths no other tile is ahead by more than
+// 2 % (149 rows × 5120 × 151936, forward: 401 µs; 256 × 128 457, 128 × 128 567), but under 40
+// rows at 1024 wide (122 µs against 142 for 128 × 128 forward, 229 against 195 backward).
+constexpr int kRun = 128;  // columns of a wave's tile
+// K slices of the dH product, most: 8 tiles (500 rows × 1024) fill the CUs 32 times
+// (349 µs; 16 slices 414, 8 580).
+constexpr int kMaxSlices = 32;
 
 struct LPStat {
   float ref, sum;  // Σ exp(logit − ref) over a run, the label left out
@@ -177,24 +187,6 @@ struct EpiProb {
   }
 };
 
-constexpr int lp_run(int cfg) {
-  return cfg == GEMM_BIG ? 128 : cfg == GEMM_NARROW || cfg == GEMM_SKINNY ? 32 : 64;
-}
-
-// The logits products' tile: by cost, `ob` bytes stored per logit.
-int lp_cfg(int n, int D, int V, double ob) {
-  int best = GEMM_BIG;
-  double bt = 0;
-  for (int cfg = 0; cfg < kGemmCfgs; ++cfg) {
-    const double c = gemm_cost(n, V, D, ob, cfg, 1);
-    if (bt == 0 || c < bt) {
-      bt = c;
-      best = cfg;
-    }
-  }
-  return best;
-}
-
 // Workspace pieces, 256-byte aligned; with a null base only the size is meant.
 struct Carve {
   char* p;
@@ -207,40 +199,20 @@ struct Carve {
   }
 };
 
-// The backward's products: `vchunk` columns of the vocabulary at a time (a multiple of
-// 256), the tile of the logits product and the width of its runs, and the tile and most K
-// slices of the dH product.
+// The backward's chunks of the vocabulary (`vchunk` columns, a multiple of 256) and the
+// room of the dH product's accumulators, all slices together: 2^24 elements are a tile for
+// each CU; half as many again, or three times n rows where that is more.
 struct LPPlan {
-  int vchunk, prob_cfg, run, runs, dh_cfg, dh_bm, dh_bn, dh_ks;
+  int vchunk;
   long part_elems;
 };
 LPPlan lp_plan(int n, int D, int V) {
-  LPPlan q{};
-  const long vr = ((long)V + 255) / 256 * 256;
-  const long units = (vr * n + kProbElems - 1) / kProbElems;
-  q.vchunk = (int)((vr / 256 + units - 1) / units * 256);
-  q.prob_cfg = lp_cfg(n, D, q.vchunk, 2.0);
-  q.run = lp_run(q.prob_cfg);
-  q.runs = (V + q.run - 1) / q.run;
-  // accumulators of all slices: three times the rows, and up to eight slices
-  q.dh_ks = kMaxSlices;
-  q.part_elems = (n > 2048 ? 3L : (long)kMaxSlices) * n * D;
-  double bt = 0;
-  for (int cfg = 0; cfg < kGemmCfgs; ++cfg) {
-    const GemmTile t = gemm_tile(cfg);
-    const int ks = live_split(n, D, q.vchunk, t.bm, t.bn, q.dh_ks, q.part_elems);
-    const long blocks = (long)((n + t.bm - 1) / t.bm) * ((D + t.bn - 1) / t.bn) * ks;
-    const double steps = ((q.vchunk + 63) / 64 + ks - 1) / ks;
-    const double c = std::max(std::ceil((double)blocks / kGemmCus) * steps * t.step,
-                              2.0 * q.vchunk * ((double)n + D) / 6.8e6) +
-                     4.0 * ks * n * D / 3.9e6;
-    if (bt == 0 || c < bt) {
-      bt = c;
-      q.dh_cfg = cfg;
-      q.dh_bm = t.bm;
-      q.dh_bn = t.bn;
-    }
-  }
+  const long blocks = ((long)V + 255) / 256;
+  const long units = std::max((blocks * 256 * n + kProbElems - 1) / kProbElems,
+                              (blocks + kMaxChunk / 256 - 1) / (kMaxChunk / 256));
+  LPPlan q;
+  q.vchunk = (int)((blocks + units - 1) / units * 256);
+  q.part_elems = std::min((long)kMaxSlices * n * D, std::max(3L << 23, 3L * n * D));
   return q;
 }
 
@@ -252,7 +224,8 @@ struct LPWork {
   float* ref;
   float* tgt;
   bf16* X;      // [n, D] the scored rows
-  LPStat* stats;
+  int runs;       // ceil(V / kRun)
+  LPStat* stats;  // forward: [runs, n]
   // backward
   float* rsum;   // [n, runs]
   bf16* P;       // [n, vchunk]
@@ -264,6 +237,7 @@ LPWork lp_layout(int n, int D, int V, bool backward, void* base, size_t* bytes) 
   Carve c{(char*)base};
   LPWork w{};
   const size_t N = (size_t)n;
+  w.runs = (V + kRun - 1) / kRun;
   w.count = c.take<int>(1);
   w.rows = c.take<int>(N);
   w.place = c.take<int>(N);
@@ -272,11 +246,10 @@ LPWork lp_layout(int n, int D, int V, bool backward, void* base, size_t* bytes) 
   w.tgt = c.take<float>(N);
   w.X = c.take<bf16>(N * D);
   if (!backward) {
-    const int run = lp_run(lp_cfg(n, D, V, 0.0));
-    w.stats = c.take<LPStat>(N * ((V + run - 1) / run));
+    w.stats = c.take<LPStat>(N * w.runs);
   } else {
     w.plan = lp_plan(n, D, V);
-    w.rsum = c.take<float>(N * w.plan.runs);
+    w.rsum = c.take<float>(N * w.runs);
     w.P = c.take<bf16>(N * w.plan.vchunk);
     w.part = c.take<float>((size_t)w.plan.part_elems);
   }
@@ -286,9 +259,9 @@ LPWork lp_layout(int n, int D, int V, bool backward, void* base, size_t* bytes) 
 
 }  // namespace
 
-// Single block: the scored rows' indices in order and their count. A row is scored
-// when 0 <= label < V and, with dlogp, dlogp ≠ 0 and logp < 0 (NaN: scored). Without
-// dlogp the other rows' outputs are written here: 0, or NaN for a label past V.
+// Single block, four rows to a thread: the scored rows' indices in order and their count. A
+// row is scored when 0 <= label < V and, with dlogp, dlogp ≠ 0 and logp < 0 (NaN: scored).
+// Without dlogp the other rows' outputs are written here: 0, or NaN for a label past V.
 __global__ __launch_bounds__(1024) void lp_rows_kernel(const int64_t* __restrict__ labels, int n,
                                                        int V, const float* __restrict__ dlogp,
                                                        const float* __restrict__ logp_in,
@@ -297,34 +270,46 @@ __global__ __launch_bounds__(1024) void lp_rows_kernel(const int64_t* __restrict
   __shared__ int tot[16];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   int base = 0;
-  for (int r0 = 0; r0 < n; r0 += 1024) {
-    const int r = r0 + tid;
-    int state = -1;
-    if (r < n) {
-      const int64_t lab = labels[r];
-      if (lab >= V)
-        state = -2;
-      else if (lab >= 0)
-        state = !dlogp || !(dlogp[r] == 0.f || logp_in[r] >= 0.f) ? 0 : -1;
-      if (state == -2 && dlogp && dlogp[r] == 0.f) state = -1;
+  for (int r0 = 0; r0 < n; r0 += 4096) {
+    const int r = r0 + 4 * tid;
+    int64_t lab[4];
+    float g[4], p[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bool in = r + i < n;
+      lab[i] = in ? labels[r + i] : -1;
+      g[i] = in && dlogp ? dlogp[r + i] : 1.f;
+      p[i] = in && dlogp ? logp_in[r + i] : -1.f;
     }
-    const unsigned long long live = __ballot(state == 0);
-    if (lane == 0) tot[wave] = __popcll(live);
+    int state[4], mine = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      state[i] = lab[i] < 0 || g[i] == 0.f ? -1 : lab[i] >= V ? -2 : p[i] >= 0.f ? -1 : 0;
+      mine += state[i] == 0;
+    }
+    int before = mine;  // of the wave's lanes up to this one
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int x = __shfl_up(before, o, 64);
+      before += lane >= o ? x : 0;
+    }
+    if (lane == 63) tot[wave] = before;
     __syncthreads();
-    int before = 0, all = 0;
+    int all = 0, at = base + before - mine;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      before += i < wave ? tot[i] : 0;
+      at += i < wave ? tot[i] : 0;
       all += tot[i];
     }
-    if (r < n) {
-      const int at = base + before + __popcll(live & ((1ull << lane) - 1));
-      if (state == 0) w.rows[at] = r;
-      w.place[r] = state == 0 ? at : state;
-      if (!dlogp && state < 0) {
-        const float v = state == -2 ? NAN : 0.f;
-        logp[r] = v;
-        other[r] = v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (r + i >= n) break;
+      w.place[r + i] = state[i] == 0 ? at : state[i];
+      if (state[i] == 0) w.rows[at++] = r + i;
+      if (!dlogp && state[i] < 0) {
+        const float v = state[i] == -2 ? NAN : 0.f;
+        logp[r + i] = v;
+        other[r + i] = v;
       }
     }
     base += all;
@@ -333,22 +318,22 @@ __global__ __launch_bounds__(1024) void lp_rows_kernel(const int64_t* __restrict
   if (tid == 0) *w.count = base;
 }
 
-// One wave per scored row: the row copied to its place, its label, and its softmax
+// One block per scored row: the row copied to its place, its label, and its softmax
 // reference: forward the dot with W[label], backward the forward's `other`.
 __global__ __launch_bounds__(256) void lp_gather_kernel(const bf16* __restrict__ H, long ldh,
                                                         const bf16* __restrict__ W,
                                                         const int64_t* __restrict__ labels, int D,
                                                         const float* __restrict__ other,
                                                         LPWork w) {
-  const int m = blockIdx.x * 4 + (threadIdx.x >> 6), l = threadIdx.x & 63;
+  __shared__ float red[4];
+  const int m = blockIdx.x;
   if (m >= *w.count) return;
   const int r = w.rows[m], lab = (int)labels[r];
   const bf16 *x = H + (long)r * ldh, *wt = W + (long)lab * D;
   bf16* o = w.X + (long)m * D;
   float dot = 0.f;
-  for (int k = l; k < D / 8; k += 64) {
+  for (int k = threadIdx.x; k < D / 8; k += 256) {
     const u32x4 v = ldg128(x + 8 * k);
-    stg128(o + 8 * k, v);
     if (!other) {
       float xf[8], wf[8];
       unpack8(v, xf);
@@ -356,32 +341,39 @@ __global__ __launch_bounds__(256) void lp_gather_kernel(const bf16* __restrict__
 #pragma unroll
       for (int e = 0; e < 8; ++e) dot += xf[e] * wf[e];
     }
+    stg128(o + 8 * k, v);
   }
-  if (!other) dot = wave_sum(dot);
-  if (l == 0) {
+  if (!other) dot = block_sum<256>(dot, red);
+  if (threadIdx.x == 0) {
     w.labels[m] = lab;
     w.ref[m] = other ? other[r] : dot;
   }
 }
 
-// 16 scored rows per block, 16 threads' shares of the runs each: the runs' sums
-// brought to one reference M, then logp and other = M + ln L.
-__global__ __launch_bounds__(256) void lp_finish_kernel(LPWork w, int cap, int runs,
-                                                        float* __restrict__ logp,
-                                                        float* __restrict__ other) {
-  __shared__ float ms[16][17], ls[16][17];
+// 16 scored rows per block, 64 threads' shares of the runs each: the runs' sums brought to
+// one reference M, then logp and other = M + ln L. Nearly always every run has the row's own
+// reference, and its sums are added as they are.
+__global__ __launch_bounds__(1024) void lp_finish_kernel(LPWork w, int cap,
+                                                         float* __restrict__ logp,
+                                                         float* __restrict__ other) {
+  __shared__ float ms[64][17], ls[64][17];
   const int i = threadIdx.x & 15, part = threadIdx.x >> 4, m = blockIdx.x * 16 + i;
   const int M = *w.count;
   if ((int)blockIdx.x * 16 >= M) return;  // uniform
   const float ref = m < M ? w.ref[m] : 0.f;
   float mx = ref, L = 0.f;
   if (m < M) {
-#pragma unroll 4
-    for (int t = part; t < runs; t += 16) {
+    bool other_ref = false;
+#pragma unroll 8
+    for (int t = part; t < w.runs; t += 64) {
       const LPStat s = w.stats[(long)t * cap + m];
-      if (s.ref == mx) {
-        L += s.sum;
-      } else {
+      L += s.sum;
+      other_ref |= s.ref != ref;
+    }
+    if (other_ref) {
+      L = 0.f;
+      for (int t = part; t < w.runs; t += 64) {
+        const LPStat s = w.stats[(long)t * cap + m];
         const float mn = fmaxf(mx, s.ref);
         L = L * __expf(mx - mn) + s.sum * __expf(s.ref - mn);
         mx = mn;
@@ -391,10 +383,13 @@ __global__ __launch_bounds__(256) void lp_finish_kernel(LPWork w, int cap, int r
   ms[part][i] = mx;
   ls[part][i] = L;
   __syncthreads();
-  if (part || m >= M) return;
-  for (int k = 1; k < 16; ++k) mx = fmaxf(mx, ms[k][i]);
+  if (part >= 4) return;  // the first wave: 4 threads to a row, in a fixed order
+  for (int k = 0; k < 64; ++k) mx = fmaxf(mx, ms[k][i]);
   L = 0.f;
-  for (int k = 0; k < 16; ++k) L += ls[k][i] * __expf(ms[k][i] - mx);
+  for (int k = part; k < 64; k += 4) L += ls[k][i] * __expf(ms[k][i] - mx);
+  L += __shfl_xor(L, 16, 64);
+  L += __shfl_xor(L, 32, 64);
+  if (part || m >= M) return;
   const float xt = w.tgt[m], d = xt - mx, et = __expf(d);
   const int r = w.rows[m];
   // log(1 + L/e_t), exact in L where the sum would round it away
@@ -402,32 +397,31 @@ __global__ __launch_bounds__(256) void lp_finish_kernel(LPWork w, int cap, int r
   other[r] = mx + logf(L);
 }
 
-// One wave per row: dH = g·(1 − p_t)·(W_t − acc/R) with R = Σ of the probabilities as
-// bf16 holds them (their common rounding falls out), acc the sum of the K slices'
-// accumulators; zeros for rows left out, NaN for a label past V. The row is rounded
-// once, to the output's type.
-__global__ __launch_bounds__(256) void lp_dh_kernel(const bf16* __restrict__ W, int n, int D,
-                                                    LPWork a, const float* __restrict__ logp,
+// One block per row: dH = g·(1 − p_t)·(W_t − acc/R) with R = Σ of the probabilities as bf16
+// holds them (their common rounding falls out), acc the sum of the K slices' accumulators;
+// zeros for rows left out, NaN for a label past V. The row is rounded once, to the output's
+// type.
+__global__ __launch_bounds__(256) void lp_dh_kernel(const bf16* __restrict__ W, int D, LPWork a,
+                                                    const float* __restrict__ logp,
                                                     const float* __restrict__ g, void* out,
                                                     long ldo, bool f32) {
-  const int r = blockIdx.x * 4 + (threadIdx.x >> 6), l = threadIdx.x & 63;
-  if (r >= n) return;
+  __shared__ float red[4];
+  const int r = blockIdx.x, tid = threadIdx.x;
   const int m = a.place[r], M = *a.count;
-  const LPPlan& q = a.plan;
   float f = m == -2 ? NAN : 0.f, R = 0.f;
   const bf16* w = W;
   const float* src = a.part;
   int ks = 1;
   if (m >= 0) {
-    for (int j = l; j < q.runs; j += 64) R += a.rsum[(long)m * q.runs + j];
-    R = wave_sum(R);
+    for (int j = tid; j < a.runs; j += 256) R += a.rsum[(long)m * a.runs + j];
+    R = block_sum<256>(R, red);
     f = -expm1f(logp[r]) * g[r] / R;
     w += (long)a.labels[m] * D;
     src += (long)m * D;
-    ks = live_split(M, D, q.vchunk, q.dh_bm, q.dh_bn, q.dh_ks, q.part_elems);
+    ks = live_split(M, D, a.plan.vchunk, 256, 256, kMaxSlices, a.plan.part_elems);
   }
   const long plane = (long)M * D;
-  for (int k = l; k < D / 8; k += 64) {
+  for (int k = tid; k < D / 8; k += 256) {
     float o[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) o[e] = f;
@@ -475,15 +469,13 @@ hipError_t token_logprobs(const bf16* normed, long ldh, const bf16* W, const int
   const LPWork w = lp_layout(n, D, V, false, work, &bytes);
   hipLaunchKernelGGL(lp_rows_kernel, dim3(1), dim3(1024), 0, s, labels, n, V,
                      (const float*)nullptr, (const float*)nullptr, logp, other, w);
-  hipLaunchKernelGGL(lp_gather_kernel, dim3((n + 3) / 4), dim3(256), 0, s, normed, ldh, W, labels, D,
+  hipLaunchKernelGGL(lp_gather_kernel, dim3(n), dim3(256), 0, s, normed, ldh, W, labels, D,
                      (const float*)nullptr, w);
   LPCK(hipGetLastError());
-  const int cfg = lp_cfg(n, D, V, 0.0), run = lp_run(cfg);
   GemmProblem p{w.X, (long)D, W, (long)D, nullptr, 0, nullptr, 0, n, V, D, 0, w.count};
   p.live = 1;
-  LPCK(launch_gemm(p, EpiLogProb{w.stats, n, V, w.ref, w.labels, w.tgt}, s, cfg));
-  hipLaunchKernelGGL(lp_finish_kernel, dim3((n + 15) / 16), dim3(256), 0, s, w, n,
-                     (V + run - 1) / run, logp, other);
+  LPCK((launch_gemm_cfg<256, 256, 2, 2>(p, EpiLogProb{w.stats, n, V, w.ref, w.labels, w.tgt}, s)));
+  hipLaunchKernelGGL(lp_finish_kernel, dim3((n + 15) / 16), dim3(1024), 0, s, w, n, logp, other);
   return hipGetLastError();
 }
 
@@ -492,36 +484,32 @@ hipError_t token_logprobs_bwd(const bf16* normed, long ldh, const bf16* W, const
                               const float* dlogp, void* dH, long lddh, bool out_f32, void* work,
                               hipStream_t s) {
   size_t bytes = 0;
-  LPWork w = lp_layout(n, D, V, true, work, &bytes);
+  const LPWork w = lp_layout(n, D, V, true, work, &bytes);
   hipLaunchKernelGGL(lp_rows_kernel, dim3(1), dim3(1024), 0, s, labels, n, V, dlogp, logp,
                      (float*)nullptr, (float*)nullptr, w);
-  hipLaunchKernelGGL(lp_gather_kernel, dim3((n + 3) / 4), dim3(256), 0, s, normed, ldh, W, labels, D,
-                     other, w);
+  hipLaunchKernelGGL(lp_gather_kernel, dim3(n), dim3(256), 0, s, normed, ldh, W, labels, D, other, w);
   LPCK(hipGetLastError());
-  const LPPlan& q = w.plan;
-  for (int c0 = 0; c0 < V; c0 += q.vchunk) {
-    const int Vc = std::min(q.vchunk, V - c0), Nc8 = (Vc + 7) / 8 * 8;
-    GemmProblem p{w.X, (long)D, W + (long)c0 * D, (long)D, nullptr, 0, nullptr, 0,
-                  n,   Vc,      D,                0,       w.count};
+  const int vchunk = w.plan.vchunk;
+  for (int c0 = 0; c0 < V; c0 += vchunk) {
+    const int Vc = std::min(vchunk, V - c0), Nc8 = (Vc + 7) / 8 * 8;
+    const bf16* Wc = W + (long)c0 * D;
+    GemmProblem p{w.X, (long)D, Wc, (long)D, nullptr, 0, nullptr, 0, n, Vc, D, 0, w.count};
     p.live = 1;
-    LPCK(launch_gemm(p,
-                     EpiProb{w.rsum, q.runs, w.P, (long)q.vchunk, c0, Vc, Nc8, w.ref, w.labels}, s,
-                     q.prob_cfg));
+    const EpiProb epi{w.rsum, w.runs, w.P, (long)vchunk, c0, Vc, Nc8, w.ref, w.labels};
+    LPCK((launch_gemm_cfg<256, 256, 2, 2>(p, epi, s)));
     // the head read in place as the [K, N] operand; each slice adds up its own partial
-    GemmProblem h{w.P, (long)q.vchunk, W + (long)c0 * D, (long)D, nullptr, 0, nullptr, 0,
-                  n,   D,              Nc8,              0,       w.count};
+    GemmProblem h{w.P, (long)vchunk, Wc, (long)D, nullptr, 0, nullptr, 0, n, D, Nc8, 0, w.count};
     h.b_kn = 1;
     h.kb_rows = Vc;
     h.part = w.part;
     h.part_acc = c0 > 0 ? 1 : 0;
     h.live = 1;
-    h.live_k = q.vchunk;
-    h.live_ks = q.dh_ks;
-    h.live_elems = q.part_elems;
-    LPCK(launch_gemm(h, EpiF32{w.part, (long)D, D, 0}, s, q.dh_cfg));
+    h.live_k = vchunk;
+    h.live_ks = kMaxSlices;
+    h.live_elems = w.plan.part_elems;
+    LPCK((launch_gemm_cfg<256, 256, 2, 2>(h, EpiF32{w.part, (long)D, D, 0}, s)));
   }
-  hipLaunchKernelGGL(lp_dh_kernel, dim3((n + 3) / 4), dim3(256), 0, s, W, n, D, w, logp, dlogp, dH,
-                     lddh, out_f32);
+  hipLaunchKernelGGL(lp_dh_kernel, dim3(n), dim3(256), 0, s, W, D, w, logp, dlogp, dH, lddh, out_f32);
   return hipGetLastError();
 }
 
