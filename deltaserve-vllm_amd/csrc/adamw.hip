@@ -150,59 +150,127 @@ __global__ void adam_hyper_kernel(const float* lr_dev, const int64_t* step_dev, 
                     step_dev ? *step_dev : step, seed);
 }
 
-// Σ g² of a chunk, in 64 bits (gradients of any finite size).
+// Σ g² of a chunk, in 64 bits (gradients of any finite size): a wave to a chunk, all its loads
+// of 16 bytes a lane in flight at once.
 __global__ __launch_bounds__(256) void adam_sumsq_kernel(const dsb_adam_tensor* __restrict__ T,
                                                          const int2* __restrict__ chunks,
+                                                         int nchunks,
                                                          double* __restrict__ partial) {
-  __shared__ double red[4];
-  const int2 ck = chunks[blockIdx.x];
+  const int c = blockIdx.x * 4 + (threadIdx.x >> 6), l = threadIdx.x & 63;
+  if (c >= nchunks) return;
+  const int2 ck = chunks[c];
   const dsb_adam_tensor t = T[ck.x];
-  const bool bf = (t.dtypes >> 8) == DSB_DT_BF16, vec = aligned4(t.g, bf);
-  const long e0 = (long)ck.y * kChunk + 4 * threadIdx.x;
+  const bool bf = (t.dtypes >> 8) == DSB_DT_BF16;
+  const long e0 = (long)ck.y * kChunk;
   double s = 0.0;
+  if (((unsigned long)t.g & 15) == 0 && e0 + kChunk <= t.numel) {
+    if (bf) {
+      u32x4 v[kChunk / 512];
 #pragma unroll
-  for (int k = 0; k < kChunk / 1024; ++k) {
-    const f32x4 g = load4(t.g, e0 + 1024 * k, t.numel, bf, vec);
+      for (int k = 0; k < kChunk / 512; ++k) v[k] = ldg128((const bf16*)t.g + e0 + 512 * k + 8 * l);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) s += (double)g[i] * (double)g[i];
+      for (int k = 0; k < kChunk / 512; ++k) {
+        float g[8];
+        unpack8(v[k], g);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s += (double)g[i] * (double)g[i];
+      }
+    } else {
+      f32x4 v[kChunk / 256];
+#pragma unroll
+      for (int k = 0; k < kChunk / 256; ++k)
+        v[k] = *reinterpret_cast<const f32x4*>((const float*)t.g + e0 + 256 * k + 4 * l);
+#pragma unroll
+      for (int k = 0; k < kChunk / 256; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s += (double)v[k][i] * (double)v[k][i];
+    }
+  } else {
+    const bool vec = aligned4(t.g, bf);
+#pragma unroll 4
+    for (int k = 0; k < kChunk / 256; ++k) {
+      const f32x4 g = load4(t.g, e0 + 256 * k + 4 * l, t.numel, bf, vec);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s += (double)g[i] * (double)g[i];
+    }
   }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+  if (l == 0) partial[c] = s;
+}
+
+// The sum over a block of NT threads, the same for all.
+template <int NT>
+DSB_DEV double block_sum64(double s, double* red) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
   __syncthreads();
-  if (threadIdx.x == 0) partial[blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
+  s = 0.0;
+#pragma unroll
+  for (int i = 0; i < NT / 64; ++i) s += red[i];
+  return s;
+}
+DSB_DEV float clip_factor(double norm, double max_norm) {
+  const double c = max_norm / (norm + 1e-6);
+  return c > 1.0 ? 1.f : (float)c;  // NaN stays
 }
 
 // One block per group: its chunks' sums in a fixed order, the norm and the factor.
-__global__ __launch_bounds__(256) void adam_norm_kernel(const int* __restrict__ group_chunks,
-                                                        const double* __restrict__ partial,
-                                                        double max_norm, float* __restrict__ norms,
-                                                        float* __restrict__ coef) {
-  __shared__ double red[4];
+__global__ __launch_bounds__(1024) void adam_norm_kernel(const int* __restrict__ group_chunks,
+                                                         const double* __restrict__ partial,
+                                                         double max_norm, float* __restrict__ norms,
+                                                         float* __restrict__ coef) {
+  __shared__ double red[16];
   const int c0 = group_chunks[blockIdx.x], c1 = group_chunks[blockIdx.x + 1];
   double s = 0.0;
-  for (int c = c0 + threadIdx.x; c < c1; c += 256) s += partial[c];
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
-  __syncthreads();
+#pragma unroll 4
+  for (int c = c0 + threadIdx.x; c < c1; c += 1024) s += partial[c];
+  const double norm = sqrt(block_sum64<1024>(s, red));
   if (threadIdx.x == 0) {
-    const double norm = sqrt((red[0] + red[1]) + (red[2] + red[3]));
-    const double c = max_norm / (norm + 1e-6);
     norms[blockIdx.x] = (float)norm;
-    coef[blockIdx.x] = c > 1.0 ? 1.f : (float)c;  // NaN stays
+    coef[blockIdx.x] = clip_factor(norm, max_norm);
   }
 }
+
+// How a step's blocks get their group's clip factor: none, from adam_norm_kernel, or each from
+// its group's sums.
+enum { CLIP_NONE, CLIP_GIVEN, CLIP_SUM };
+struct ClipArgs {
+  int how;
+  const float* coef;
+  const int* group_chunks;
+  int ngroups;
+  const double* partial;
+  double max_norm;
+  float* norms;
+};
 
 template <int BITS>
 __global__ __launch_bounds__(256) void adam_kernel(const dsb_adam_tensor* __restrict__ T,
                                                    const int2* __restrict__ chunks, Hyper hv,
-                                                   const Hyper* __restrict__ hp,
-                                                   const float* __restrict__ coef, void* mp,
+                                                   const Hyper* __restrict__ hp, ClipArgs clip,
+                                                   void* mp,
                                                    void* vp, float* __restrict__ m_scale,
                                                    float* __restrict__ r_scale) {
-  const int2 ck = chunks[blockIdx.x];
+  __shared__ double red[4];
+  // the chunks that the norm's pass read last come first: the device's cache still holds them
+  const int chunk = gridDim.x - 1 - blockIdx.x;
+  const int2 ck = chunks[chunk];
   const dsb_adam_tensor t = T[ck.x];
+  float cf = 1.f;
+  if (clip.how == CLIP_GIVEN) {
+    cf = clip.coef[t.group];
+  } else if (clip.how == CLIP_SUM) {
+    const int c0 = clip.group_chunks[t.group], c1 = clip.group_chunks[t.group + 1];
+    const double norm =
+        sqrt(block_sum64<256>(c0 + (int)threadIdx.x < c1 ? clip.partial[c0 + threadIdx.x] : 0.0, red));
+    cf = clip_factor(norm, clip.max_norm);
+    if (chunk == c0 && threadIdx.x == 0) clip.norms[t.group] = (float)norm;
+    if (chunk == 0)  // groups without elements
+      for (int g = threadIdx.x; g < clip.ngroups; g += 256)
+        if (clip.group_chunks[g] == clip.group_chunks[g + 1]) clip.norms[g] = 0.f;
+  }
   Hyper h = hv;
   if (hp) h = *hp;
   const int l16 = threadIdx.x & 15, qb = threadIdx.x >> 4;  // 16 blocks of 256 per chunk
@@ -210,7 +278,6 @@ __global__ __launch_bounds__(256) void adam_kernel(const dsb_adam_tensor* __rest
   if (tb * kBlock >= t.numel) return;                       // the 16 lanes of a block together
   const bool wbf = (t.dtypes & 255) == DSB_DT_BF16, gbf = (t.dtypes >> 8) == DSB_DT_BF16;
   const bool wvec = aligned4(t.w, wbf), gvec = aligned4(t.g, gbf);
-  const float cf = coef ? coef[t.group] : 1.f;
   const long b = t.block0 + tb, e0 = tb * kBlock + 4 * l16, s0 = b * kBlock + 4 * l16;
   f32x4 g[4], w[4];
   float m[4][4], r[4][4];
@@ -316,20 +383,25 @@ hipError_t adam_step(const AdamArgs& a, void* work, hipStream_t s) {
                        a.beta1, a.beta2, a.eps, a.wd, a.seed, hp);
   else
     hv = make_hyper(a.lr, a.beta1, a.beta2, a.eps, a.wd, a.step, a.seed);
+  ClipArgs c{CLIP_NONE, coef, a.group_chunks, a.ngroups, partial, a.max_norm, a.norms};
   if (clip) {
     if (a.nchunks > 0)
-      hipLaunchKernelGGL(adam_sumsq_kernel, dim3(a.nchunks), dim3(256), 0, s, a.tensors, a.chunks,
-                         partial);
-    hipLaunchKernelGGL(adam_norm_kernel, dim3(a.ngroups), dim3(256), 0, s, a.group_chunks, partial,
-                       a.max_norm, a.norms, coef);
+      hipLaunchKernelGGL(adam_sumsq_kernel, dim3((a.nchunks + 3) / 4), dim3(256), 0, s, a.tensors,
+                         a.chunks, a.nchunks, partial);
+    // Groups of at most 256 chunks (a million elements) are added up by each of their blocks,
+    // which saves a launch.
+    c.how = a.most_chunks <= 256 && a.nchunks > 0 ? CLIP_SUM : CLIP_GIVEN;
+    if (c.how == CLIP_GIVEN)
+      hipLaunchKernelGGL(adam_norm_kernel, dim3(a.ngroups), dim3(1024), 0, s, a.group_chunks, partial,
+                         a.max_norm, a.norms, coef);
   }
   if (a.nchunks > 0) {
     if (a.bits == 8)
       hipLaunchKernelGGL(adam_kernel<8>, dim3(a.nchunks), dim3(256), 0, s, a.tensors, a.chunks, hv,
-                         dev ? hp : nullptr, clip ? coef : nullptr, a.m, a.v, a.m_scale, a.r_scale);
+                         dev ? hp : nullptr, c, a.m, a.v, a.m_scale, a.r_scale);
     else
       hipLaunchKernelGGL(adam_kernel<32>, dim3(a.nchunks), dim3(256), 0, s, a.tensors, a.chunks, hv,
-                         dev ? hp : nullptr, clip ? coef : nullptr, a.m, a.v, a.m_scale, a.r_scale);
+                         dev ? hp : nullptr, c, a.m, a.v, a.m_scale, a.r_scale);
   }
   return hipGetLastError();
 }

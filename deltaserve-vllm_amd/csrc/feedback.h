@@ -48,7 +48,7 @@ struct AdamArgs {
   const int2* chunks;       // (tensor, 4096-element chunk of it)
   int nchunks;
   const int* group_chunks;  // [ngroups + 1] first chunk of each group
-  int ngroups;
+  int ngroups, most_chunks;
   void *m, *v;              // 8 bits: e4m3 codes of m and of sqrt(v); 32 bits: fp32 m and v
   float *m_scale, *r_scale;
   int bits;

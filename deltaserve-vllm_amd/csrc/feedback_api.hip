@@ -38,6 +38,7 @@ const char* check_logprob(const void* normed, int64_t ldh, const void* lm_w, con
   return nullptr;
 }
 const char* check_work(const void* work, int64_t have, int64_t need) {
+  if (need == 0) return nullptr;
   if (have < need || !work) return "the workspace is too small";
   if (misaligned(work, 256)) return "the workspace must be 256-byte aligned";
   return nullptr;
@@ -223,13 +224,14 @@ int dsb_op_adam_workspace(int nchunks, int ngroups, int64_t* bytes) {
 }
 
 int dsb_op_adam_step(const dsb_adam_tensor* tensors, const int32_t* chunks, int nchunks,
-                     const int32_t* group_chunks, int ngroups, void* m, void* v, float* m_scale,
-                     float* r_scale, int bits, double lr, double beta1, double beta2, double eps,
+                     const int32_t* group_chunks, int ngroups, int most_chunks, void* m, void* v,
+                     float* m_scale, float* r_scale, int bits, double lr, double beta1, double beta2, double eps,
                      double weight_decay, double max_norm, int64_t step, uint32_t seed,
                      const float* lr_dev, const int64_t* step_dev, float* norms, void* work,
                      int64_t work_bytes, void* stream) {
   const char* what = "dsb_op_adam_step";
-  if (nchunks < 0 || ngroups < 1) return bad(what, "bad sizes");
+  if (nchunks < 0 || ngroups < 1 || most_chunks < 0 || most_chunks > nchunks)
+    return bad(what, "bad sizes");
   if (bits != 8 && bits != 32) return bad(what, "the moments have 8 or 32 bits");
   if (!(beta1 >= 0 && beta1 < 1) || !(beta2 >= 0 && beta2 < 1))
     return bad(what, "beta1 and beta2 lie in [0, 1)");
@@ -248,6 +250,7 @@ int dsb_op_adam_step(const dsb_adam_tensor* tensors, const int32_t* chunks, int 
   a.nchunks = nchunks;
   a.group_chunks = group_chunks;
   a.ngroups = ngroups;
+  a.most_chunks = most_chunks;
   a.m = m;
   a.v = v;
   a.m_scale = m_scale;

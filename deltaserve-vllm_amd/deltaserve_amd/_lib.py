@@ -191,8 +191,8 @@ _SIGS = {
                                    c_double, c_double, c_void_p, c_void_p, c_void_p, c_int64,
                                    c_void_p]),
     "dsb_op_adam_workspace": (c_int, [c_int, c_int, POINTER(c_int64)]),
-    "dsb_op_adam_step": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p,
-                                 c_void_p, c_void_p, c_int, c_double, c_double, c_double, c_double,
+    "dsb_op_adam_step": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_void_p,
+                                 c_void_p, c_void_p, c_void_p, c_int, c_double, c_double, c_double, c_double,
                                  c_double, c_double, c_int64, c_uint32, c_void_p, c_void_p, c_void_p,
                                  c_void_p, c_int64, c_void_p]),
 }

@@ -328,23 +328,36 @@ _HERE = contextlib.nullcontext()
 
 def _on(what, *ts):
     """A context in which the device that holds all tensors (None: left out) is the current one."""
-    dev = None
+    dev = -1
     for t in ts:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise ValueError(f"{what}: takes CUDA (HIP) tensors")
-        if dev is not None and t.device != dev:
-            raise ValueError(f"{what}: the tensors are on different devices")
-        dev = t.device
-    return _HERE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+        if t is not None:
+            d = t.get_device()  # -1: not on a device
+            if d != dev:
+                if d < 0:
+                    raise ValueError(f"{what}: takes CUDA (HIP) tensors")
+                if dev >= 0:
+                    raise ValueError(f"{what}: the tensors are on different devices")
+                dev = d
+    if dev < 0:
+        raise ValueError(f"{what}: takes CUDA (HIP) tensors")
+    return _HERE if torch.cuda.current_device() == dev else torch.cuda.device(dev)
 
 
 def _vec(what, name, t, n, *dtypes):
     """A contiguous vector of n elements of one of the dtypes."""
-    if t.dtype not in dtypes or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+    if t.dtype not in dtypes or t.shape != (n,) or not t.is_contiguous():
         raise ValueError(f"{what}: {name} must be a contiguous vector of {n} elements of "
                          f"{' or '.join(str(d) for d in dtypes)}")
+
+
+def _at(t):
+    """A tensor's address for ctypes (None for None)."""
+    return None if t is None else t.data_ptr()
+
+
+def _now():
+    # (torch.cuda.current_stream() builds a stream object: 2.8 µs, this 0.1)
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def _work(nbytes, device):
@@ -355,7 +368,7 @@ class PackPlan:
     """Sequences packed row after row: their tables on the device, built once per packing by
     :func:`pack_plan` and read by the losses. ``n`` rows, ``nseq`` sequences."""
 
-    __slots__ = ("n", "nseq", "device", "c", "tables", "loss_bytes")
+    __slots__ = ("n", "nseq", "device", "c", "ref", "tables", "loss_bytes")
 
     def __init__(self, seq_lens, device):
         lib = L.load()
@@ -376,6 +389,7 @@ class PackPlan:
         self.tables.copy_(host)
         L.check(lib.dsb_op_loss_workspace(byref(c), byref(nbytes)), what="dsb_op_loss_workspace")
         self.c, self.n, self.nseq, self.loss_bytes = c, c.n, c.nseq, nbytes.value
+        self.ref = byref(c)
 
 
 def pack_plan(seq_lens, device="cuda"):
@@ -398,8 +412,8 @@ def next_token_labels(ids, plan, mask=None):
     with _on(what, ids, mask, plan.tables):
         labels = torch.empty_like(ids)
         rows = torch.empty(plan.n, dtype=torch.bool, device=ids.device)
-        L.check(L.load().dsb_op_next_token_labels(_p(ids), _p(mask), byref(plan.c), _p(labels),
-                                                  _p(rows), _stream()),
+        L.check(L.load().dsb_op_next_token_labels(_at(ids), _at(mask), plan.ref, _at(labels),
+                                                  _at(rows), _now()),
                 what="dsb_op_next_token_labels")
     return labels, rows
 
@@ -436,8 +450,8 @@ def token_logprobs(normed, lm_w, labels):
         logp = torch.empty(n, dtype=torch.float32, device=normed.device)
         other = torch.empty_like(logp)
         work, nbytes = _logprob_work(n, D, V, 0, normed.device)
-        L.check(L.load().dsb_op_token_logprobs(_p(normed), ld, _p(lm_w), _p(labels), n, D, V,
-                                               _p(logp), _p(other), _p(work), nbytes, _stream()),
+        L.check(L.load().dsb_op_token_logprobs(_at(normed), ld, _at(lm_w), _at(labels), n, D, V,
+                                               _at(logp), _at(other), _at(work), nbytes, _now()),
                 what="dsb_op_token_logprobs")
     return logp, other
 
@@ -455,8 +469,8 @@ def token_logprobs_backward(normed, lm_w, labels, logp, other, dlogp, out_dtype=
         dH = torch.empty(n, D, dtype=out_dtype, device=normed.device)
         work, nbytes = _logprob_work(n, D, V, 1, normed.device)
         L.check(L.load().dsb_op_token_logprobs_bwd(
-            _p(normed), ld, _p(lm_w), _p(labels), n, D, V, _p(logp), _p(other), _p(dlogp), _p(dH), D,
-            int(out_dtype == torch.float32), _p(work), nbytes, _stream()),
+            _at(normed), ld, _at(lm_w), _at(labels), n, D, V, _at(logp), _at(other), _at(dlogp),
+            _at(dH), D, int(out_dtype == torch.float32), _at(work), nbytes, _now()),
             what="dsb_op_token_logprobs_bwd")
     return dH
 
@@ -481,12 +495,11 @@ def preference_loss(logp, ref_logp, plan, mask=None, kind="sigmoid", beta=0.1, l
     with _on(what, logp, ref_logp, mask, plan.tables):
         dlogp = torch.empty_like(logp)
         out = torch.empty(1 + plan.nseq, dtype=torch.float32, device=logp.device)
-        work = _work(plan.loss_bytes, logp.device)
+        work = _work(plan.loss_bytes, logp.device) if plan.loss_bytes else None
         L.check(L.load().dsb_op_preference_loss(
-            _p(logp), _p(ref_logp), _p(mask), byref(plan.c), L.PREF_KINDS[kind], beta,
-            label_smoothing, margin, int(average), grad_scale, _p(out),
-            c_void_p(out.data_ptr() + 4), _p(dlogp), _p(work), work.numel(), _stream()),
-            what="dsb_op_preference_loss")
+            _at(logp), _at(ref_logp), _at(mask), plan.ref, L.PREF_KINDS[kind], beta, label_smoothing,
+            margin, average, grad_scale, _at(out), out.data_ptr() + 4, _at(dlogp), _at(work),
+            plan.loss_bytes, _now()), what="dsb_op_preference_loss")
     return out[0], out[1:], dlogp
 
 
@@ -518,12 +531,11 @@ def policy_loss(logp, old_logp, adv, plan, mask=None, ref_logp=None, clip_low=0.
     with _on(what, logp, old_logp, adv, ref_logp, mask, plan.tables):
         dlogp = torch.empty_like(logp)
         out = torch.empty(4, dtype=torch.float32, device=logp.device)
-        work = _work(plan.loss_bytes, logp.device)
+        work = _work(plan.loss_bytes, logp.device) if plan.loss_bytes else None
         L.check(L.load().dsb_op_policy_loss(
-            _p(logp), _p(old_logp), _p(ref_logp), _p(adv), int(by_row), _p(mask), byref(plan.c),
-            clip_low, clip_high, kl_coef, L.KL_KINDS[kl], L.REDUCTIONS[reduction], divisor,
-            grad_scale, _p(out), _p(dlogp), _p(work), work.numel(), _stream()),
-            what="dsb_op_policy_loss")
+            _at(logp), _at(old_logp), _at(ref_logp), _at(adv), by_row, _at(mask), plan.ref, clip_low,
+            clip_high, kl_coef, L.KL_KINDS[kl], L.REDUCTIONS[reduction], divisor, grad_scale,
+            _at(out), _at(dlogp), _at(work), plan.loss_bytes, _now()), what="dsb_op_policy_loss")
     return out[0], out[1:], dlogp
 
 
@@ -578,6 +590,7 @@ class AdamW:
             tensor = np.repeat(np.arange(len(ws)), chunks)
             table = np.stack([tensor, np.arange(self.nchunks) - first[tensor]], 1).astype(np.int32)
             per = np.bincount(np.array(groups), weights=chunks, minlength=self.ngroups)
+            most = int(per.max())
             ends = np.concatenate([[0], np.cumsum(per)]).astype(np.int32)
 
             def dev(a):
@@ -600,6 +613,10 @@ class AdamW:
                                "r_scale": zeros(self.nblocks, torch.float32)}
             else:
                 self._state = {"m": zeros(n, torch.float32), "v": zeros(n, torch.float32)}
+            s = self._state
+            self._args = (_at(self._tensors), _at(self._chunks), self.nchunks, _at(self._ends),
+                          self.ngroups, most, _at(s["m"]), _at(s["r" if bits == 8 else "v"]),
+                          _at(s.get("m_scale")), _at(s.get("r_scale")), bits)
 
     def state(self):
         """The moments by name (the optimizer's own tensors)."""
@@ -621,17 +638,14 @@ class AdamW:
                 raise ValueError(f"{what}: a {name} tensor holds one element of {dt}")
         if max_norm is not None and not max_norm >= 0:
             raise ValueError(f"{what}: max_norm must not be negative")
-        s = self._state
         with _on(what, self._tensors, lr_t, step_t):
             norms = None
             if max_norm is not None:
                 norms = torch.empty(self.ngroups, dtype=torch.float32, device=self.device)
             work = _work(self._bytes, self.device)
             L.check(L.load().dsb_op_adam_step(
-                _p(self._tensors), _p(self._chunks), self.nchunks, _p(self._ends), self.ngroups,
-                _p(s["m"]), _p(s["r" if self.bits == 8 else "v"]), _p(s.get("m_scale")),
-                _p(s.get("r_scale")), self.bits, 0.0 if lr_t is not None else lr, beta1, beta2, eps,
-                wd, -1.0 if max_norm is None else max_norm, 0 if step_t is not None else step,
-                seed & 0xffffffff, _p(lr_t), _p(step_t), _p(norms), _p(work), work.numel(),
-                _stream()), what="dsb_op_adam_step")
+                *self._args, 0.0 if lr_t is not None else lr, beta1, beta2, eps, wd,
+                -1.0 if max_norm is None else max_norm, 0 if step_t is not None else step,
+                seed & 0xffffffff, _at(lr_t), _at(step_t), _at(norms), _at(work), self._bytes, _now()),
+                what="dsb_op_adam_step")
         return norms

@@ -437,6 +437,7 @@ int dsb_plan_fill(const int32_t* seq_lens, dsb_pack_plan* plan, int32_t* tables,
 int dsb_op_next_token_labels(const int64_t* ids, const uint8_t* mask, const dsb_pack_plan* plan,
                              int64_t* labels, uint8_t* rows, void* stream);
 
+/* 0 for a batch that one workgroup takes (work may be null then). */
 int dsb_op_loss_workspace(const dsb_pack_plan* plan, int64_t* bytes);
 /* Preference loss over pairs: sequences 2i (preferred) and 2i + 1 of the plan.
  * s_y = Σ over the scored rows of y of (logp − ref) (its mean with `average`; 0 where
@@ -485,7 +486,8 @@ typedef struct dsb_adam_tensor {
 /* Clip by group and AdamW over many tensors (the arithmetic of dsb_op_clip_adamw; the
  * gradients are left as they are). tensors, chunks ((tensor, chunk of it) int32 pairs,
  * chunks of DSB_ADAM_CHUNK elements, in order of the tensors' groups) and group_chunks
- * [ngroups + 1] (first chunk of each group) live on the device.
+ * [ngroups + 1] (first chunk of each group) live on the device; most_chunks: those of the
+ * largest group.
  * bits 32: m and v fp32 by block. bits 8: m holds e4m3 codes of m / m_scale and v those
  * of sqrt(v) / r_scale, scales fp32 by block, the block's largest magnitude / 448; m is
  * rounded to nearest, sqrt(v) up or down at random in proportion (a function of seed, step,
@@ -495,8 +497,8 @@ typedef struct dsb_adam_tensor {
  * and the step count (int64) are read on the device, for a captured step. */
 int dsb_op_adam_workspace(int nchunks, int ngroups, int64_t* bytes);
 int dsb_op_adam_step(const dsb_adam_tensor* tensors, const int32_t* chunks, int nchunks,
-                     const int32_t* group_chunks, int ngroups, void* m, void* v, float* m_scale,
-                     float* r_scale, int bits, double lr, double beta1, double beta2, double eps,
+                     const int32_t* group_chunks, int ngroups, int most_chunks, void* m, void* v,
+                     float* m_scale, float* r_scale, int bits, double lr, double beta1, double beta2, double eps,
                      double weight_decay, double max_norm, int64_t step, uint32_t seed,
                      const float* lr_dev, const int64_t* step_dev, float* norms, void* work,
                      int64_t work_bytes, void* stream);

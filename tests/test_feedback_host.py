@@ -160,7 +160,7 @@ NAN, INF = float("nan"), float("inf")
                                  dict(work=None), dict(nbytes=1), dict(plan=None)])
 def test_preference_refusals(bad):
     L, lib = _lib()
-    c, pref, _ = _losses(lib, L, [4, 5])
+    c, pref, _ = _losses(lib, L, [4000, 5000])
     assert pref(**bad) != 0 and L.last_error()
 
 
@@ -177,7 +177,7 @@ def test_preference_needs_pairs(lens):
                                  dict(d=None), dict(adv=FAKE + 1), dict(nbytes=1), dict(plan=None)])
 def test_policy_refusals(bad):
     L, lib = _lib()
-    c, _, policy = _losses(lib, L, [4, 5])
+    c, _, policy = _losses(lib, L, [4000, 5000])
     assert policy(**bad) != 0 and L.last_error()
 
 
@@ -185,10 +185,11 @@ def test_policy_refusals(bad):
                                  dict(eps=INF), dict(lr=NAN), dict(wd=INF), dict(step=0), dict(maxn=NAN),
                                  dict(maxn=1.0, norms=None), dict(m=None), dict(v=FAKE + 4),
                                  dict(ms=None), dict(tensors=None), dict(ngroups=0), dict(nbytes=8),
-                                 dict(work=FAKE + 8), dict(nchunks=-1)])
+                                 dict(work=FAKE + 8), dict(nchunks=-1), dict(most=2),
+                                 dict(most=-1)])
 def test_adam_refusals(bad):
     L, lib = _lib()
-    a = dict(tensors=FAKE, chunks=FAKE, nchunks=1, gc=FAKE, ngroups=1, m=FAKE, v=FAKE, ms=FAKE, rs=FAKE,
+    a = dict(tensors=FAKE, chunks=FAKE, nchunks=1, gc=FAKE, ngroups=1, most=1, m=FAKE, v=FAKE, ms=FAKE, rs=FAKE,
              bits=8, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, wd=0.0, maxn=-1.0, step=1, seed=0,
              lrd=None, stepd=None, norms=FAKE, work=FAKE, nbytes=BIG)
     a.update(bad)
