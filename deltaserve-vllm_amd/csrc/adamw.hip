@@ -63,8 +63,8 @@ __host__ __device__ inline Hyper make_hyper(double lr, double beta1, double beta
   return h;
 }
 
-// 4 consecutive elements from e of a tensor of `numel`, as fp32; zeros past its end
-DSB_DEV f32x4 load4(const void* p, long e, long numel, bool bf, bool vec) {
+// 4 consecutive elements from e of a chunk of `numel`, as fp32; zeros past its end
+DSB_DEV f32x4 load4(const void* p, int e, int numel, bool bf, bool vec) {
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
   if (vec && e + 4 <= numel) {
     if (bf) {
@@ -81,7 +81,7 @@ DSB_DEV f32x4 load4(const void* p, long e, long numel, bool bf, bool vec) {
     if (e + i < numel) o[i] = bf ? (float)((const bf16*)p)[e + i] : ((const float*)p)[e + i];
   return o;
 }
-DSB_DEV void store4(void* p, long e, long numel, bool bf, bool vec, f32x4 v) {
+DSB_DEV void store4(void* p, int e, int numel, bool bf, bool vec, f32x4 v) {
   if (vec && e + 4 <= numel) {
     if (bf)
       *reinterpret_cast<bf16x4*>((bf16*)p + e) =
@@ -152,22 +152,19 @@ __global__ void adam_hyper_kernel(const float* lr_dev, const int64_t* step_dev, 
 
 // Σ g² of a chunk, in 64 bits (gradients of any finite size): a wave to a chunk, all its loads
 // of 16 bytes a lane in flight at once.
-__global__ __launch_bounds__(256) void adam_sumsq_kernel(const dsb_adam_tensor* __restrict__ T,
-                                                         const int2* __restrict__ chunks,
+__global__ __launch_bounds__(256) void adam_sumsq_kernel(const dsb_adam_chunk* __restrict__ chunks,
                                                          int nchunks,
                                                          double* __restrict__ partial) {
   const int c = blockIdx.x * 4 + (threadIdx.x >> 6), l = threadIdx.x & 63;
   if (c >= nchunks) return;
-  const int2 ck = chunks[c];
-  const dsb_adam_tensor t = T[ck.x];
+  const dsb_adam_chunk t = chunks[c];
   const bool bf = (t.dtypes >> 8) == DSB_DT_BF16;
-  const long e0 = (long)ck.y * kChunk;
   double s = 0.0;
-  if (((unsigned long)t.g & 15) == 0 && e0 + kChunk <= t.numel) {
+  if (((unsigned long)t.g & 15) == 0 && t.count == kChunk) {
     if (bf) {
       u32x4 v[kChunk / 512];
 #pragma unroll
-      for (int k = 0; k < kChunk / 512; ++k) v[k] = ldg128((const bf16*)t.g + e0 + 512 * k + 8 * l);
+      for (int k = 0; k < kChunk / 512; ++k) v[k] = ldg128((const bf16*)t.g + 512 * k + 8 * l);
 #pragma unroll
       for (int k = 0; k < kChunk / 512; ++k) {
         float g[8];
@@ -179,7 +176,7 @@ __global__ __launch_bounds__(256) void adam_sumsq_kernel(const dsb_adam_tensor* 
       f32x4 v[kChunk / 256];
 #pragma unroll
       for (int k = 0; k < kChunk / 256; ++k)
-        v[k] = *reinterpret_cast<const f32x4*>((const float*)t.g + e0 + 256 * k + 4 * l);
+        v[k] = *reinterpret_cast<const f32x4*>((const float*)t.g + 256 * k + 4 * l);
 #pragma unroll
       for (int k = 0; k < kChunk / 256; ++k)
 #pragma unroll
@@ -189,7 +186,7 @@ __global__ __launch_bounds__(256) void adam_sumsq_kernel(const dsb_adam_tensor* 
     const bool vec = aligned4(t.g, bf);
 #pragma unroll 4
     for (int k = 0; k < kChunk / 256; ++k) {
-      const f32x4 g = load4(t.g, e0 + 256 * k + 4 * l, t.numel, bf, vec);
+      const f32x4 g = load4(t.g, 256 * k + 4 * l, t.count, bf, vec);
 #pragma unroll
       for (int i = 0; i < 4; ++i) s += (double)g[i] * (double)g[i];
     }
@@ -247,17 +244,48 @@ struct ClipArgs {
 };
 
 template <int BITS>
-__global__ __launch_bounds__(256) void adam_kernel(const dsb_adam_tensor* __restrict__ T,
-                                                   const int2* __restrict__ chunks, Hyper hv,
-                                                   const Hyper* __restrict__ hp, ClipArgs clip,
-                                                   void* mp,
-                                                   void* vp, float* __restrict__ m_scale,
+__global__ __launch_bounds__(256) void adam_kernel(const dsb_adam_chunk* __restrict__ chunks,
+                                                   Hyper hv, const Hyper* __restrict__ hp,
+                                                   ClipArgs clip, void* mp, void* vp,
+                                                   float* __restrict__ m_scale,
                                                    float* __restrict__ r_scale) {
   __shared__ double red[4];
   // the chunks that the norm's pass read last come first: the device's cache still holds them
   const int chunk = gridDim.x - 1 - blockIdx.x;
-  const int2 ck = chunks[chunk];
-  const dsb_adam_tensor t = T[ck.x];
+  const dsb_adam_chunk t = chunks[chunk];
+  const int l16 = threadIdx.x & 15, qb = threadIdx.x >> 4;  // 16 blocks of 256 per chunk
+  const bool live = qb * kBlock < t.count;                  // the 16 lanes of a block together
+  const bool wbf = (t.dtypes & 255) == DSB_DT_BF16, gbf = (t.dtypes >> 8) == DSB_DT_BF16;
+  const bool wvec = aligned4(t.w, wbf), gvec = aligned4(t.g, gbf);
+  const int e0 = qb * kBlock + 4 * l16;
+  const long b = t.block + qb, s0 = b * kBlock + 4 * l16;
+  f32x4 g[4], w[4];
+  float m[4][4], r[4][4];
+  unsigned mc[4], rc[4];
+  float ms = 0.f, rs = 0.f;
+  if (live) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) g[k] = load4(t.g, e0 + 64 * k, t.count, gbf, gvec);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] = load4(t.w, e0 + 64 * k, t.count, wbf, wvec);
+    if constexpr (BITS == 8) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        mc[k] = *reinterpret_cast<const unsigned*>((const uint8_t*)mp + s0 + 64 * k);
+        rc[k] = *reinterpret_cast<const unsigned*>((const uint8_t*)vp + s0 + 64 * k);
+      }
+      ms = m_scale[b];
+      rs = r_scale[b];
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        *reinterpret_cast<f32x4*>(m[k]) =
+            *reinterpret_cast<const f32x4*>((const float*)mp + s0 + 64 * k);
+        *reinterpret_cast<f32x4*>(r[k]) =
+            *reinterpret_cast<const f32x4*>((const float*)vp + s0 + 64 * k);
+      }
+    }
+  }
   float cf = 1.f;
   if (clip.how == CLIP_GIVEN) {
     cf = clip.coef[t.group];
@@ -271,37 +299,9 @@ __global__ __launch_bounds__(256) void adam_kernel(const dsb_adam_tensor* __rest
       for (int g = threadIdx.x; g < clip.ngroups; g += 256)
         if (clip.group_chunks[g] == clip.group_chunks[g + 1]) clip.norms[g] = 0.f;
   }
+  if (!live) return;
   Hyper h = hv;
   if (hp) h = *hp;
-  const int l16 = threadIdx.x & 15, qb = threadIdx.x >> 4;  // 16 blocks of 256 per chunk
-  const long tb = (long)ck.y * (kChunk / kBlock) + qb;      // block within the tensor
-  if (tb * kBlock >= t.numel) return;                       // the 16 lanes of a block together
-  const bool wbf = (t.dtypes & 255) == DSB_DT_BF16, gbf = (t.dtypes >> 8) == DSB_DT_BF16;
-  const bool wvec = aligned4(t.w, wbf), gvec = aligned4(t.g, gbf);
-  const long b = t.block0 + tb, e0 = tb * kBlock + 4 * l16, s0 = b * kBlock + 4 * l16;
-  f32x4 g[4], w[4];
-  float m[4][4], r[4][4];
-  unsigned mc[4], rc[4];
-  float ms = 0.f, rs = 0.f;
-#pragma unroll
-  for (int k = 0; k < 4; ++k) g[k] = load4(t.g, e0 + 64 * k, t.numel, gbf, gvec);
-#pragma unroll
-  for (int k = 0; k < 4; ++k) w[k] = load4(t.w, e0 + 64 * k, t.numel, wbf, wvec);
-  if constexpr (BITS == 8) {
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      mc[k] = *reinterpret_cast<const unsigned*>((const uint8_t*)mp + s0 + 64 * k);
-      rc[k] = *reinterpret_cast<const unsigned*>((const uint8_t*)vp + s0 + 64 * k);
-    }
-    ms = m_scale[b];
-    rs = r_scale[b];
-  } else {
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      *reinterpret_cast<f32x4*>(m[k]) = *reinterpret_cast<const f32x4*>((const float*)mp + s0 + 64 * k);
-      *reinterpret_cast<f32x4*>(r[k]) = *reinterpret_cast<const f32x4*>((const float*)vp + s0 + 64 * k);
-    }
-  }
   unsigned mtop = 0, rtop = 0;
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
@@ -331,7 +331,7 @@ __global__ __launch_bounds__(256) void adam_kernel(const dsb_adam_tensor* __rest
                       __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v) * h.rbc2 + h.eps);
       }
     }
-    store4(t.w, e0 + 64 * k, t.numel, wbf, wvec, w[k]);
+    store4(t.w, e0 + 64 * k, t.count, wbf, wvec, w[k]);
     if constexpr (BITS == 32) {
       *reinterpret_cast<f32x4*>((float*)mp + s0 + 64 * k) = *reinterpret_cast<f32x4*>(m[k]);
       *reinterpret_cast<f32x4*>((float*)vp + s0 + 64 * k) = *reinterpret_cast<f32x4*>(r[k]);
@@ -341,8 +341,8 @@ __global__ __launch_bounds__(256) void adam_kernel(const dsb_adam_tensor* __rest
     const float mt = __builtin_bit_cast(float, max16(mtop));
     const float rt = __builtin_bit_cast(float, max16(rtop));
     // not below kTiny (so NaN and infinity show in the scale)
-    const float im = mt < kTiny ? 0.f : 448.f * __builtin_amdgcn_rcpf(mt);
-    const float ir = rt < kTiny ? 0.f : 448.f * __builtin_amdgcn_rcpf(rt);
+    const float im = mt < kTiny ? 0.f : 448.f / mt;
+    const float ir = rt < kTiny ? 0.f : 448.f / rt;
     const unsigned key = mix32(h.key ^ mix32((unsigned)b));
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -386,8 +386,8 @@ hipError_t adam_step(const AdamArgs& a, void* work, hipStream_t s) {
   ClipArgs c{CLIP_NONE, coef, a.group_chunks, a.ngroups, partial, a.max_norm, a.norms};
   if (clip) {
     if (a.nchunks > 0)
-      hipLaunchKernelGGL(adam_sumsq_kernel, dim3((a.nchunks + 3) / 4), dim3(256), 0, s, a.tensors,
-                         a.chunks, a.nchunks, partial);
+      hipLaunchKernelGGL(adam_sumsq_kernel, dim3((a.nchunks + 3) / 4), dim3(256), 0, s, a.chunks,
+                         a.nchunks, partial);
     // Groups of at most 256 chunks (a million elements) are added up by each of their blocks,
     // which saves a launch.
     c.how = a.most_chunks <= 256 && a.nchunks > 0 ? CLIP_SUM : CLIP_GIVEN;
@@ -397,10 +397,10 @@ hipError_t adam_step(const AdamArgs& a, void* work, hipStream_t s) {
   }
   if (a.nchunks > 0) {
     if (a.bits == 8)
-      hipLaunchKernelGGL(adam_kernel<8>, dim3(a.nchunks), dim3(256), 0, s, a.tensors, a.chunks, hv,
+      hipLaunchKernelGGL(adam_kernel<8>, dim3(a.nchunks), dim3(256), 0, s, a.chunks, hv,
                          dev ? hp : nullptr, c, a.m, a.v, a.m_scale, a.r_scale);
     else
-      hipLaunchKernelGGL(adam_kernel<32>, dim3(a.nchunks), dim3(256), 0, s, a.tensors, a.chunks, hv,
+      hipLaunchKernelGGL(adam_kernel<32>, dim3(a.nchunks), dim3(256), 0, s, a.chunks, hv,
                          dev ? hp : nullptr, c, a.m, a.v, a.m_scale, a.r_scale);
   }
   return hipGetLastError();

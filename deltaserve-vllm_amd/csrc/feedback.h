@@ -44,8 +44,7 @@ hipError_t policy_loss(const float* logp, const float* old, const float* ref, co
 
 // ---- adamw.hip
 struct AdamArgs {
-  const dsb_adam_tensor* tensors;
-  const int2* chunks;       // (tensor, 4096-element chunk of it)
+  const dsb_adam_chunk* chunks;
   int nchunks;
   const int* group_chunks;  // [ngroups + 1] first chunk of each group
   int ngroups, most_chunks;

@@ -223,9 +223,9 @@ int dsb_op_adam_workspace(int nchunks, int ngroups, int64_t* bytes) {
   return 0;
 }
 
-int dsb_op_adam_step(const dsb_adam_tensor* tensors, const int32_t* chunks, int nchunks,
-                     const int32_t* group_chunks, int ngroups, int most_chunks, void* m, void* v,
-                     float* m_scale, float* r_scale, int bits, double lr, double beta1, double beta2, double eps,
+int dsb_op_adam_step(const dsb_adam_chunk* chunks, int nchunks, const int32_t* group_chunks,
+                     int ngroups, int most_chunks, void* m, void* v, float* m_scale,
+                     float* r_scale, int bits, double lr, double beta1, double beta2, double eps,
                      double weight_decay, double max_norm, int64_t step, uint32_t seed,
                      const float* lr_dev, const int64_t* step_dev, float* norms, void* work,
                      int64_t work_bytes, void* stream) {
@@ -240,13 +240,12 @@ int dsb_op_adam_step(const dsb_adam_tensor* tensors, const int32_t* chunks, int 
   if (!step_dev && step < 1) return bad(what, "step counts from 1");
   if (std::isnan(max_norm)) return bad(what, "max_norm is NaN");
   if (max_norm >= 0 && (!norms || !group_chunks)) return bad(what, "null argument");
-  if (nchunks > 0 && (!tensors || !chunks || !m || !v || (bits == 8 && (!m_scale || !r_scale))))
+  if (nchunks > 0 && (!chunks || !m || !v || (bits == 8 && (!m_scale || !r_scale))))
     return bad(what, "null argument");
   if (misaligned(m, 16) || misaligned(v, 16)) return bad(what, "the moments must be 16-byte aligned");
   if (const char* e = check_work(work, work_bytes, adam_bytes(nchunks, ngroups))) return bad(what, e);
   AdamArgs a{};
-  a.tensors = tensors;
-  a.chunks = (const int2*)chunks;
+  a.chunks = chunks;
   a.nchunks = nchunks;
   a.group_chunks = group_chunks;
   a.ngroups = ngroups;

@@ -84,9 +84,9 @@ class DsbPackPlan(Structure):
         (k, c_int32) for k in ("ntiles", "nseq", "n", "npred", "nonempty")]
 
 
-class DsbAdamTensor(Structure):
-    _fields_ = [("w", c_void_p), ("g", c_void_p), ("numel", c_int64), ("block0", c_int64),
-                ("group", c_int32), ("dtypes", c_int32)]
+class DsbAdamChunk(Structure):
+    _fields_ = [("w", c_void_p), ("g", c_void_p), ("block", c_int64), ("count", c_int32),
+                ("group", c_int32), ("dtypes", c_int32), ("pad", c_int32)]
 
 
 # name -> (restype, argtypes)
@@ -191,7 +191,7 @@ _SIGS = {
                                    c_double, c_double, c_void_p, c_void_p, c_void_p, c_int64,
                                    c_void_p]),
     "dsb_op_adam_workspace": (c_int, [c_int, c_int, POINTER(c_int64)]),
-    "dsb_op_adam_step": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_void_p,
+    "dsb_op_adam_step": (c_int, [c_void_p, c_int, c_void_p, c_int, c_int, c_void_p,
                                  c_void_p, c_void_p, c_void_p, c_int, c_double, c_double, c_double, c_double,
                                  c_double, c_double, c_int64, c_uint32, c_void_p, c_void_p, c_void_p,
                                  c_void_p, c_int64, c_void_p]),

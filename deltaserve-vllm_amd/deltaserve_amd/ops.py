@@ -582,22 +582,27 @@ class AdamW:
             self.nblocks, self.nchunks = int(blocks.sum()), int(chunks.sum())
             if self.nchunks > 0x7fffffff:
                 raise ValueError(f"{what}: too many elements")
-            rec = (L.DsbAdamTensor * len(ws))(*[
-                L.DsbAdamTensor(w.data_ptr(), g.data_ptr(), int(numel[i]), int(block0[i]), groups[i],
-                                code[w.dtype] + 256 * code[g.dtype])
-                for i, (w, g) in enumerate(zip(ws, gs))])
-            first = np.cumsum(chunks) - chunks
-            tensor = np.repeat(np.arange(len(ws)), chunks)
-            table = np.stack([tensor, np.arange(self.nchunks) - first[tensor]], 1).astype(np.int32)
+            # a record per chunk: one table to read, no second one behind it
+            t = np.repeat(np.arange(len(ws)), chunks)
+            at = (np.arange(self.nchunks) - (np.cumsum(chunks) - chunks)[t]) * L.ADAM_CHUNK
+            table = np.zeros(self.nchunks, dtype=np.dtype(L.DsbAdamChunk))
+            for name, ts in (("w", ws), ("g", gs)):
+                base = np.array([x.data_ptr() for x in ts], dtype=np.uint64)
+                size = np.array([x.element_size() for x in ts], dtype=np.int64)
+                table[name] = base[t] + (at * size[t]).astype(np.uint64)
+            table["block"] = block0[t] + at // L.ADAM_BLOCK
+            table["count"] = np.minimum(numel[t] - at, L.ADAM_CHUNK)
+            table["group"] = np.array(groups)[t]
+            table["dtypes"] = np.array([code[w.dtype] + 256 * code[g.dtype] for w, g in zip(ws, gs)])[t]
             per = np.bincount(np.array(groups), weights=chunks, minlength=self.ngroups)
             most = int(per.max())
             ends = np.concatenate([[0], np.cumsum(per)]).astype(np.int32)
 
             def dev(a):
-                raw = np.frombuffer(bytes(a), dtype=np.uint8).copy()
+                raw = np.frombuffer(a.tobytes(), dtype=np.uint8).copy()
                 return torch.from_numpy(raw).to(self.device) if raw.size else _work(0, self.device)
 
-            self._tensors, self._chunks, self._ends = dev(rec), dev(table), dev(ends)
+            self._chunks, self._ends = dev(table), dev(ends)
             self._kept = [t.untyped_storage() for t in (*ws, *gs)]
             nbytes = c_int64()
             L.check(L.load().dsb_op_adam_workspace(self.nchunks, self.ngroups, byref(nbytes)),
@@ -614,9 +619,9 @@ class AdamW:
             else:
                 self._state = {"m": zeros(n, torch.float32), "v": zeros(n, torch.float32)}
             s = self._state
-            self._args = (_at(self._tensors), _at(self._chunks), self.nchunks, _at(self._ends),
-                          self.ngroups, most, _at(s["m"]), _at(s["r" if bits == 8 else "v"]),
-                          _at(s.get("m_scale")), _at(s.get("r_scale")), bits)
+            self._args = (_at(self._chunks), self.nchunks, _at(self._ends), self.ngroups, most,
+                          _at(s["m"]), _at(s["r" if bits == 8 else "v"]), _at(s.get("m_scale")),
+                          _at(s.get("r_scale")), bits)
 
     def state(self):
         """The moments by name (the optimizer's own tensors)."""
@@ -638,7 +643,7 @@ class AdamW:
                 raise ValueError(f"{what}: a {name} tensor holds one element of {dt}")
         if max_norm is not None and not max_norm >= 0:
             raise ValueError(f"{what}: max_norm must not be negative")
-        with _on(what, self._tensors, lr_t, step_t):
+        with _on(what, self._chunks, lr_t, step_t):
             norms = None
             if max_norm is not None:
                 norms = torch.empty(self.ngroups, dtype=torch.float32, device=self.device)

@@ -471,21 +471,22 @@ int dsb_op_policy_loss(const float* logp, const float* old_logp, const float* re
                        double kl_coef, int kl, int reduction, double divisor, double grad_scale,
                        float* out, float* dlogp, void* work, int64_t work_bytes, void* stream);
 
-/* One tensor of an AdamW step. w and g: element type by dtypes (DSB_DT_BF16 or
- * DSB_DT_F32, w + 256·g), aligned to their type. block0: its first block of
- * DSB_ADAM_BLOCK elements in the moments (a tensor starts on a block). */
+/* Up to DSB_ADAM_CHUNK elements of one tensor of an AdamW step, from a multiple of that: their
+ * address in the weights and in the gradients (element types by dtypes: DSB_DT_BF16 or
+ * DSB_DT_F32, w + 256·g; aligned to their type), the first of their blocks of DSB_ADAM_BLOCK
+ * elements in the moments (a tensor starts on a block), their number and their group. */
 enum { DSB_ADAM_BLOCK = 256, DSB_ADAM_CHUNK = 4096 };
-typedef struct dsb_adam_tensor {
+typedef struct dsb_adam_chunk {
   void* w;
   const void* g;
-  int64_t numel;
-  int64_t block0;
+  int64_t block;
+  int32_t count;
   int32_t group;
   int32_t dtypes;
-} dsb_adam_tensor;
+  int32_t pad;
+} dsb_adam_chunk;
 /* Clip by group and AdamW over many tensors (the arithmetic of dsb_op_clip_adamw; the
- * gradients are left as they are). tensors, chunks ((tensor, chunk of it) int32 pairs,
- * chunks of DSB_ADAM_CHUNK elements, in order of the tensors' groups) and group_chunks
+ * gradients are left as they are). chunks, in order of their groups, and group_chunks
  * [ngroups + 1] (first chunk of each group) live on the device; most_chunks: those of the
  * largest group.
  * bits 32: m and v fp32 by block. bits 8: m holds e4m3 codes of m / m_scale and v those
@@ -496,9 +497,9 @@ typedef struct dsb_adam_tensor {
  * gets each group's gradient norm. lr_dev / step_dev: when set, the learning rate (fp32)
  * and the step count (int64) are read on the device, for a captured step. */
 int dsb_op_adam_workspace(int nchunks, int ngroups, int64_t* bytes);
-int dsb_op_adam_step(const dsb_adam_tensor* tensors, const int32_t* chunks, int nchunks,
-                     const int32_t* group_chunks, int ngroups, int most_chunks, void* m, void* v,
-                     float* m_scale, float* r_scale, int bits, double lr, double beta1, double beta2, double eps,
+int dsb_op_adam_step(const dsb_adam_chunk* chunks, int nchunks, const int32_t* group_chunks,
+                     int ngroups, int most_chunks, void* m, void* v, float* m_scale,
+                     float* r_scale, int bits, double lr, double beta1, double beta2, double eps,
                      double weight_decay, double max_norm, int64_t step, uint32_t seed,
                      const float* lr_dev, const int64_t* step_dev, float* norms, void* work,
                      int64_t work_bytes, void* stream);

@@ -79,7 +79,7 @@ def test_plan_refusals():
 
 def test_struct_layouts(tmp_path):
     L, _ = _lib()
-    structs = {"dsb_pack_plan": L.DsbPackPlan, "dsb_adam_tensor": L.DsbAdamTensor}
+    structs = {"dsb_pack_plan": L.DsbPackPlan, "dsb_adam_chunk": L.DsbAdamChunk}
     lines = ["#include <stdio.h>", "#include <stddef.h>", '#include "dsb.h"', "int main(void) {"]
     for name, cls in structs.items():
         lines.append(f'  printf("%zu", sizeof({name}));')
@@ -184,12 +184,12 @@ def test_policy_refusals(bad):
 @pytest.mark.parametrize("bad", [dict(bits=4), dict(beta1=1.0), dict(beta2=-0.1), dict(eps=-1.0),
                                  dict(eps=INF), dict(lr=NAN), dict(wd=INF), dict(step=0), dict(maxn=NAN),
                                  dict(maxn=1.0, norms=None), dict(m=None), dict(v=FAKE + 4),
-                                 dict(ms=None), dict(tensors=None), dict(ngroups=0), dict(nbytes=8),
+                                 dict(ms=None), dict(chunks=None), dict(ngroups=0), dict(nbytes=8),
                                  dict(work=FAKE + 8), dict(nchunks=-1), dict(most=2),
                                  dict(most=-1)])
 def test_adam_refusals(bad):
     L, lib = _lib()
-    a = dict(tensors=FAKE, chunks=FAKE, nchunks=1, gc=FAKE, ngroups=1, most=1, m=FAKE, v=FAKE, ms=FAKE, rs=FAKE,
+    a = dict(chunks=FAKE, nchunks=1, gc=FAKE, ngroups=1, most=1, m=FAKE, v=FAKE, ms=FAKE, rs=FAKE,
              bits=8, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, wd=0.0, maxn=-1.0, step=1, seed=0,
              lrd=None, stepd=None, norms=FAKE, work=FAKE, nbytes=BIG)
     a.update(bad)

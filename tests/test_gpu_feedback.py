@@ -264,7 +264,8 @@ def _scored(lens, mask):
 
 
 LENS = {"one": [1, 1], "empty": [0, 0], "pair": [5, 3], "ragged": [7, 0, 1, 130, 64, 65, 2, 0],
-        "tiles": [4097, 4096, 1, 300, 8193, 2], "many": [3, 1, 0, 2] * 300, "long": [20011, 9003]}
+        "tiles": [4097, 4096, 1, 300, 8193, 2], "many": [3, 1, 0, 2] * 300, "long": [20011, 9003],
+        "pairs": [3, 0, 700, 5, 1, 2, 2, 4, 1, 3] * 420, "crowd": [1, 2, 0, 3, 2, 1, 4, 1] * 2100}
 
 
 @pytest.mark.parametrize("masked", [False, True])
