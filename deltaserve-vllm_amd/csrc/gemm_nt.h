@@ -92,24 +92,22 @@ struct GemmProblem {
   // K1 load as zeros (the LM head's last vocabulary chunk runs K to a
   // multiple of 8 past the vocabulary)
   int kb_rows = 0;
-  // Tiles counted and dealt to the XCDs over the live rows (M_dev) instead of
-  // M: of a batch of which an unknown part is live, whole XCDs would
-  // otherwise hold no live tile. The grid is one-dimensional, live_grid
-  // blocks. With `part`, K is split on the device by the live tiles, over
-  // live_split(...) <= live_ks slices (those of a product of live_k, the same
-  // for every chunk of a longer K) whose partials lie live rows · N apart and
-  // take at most live_elems floats.
-  int live = 0;
-  int live_k = 0;
-  int live_ks = 1;
-  long live_elems = 0;
 };
+
+// Live epilogues (a type with kLive): tiles are counted and dealt to the XCDs over
+// the live rows (M_dev) instead of M, since of a batch of which an unknown part is
+// live whole XCDs would otherwise hold no live tile. The grid is one-dimensional.
+// K is split on the device by the live tiles: the epilogue's slices(M, N, BM, BN)
+// for M live rows, and at(slice, M, N) is what a slice's block runs.
+template <class E, class = void>
+struct IsLive : std::false_type {};
+template <class E>
+struct IsLive<E, std::void_t<decltype(E::kLive)>> : std::true_type {};
 
 // Slices of K that `tiles` output tiles of nk K tiles are split over so that
 // the device's 256 CUs are evenly loaded: the least number of K steps on the
 // busiest one, a block's epilogue (an fp32 tile stored while the others store
-// theirs) counting as `epi` steps. `most`: as many as their partials have room
-// for.
+// theirs) counting as `epi` steps.
 __host__ __device__ inline int live_slices(int tiles, int nk, int most, int epi) {
   int best = 1, least = 0x7fffffff;
   for (int ks = 1; ks <= most; ++ks) {
@@ -120,14 +118,6 @@ __host__ __device__ inline int live_slices(int tiles, int nk, int most, int epi)
     }
   }
   return best;
-}
-constexpr int kLiveEpi = 16;
-// The slices of a product of `rows` live rows.
-__host__ __device__ inline int live_split(int rows, int N, int K, int BM, int BN, int live_ks,
-                                          long live_elems) {
-  const int tiles = (rows + BM - 1) / BM * ((N + BN - 1) / BN);
-  const long fit = live_elems / ((long)max(rows, 1) * N);
-  return live_slices(tiles, (K + 63) / 64, (int)min((long)live_ks, max(fit, 1L)), kLiveEpi);
 }
 // Block `bid`'s place among `total` dealt to the 8 XCDs in contiguous runs
 // (blocks start round-robin over them).
@@ -413,11 +403,11 @@ __attribute__((amdgpu_waves_per_eu(WM* WN / 4, WM* WN / 4))) void gemm_nt_kernel
 
   int M = p.M;
   if (p.M_dev) M = min(M, *p.M_dev);
-  const int nbm = ((p.live ? M : p.M) + BM - 1) / BM, nbn = (p.N + BN - 1) / BN;
+  const int nbm = ((IsLive<Epi>::value ? M : p.M) + BM - 1) / BM, nbn = (p.N + BN - 1) / BN;
   int pm, pn, slice = blockIdx.y, slices = gridDim.y;
-  if (p.live) {
+  if constexpr (IsLive<Epi>::value) {
     if (M <= 0) return;
-    slices = p.part ? live_split(M, p.N, p.live_k, BM, BN, p.live_ks, p.live_elems) : 1;
+    slices = epi.slices(M, p.N, BM, BN);
     const int tiles = nbm * nbn;
     if ((int)blockIdx.x >= tiles * slices) return;
     const int at = xcd_run(blockIdx.x, tiles * slices);
@@ -799,8 +789,8 @@ __attribute__((amdgpu_waves_per_eu(WM* WN / 4, WM* WN / 4))) void gemm_nt_kernel
 
   if constexpr (SplitPart<Epi>::enabled) {
     if (p.part) {
-      const typename SplitPart<Epi>::type ep{p.part + (long)slice * (p.live ? M : p.M) * p.N,
-                                             (long)p.N, p.N, p.part_acc, p.part_scale};
+      const typename SplitPart<Epi>::type ep{p.part + (long)blockIdx.y * p.M * p.N, (long)p.N,
+                                             p.N, p.part_acc, p.part_scale};
       ep.template run<FM, FN, WM, WN>(acc, m0 + wm * TM, n0 + wn * TN, M, lane, wave,
                                       (void*)smem);
       return;
@@ -816,10 +806,12 @@ __attribute__((amdgpu_waves_per_eu(WM* WN / 4, WM* WN / 4))) void gemm_nt_kernel
       return;
     }
   }
-  {
+  if constexpr (IsLive<Epi>::value)
+    epi.at(slice, M, p.N).template run<FM, FN, WM, WN>(acc, m0 + wm * TM, n0 + wn * TN, M, lane,
+                                                       wave, (void*)smem);
+  else
     epi.template run<FM, FN, WM, WN>(acc, m0 + wm * TM, n0 + wn * TN, M, lane, wave,
                                      (void*)smem);
-  }
 }
 
 // ---------------------------------------------------------------- epilogues
@@ -1090,6 +1082,27 @@ struct EpiF32 {
   }
 };
 
+// fp32 partials of a live launch's K slices, live rows · N apart, `elems` floats in
+// all, added to what they hold with `accumulate`; K is split as for a product of k (the
+// same for every chunk of a longer K) into at most `ks`.
+struct EpiLivePart {
+  static constexpr bool kLive = true;
+  float* part;
+  int accumulate;
+  int k, ks;
+  long elems;
+  __host__ __device__ int most_slices(int M, int N) const {
+    const long fit = elems / ((long)M * N);
+    return fit < 1 ? 1 : fit < ks ? (int)fit : ks;
+  }
+  __host__ __device__ int slices(int M, int N, int BM, int BN) const {
+    return live_slices((M + BM - 1) / BM * ((N + BN - 1) / BN), (k + 63) / 64, most_slices(M, N), 16);
+  }
+  DSB_DEV EpiF32 at(int slice, int M, int N) const {
+    return EpiF32{part + (long)slice * M * N, (long)N, N, accumulate};
+  }
+};
+
 // Tile configurations, all of 4 waves (2×2). LDS slots (A, B) and the blocks
 // a CU holds by LDS: 256×256 (2, 3) 160 KB, 1; 256×128 (3, 3) 144 KB, 1;
 // 128×128 (2, 3) 80 KB, 2; 128×64 (3, 3) 72 KB, 2; 64×64 (5, 5) 80 KB, 2.
@@ -1200,28 +1213,23 @@ __global__ __launch_bounds__(256) void gemm_split_reduce_kernel(GemmProblem p, i
   epi.apply8(m, n, v);
 }
 
-// Blocks of a live launch: the most tiles · slices over 1 .. M live rows.
-inline long live_grid(const GemmProblem& p, int BM, int BN) {
-  const int nbn = (p.N + BN - 1) / BN;
+// Blocks of a live launch: the most tiles · slices over 1 .. M live rows (the slices
+// fall with the rows while their tiles stay the same).
+template <class Epi>
+unsigned live_grid(const GemmProblem& p, const Epi& e, int BM, int BN) {
   long most = 0;
-  for (int rows = 1; rows <= p.M; rows += BM) {
-    // the slices fall with the rows while their tiles stay the same
-    const long tiles = (long)((rows + BM - 1) / BM) * nbn;
-    int ks = 1;
-    if (p.part) {
-      const long fit = p.live_elems / ((long)rows * p.N);
-      ks = (int)std::min((long)p.live_ks, std::max(fit, 1L));
-    }
-    most = std::max(most, tiles * ks);
-  }
-  return most;
+  for (int rows = 1; rows <= p.M; rows += BM)
+    most = std::max(most, (long)((rows + BM - 1) / BM) * ((p.N + BN - 1) / BN) *
+                              e.most_slices(rows, p.N));
+  return (unsigned)most;
 }
 
 template <int BM, int BN, int WM, int WN, int NA = 2, int NB = 3, class Epi>
 hipError_t launch_gemm_cfg(const GemmProblem& p, const Epi& e, hipStream_t s, int ks = 1) {
   const int nbm = (p.M + BM - 1) / BM, nbn = (p.N + BN - 1) / BN;
   if (nbm == 0 || nbn == 0) return hipSuccess;
-  const dim3 grid(p.live ? (unsigned)live_grid(p, BM, BN) : (unsigned)(nbm * nbn), ks);
+  dim3 grid(nbm * nbn, ks);
+  if constexpr (IsLive<Epi>::value) grid = dim3(live_grid(p, e, BM, BN));
   if (p.b_kn)
     hipLaunchKernelGGL((gemm_nt_kernel<BM, BN, WM, WN, Epi, true, NA, NB>), grid, dim3(WM * WN * 64), 0,
                        s, p, e);

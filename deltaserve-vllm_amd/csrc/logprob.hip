@@ -46,6 +46,10 @@ struct LPStat {
 // a fragment are neighbours, so a store is one 128-byte line) and the label's logit
 // into tgt[m]. A lane holds 4·FN columns of a row.
 struct EpiLogProb {
+  static constexpr bool kLive = true;
+  __host__ __device__ int most_slices(int, int) const { return 1; }
+  DSB_DEV int slices(int, int, int, int) const { return 1; }
+  DSB_DEV const EpiLogProb& at(int, int, int) const { return *this; }
   LPStat* stats;
   int cap, V;
   const float* ref;
@@ -118,6 +122,10 @@ struct EpiLogProb {
 // matrix cores). Only runs that hold a label (one in V / TN of a row's) test their columns
 // for it; its exponential, which may be infinite, is left out by a select.
 struct EpiProb {
+  static constexpr bool kLive = true;
+  __host__ __device__ int most_slices(int, int) const { return 1; }
+  DSB_DEV int slices(int, int, int, int) const { return 1; }
+  DSB_DEV const EpiProb& at(int, int, int) const { return *this; }
   float* rsum;
   int runs;
   bf16* P;
@@ -232,6 +240,11 @@ struct LPWork {
   float* part;   // the dH product's accumulators
   LPPlan plan;
 };
+
+// The dH product's epilogue; its K slices at any live row count.
+__host__ __device__ inline EpiLivePart lp_part(const LPWork& w, int accumulate) {
+  return EpiLivePart{w.part, accumulate, w.plan.vchunk, kMaxSlices, w.plan.part_elems};
+}
 
 LPWork lp_layout(int n, int D, int V, bool backward, void* base, size_t* bytes) {
   Carve c{(char*)base};
@@ -418,7 +431,7 @@ __global__ __launch_bounds__(256) void lp_dh_kernel(const bf16* __restrict__ W, 
     f = -expm1f(logp[r]) * g[r] / R;
     w += (long)a.labels[m] * D;
     src += (long)m * D;
-    ks = live_split(M, D, a.plan.vchunk, 256, 256, kMaxSlices, a.plan.part_elems);
+    ks = lp_part(a, 0).slices(M, D, 256, 256);
   }
   const long plane = (long)M * D;
   for (int k = tid; k < D / 8; k += 256) {
@@ -473,7 +486,6 @@ hipError_t token_logprobs(const bf16* normed, long ldh, const bf16* W, const int
                      (const float*)nullptr, w);
   LPCK(hipGetLastError());
   GemmProblem p{w.X, (long)D, W, (long)D, nullptr, 0, nullptr, 0, n, V, D, 0, w.count};
-  p.live = 1;
   LPCK((launch_gemm_cfg<256, 256, 2, 2>(p, EpiLogProb{w.stats, n, V, w.ref, w.labels, w.tgt}, s)));
   hipLaunchKernelGGL(lp_finish_kernel, dim3((n + 15) / 16), dim3(1024), 0, s, w, n, logp, other);
   return hipGetLastError();
@@ -494,20 +506,13 @@ hipError_t token_logprobs_bwd(const bf16* normed, long ldh, const bf16* W, const
     const int Vc = std::min(vchunk, V - c0), Nc8 = (Vc + 7) / 8 * 8;
     const bf16* Wc = W + (long)c0 * D;
     GemmProblem p{w.X, (long)D, Wc, (long)D, nullptr, 0, nullptr, 0, n, Vc, D, 0, w.count};
-    p.live = 1;
     const EpiProb epi{w.rsum, w.runs, w.P, (long)vchunk, c0, Vc, Nc8, w.ref, w.labels};
     LPCK((launch_gemm_cfg<256, 256, 2, 2>(p, epi, s)));
     // the head read in place as the [K, N] operand; each slice adds up its own partial
     GemmProblem h{w.P, (long)vchunk, Wc, (long)D, nullptr, 0, nullptr, 0, n, D, Nc8, 0, w.count};
     h.b_kn = 1;
     h.kb_rows = Vc;
-    h.part = w.part;
-    h.part_acc = c0 > 0 ? 1 : 0;
-    h.live = 1;
-    h.live_k = vchunk;
-    h.live_ks = kMaxSlices;
-    h.live_elems = w.plan.part_elems;
-    LPCK((launch_gemm_cfg<256, 256, 2, 2>(h, EpiF32{w.part, (long)D, D, 0}, s)));
+    LPCK((launch_gemm_cfg<256, 256, 2, 2>(h, lp_part(w, c0 > 0), s)));
   }
   hipLaunchKernelGGL(lp_dh_kernel, dim3(n), dim3(256), 0, s, W, D, w, logp, dlogp, dH, lddh, out_f32);
   return hipGetLastError();
