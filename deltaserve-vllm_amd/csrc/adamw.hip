@@ -259,6 +259,8 @@ __global__ __launch_bounds__(256) void adam_kernel(const dsb_adam_chunk* __restr
   const bool wvec = aligned4(t.w, wbf), gvec = aligned4(t.g, gbf);
   const int e0 = qb * kBlock + 4 * l16;
   const long b = t.block + qb, s0 = b * kBlock + 4 * l16;
+  const double mine =
+      clip.how == CLIP_SUM && t.c0 + (int)threadIdx.x < t.c1 ? clip.partial[t.c0 + threadIdx.x] : 0.0;
   f32x4 g[4], w[4];
   float m[4][4], r[4][4];
   unsigned mc[4], rc[4];
@@ -290,11 +292,9 @@ __global__ __launch_bounds__(256) void adam_kernel(const dsb_adam_chunk* __restr
   if (clip.how == CLIP_GIVEN) {
     cf = clip.coef[t.group];
   } else if (clip.how == CLIP_SUM) {
-    const int c0 = clip.group_chunks[t.group], c1 = clip.group_chunks[t.group + 1];
-    const double norm =
-        sqrt(block_sum64<256>(c0 + (int)threadIdx.x < c1 ? clip.partial[c0 + threadIdx.x] : 0.0, red));
+    const double norm = sqrt(block_sum64<256>(mine, red));
     cf = clip_factor(norm, clip.max_norm);
-    if (chunk == c0 && threadIdx.x == 0) clip.norms[t.group] = (float)norm;
+    if (chunk == t.c0 && threadIdx.x == 0) clip.norms[t.group] = (float)norm;
     if (chunk == 0)  // groups without elements
       for (int g = threadIdx.x; g < clip.ngroups; g += 256)
         if (clip.group_chunks[g] == clip.group_chunks[g + 1]) clip.norms[g] = 0.f;

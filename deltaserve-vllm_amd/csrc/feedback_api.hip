@@ -30,8 +30,8 @@ int64_t plan_part(int64_t elems) { return (elems + 3) / 4 * 4; }
 
 const char* check_logprob(const void* normed, int64_t ldh, const void* lm_w, const int64_t* labels,
                           int n, int D, int V) {
-  if (n < 0 || V < 2 || D < 8 || D % 8 || D > 65536 || V > (1 << 24))
-    return "D a multiple of 8 up to 65536 and V from 2 to 2^24 are taken";
+  if (n < 0 || n > (1 << 30) || V < 2 || D < 8 || D % 8 || D > 65536 || V > (1 << 24))
+    return "n up to 2^30, D a multiple of 8 up to 65536 and V from 2 to 2^24 are taken";
   if (ldh < D || ldh % 8) return "ldh must be a multiple of 8 and >= D";
   if (n > 0 && (!normed || !lm_w || !labels)) return "null argument";
   if (misaligned(normed, 16) || misaligned(lm_w, 16)) return "normed and lm_w must be 16-byte aligned";
@@ -88,7 +88,7 @@ int dsb_op_token_logprobs_bwd(const void* normed, int64_t ldh, const void* lm_w,
 int dsb_plan_sizes(const int32_t* seq_lens, int nseq, dsb_pack_plan* plan, int64_t* elems) {
   const char* what = "dsb_plan_sizes";
   if (!plan || !elems || nseq < 0 || (nseq > 0 && !seq_lens)) return bad(what, "bad argument");
-  int64_t n = 0, tiles = 0, npred = 0, nonempty = 0;
+  int64_t n = 0, tiles = 0, npred = 0, nonempty = 0, longest = 0;
   for (int i = 0; i < nseq; ++i) {
     const int64_t len = seq_lens[i];
     if (len < 0) return bad(what, "a sequence's length is negative");
@@ -96,6 +96,7 @@ int dsb_plan_sizes(const int32_t* seq_lens, int nseq, dsb_pack_plan* plan, int64
     tiles += (len + DSB_TILE_ROWS - 1) / DSB_TILE_ROWS;
     npred += len > 1 ? len - 1 : 0;
     nonempty += len > 1;
+    longest = len > longest ? len : longest;
   }
   if (n > 0x7fffffffLL - DSB_CHUNK_ROWS) return bad(what, "the sequences hold too many rows");
   plan->ntiles = (int)tiles;
@@ -103,6 +104,7 @@ int dsb_plan_sizes(const int32_t* seq_lens, int nseq, dsb_pack_plan* plan, int64
   plan->n = (int)n;
   plan->npred = (int)npred;
   plan->nonempty = (int)nonempty;
+  plan->longest = (int)longest;
   *elems = plan_part(4 * tiles) + 2 * plan_part(nseq + 1) +
            plan_part((n + DSB_CHUNK_ROWS - 1) / DSB_CHUNK_ROWS + 1);
   return 0;

@@ -38,6 +38,15 @@ constexpr int kRun = 128;  // columns of a wave's tile
 // (349 µs; 16 slices 414, 8 580).
 constexpr int kMaxSlices = 32;
 
+// An accumulator's value, read from its AGPR here: left to itself the compiler reads all 256
+// at the start of the epilogue and spills what else is live. (volatile: stays behind the
+// wait for the last products.)
+DSB_DEV float acc_read(const float& a) {
+  float v;
+  asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(v) : "a"(a));
+  return v;
+}
+
 struct LPStat {
   float ref, sum;  // Σ exp(logit − ref) over a run, the label left out
 };
@@ -51,10 +60,11 @@ struct EpiLogProb {
   DSB_DEV int slices(int, int, int, int) const { return 1; }
   DSB_DEV const EpiLogProb& at(int, int, int) const { return *this; }
   LPStat* stats;
-  int cap, V;
+  int cap, V;  // V: the product's columns, from c0 of the vocabulary on
   const float* ref;
   const int* labels;
   float* tgt;
+  int c0;
   template <int FM, int FN, int WM, int WN>
   DSB_DEV void run(const f32x4 (&acc)[FM][FN], int mw, int nw, int M, int lane, int,
                    void*) const {
@@ -63,27 +73,29 @@ struct EpiLogProb {
     const int l16 = lane & 15, lq = lane >> 4;
     const bool whole = nw + TN <= V;
     LPStat* out = stats + (long)(nw / TN) * cap;
-    float ref0[FM];
-    int tcol[FM];
-#pragma unroll
-    for (int fm = 0; fm < FM; ++fm) {
-      const int m = min(mw + fm * 16 + l16, M - 1);
-      ref0[fm] = ref[m];
-      tcol[fm] = labels[m] - nw;
-    }
+    // a fragment's references and labels are loaded during the one before (all of them ahead
+    // spill)
+    float ref1 = ref[min(mw + l16, M - 1)];
+    int lab1 = labels[min(mw + l16, M - 1)];
 #pragma unroll
     for (int fm = 0; fm < FM; ++fm) {
       if (mw + fm * 16 >= M) break;
-      const float tl = (float)(tcol[fm] - 4 * lq);
+      const float ref0 = ref1;
+      const int tc = lab1 - (c0 + nw);
+      ref1 = ref[min(mw + fm * 16 + 16 + l16, M - 1)];
+      lab1 = labels[min(mw + fm * 16 + 16 + l16, M - 1)];
+      const float tl = (float)(tc - 4 * lq);
       auto take = [&](float r, auto skips) {
         float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int fn = 0; fn < FN; ++fn)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            float e = __expf(acc[fm][fn][i] - r);
+            float e = __expf(acc_read(acc[fm][fn][i]) - r);
             if (!whole) e = nw + fn * 16 + 4 * lq + i < V ? e : 0.f;
-            if (decltype(skips)::value) e = (float)(fn * 16 + i) == tl ? 0.f : e;
+            // the label's own column (whose e is at most about 1, r being its logit or more) by
+            // a factor of 0: as tests the masks of 128 columns spill
+            if (decltype(skips)::value) e *= fminf(fabsf((float)(fn * 16 + i) - tl), 1.f);
             part[i] += e;
           }
         float v = (part[0] + part[1]) + (part[2] + part[3]);
@@ -91,26 +103,26 @@ struct EpiLogProb {
         return LPStat{r, v + __shfl_xor(v, 32, 64)};
       };
       const int m = mw + fm * 16 + l16;
-      LPStat st = take(ref0[fm], std::false_type{});
-      if (__any(!(st.sum <= kRunLimit) || (unsigned)tcol[fm] < (unsigned)TN)) {
+      LPStat st = take(ref0, std::false_type{});
+      if (__any(!(st.sum <= kRunLimit) || (unsigned)tc < (unsigned)TN)) {
         // rare: a row with its label in the run, or past the limit
         float v = -INFINITY, xt = 0.f;
 #pragma unroll
         for (int fn = 0; fn < FN; ++fn)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float x = acc[fm][fn][i];
-            const bool mine = (float)(fn * 16 + i) == tl;
-            if (mine) xt = x;
-            v = !mine && (whole || nw + fn * 16 + 4 * lq + i < V) ? fmaxf(v, x) : v;
+            const float x = acc_read(acc[fm][fn][i]);
+            v = whole || nw + fn * 16 + 4 * lq + i < V ? fmaxf(v, x) : v;
+            xt = (float)(fn * 16 + i) == tl ? x : xt;
           }
-        const int tc = tcol[fm];
         if ((unsigned)tc < (unsigned)TN && ((tc >> 2) & 3) == lq && m < M) tgt[m] = xt;
         v = fmaxf(v, __shfl_xor(v, 16, 64));
         v = fmaxf(v, __shfl_xor(v, 32, 64));
         st = take(st.sum <= kRunLimit ? st.ref : fmaxf(st.ref, v), std::true_type{});
       }
       if (lq == 0 && m < M) out[m] = st;
+      // one fragment's values at a time: with several in flight the registers spill
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
 };
@@ -126,8 +138,8 @@ struct EpiProb {
   __host__ __device__ int most_slices(int, int) const { return 1; }
   DSB_DEV int slices(int, int, int, int) const { return 1; }
   DSB_DEV const EpiProb& at(int, int, int) const { return *this; }
-  float* rsum;
-  int runs;
+  float* rsum;  // the chunk's first run of row 0
+  int runs;     // row pitch
   bf16* P;
   long ldp;
   int c0, Vc, Nc8;
@@ -141,12 +153,15 @@ struct EpiProb {
     const int l16 = lane & 15, lq = lane >> 4;
     const bool whole = nw + TN <= Vc;
     bf16* buf = reinterpret_cast<bf16*>(smem) + wave * 32 * PITCH;
-    float ref0[FM];
+    // e^(x − ref) = 2^(x·log2(e) − ref·log2(e)) with one multiply-add: what the second
+    // product's rounding changes is a factor of the whole row, which the division by R takes out
+    constexpr float kLog2e = 1.44269504088896340736f;
+    float ref2[FM];
     int tcol[FM];
 #pragma unroll
     for (int fm = 0; fm < FM; ++fm) {
       const int m = min(mw + fm * 16 + l16, M - 1);
-      ref0[fm] = ref[m];
+      ref2[fm] = -ref[m] * kLog2e;
       tcol[fm] = labels[m] - (c0 + nw);
     }
 #pragma unroll
@@ -162,7 +177,7 @@ struct EpiProb {
           for (int fn = 0; fn < FN; ++fn)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              float e = __expf(acc[fm][fn][i] - ref0[fm]);
+              float e = __builtin_amdgcn_exp2f(fmaf(acc_read(acc[fm][fn][i]), kLog2e, ref2[fm]));
               if (!whole) e = nw + fn * 16 + 4 * lq + i < Vc ? e : 0.f;
               if (decltype(skips)::value) e = (float)(fn * 16 + i) == tl ? 0.f : e;
               pk[fn][i] = (bf16)e;
@@ -182,7 +197,7 @@ struct EpiProb {
         for (int fn = 0; fn < FN; ++fn)
           *reinterpret_cast<bf16x4*>(buf + (16 * h + l16) * PITCH + fn * 16 + 4 * lq) = pk[fn];
         const int m = mw + fm * 16 + l16;
-        if (lq == 0 && m < M) rsum[(long)m * runs + (c0 + nw) / TN] = r[0];
+        if (lq == 0 && m < M) rsum[(long)m * runs + nw / TN] = r[0];
       }
 #pragma unroll
       for (int it = 0; it < 32 * CG / 64; ++it) {
@@ -224,6 +239,17 @@ LPPlan lp_plan(int n, int D, int V) {
   return q;
 }
 
+// Columns, the last ones of the vocabulary, that the forward's product takes in 256 × 128
+// tiles: over one block of rows the head is streamed by whole rounds of the device's CUs, and
+// where the last round of 256 × 256 tiles is at most half full, half-wide ones fill it better
+// (149 rows × 5120 × 151936, 82 tiles in the third round: 386 → 355 µs).
+int lp_narrow(int n, int V) {
+  const int tiles = (V + 255) / 256, last = tiles % kGemmCus;
+  return n <= 256 && tiles > kGemmCus && last > 0 && last <= kGemmCus / 2
+             ? V - (tiles - last) * 256
+             : 0;
+}
+
 struct LPWork {
   int* count;   // scored rows
   int* rows;    // [n] their rows in order
@@ -232,7 +258,8 @@ struct LPWork {
   float* ref;
   float* tgt;
   bf16* X;      // [n, D] the scored rows
-  int runs;       // ceil(V / kRun)
+  int runs;       // of all columns
+  int narrow;     // columns that the narrower tiles take (lp_narrow)
   LPStat* stats;  // forward: [runs, n]
   // backward
   float* rsum;   // [n, runs]
@@ -250,7 +277,8 @@ LPWork lp_layout(int n, int D, int V, bool backward, void* base, size_t* bytes) 
   Carve c{(char*)base};
   LPWork w{};
   const size_t N = (size_t)n;
-  w.runs = (V + kRun - 1) / kRun;
+  w.narrow = backward ? 0 : lp_narrow(n, V);
+  w.runs = (V - w.narrow + kRun - 1) / kRun + (w.narrow + kRun / 2 - 1) / (kRun / 2);
   w.count = c.take<int>(1);
   w.rows = c.take<int>(N);
   w.place = c.take<int>(N);
@@ -485,8 +513,15 @@ hipError_t token_logprobs(const bf16* normed, long ldh, const bf16* W, const int
   hipLaunchKernelGGL(lp_gather_kernel, dim3(n), dim3(256), 0, s, normed, ldh, W, labels, D,
                      (const float*)nullptr, w);
   LPCK(hipGetLastError());
-  GemmProblem p{w.X, (long)D, W, (long)D, nullptr, 0, nullptr, 0, n, V, D, 0, w.count};
-  LPCK((launch_gemm_cfg<256, 256, 2, 2>(p, EpiLogProb{w.stats, n, V, w.ref, w.labels, w.tgt}, s)));
+  const int V1 = V - w.narrow;
+  GemmProblem p{w.X, (long)D, W, (long)D, nullptr, 0, nullptr, 0, n, V1, D, 0, w.count};
+  LPCK((launch_gemm_cfg<256, 256, 2, 2>(p, EpiLogProb{w.stats, n, V1, w.ref, w.labels, w.tgt, 0}, s)));
+  if (w.narrow) {
+    p.B = W + (long)V1 * D;
+    p.N = w.narrow;
+    const EpiLogProb epi{w.stats + (long)(V1 / kRun) * n, n, w.narrow, w.ref, w.labels, w.tgt, V1};
+    LPCK((launch_gemm_cfg<256, 128, 2, 2, 3, 3>(p, epi, s)));
+  }
   hipLaunchKernelGGL(lp_finish_kernel, dim3((n + 15) / 16), dim3(1024), 0, s, w, n, logp, other);
   return hipGetLastError();
 }
@@ -506,7 +541,7 @@ hipError_t token_logprobs_bwd(const bf16* normed, long ldh, const bf16* W, const
     const int Vc = std::min(vchunk, V - c0), Nc8 = (Vc + 7) / 8 * 8;
     const bf16* Wc = W + (long)c0 * D;
     GemmProblem p{w.X, (long)D, Wc, (long)D, nullptr, 0, nullptr, 0, n, Vc, D, 0, w.count};
-    const EpiProb epi{w.rsum, w.runs, w.P, (long)vchunk, c0, Vc, Nc8, w.ref, w.labels};
+    const EpiProb epi{w.rsum + c0 / kRun, w.runs, w.P, (long)vchunk, c0, Vc, Nc8, w.ref, w.labels};
     LPCK((launch_gemm_cfg<256, 256, 2, 2>(p, epi, s)));
     // the head read in place as the [K, N] operand; each slice adds up its own partial
     GemmProblem h{w.P, (long)vchunk, Wc, (long)D, nullptr, 0, nullptr, 0, n, D, Nc8, 0, w.count};

@@ -174,9 +174,10 @@ DSB_DEV Pair pair_eval(const PrefHyper& h, int npairs, const double (&sum)[2], c
   if (h.kind == DSB_PREF_SIGMOID) {
     const double e = exp(-fabs(z)), l = log1p(e), q = 1.0 / (1.0 + e);
     const double up = z >= 0 ? q : e * q, down = z >= 0 ? e * q : q;  // σ(z), σ(−z)
-    o.loss = (1.0 - h.smooth) * (fmax(-z, 0.0) + l) + h.smooth * (fmax(z, 0.0) + l);
+    // a term of weight 0 stays out: it may be infinite
+    o.loss = (h.smooth < 1.0 ? (1.0 - h.smooth) * (fmax(-z, 0.0) + l) : 0.0) +
+             (h.smooth > 0.0 ? h.smooth * (fmax(z, 0.0) + l) : 0.0);
     g = h.beta * (h.smooth * up - (1.0 - h.smooth) * down);
-    if (z != z) o.loss = z;
   } else if (h.kind == DSB_PREF_HINGE) {
     o.loss = z >= 1.0 ? 0.0 : 1.0 - z;
     g = z >= 1.0 ? 0.0 : z < 1.0 ? -h.beta : z;
@@ -812,7 +813,7 @@ hipError_t preference_loss(const float* logp, const float* ref, const uint8_t* m
   }
   int64_t bytes;
   const LossWork w = loss_layout(p, work, &bytes);
-  if (p.ntiles <= p.nseq) {
+  if (p.longest <= DSB_TILE_ROWS) {
     const int pairs = p.nseq / 2;
     auto go = [&](auto nt, auto nb) {
       constexpr int NT = decltype(nt)::value, NB = decltype(nb)::value;

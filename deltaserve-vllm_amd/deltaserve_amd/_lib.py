@@ -81,12 +81,13 @@ class DsbCycleInfo(Structure):
 
 class DsbPackPlan(Structure):
     _fields_ = [(k, c_void_p) for k in ("tiles", "seq_tile", "starts", "chunk_seq")] + [
-        (k, c_int32) for k in ("ntiles", "nseq", "n", "npred", "nonempty")]
+        (k, c_int32) for k in ("ntiles", "nseq", "n", "npred", "nonempty", "longest")]
 
 
 class DsbAdamChunk(Structure):
     _fields_ = [("w", c_void_p), ("g", c_void_p), ("block", c_int64), ("count", c_int32),
-                ("group", c_int32), ("dtypes", c_int32), ("pad", c_int32)]
+                ("group", c_int32), ("c0", c_int32), ("c1", c_int32), ("dtypes", c_int32),
+                ("pad", c_int32)]
 
 
 # name -> (restype, argtypes)

@@ -422,6 +422,8 @@ def _head_args(what, normed, lm_w, labels):
     if normed.dtype != BF16 or lm_w.dtype != BF16 or normed.dim() != 2 or lm_w.dim() != 2:
         raise ValueError(f"{what}: normed and lm_w must be bf16 matrices")
     n, D = normed.shape
+    if max(n, D, lm_w.shape[0]) >= 1 << 31:
+        raise ValueError(f"{what}: a dimension is too large")
     if lm_w.shape[1] != D or not lm_w.is_contiguous():
         raise ValueError(f"{what}: lm_w must be a contiguous [V, {D}]")
     if n and D > 1 and normed.stride(1) != 1:
@@ -544,7 +546,7 @@ class AdamW:
     32 bits (:func:`clip_adamw_` keeps fp32 moments of the caller's).
 
     ws, gs: weights and their gradient buffers, fp32 or bf16 each, contiguous, on one device, no
-    two weights overlapping; they are bound: each step reads the gradients from, and writes the
+    weight overlapping another or a gradient; they are bound: each step reads the gradients from, and writes the
     weights to, the memory that these tensors had here (which is kept alive). groups:
     non-decreasing group numbers from 0 (default: one group).
 
@@ -561,18 +563,23 @@ class AdamW:
             raise ValueError(f"{what}: bits is 8 or 32")
         if not ws or len(gs) != len(ws) or len(groups) != len(ws):
             raise ValueError(f"{what}: takes as many gradients and groups as weights, at least one")
-        if groups[0] < 0 or any(b < a for a, b in zip(groups, groups[1:])):
-            raise ValueError(f"{what}: groups must be non-decreasing, from 0")
+        if groups[0] < 0 or groups[-1] >= 1 << 20 or any(b < a for a, b in zip(groups, groups[1:])):
+            raise ValueError(f"{what}: groups must be non-decreasing numbers below 2^20")
         code = {BF16: L.DT_BF16, torch.float32: L.DT_F32}
         for w, g in zip(ws, gs):
             if w.dtype not in code or g.dtype not in code:
                 raise ValueError(f"{what}: weights and gradients are fp32 or bf16")
             if w.shape != g.shape or not w.is_contiguous() or not g.is_contiguous():
                 raise ValueError(f"{what}: a weight and its gradient are contiguous, of one shape")
-        span = sorted((w.data_ptr(), w.data_ptr() + w.numel() * w.element_size()) for w in ws
-                      if w.numel())
-        if any(b[0] < a[1] for a, b in zip(span, span[1:])):
-            raise ValueError(f"{what}: two weights overlap in memory")
+        # by address: each weight's end before the next weight and the next gradient begin, and each
+        # gradient's before the next weight (gradients may be shared)
+        span = sorted((x.data_ptr(), x.data_ptr() + x.numel() * x.element_size(), k)
+                      for k, xs in enumerate((ws, gs)) for x in xs if x.numel())
+        end = [0, 0]
+        for a, b, k in span:
+            if a < end[0] or (k == 0 and a < end[1]):
+                raise ValueError(f"{what}: a weight overlaps another weight or a gradient in memory")
+            end[k] = max(end[k], b)
         with _on(what, *ws, *gs):
             self.device, self.bits, self.ngroups = ws[0].device, bits, groups[-1] + 1
             numel = np.array([w.numel() for w in ws], dtype=np.int64)
@@ -592,11 +599,12 @@ class AdamW:
                 table[name] = base[t] + (at * size[t]).astype(np.uint64)
             table["block"] = block0[t] + at // L.ADAM_BLOCK
             table["count"] = np.minimum(numel[t] - at, L.ADAM_CHUNK)
-            table["group"] = np.array(groups)[t]
             table["dtypes"] = np.array([code[w.dtype] + 256 * code[g.dtype] for w, g in zip(ws, gs)])[t]
             per = np.bincount(np.array(groups), weights=chunks, minlength=self.ngroups)
             most = int(per.max())
             ends = np.concatenate([[0], np.cumsum(per)]).astype(np.int32)
+            table["group"] = group = np.array(groups)[t]
+            table["c0"], table["c1"] = ends[group], ends[group + 1]
 
             def dev(a):
                 raw = np.frombuffer(a.tobytes(), dtype=np.uint8).copy()

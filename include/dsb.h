@@ -415,14 +415,15 @@ int dsb_op_token_logprobs_bwd(const void* normed, int64_t ldh, const void* lm_w,
  * DSB_TILE_ROWS rows of a sequence; seq_tile [nseq + 1]: a sequence's first tile;
  * starts [nseq + 1]: its first row; chunk_seq [ceil(n / DSB_CHUNK_ROWS) + 1]: the
  * sequence that holds row DSB_CHUNK_ROWS·c (the last entry: nseq − 1). npred:
- * rows that are not the last of their sequence; nonempty: sequences with one. */
+ * rows that are not the last of their sequence; nonempty: sequences with one; longest: the
+ * most rows of a sequence. */
 enum { DSB_TILE_ROWS = 4096, DSB_CHUNK_ROWS = 4096 };
 typedef struct dsb_pack_plan {
   const int32_t* tiles;
   const int32_t* seq_tile;
   const int32_t* starts;
   const int32_t* chunk_seq;
-  int32_t ntiles, nseq, n, npred, nonempty;
+  int32_t ntiles, nseq, n, npred, nonempty, longest;
 } dsb_pack_plan;
 /* Host only. seq_lens int32 [nseq], each >= 0, their sum below 2^31: the counts of
  * the plan (its pointers untouched) and the int32 elements of all four tables. */
@@ -474,7 +475,8 @@ int dsb_op_policy_loss(const float* logp, const float* old_logp, const float* re
 /* Up to DSB_ADAM_CHUNK elements of one tensor of an AdamW step, from a multiple of that: their
  * address in the weights and in the gradients (element types by dtypes: DSB_DT_BF16 or
  * DSB_DT_F32, w + 256·g; aligned to their type), the first of their blocks of DSB_ADAM_BLOCK
- * elements in the moments (a tensor starts on a block), their number and their group. */
+ * elements in the moments (a tensor starts on a block), their number, their group and that
+ * group's chunks, c0 to c1 - 1. */
 enum { DSB_ADAM_BLOCK = 256, DSB_ADAM_CHUNK = 4096 };
 typedef struct dsb_adam_chunk {
   void* w;
@@ -482,6 +484,7 @@ typedef struct dsb_adam_chunk {
   int64_t block;
   int32_t count;
   int32_t group;
+  int32_t c0, c1;
   int32_t dtypes;
   int32_t pad;
 } dsb_adam_chunk;

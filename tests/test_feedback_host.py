@@ -44,6 +44,7 @@ def test_plan_tables(lens):
     n = sum(lens)
     assert (c.n, c.nseq, c.npred, c.nonempty) == (n, len(lens), sum(max(x - 1, 0) for x in lens),
                                                   sum(x > 1 for x in lens))
+    assert c.longest == max(lens, default=0)
     want = np.concatenate([[0], np.cumsum(lens)]).astype(int)
     assert starts.tolist() == want.tolist()
     tiles = tiles.reshape(-1, 4)
@@ -110,7 +111,7 @@ def _lp(lib, **kw):
 @pytest.mark.parametrize("bad", [dict(ld=63), dict(ld=60), dict(D=60), dict(D=0), dict(V=1), dict(n=-1),
                                  dict(h=FAKE + 2), dict(w=FAKE + 8), dict(lab=None), dict(logp=None),
                                  dict(work=None), dict(nbytes=100), dict(work=FAKE + 16),
-                                 dict(V=(1 << 24) + 1)])
+                                 dict(V=(1 << 24) + 1), dict(n=(1 << 30) + 1)])
 def test_logprob_refusals(bad):
     L, lib = _lib()
     assert _lp(lib, **bad) != 0 and L.last_error()
@@ -211,7 +212,7 @@ def test_front_end_refusals():
     for bad in (dict(ws=[], gs=[]), dict(ws=[f], gs=[f, f]), dict(ws=[f], gs=[f], bits=16),
                 dict(ws=[f], gs=[f[:2]]), dict(ws=[f.half()], gs=[f]), dict(ws=[f], gs=[f], groups=[-1]),
                 dict(ws=[f, f.clone()], gs=[f, f], groups=[1, 0]), dict(ws=[f, f[1:]], gs=[f, f[1:]]),
-                dict(ws=[b.t()], gs=[b.t()]), dict(ws=[f], gs=[f])):
+                dict(ws=[f], gs=[f], groups=[1 << 20]), dict(ws=[b.t()], gs=[b.t()]), dict(ws=[f], gs=[f])):
         with pytest.raises(ValueError):
             ops.AdamW(**bad)
 

@@ -78,7 +78,7 @@ def _head_tol(H, W):
 
 
 SHAPES = [(1, 8, 2), (1, 64, 1000), (2, 72, 31), (5, 128, 257), (33, 64, 3), (130, 256, 5001),
-          (257, 104, 20001), (300, 1024, 2000), (3001, 64, 50003)]
+          (257, 104, 20001), (300, 1024, 2000), (3001, 64, 50003), (130, 64, 70001)]
 
 
 @pytest.mark.parametrize("scored", ["all", "some", "none"])
@@ -121,6 +121,31 @@ def test_token_logprobs_backward(n, D, V, out_dtype):
     tol = tol + (U16 if out_dtype == BF16 else 4 * U32) * want.abs() + 2.0 ** -120
     _within(got, want, tol)
     assert (got[(~live) | (d == 0)] == 0).all()
+
+
+def test_logprobs_of_many_rows_in_chunks():
+    """More probabilities than one chunk of the vocabulary holds: the gradient's accumulators carry
+    over, at two shares of scored rows (different K slices). Checked on a tenth of the rows."""
+    ops = _ops()
+    n, D, V = 8200, 64, 70001
+    for seed, part in ((1, 0.7), (2, 0.05)):
+        H, W, lab = _head_inputs(n, D, V, seed, "all")
+        lab[torch.rand(n, generator=_gen(seed), device=DEV) >= part] = -1
+        d = torch.randn(n, generator=_gen(9), device=DEV)
+        logp, other = ops.token_logprobs(H, W, lab)
+        got = ops.token_logprobs_backward(H, W, lab, logp, other, d, out_dtype=F32)
+        assert (got[lab < 0] == 0).all()
+        some = (lab >= 0).nonzero()[:, 0][::10]
+        e_logp, e_other, q = _head_exact(H[some], W, lab[some])
+        ex, tol = _head_tol(H[some], W)
+        _within(logp[some], e_logp, tol + 4 * U32 * e_logp.abs())
+        _within(other[some], e_other, tol + 4 * U32 * e_other.abs())
+        W64, g = W.double(), d[some].double().abs() * -e_logp.expm1()
+        want = (d[some].double() * -e_logp.expm1())[:, None] * (W64[lab[some]] - q @ W64)
+        spread = q @ W64.abs() + W64[lab[some]].abs()
+        rel = 2 * (U16 + ex + tol + 256 * U32) + (64 + V / 64) * U32
+        bound = (g * rel)[:, None] * spread + (d[some].double().abs() * tol)[:, None] * spread
+        _within(got[some], want, bound + 4 * U32 * want.abs() + 2.0 ** -120)
 
 
 def test_logprobs_of_sure_and_hopeless_labels():
@@ -265,6 +290,7 @@ def _scored(lens, mask):
 
 LENS = {"one": [1, 1], "empty": [0, 0], "pair": [5, 3], "ragged": [7, 0, 1, 130, 64, 65, 2, 0],
         "tiles": [4097, 4096, 1, 300, 8193, 2], "many": [3, 1, 0, 2] * 300, "long": [20011, 9003],
+        "mostly_empty": [0] * 39 + [70001] + [0] * 20,
         "pairs": [3, 0, 700, 5, 1, 2, 2, 4, 1, 3] * 420, "crowd": [1, 2, 0, 3, 2, 1, 4, 1] * 2100}
 
 
@@ -345,6 +371,28 @@ def test_preference_loss_ignores_unscored_values(lens):
     # nothing scored at all: log 2, no gradient
     loss, rewards, d = ops.preference_loss(logp, ref, plan, mask=torch.zeros_like(mask))
     assert abs(loss.item() - math.log(2)) < 1e-7 and (rewards == 0).all() and (d == 0).all()
+
+
+@pytest.mark.parametrize("lens", [[4, 3, 5, 2], [4000, 3000, 5000, 2000], [3000] * 4], ids=["small", "tiles", "pairs"])
+def test_preference_loss_of_impossible_answers(lens):
+    """A rejected answer of probability 0 costs nothing, a preferred one costs infinitely much; without a
+    weight of its own the other term does not make it NaN."""
+    ops = _ops()
+    plan, seq, mask, logp, ref = _packing(lens, 3, 2, masked=False)
+    first = [sum(lens[:i]) for i in range(4)]
+    a = logp.clone()
+    a[first[1]] = -float("inf")  # the first pair's rejected one
+    loss, rewards, d = ops.preference_loss(a, ref, plan)
+    assert rewards[1] == -float("inf") and loss.isfinite() and d.isfinite().all()
+    assert (d[: first[2]] == 0).all()
+    e = _pref_exact(logp, ref, seq, _scored(lens, None), 4, "sigmoid", 0.1, 0.0, 0.0, False)
+    one = ops.preference_loss(logp[first[2]:].contiguous(), ref[first[2]:].contiguous(), ops.pack_plan(lens[2:]))
+    _within(loss, one[0].double() / 2, 2 * U32 * loss.double() + 1e-12)
+    assert e[0].isfinite()
+    a = logp.clone()
+    a[first[0]] = -float("inf")
+    assert ops.preference_loss(a, ref, plan)[0] == float("inf")
+    assert ops.preference_loss(a, ref, plan, label_smoothing=1.0)[0].isfinite()
 
 
 @pytest.mark.parametrize("lens", [LENS["ragged"], LENS["tiles"]], ids=["ragged", "tiles"])
@@ -528,6 +576,18 @@ def test_losses_captured_and_on_a_side_stream():
             got = make()
         side.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_losses_of_nothing():
+    ops = _ops()
+    plan, none = ops.pack_plan([]), torch.empty(0, device=DEV)
+    assert plan.n == 0 and plan.nseq == 0
+    loss, stats, d = ops.policy_loss(none, none, none, plan, ref_logp=none, kl_coef=0.1, reduction="sequence")
+    assert loss == 0 and (stats == 0).all() and d.shape == (0,)
+    labels, rows = ops.next_token_labels(none.long(), plan)
+    assert labels.shape == rows.shape == (0,)
+    with pytest.raises(RuntimeError):
+        ops.preference_loss(none, none, plan)
 
 
 def test_loss_refusals_on_the_device():
@@ -792,6 +852,28 @@ def test_adamw_captured_with_device_lr_and_step(bits):
             assert torch.equal(a, b), k
         for a, b in zip(opt.state().values(), eager.state().values()):
             assert torch.equal(a.view(torch.uint8), b.view(torch.uint8)), k
+
+
+def test_adamw_refusals_on_the_device():
+    ops = _ops()
+    x = torch.zeros(1000, device=DEV)
+    y = torch.zeros(1000, device=DEV)
+    for bad in (dict(ws=[x, x], gs=[y, y]), dict(ws=[x[:600], x[500:]], gs=[y[:600], y[500:]]),
+                dict(ws=[x[:500]], gs=[x[499:999]]), dict(ws=[x], gs=[y.cpu()]), dict(ws=[x[::2]], gs=[y[::2]])):
+        with pytest.raises(ValueError):
+            ops.AdamW(**bad)
+    opt = ops.AdamW([x[:500], x[500:]], [y[:500], y[:500]])  # a gradient may be shared
+    for bad in (dict(step=0), dict(lr=float("nan")), dict(beta1=1.0), dict(eps=-1.0)):
+        with pytest.raises(RuntimeError):
+            opt.step(**{"lr": 1e-3, "step": 1, **bad})
+    for bad in (dict(max_norm=-1.0), dict(lr=torch.zeros(2, device=DEV)), dict(step=torch.zeros(1, device=DEV))):
+        with pytest.raises(ValueError):
+            opt.step(**{"lr": 1e-3, "step": 1, **bad})
+    empty = ops.AdamW([x[:0]], [y[:0]])
+    assert empty.step(1e-3, 1, max_norm=1.0).tolist() == [0.0]
+    gaps = ops.AdamW([x[:10], x[10:20]], [y[:10], y[10:20]], groups=[1, 4])
+    y[:20] = 3.0
+    assert gaps.step(1e-3, 1, max_norm=1.0).tolist() == [0.0, y[:10].norm().item(), 0.0, 0.0, y[:10].norm().item()]
 
 
 def test_adamw_matches_the_fp32_step():
