@@ -28,6 +28,7 @@ namespace dsb {
 namespace {
 
 constexpr int kBlock = DSB_ADAM_BLOCK, kChunk = DSB_ADAM_CHUNK;
+constexpr int kThreads = kChunk / 16;  // of a chunk's workgroup in the step
 constexpr float kTiny = 0x1p-100f;
 
 struct Hyper {
@@ -63,44 +64,96 @@ __host__ __device__ inline Hyper make_hyper(double lr, double beta1, double beta
   return h;
 }
 
-// 4 consecutive elements from e of a chunk of `numel`, as fp32; zeros past its end
-DSB_DEV f32x4 load4(const void* p, int e, int numel, bool bf, bool vec) {
-  f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  if (vec && e + 4 <= numel) {
-    if (bf) {
-      const bf16x4 b = *reinterpret_cast<const bf16x4*>((const bf16*)p + e);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = (float)b[i];
-    } else {
-      o = *reinterpret_cast<const f32x4*>((const float*)p + e);
-    }
-    return o;
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (e + i < numel) o[i] = bf ? (float)((const bf16*)p)[e + i] : ((const float*)p)[e + i];
-  return o;
+// Tensors' addresses come from a table in memory, of which the compiler does not know that they
+// are device memory: without these casts every access is a flat one, which waits on the LDS
+// counter too.
+template <class T>
+using Global = __attribute__((address_space(1))) T;
+template <class T>
+DSB_DEV T gload(const void* p, int e) {
+  return reinterpret_cast<const Global<T>*>((unsigned long)p)[e];
 }
-DSB_DEV void store4(void* p, int e, int numel, bool bf, bool vec, f32x4 v) {
-  if (vec && e + 4 <= numel) {
+template <class T>
+DSB_DEV void gstore(void* p, int e, T v) {
+  reinterpret_cast<Global<T>*>((unsigned long)p)[e] = v;
+}
+
+typedef unsigned u32x4h __attribute__((ext_vector_type(4), aligned(2)));
+typedef unsigned u32x4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef unsigned u32x2u __attribute__((ext_vector_type(2), aligned(2)));
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef __bf16 bf16x4u __attribute__((ext_vector_type(4), aligned(2)));
+
+// N fours of consecutive elements of a chunk, from e, e + step, ..., as they lie (bf16: in the
+// low half), zeros past its `count`; wherever they start (these loads need their elements'
+// alignment only). The type is tested once and what is left of a last four comes after, so that
+// all the loads are on their way together.
+template <bool BF>
+DSB_DEV u32x4 load4(const void* p, int e) {
+  if constexpr (BF) {
+    const u32x2u x = *reinterpret_cast<const Global<u32x2u>*>((unsigned long)p + 2l * e);
+    return u32x4{x[0], x[1], 0, 0};
+  } else {
+    return *reinterpret_cast<const Global<u32x4u>*>((unsigned long)p + 4l * e);
+  }
+}
+template <bool WHOLE, bool BF, int N>
+DSB_DEV void load_fours(u32x4 (&o)[N], const void* p, int e, int step, int count) {
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    if (WHOLE) {
+      o[k] = load4<BF>(p, e + step * k);
+    } else {
+      o[k] = u32x4{0, 0, 0, 0};
+      if (e + step * k + 4 <= count) o[k] = load4<BF>(p, e + step * k);
+    }
+  }
+  if (!WHOLE) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int at = e + step * k;
+      if (at < count && at + 4 > count) {
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+          if (at + i < count) {
+            if (BF)
+              o[k][i / 2] |= (unsigned)gload<uint16_t>(p, at + i) << (16 * (i & 1));
+            else
+              o[k][i] = gload<unsigned>(p, at + i);
+          }
+      }
+    }
+  }
+}
+template <bool WHOLE, int N>
+DSB_DEV void load_fours(u32x4 (&o)[N], const void* p, int e, int step, int count, bool bf) {
+  if (bf)
+    load_fours<WHOLE, true>(o, p, e, step, count);
+  else
+    load_fours<WHOLE, false>(o, p, e, step, count);
+}
+DSB_DEV f32x4 value4(u32x4 x, bool bf) {
+  if (!bf) return __builtin_bit_cast(f32x4, x);
+  const u32x4 y = {x[0] << 16, x[0] & 0xffff0000u, x[1] << 16, x[1] & 0xffff0000u};
+  return __builtin_bit_cast(f32x4, y);
+}
+DSB_DEV void store4(void* p, int e, int count, bool bf, f32x4 v) {
+  const bf16x4 b = {(bf16)v[0], (bf16)v[1], (bf16)v[2], (bf16)v[3]};
+  if (e + 4 <= count) {
     if (bf)
-      *reinterpret_cast<bf16x4*>((bf16*)p + e) =
-          bf16x4{(bf16)v[0], (bf16)v[1], (bf16)v[2], (bf16)v[3]};
+      *reinterpret_cast<Global<bf16x4u>*>((unsigned long)p + 2l * e) = b;
     else
-      *reinterpret_cast<f32x4*>((float*)p + e) = v;
+      *reinterpret_cast<Global<f32x4u>*>((unsigned long)p + 4l * e) = v;
     return;
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (e + i < numel) {
+  for (int i = 0; i < 3; ++i)
+    if (e + i < count) {
       if (bf)
-        ((bf16*)p)[e + i] = (bf16)v[i];
+        gstore(p, e + i, b[i]);
       else
-        ((float*)p)[e + i] = v[i];
+        gstore(p, e + i, v[i]);
     }
-}
-DSB_DEV bool aligned4(const void* p, bool bf) {
-  return ((unsigned long)p & (bf ? 7 : 15)) == 0;
 }
 
 // The largest of the 16 lanes of a block, as unsigned bits (of magnitudes: NaN wins).
@@ -160,11 +213,12 @@ __global__ __launch_bounds__(256) void adam_sumsq_kernel(const dsb_adam_chunk* _
   const dsb_adam_chunk t = chunks[c];
   const bool bf = (t.dtypes >> 8) == DSB_DT_BF16;
   double s = 0.0;
-  if (((unsigned long)t.g & 15) == 0 && t.count == kChunk) {
+  if (t.count == kChunk) {
     if (bf) {
       u32x4 v[kChunk / 512];
 #pragma unroll
-      for (int k = 0; k < kChunk / 512; ++k) v[k] = ldg128((const bf16*)t.g + 512 * k + 8 * l);
+      for (int k = 0; k < kChunk / 512; ++k)
+        v[k] = *reinterpret_cast<const Global<u32x4h>*>((unsigned long)t.g + 16 * (64 * k + l));
 #pragma unroll
       for (int k = 0; k < kChunk / 512; ++k) {
         float g[8];
@@ -173,22 +227,25 @@ __global__ __launch_bounds__(256) void adam_sumsq_kernel(const dsb_adam_chunk* _
         for (int i = 0; i < 8; ++i) s += (double)g[i] * (double)g[i];
       }
     } else {
-      f32x4 v[kChunk / 256];
+      u32x4 v[kChunk / 256];
+      load_fours<true, false>(v, t.g, 4 * l, 256, t.count);
 #pragma unroll
-      for (int k = 0; k < kChunk / 256; ++k)
-        v[k] = *reinterpret_cast<const f32x4*>((const float*)t.g + 256 * k + 4 * l);
+      for (int k = 0; k < kChunk / 256; ++k) {
+        const f32x4 g = value4(v[k], false);
 #pragma unroll
-      for (int k = 0; k < kChunk / 256; ++k)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s += (double)v[k][i] * (double)v[k][i];
+        for (int i = 0; i < 4; ++i) s += (double)g[i] * (double)g[i];
+      }
     }
   } else {
-    const bool vec = aligned4(t.g, bf);
-#pragma unroll 4
-    for (int k = 0; k < kChunk / 256; ++k) {
-      const f32x4 g = load4(t.g, 256 * k + 4 * l, t.count, bf, vec);
+    for (int k0 = 0; k0 < kChunk / 256; k0 += 4) {
+      u32x4 v[4];
+      load_fours<false>(v, t.g, 256 * k0 + 4 * l, 256, t.count, bf);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s += (double)g[i] * (double)g[i];
+      for (int k = 0; k < 4; ++k) {
+        const f32x4 g = value4(v[k], bf);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s += (double)g[i] * (double)g[i];
+      }
     }
   }
 #pragma unroll
@@ -244,32 +301,34 @@ struct ClipArgs {
 };
 
 template <int BITS>
-__global__ __launch_bounds__(256) void adam_kernel(const dsb_adam_chunk* __restrict__ chunks,
+__global__ __launch_bounds__(kThreads) void adam_kernel(const dsb_adam_chunk* __restrict__ chunks,
                                                    Hyper hv, const Hyper* __restrict__ hp,
                                                    ClipArgs clip, void* mp, void* vp,
                                                    float* __restrict__ m_scale,
                                                    float* __restrict__ r_scale) {
-  __shared__ double red[4];
+  __shared__ double red[kThreads / 64];
   // the chunks that the norm's pass read last come first: the device's cache still holds them
   const int chunk = gridDim.x - 1 - blockIdx.x;
   const dsb_adam_chunk t = chunks[chunk];
   const int l16 = threadIdx.x & 15, qb = threadIdx.x >> 4;  // 16 blocks of 256 per chunk
   const bool live = qb * kBlock < t.count;                  // the 16 lanes of a block together
   const bool wbf = (t.dtypes & 255) == DSB_DT_BF16, gbf = (t.dtypes >> 8) == DSB_DT_BF16;
-  const bool wvec = aligned4(t.w, wbf), gvec = aligned4(t.g, gbf);
   const int e0 = qb * kBlock + 4 * l16;
   const long b = t.block + qb, s0 = b * kBlock + 4 * l16;
   const double mine =
       clip.how == CLIP_SUM && t.c0 + (int)threadIdx.x < t.c1 ? clip.partial[t.c0 + threadIdx.x] : 0.0;
-  f32x4 g[4], w[4];
+  u32x4 graw[4], wraw[4];
   float m[4][4], r[4][4];
   unsigned mc[4], rc[4];
   float ms = 0.f, rs = 0.f;
   if (live) {
-#pragma unroll
-    for (int k = 0; k < 4; ++k) g[k] = load4(t.g, e0 + 64 * k, t.count, gbf, gvec);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) w[k] = load4(t.w, e0 + 64 * k, t.count, wbf, wvec);
+    if (t.count == kChunk) {
+      load_fours<true>(graw, t.g, e0, 64, t.count, gbf);
+      load_fours<true>(wraw, t.w, e0, 64, t.count, wbf);
+    } else {
+      load_fours<false>(graw, t.g, e0, 64, t.count, gbf);
+      load_fours<false>(wraw, t.w, e0, 64, t.count, wbf);
+    }
     if constexpr (BITS == 8) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -292,11 +351,11 @@ __global__ __launch_bounds__(256) void adam_kernel(const dsb_adam_chunk* __restr
   if (clip.how == CLIP_GIVEN) {
     cf = clip.coef[t.group];
   } else if (clip.how == CLIP_SUM) {
-    const double norm = sqrt(block_sum64<256>(mine, red));
+    const double norm = sqrt(block_sum64<kThreads>(mine, red));
     cf = clip_factor(norm, clip.max_norm);
     if (chunk == t.c0 && threadIdx.x == 0) clip.norms[t.group] = (float)norm;
     if (chunk == 0)  // groups without elements
-      for (int g = threadIdx.x; g < clip.ngroups; g += 256)
+      for (int g = threadIdx.x; g < clip.ngroups; g += kThreads)
         if (clip.group_chunks[g] == clip.group_chunks[g + 1]) clip.norms[g] = 0.f;
   }
   if (!live) return;
@@ -309,9 +368,11 @@ __global__ __launch_bounds__(256) void adam_kernel(const dsb_adam_chunk* __restr
       unpack4_e4m3(mc[k], m[k]);
       unpack4_e4m3(rc[k], r[k]);
     }
+    const f32x4 g = value4(graw[k], gbf);
+    f32x4 w = value4(wraw[k], wbf);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float gi = g[k][i] * cf;
+      const float gi = g[i] * cf;
       float v;
       if constexpr (BITS == 8) {
         const float ro = r[k][i] * rs;
@@ -320,18 +381,18 @@ __global__ __launch_bounds__(256) void adam_kernel(const dsb_adam_chunk* __restr
         r[k][i] = __builtin_amdgcn_sqrtf(v);
         mtop = max(mtop, mag(m[k][i]));
         rtop = max(rtop, mag(r[k][i]));
-        w[k][i] = w[k][i] * h.decay -
+        w[i] = w[i] * h.decay -
                   h.step_size * m[k][i] * __builtin_amdgcn_rcpf(r[k][i] * h.rbc2 + h.eps);
       } else {
         v = h.b2 * r[k][i] + h.ob2 * (gi * gi);
         m[k][i] = h.b1 * m[k][i] + h.ob1 * gi;
         r[k][i] = v;
-        w[k][i] = w[k][i] * h.decay -
+        w[i] = w[i] * h.decay -
                   h.step_size * m[k][i] *
                       __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v) * h.rbc2 + h.eps);
       }
     }
-    store4(t.w, e0 + 64 * k, t.count, wbf, wvec, w[k]);
+    store4(t.w, e0 + 64 * k, t.count, wbf, w);
     if constexpr (BITS == 32) {
       *reinterpret_cast<f32x4*>((float*)mp + s0 + 64 * k) = *reinterpret_cast<f32x4*>(m[k]);
       *reinterpret_cast<f32x4*>((float*)vp + s0 + 64 * k) = *reinterpret_cast<f32x4*>(r[k]);
@@ -390,17 +451,17 @@ hipError_t adam_step(const AdamArgs& a, void* work, hipStream_t s) {
                          a.nchunks, partial);
     // Groups of at most 256 chunks (a million elements) are added up by each of their blocks,
     // which saves a launch.
-    c.how = a.most_chunks <= 256 && a.nchunks > 0 ? CLIP_SUM : CLIP_GIVEN;
+    c.how = a.most_chunks <= kThreads && a.nchunks > 0 ? CLIP_SUM : CLIP_GIVEN;
     if (c.how == CLIP_GIVEN)
       hipLaunchKernelGGL(adam_norm_kernel, dim3(a.ngroups), dim3(1024), 0, s, a.group_chunks, partial,
                          a.max_norm, a.norms, coef);
   }
   if (a.nchunks > 0) {
     if (a.bits == 8)
-      hipLaunchKernelGGL(adam_kernel<8>, dim3(a.nchunks), dim3(256), 0, s, a.chunks, hv,
+      hipLaunchKernelGGL(adam_kernel<8>, dim3(a.nchunks), dim3(kThreads), 0, s, a.chunks, hv,
                          dev ? hp : nullptr, c, a.m, a.v, a.m_scale, a.r_scale);
     else
-      hipLaunchKernelGGL(adam_kernel<32>, dim3(a.nchunks), dim3(256), 0, s, a.chunks, hv,
+      hipLaunchKernelGGL(adam_kernel<32>, dim3(a.nchunks), dim3(kThreads), 0, s, a.chunks, hv,
                          dev ? hp : nullptr, c, a.m, a.v, a.m_scale, a.r_scale);
   }
   return hipGetLastError();

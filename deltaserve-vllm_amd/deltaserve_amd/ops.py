@@ -496,13 +496,14 @@ def preference_loss(logp, ref_logp, plan, mask=None, kind="sigmoid", beta=0.1, l
     _mask(what, mask, plan.n)
     with _on(what, logp, ref_logp, mask, plan.tables):
         dlogp = torch.empty_like(logp)
-        out = torch.empty(1 + plan.nseq, dtype=torch.float32, device=logp.device)
+        loss = torch.empty((), dtype=torch.float32, device=logp.device)
+        rewards = torch.empty(plan.nseq, dtype=torch.float32, device=logp.device)
         work = _work(plan.loss_bytes, logp.device) if plan.loss_bytes else None
         L.check(L.load().dsb_op_preference_loss(
             _at(logp), _at(ref_logp), _at(mask), plan.ref, L.PREF_KINDS[kind], beta, label_smoothing,
-            margin, average, grad_scale, _at(out), out.data_ptr() + 4, _at(dlogp), _at(work),
+            margin, average, grad_scale, _at(loss), _at(rewards), _at(dlogp), _at(work),
             plan.loss_bytes, _now()), what="dsb_op_preference_loss")
-    return out[0], out[1:], dlogp
+    return loss, rewards, dlogp
 
 
 def policy_loss(logp, old_logp, adv, plan, mask=None, ref_logp=None, clip_low=0.2, clip_high=0.2,
