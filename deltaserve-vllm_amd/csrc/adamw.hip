@@ -17,7 +17,12 @@
 //
 // A workgroup takes a chunk of 4096 elements, a wave 4 blocks, 16 lanes a block:
 // every load of 4 elements a lane covers whole 256-byte runs, and the block's
-// maxima are 4 DPP steps.
+// maxima are 4 DPP steps. The step is bound by its bytes, which nothing reads again:
+// its loads and stores bypass the caches, where they only push out what the norm's pass
+// left of the gradients (54 M fp32 elements with fp32 moments 320 → 259 µs, 6.7 TB/s;
+// 252 M bf16 ones with 8-bit moments 575 → 518; 84 M fp32 ones, no clip, 252 → 230; the
+// stores alone 321, 592, 272, the moments' loads alone 312, 571, 241). The norm's pass
+// reads through them (past them: 285, 556).
 #include <cmath>
 #include <type_traits>
 
@@ -87,25 +92,27 @@ typedef __bf16 bf16x4u __attribute__((ext_vector_type(4), aligned(2)));
 // N fours of consecutive elements of a chunk, from e, e + step, ..., as they lie (bf16: in the
 // low half), zeros past its `count`; wherever they start (these loads need their elements'
 // alignment only). The type is tested once and what is left of a last four comes after, so that
-// all the loads are on their way together.
-template <bool BF>
+// all the loads are on their way together. NT: loads past the caches.
+template <bool BF, bool NT>
 DSB_DEV u32x4 load4(const void* p, int e) {
   if constexpr (BF) {
-    const u32x2u x = *reinterpret_cast<const Global<u32x2u>*>((unsigned long)p + 2l * e);
+    const auto* q = reinterpret_cast<const Global<u32x2u>*>((unsigned long)p + 2l * e);
+    const u32x2u x = NT ? __builtin_nontemporal_load(q) : *q;
     return u32x4{x[0], x[1], 0, 0};
   } else {
-    return *reinterpret_cast<const Global<u32x4u>*>((unsigned long)p + 4l * e);
+    const auto* q = reinterpret_cast<const Global<u32x4u>*>((unsigned long)p + 4l * e);
+    return NT ? __builtin_nontemporal_load(q) : *q;
   }
 }
-template <bool WHOLE, bool BF, int N>
+template <bool WHOLE, bool BF, bool NT, int N>
 DSB_DEV void load_fours(u32x4 (&o)[N], const void* p, int e, int step, int count) {
 #pragma unroll
   for (int k = 0; k < N; ++k) {
     if (WHOLE) {
-      o[k] = load4<BF>(p, e + step * k);
+      o[k] = load4<BF, NT>(p, e + step * k);
     } else {
       o[k] = u32x4{0, 0, 0, 0};
-      if (e + step * k + 4 <= count) o[k] = load4<BF>(p, e + step * k);
+      if (e + step * k + 4 <= count) o[k] = load4<BF, NT>(p, e + step * k);
     }
   }
   if (!WHOLE) {
@@ -125,12 +132,21 @@ DSB_DEV void load_fours(u32x4 (&o)[N], const void* p, int e, int step, int count
     }
   }
 }
-template <bool WHOLE, int N>
+template <bool WHOLE, bool NT, int N>
 DSB_DEV void load_fours(u32x4 (&o)[N], const void* p, int e, int step, int count, bool bf) {
   if (bf)
-    load_fours<WHOLE, true>(o, p, e, step, count);
+    load_fours<WHOLE, true, NT>(o, p, e, step, count);
   else
-    load_fours<WHOLE, false>(o, p, e, step, count);
+    load_fours<WHOLE, false, NT>(o, p, e, step, count);
+}
+// The moments: kernel arguments, aligned.
+template <class T>
+DSB_DEV T nt_load(const void* base, long at) {
+  return __builtin_nontemporal_load(reinterpret_cast<const T*>(base) + at);
+}
+template <class T>
+DSB_DEV void nt_store(void* base, long at, T v) {
+  __builtin_nontemporal_store(v, reinterpret_cast<T*>(base) + at);
 }
 DSB_DEV f32x4 value4(u32x4 x, bool bf) {
   if (!bf) return __builtin_bit_cast(f32x4, x);
@@ -141,9 +157,11 @@ DSB_DEV void store4(void* p, int e, int count, bool bf, f32x4 v) {
   const bf16x4 b = {(bf16)v[0], (bf16)v[1], (bf16)v[2], (bf16)v[3]};
   if (e + 4 <= count) {
     if (bf)
-      *reinterpret_cast<Global<bf16x4u>*>((unsigned long)p + 2l * e) = b;
+      __builtin_nontemporal_store((bf16x4u)b,
+                                  reinterpret_cast<Global<bf16x4u>*>((unsigned long)p + 2l * e));
     else
-      *reinterpret_cast<Global<f32x4u>*>((unsigned long)p + 4l * e) = v;
+      __builtin_nontemporal_store((f32x4u)v,
+                                  reinterpret_cast<Global<f32x4u>*>((unsigned long)p + 4l * e));
     return;
   }
 #pragma unroll
@@ -228,7 +246,7 @@ __global__ __launch_bounds__(256) void adam_sumsq_kernel(const dsb_adam_chunk* _
       }
     } else {
       u32x4 v[kChunk / 256];
-      load_fours<true, false>(v, t.g, 4 * l, 256, t.count);
+      load_fours<true, false, false>(v, t.g, 4 * l, 256, t.count);
 #pragma unroll
       for (int k = 0; k < kChunk / 256; ++k) {
         const f32x4 g = value4(v[k], false);
@@ -239,7 +257,7 @@ __global__ __launch_bounds__(256) void adam_sumsq_kernel(const dsb_adam_chunk* _
   } else {
     for (int k0 = 0; k0 < kChunk / 256; k0 += 4) {
       u32x4 v[4];
-      load_fours<false>(v, t.g, 256 * k0 + 4 * l, 256, t.count, bf);
+      load_fours<false, false>(v, t.g, 256 * k0 + 4 * l, 256, t.count, bf);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const f32x4 g = value4(v[k], bf);
@@ -307,8 +325,7 @@ __global__ __launch_bounds__(kThreads) void adam_kernel(const dsb_adam_chunk* __
                                                    float* __restrict__ m_scale,
                                                    float* __restrict__ r_scale) {
   __shared__ double red[kThreads / 64];
-  // the chunks that the norm's pass read last come first: the device's cache still holds them
-  const int chunk = gridDim.x - 1 - blockIdx.x;
+  const int chunk = blockIdx.x;
   const dsb_adam_chunk t = chunks[chunk];
   const int l16 = threadIdx.x & 15, qb = threadIdx.x >> 4;  // 16 blocks of 256 per chunk
   const bool live = qb * kBlock < t.count;                  // the 16 lanes of a block together
@@ -323,27 +340,25 @@ __global__ __launch_bounds__(kThreads) void adam_kernel(const dsb_adam_chunk* __
   float ms = 0.f, rs = 0.f;
   if (live) {
     if (t.count == kChunk) {
-      load_fours<true>(graw, t.g, e0, 64, t.count, gbf);
-      load_fours<true>(wraw, t.w, e0, 64, t.count, wbf);
+      load_fours<true, true>(graw, t.g, e0, 64, t.count, gbf);
+      load_fours<true, true>(wraw, t.w, e0, 64, t.count, wbf);
     } else {
-      load_fours<false>(graw, t.g, e0, 64, t.count, gbf);
-      load_fours<false>(wraw, t.w, e0, 64, t.count, wbf);
+      load_fours<false, true>(graw, t.g, e0, 64, t.count, gbf);
+      load_fours<false, true>(wraw, t.w, e0, 64, t.count, wbf);
     }
     if constexpr (BITS == 8) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        mc[k] = *reinterpret_cast<const unsigned*>((const uint8_t*)mp + s0 + 64 * k);
-        rc[k] = *reinterpret_cast<const unsigned*>((const uint8_t*)vp + s0 + 64 * k);
+        mc[k] = nt_load<unsigned>(mp, s0 / 4 + 16 * k);
+        rc[k] = nt_load<unsigned>(vp, s0 / 4 + 16 * k);
       }
       ms = m_scale[b];
       rs = r_scale[b];
     } else {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        *reinterpret_cast<f32x4*>(m[k]) =
-            *reinterpret_cast<const f32x4*>((const float*)mp + s0 + 64 * k);
-        *reinterpret_cast<f32x4*>(r[k]) =
-            *reinterpret_cast<const f32x4*>((const float*)vp + s0 + 64 * k);
+        *reinterpret_cast<f32x4*>(m[k]) = nt_load<f32x4>(mp, s0 / 4 + 16 * k);
+        *reinterpret_cast<f32x4*>(r[k]) = nt_load<f32x4>(vp, s0 / 4 + 16 * k);
       }
     }
   }
@@ -394,8 +409,8 @@ __global__ __launch_bounds__(kThreads) void adam_kernel(const dsb_adam_chunk* __
     }
     store4(t.w, e0 + 64 * k, t.count, wbf, w);
     if constexpr (BITS == 32) {
-      *reinterpret_cast<f32x4*>((float*)mp + s0 + 64 * k) = *reinterpret_cast<f32x4*>(m[k]);
-      *reinterpret_cast<f32x4*>((float*)vp + s0 + 64 * k) = *reinterpret_cast<f32x4*>(r[k]);
+      nt_store(mp, s0 / 4 + 16 * k, *reinterpret_cast<f32x4*>(m[k]));
+      nt_store(vp, s0 / 4 + 16 * k, *reinterpret_cast<f32x4*>(r[k]));
     }
   }
   if constexpr (BITS == 8) {
@@ -419,8 +434,8 @@ __global__ __launch_bounds__(kThreads) void adam_kernel(const dsb_adam_chunk* __
         p[2 * j] = round_random(p[2 * j], x & 0xffffu);
         p[2 * j + 1] = round_random(p[2 * j + 1], x >> 16);
       }
-      *reinterpret_cast<unsigned*>((uint8_t*)mp + s0 + 64 * k) = pack4_e4m3(q);
-      *reinterpret_cast<unsigned*>((uint8_t*)vp + s0 + 64 * k) = pack4_e4m3(p);
+      nt_store(mp, s0 / 4 + 16 * k, pack4_e4m3(q));
+      nt_store(vp, s0 / 4 + 16 * k, pack4_e4m3(p));
     }
     if (l16 == 0) {
       m_scale[b] = mt < kTiny ? 0.f : mt * (1.f / 448.f);
@@ -450,7 +465,8 @@ hipError_t adam_step(const AdamArgs& a, void* work, hipStream_t s) {
       hipLaunchKernelGGL(adam_sumsq_kernel, dim3((a.nchunks + 3) / 4), dim3(256), 0, s, a.chunks,
                          a.nchunks, partial);
     // Groups of at most 256 chunks (a million elements) are added up by each of their blocks,
-    // which saves a launch.
+    // which saves a launch (2.3 M elements in 28 groups: 15.3 µs, 17.2 with it); a thread of a
+    // block reads one sum.
     c.how = a.most_chunks <= kThreads && a.nchunks > 0 ? CLIP_SUM : CLIP_GIVEN;
     if (c.how == CLIP_GIVEN)
       hipLaunchKernelGGL(adam_norm_kernel, dim3(a.ngroups), dim3(1024), 0, s, a.group_chunks, partial,

@@ -68,11 +68,12 @@ DSB_DEV double block_sumd(double v, double* red) {
   return s[0];
 }
 
-// Rows r .. r+k-1 (k <= 4; Int<4>: one access), zeros after them.
-template <class K>
+// Rows r .. r+k-1 (k <= 4; Int<4>: one access), zeros after them. NT: past the caches.
+template <bool NT = false, class K>
 DSB_DEV f32x4 get4(const float* p, int r, K k) {
   if constexpr (std::is_same<K, Int<4>>::value) {
-    return *reinterpret_cast<const f32x4u*>(p + r);
+    const auto* q = reinterpret_cast<const f32x4u*>(p + r);
+    return NT ? __builtin_nontemporal_load(q) : *q;
   } else {
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -81,10 +82,14 @@ DSB_DEV f32x4 get4(const float* p, int r, K k) {
     return o;
   }
 }
-template <class K>
+template <bool NT = false, class K>
 DSB_DEV void put4(float* p, int r, K k, f32x4 v) {
   if constexpr (std::is_same<K, Int<4>>::value) {
-    *reinterpret_cast<f32x4u*>(p + r) = v;
+    auto* q = reinterpret_cast<f32x4u*>(p + r);
+    if (NT)
+      __builtin_nontemporal_store((f32x4u)v, q);
+    else
+      *q = v;
   } else {
 #pragma unroll
     for (int i = 0; i < 3; ++i)
@@ -238,7 +243,9 @@ DSB_DEV double tile_sum(const PrefIn& in, const Tile& t, int last, int lane, int
   return wave_sumd(s);
 }
 
-// One wave: a tile's rows of the gradient.
+// One wave: a tile's rows of the gradient. Large batches store it past the caches (4096 pairs of
+// 1024 rows by pair: 18.4 → 17.5 µs; their loads past them too 18.3).
+template <bool NT>
 DSB_DEV void tile_grads(const PrefIn& in, const Tile& t, int last, float coef, float* dlogp,
                         int lane) {
   for_rows<64, 4>(
@@ -249,7 +256,7 @@ DSB_DEV void tile_grads(const PrefIn& in, const Tile& t, int last, float coef, f
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           v[i] = (in.mask ? m >> i & 1 : r + i != last) ? coef : 0.f;
-        put4(dlogp, r, k, v);
+        put4<NT>(dlogp, r, k, v);
       });
 }
 
@@ -302,7 +309,7 @@ __global__ __launch_bounds__(1024) void pref_small_kernel(PrefIn in, dsb_pack_pl
   if (threadIdx.x == 0) *loss = (float)(total / npairs);
   for (int t = wave; t < p.ntiles; t += 16) {
     const Tile tl = get_tile(p, t);
-    tile_grads(in, tl, p.starts[tl.seq + 1] - 1, coef[tl.seq], dlogp, lane);
+    tile_grads<false>(in, tl, p.starts[tl.seq + 1] - 1, coef[tl.seq], dlogp, lane);
   }
 }
 
@@ -379,7 +386,7 @@ __global__ __launch_bounds__(NB) void pref_pair_kernel(PrefIn in, dsb_pack_plan 
           const bool on = in.mask ? m >> j & 1 : r + j != b - 1 && r + j != c - 1;
           v[j] = on ? r + j >= b ? d1 : d0 : 0.f;
         }
-        put4(dlogp, r, k, v);
+        put4<true>(dlogp, r, k, v);
       });
 }
 
@@ -441,7 +448,7 @@ __global__ __launch_bounds__(256) void pref_grads_kernel(PrefIn in, dsb_pack_pla
   const int t = (blockIdx.x - 1) * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
   if (t >= p.ntiles) return;
   const Tile tl = get_tile(p, t);
-  tile_grads(in, tl, p.starts[tl.seq + 1] - 1, coef[tl.seq], dlogp, lane);
+  tile_grads<true>(in, tl, p.starts[tl.seq + 1] - 1, coef[tl.seq], dlogp, lane);
 }
 
 // ---------------------------------------------------------------- policy loss
@@ -521,10 +528,10 @@ struct PolicyIn {
   const float *logp, *old, *ref, *adv;
   const uint8_t* mask;
   bool adv_rows;
-  template <class K>
-  DSB_DEV Rows operator()(int r, K k) const {
-    return Rows{get4(logp, r, k), get4(old, r, k), get4(ref ? ref : logp, r, k),
-                get4(adv_rows ? adv : logp, r, k),
+  template <bool NT = false, class K>
+  DSB_DEV Rows load(int r, K k) const {
+    return Rows{get4<NT>(logp, r, k), get4<NT>(old, r, k), get4<NT>(ref ? ref : logp, r, k),
+                get4<NT>(adv_rows ? adv : logp, r, k),
                 mask4(mask ? mask : (const uint8_t*)logp, r, k)};
   }
 };
@@ -584,9 +591,9 @@ __global__ __launch_bounds__(1024) void policy_small_kernel(PolicyIn in, dsb_pac
     const int r = 4 * (tid + 1024 * j);
     left[j] = min(max(p.n - r, 0), 4);
     if (left[j] == 4)
-      x[j] = in(r, Int<4>{});
+      x[j] = in.load(r, Int<4>{});
     else if (left[j] > 0)
-      x[j] = in(r, left[j]);
+      x[j] = in.load(r, left[j]);
   }
   if (need_seq)
     for (int s = tid; s <= p.nseq; s += 1024) starts[s] = p.starts[s];
@@ -724,9 +731,13 @@ __global__ __launch_bounds__(256) void policy_kernel(PolicyIn in, dsb_pack_plan 
   };
   PolicySums sums;
   const int r0 = blockIdx.x * kChunkRows, r1 = min(p.n - r0, kChunkRows) + r0;
-  for_rows<256, 2>(r0, r1, threadIdx.x, in, [&](int r, auto k, const Rows& x) {
-    policy_rows4(in, p.starts, h, r, k, x, lo, hi, need_seq, weight, dlogp, sums);
-  });
+  // rows are read once, past the caches (16 M rows with a reference and advantages by row: 80.9
+  // → 70.6 µs; the gradients past them too 72.3)
+  for_rows<256, 2>(
+      r0, r1, threadIdx.x, [&](int r, auto k) { return in.load<true>(r, k); },
+      [&](int r, auto k, const Rows& x) {
+        policy_rows4(in, p.starts, h, r, k, x, lo, hi, need_seq, weight, dlogp, sums);
+      });
   double v[4] = {sums.pol, sums.kl, (double)sums.clipped, (double)sums.count};
   block_sums<256>(v, red4);
   if (threadIdx.x == 0)
