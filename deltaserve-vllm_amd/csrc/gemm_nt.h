@@ -104,6 +104,14 @@ struct IsLive : std::false_type {};
 template <class E>
 struct IsLive<E, std::void_t<decltype(E::kLive)>> : std::true_type {};
 
+// Epilogues with a true kStreamB: each block's B is its own (one tile of rows), and its
+// loads bypass the caches.
+template <class E, class = void>
+struct StreamsB : std::false_type {};
+template <class E>
+struct StreamsB<E, std::void_t<decltype(E::kStreamB)>>
+    : std::integral_constant<bool, E::kStreamB> {};
+
 // Slices of K that `tiles` output tiles of nk K tiles are split over so that
 // the device's 256 CUs are evenly loaded: the least number of K steps on the
 // busiest one, a block's epilogue (an fp32 tile stored while the others store
@@ -172,6 +180,10 @@ DSB_DEV void set_m0(unsigned lds_addr) {
 }
 DSB_DEV void dma16_m0(u32x4 rsrc, int voff) {
   asm volatile("buffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(rsrc) : "memory");
+}
+// past the caches, for an operand that one block alone reads
+DSB_DEV void dma16_m0_nt(u32x4 rsrc, int voff) {
+  asm volatile("buffer_load_dwordx4 %0, %1, 0 offen nt lds" ::"v"(voff), "s"(rsrc) : "memory");
 }
 #pragma clang diagnostic pop
 
@@ -565,6 +577,12 @@ __attribute__((amdgpu_waves_per_eu(WM* WN / 4, WM* WN / 4))) void gemm_nt_kernel
   auto pre_one = [&](const auto& f, int j) __attribute__((always_inline)) {
     set_m0(j < IA ? f.dstA + j * 8 * NW * BK * 2 : f.dstB + (SA + (j - IA) * 8 * NW * BK) * 2);
   };
+  auto dma_b = [](u32x4 rsrc, int voff) __attribute__((always_inline)) {
+    if constexpr (StreamsB<Epi>::value)
+      dma16_m0_nt(rsrc, voff);
+    else
+      dma16_m0(rsrc, voff);
+  };
   auto go_one = [&](const auto& f, int j) __attribute__((always_inline)) {
     constexpr bool EDGE = std::decay_t<decltype(f)>::kEdge;
     if (j < IA) {
@@ -574,13 +592,13 @@ __attribute__((amdgpu_waves_per_eu(WM* WN / 4, WM* WN / 4))) void gemm_nt_kernel
       const int off = f.s1B ? vkn1[j - IA] : vkn2[j - IA];
       if constexpr (EDGE) {
         const int none = mask(!ring_kn_live(RPL * (wave + (j - IA) * NW), f.liveB));
-        dma16_m0(pick_rsrc(none, zs, f.dB), pick(none, lane * 16, off));
+        dma_b(pick_rsrc(none, zs, f.dB), pick(none, lane * 16, off));
       } else {
-        dma16_m0(f.dB, off);
+        dma_b(f.dB, off);
       }
     } else {
       const int off = f.s1B ? boff1[j - IA] : boff2[j - IA];
-      dma16_m0(f.dB, f.voB + (EDGE ? pick(f.pastB, 0, off) : off));
+      dma_b(f.dB, f.voB + (EDGE ? pick(f.pastB, 0, off) : off));
     }
   };
   auto issue_one = [&](const auto& f, int j) __attribute__((always_inline)) {
@@ -1085,8 +1103,9 @@ struct EpiF32 {
 // fp32 partials of a live launch's K slices, live rows · N apart, `elems` floats in
 // all, added to what they hold with `accumulate`; K is split as for a product of k (the
 // same for every chunk of a longer K) into at most `ks`.
+template <bool STREAM>
 struct EpiLivePart {
-  static constexpr bool kLive = true;
+  static constexpr bool kLive = true, kStreamB = STREAM;
   float* part;
   int accumulate;
   int k, ks;

@@ -54,8 +54,9 @@ struct LPStat {
 // Per run of TN columns and row: LPStat into stats[run · cap + m] (the 16 rows of
 // a fragment are neighbours, so a store is one 128-byte line) and the label's logit
 // into tgt[m]. A lane holds 4·FN columns of a row.
+template <bool STREAM>
 struct EpiLogProb {
-  static constexpr bool kLive = true;
+  static constexpr bool kLive = true, kStreamB = STREAM;
   __host__ __device__ int most_slices(int, int) const { return 1; }
   DSB_DEV int slices(int, int, int, int) const { return 1; }
   DSB_DEV const EpiLogProb& at(int, int, int) const { return *this; }
@@ -133,8 +134,9 @@ struct EpiLogProb {
 // the sum of the rounded values goes to rsum[m · runs + run] (products with ones on the
 // matrix cores). Only runs that hold a label (one in V / TN of a row's) test their columns
 // for it; its exponential, which may be infinite, is left out by a select.
+template <bool STREAM>
 struct EpiProb {
-  static constexpr bool kLive = true;
+  static constexpr bool kLive = true, kStreamB = STREAM;
   __host__ __device__ int most_slices(int, int) const { return 1; }
   DSB_DEV int slices(int, int, int, int) const { return 1; }
   DSB_DEV const EpiProb& at(int, int, int) const { return *this; }
@@ -242,7 +244,7 @@ LPPlan lp_plan(int n, int D, int V) {
 // Columns, the last ones of the vocabulary, that the forward's product takes in 256 × 128
 // tiles: over one block of rows the head is streamed by whole rounds of the device's CUs, and
 // where the last round of 256 × 256 tiles is at most half full, half-wide ones fill it better
-// (149 rows × 5120 × 151936, 82 tiles in the third round: 386 → 355 µs).
+// (149 rows × 5120 × 151936, 82 tiles in the third round: 386 → 355 µs, both through the caches).
 int lp_narrow(int n, int V) {
   const int tiles = (V + 255) / 256, last = tiles % kGemmCus;
   return n <= 256 && tiles > kGemmCus && last > 0 && last <= kGemmCus / 2
@@ -269,8 +271,9 @@ struct LPWork {
 };
 
 // The dH product's epilogue; its K slices at any live row count.
-__host__ __device__ inline EpiLivePart lp_part(const LPWork& w, int accumulate) {
-  return EpiLivePart{w.part, accumulate, w.plan.vchunk, kMaxSlices, w.plan.part_elems};
+template <bool STREAM = false>
+__host__ __device__ inline EpiLivePart<STREAM> lp_part(const LPWork& w, int accumulate) {
+  return EpiLivePart<STREAM>{w.part, accumulate, w.plan.vchunk, kMaxSlices, w.plan.part_elems};
 }
 
 LPWork lp_layout(int n, int D, int V, bool backward, void* base, size_t* bytes) {
@@ -504,6 +507,9 @@ int64_t logprob_bytes(int n, int D, int V, bool backward) {
     if (_e != hipSuccess) return _e;     \
   } while (0)
 
+// Over one block of rows (n <= 256) each block of the products reads columns of the head of its
+// own: past the caches (µs, through them → past them: 149 rows × 5120 × 151936 forward 349 → 335,
+// gradient 711 → 690; 113 × 4096 × 128256 219 → 214, 443 → 429).
 hipError_t token_logprobs(const bf16* normed, long ldh, const bf16* W, const int64_t* labels, int n,
                           int D, int V, float* logp, float* other, void* work, hipStream_t s) {
   size_t bytes = 0;
@@ -515,12 +521,20 @@ hipError_t token_logprobs(const bf16* normed, long ldh, const bf16* W, const int
   LPCK(hipGetLastError());
   const int V1 = V - w.narrow;
   GemmProblem p{w.X, (long)D, W, (long)D, nullptr, 0, nullptr, 0, n, V1, D, 0, w.count};
-  LPCK((launch_gemm_cfg<256, 256, 2, 2>(p, EpiLogProb{w.stats, n, V1, w.ref, w.labels, w.tgt, 0}, s)));
-  if (w.narrow) {
-    p.B = W + (long)V1 * D;
-    p.N = w.narrow;
-    const EpiLogProb epi{w.stats + (long)(V1 / kRun) * n, n, w.narrow, w.ref, w.labels, w.tgt, V1};
-    LPCK((launch_gemm_cfg<256, 128, 2, 2, 3, 3>(p, epi, s)));
+  if (n > 256) {
+    const EpiLogProb<false> epi{w.stats, n, V1, w.ref, w.labels, w.tgt, 0};
+    LPCK((launch_gemm_cfg<256, 256, 2, 2>(p, epi, s)));
+  } else {
+    EpiLogProb<true> epi{w.stats, n, V1, w.ref, w.labels, w.tgt, 0};
+    LPCK((launch_gemm_cfg<256, 256, 2, 2>(p, epi, s)));
+    if (w.narrow) {
+      p.B = W + (long)V1 * D;
+      p.N = w.narrow;
+      epi.stats += (long)(V1 / kRun) * n;
+      epi.V = w.narrow;
+      epi.c0 = V1;
+      LPCK((launch_gemm_cfg<256, 128, 2, 2, 3, 3>(p, epi, s)));
+    }
   }
   hipLaunchKernelGGL(lp_finish_kernel, dim3((n + 15) / 16), dim3(1024), 0, s, w, n, logp, other);
   return hipGetLastError();
@@ -541,13 +555,18 @@ hipError_t token_logprobs_bwd(const bf16* normed, long ldh, const bf16* W, const
     const int Vc = std::min(vchunk, V - c0), Nc8 = (Vc + 7) / 8 * 8;
     const bf16* Wc = W + (long)c0 * D;
     GemmProblem p{w.X, (long)D, Wc, (long)D, nullptr, 0, nullptr, 0, n, Vc, D, 0, w.count};
-    const EpiProb epi{w.rsum + c0 / kRun, w.runs, w.P, (long)vchunk, c0, Vc, Nc8, w.ref, w.labels};
-    LPCK((launch_gemm_cfg<256, 256, 2, 2>(p, epi, s)));
+    auto logits = [&](auto stream) {
+      const EpiProb<decltype(stream)::value> epi{w.rsum + c0 / kRun, w.runs, w.P,   (long)vchunk, c0,
+                                                 Vc,                 Nc8,    w.ref, w.labels};
+      return launch_gemm_cfg<256, 256, 2, 2>(p, epi, s);
+    };
+    LPCK(n > 256 ? logits(std::false_type{}) : logits(std::true_type{}));
     // the head read in place as the [K, N] operand; each slice adds up its own partial
     GemmProblem h{w.P, (long)vchunk, Wc, (long)D, nullptr, 0, nullptr, 0, n, D, Nc8, 0, w.count};
     h.b_kn = 1;
     h.kb_rows = Vc;
-    LPCK((launch_gemm_cfg<256, 256, 2, 2>(h, lp_part(w, c0 > 0), s)));
+    LPCK((n > 256 ? launch_gemm_cfg<256, 256, 2, 2>(h, lp_part<false>(w, c0 > 0), s)
+                  : launch_gemm_cfg<256, 256, 2, 2>(h, lp_part<true>(w, c0 > 0), s)));
   }
   hipLaunchKernelGGL(lp_dh_kernel, dim3(n), dim3(256), 0, s, W, D, w, logp, dlogp, dH, lddh, out_f32);
   return hipGetLastError();
