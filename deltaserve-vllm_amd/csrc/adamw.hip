@@ -13,7 +13,10 @@
 // down at random in proportion to where it lies, and the mean moves as it should. It
 // is never rounded to 0 from above, where m / (0 + ε) would leap. The step uses m' and
 // v' before they are rounded. Blocks whose largest magnitude is below 2^-100 are held as
-// zeros.
+// zeros. The moments take the formula's operations one by one in fp32, each to nearest, so
+// that their codes are those that elementary operations give, bit for bit: a code on the
+// other side of where two meet (one in a million with fused operations) is a step of 6 to
+// 12 % that later updates show.
 //
 // A workgroup takes a chunk of 4096 elements, a wave 4 blocks, 16 lanes a block:
 // loads of 16 bytes a lane cover whole 256-byte runs, and the block's
@@ -317,12 +320,38 @@ DSB_DEV double block_sum64(double s, double* red) {
   for (int i = 0; i < NT / 64; ++i) s += red[i];
   return s;
 }
+template <int BITS>
 DSB_DEV float clip_factor(double norm, double max_norm) {
+  if constexpr (BITS == 8) {
+    const float c = 1.f / ((float)norm + 1e-6f) * (float)max_norm;
+    return c > 1.f ? 1.f : c;  // NaN stays
+  }
   const double c = max_norm / (norm + 1e-6);
-  return c > 1.0 ? 1.f : (float)c;  // NaN stays
+  return c > 1.0 ? 1.f : (float)c;
+}
+// x / s to nearest, from inv = 1 / s to nearest: what the product leaves over, times inv. (s and
+// the largest x are not near the smallest numbers, so that the rest is exact.)
+DSB_DEV float divided(float x, float s, float inv) {
+  const float q = x * inv;
+  return fmaf(fmaf(-q, s, x), inv, q);
+}
+// sqrt(v) to nearest: the instruction is off by at most a step, and a neighbour s' of its s is
+// the nearer one where v − s·s' says so (not with 0, infinity or NaN, where s stays).
+DSB_DEV float root(float v) {
+  const float s = __builtin_amdgcn_sqrtf(v);
+  const float down = __builtin_bit_cast(float, __builtin_bit_cast(int, s) - 1);
+  const float up = __builtin_bit_cast(float, __builtin_bit_cast(int, s) + 1);
+  const float below = fmaf(-down, s, v), above = fmaf(-up, s, v);
+  return above > 0.f ? up : below <= 0.f ? down : s;
+}
+// β·x + (1 − β)·y, every operation rounded.
+DSB_DEV float blend(float b, float x, float ob, float y) {
+#pragma clang fp contract(off)
+  return b * x + ob * y;
 }
 
 // One block per group: its chunks' sums in a fixed order, the norm and the factor.
+template <int BITS>
 __global__ __launch_bounds__(1024) void adam_norm_kernel(const int* __restrict__ group_chunks,
                                                          const double* __restrict__ partial,
                                                          double max_norm, float* __restrict__ norms,
@@ -335,7 +364,7 @@ __global__ __launch_bounds__(1024) void adam_norm_kernel(const int* __restrict__
   const double norm = sqrt(block_sum64<1024>(s, red));
   if (threadIdx.x == 0) {
     norms[blockIdx.x] = (float)norm;
-    coef[blockIdx.x] = clip_factor(norm, max_norm);
+    coef[blockIdx.x] = clip_factor<BITS>(norm, max_norm);
   }
 }
 
@@ -417,7 +446,7 @@ DSB_DEV void adam_chunk(const AdamKernelArgs& a, const dsb_adam_chunk& t, int ch
     cf = clip.coef[t.group];
   } else if (clip.how == CLIP_SUM) {
     const double norm = sqrt(block_sum64<kThreads>(mine, red));
-    cf = clip_factor(norm, clip.max_norm);
+    cf = clip_factor<BITS>(norm, clip.max_norm);
     if (chunk == t.c0 && threadIdx.x == 0) clip.norms[t.group] = (float)norm;
     if (chunk == 0)  // groups without elements
       for (int g = threadIdx.x; g < clip.ngroups; g += kThreads)
@@ -442,9 +471,8 @@ DSB_DEV void adam_chunk(const AdamKernelArgs& a, const dsb_adam_chunk& t, int ch
       const float gi = value(graw[k], i, gbf) * cf, wi = value(wraw[k], i, wbf);
       if constexpr (BITS == 8) {
         const float ro = r[k][i] * rs;
-        const float v = h.b2 * (ro * ro) + h.ob2 * (gi * gi);
-        m[k][i] = h.b1 * (m[k][i] * ms) + h.ob1 * gi;
-        r[k][i] = __builtin_amdgcn_sqrtf(v);
+        m[k][i] = blend(h.b1, m[k][i] * ms, h.ob1, gi);
+        r[k][i] = root(blend(h.b2, ro * ro, h.ob2, gi * gi));
         mtop = max(mtop, mag(m[k][i]));
         rtop = max(rtop, mag(r[k][i]));
         w[i] = wi * h.decay -
@@ -472,15 +500,15 @@ DSB_DEV void adam_chunk(const AdamKernelArgs& a, const dsb_adam_chunk& t, int ch
     const float mt = __builtin_bit_cast(float, max16(mtop));
     const float rt = __builtin_bit_cast(float, max16(rtop));
     // not below kTiny (so NaN and infinity show in the scale)
-    const float im = mt < kTiny ? 0.f : 448.f / mt;
-    const float ir = rt < kTiny ? 0.f : 448.f / rt;
+    const float unit = mt * (1.f / 448.f), im = mt < kTiny ? 0.f : 1.f / unit;
+    const float ir = rt < kTiny ? 0.f : 1.f / rt * 448.f;
     const unsigned key = mix32(h.key ^ mix32((unsigned)b));
 #pragma unroll
     for (int k = 0; k < G; ++k) {
       float q[E], p[E];
 #pragma unroll
       for (int i = 0; i < E; ++i) {
-        q[i] = fminf(fmaxf(m[k][i] * im, -448.f), 448.f);
+        q[i] = fminf(fmaxf(divided(m[k][i], unit, im), -448.f), 448.f);
         p[i] = fminf(r[k][i] * ir, 448.f);
       }
 #pragma unroll
@@ -499,7 +527,7 @@ DSB_DEV void adam_chunk(const AdamKernelArgs& a, const dsb_adam_chunk& t, int ch
       }
     }
     if (l16 == 0) {
-      a.m_scale[b] = mt < kTiny ? 0.f : mt * (1.f / 448.f);
+      a.m_scale[b] = mt < kTiny ? 0.f : unit;
       a.r_scale[b] = rt < kTiny ? 0.f : rt * (1.f / 448.f);
     }
   }
@@ -546,7 +574,7 @@ hipError_t adam_step(const AdamArgs& a, void* work, hipStream_t s) {
     // block reads one sum.
     c.how = a.most_chunks <= kThreads && a.nchunks > 0 ? CLIP_SUM : CLIP_GIVEN;
     if (c.how == CLIP_GIVEN)
-      hipLaunchKernelGGL(adam_norm_kernel, dim3(a.ngroups), dim3(1024), 0, s, a.group_chunks, partial,
+      hipLaunchKernelGGL(a.bits == 8 ? adam_norm_kernel<8> : adam_norm_kernel<32>, dim3(a.ngroups), dim3(1024), 0, s, a.group_chunks, partial,
                          a.max_norm, a.norms, coef);
   }
   const AdamKernelArgs k{a.chunks, hv, dev ? hp : nullptr, c, a.m, a.v, a.m_scale, a.r_scale};

@@ -746,6 +746,46 @@ def test_adamw(sizes, clip, dtypes, bits):
         assert all(torch.equal(a, b) for a, b in zip(gs, kept))
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("clip", [None, 0.01])
+def test_adamw_codes_of_elementary_operations(clip, dtype):
+    """8-bit moments, codes and scales, are bit for bit those of the formula taken in fp32 with every
+    operation rounded, step after step: no tolerance. (Quotients and roots in 64 bits, then in 32, are
+    rounded as one operation in 32 is: 53 bits are 2·24 + 2 and more.)"""
+    ops = _ops()
+    sizes = [(1 << 18) + 5, 333, 4096]
+    groups = [0, 0, 1]
+    ws, gs = _adam_inputs(sizes, (dtype, dtype), 29, 0)
+    opt = ops.AdamW(ws, gs, bits=8, groups=groups)
+    b1, b2 = 0.9, 0.999
+    for step in (1, 2, 3):
+        for i, x in enumerate(gs):
+            x.copy_(torch.randn(x.shape, generator=_gen(10 * step + i), device=DEV) * 10.0 ** (step - 4))
+        ref = Ref(opt, ws, gs, groups)
+        old = {k: v.float().cpu() for k, v in opt.state().items()}
+        hyper = dict(lr=1e-3, step=step, max_norm=clip, seed=5)
+        opt.step(**hyper)
+        ref.step(**hyper)
+        g = ref.g.float().cpu()
+        if clip is not None:
+            factor = ((1 / (ref.norms.float().cpu() + 1e-6).double()).float() * clip).clamp(max=1)
+            per = torch.repeat_interleave(torch.tensor(groups), torch.tensor([-(-n // 256) for n in sizes]))
+            g = g * factor[per, None]
+        m = b1 * (old["m"].view(-1, 256) * old["m_scale"][:, None]) + (1 - b1) * g
+        r = (old["r"].view(-1, 256) * old["r_scale"][:, None]).square()
+        r = (b2 * r + (1 - b2) * g.square()).double().sqrt().float()
+        unit = torch.tensor(1 / 448)
+        ms, top = m.abs().amax(1) * unit, r.amax(1)
+        want = torch.where(ms[:, None] > 0, m.double() / ms.double()[:, None], 0.0).float().clamp(-448, 448).to(F8).float()
+        x = torch.where(top[:, None] > 0, r * ((1 / top.double()).float() * 448)[:, None], 0.0).clamp(max=448).double()
+        grid = torch.ldexp(torch.ones_like(x), torch.frexp(x)[1].clamp(min=-5) - 4)
+        q = (torch.floor(x / grid + ref.unit.double().cpu()) * grid).clamp(2.0 ** -9, 448.0)
+        got = {k: v.float().cpu() for k, v in opt.state().items()}
+        assert torch.equal(got["m_scale"], ms) and torch.equal(got["r_scale"], top * unit)
+        assert torch.equal(got["m"].view(-1, 256), want)
+        assert torch.equal(got["r"].view(-1, 256), torch.where(x > 0, q, 0.0).float())
+
+
 @pytest.mark.parametrize("bits", [8, 32])
 def test_adamw_values_of_all_sizes(bits):
     """Blocks of zeros, of one value, of gradients over 12 decades; beta1 = 0, beta2 = 0."""
