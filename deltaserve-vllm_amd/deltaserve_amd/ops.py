@@ -372,10 +372,10 @@ class PackPlan:
 
     def __init__(self, seq_lens, device):
         lib = L.load()
-        lens = np.ascontiguousarray(seq_lens, dtype=np.int64).reshape(-1)
-        if lens.size and (lens.min() < 0 or lens.max() > 0x7fffffff):
-            raise ValueError("pack_plan: lengths must lie in [0, 2^31)")
-        lens = lens.astype(np.int32)
+        lens = np.asarray(seq_lens).reshape(-1)
+        if lens.size and (lens.dtype.kind not in "iu" or lens.min() < 0 or lens.max() > 0x7fffffff):
+            raise ValueError("pack_plan: lengths must be whole numbers in [0, 2^31)")
+        lens = np.ascontiguousarray(lens, dtype=np.int32)
         p = lens.ctypes.data_as(ctypes.POINTER(c_int32))
         c, elems, nbytes = L.DsbPackPlan(), c_int64(), c_int64()
         L.check(lib.dsb_plan_sizes(p, lens.size, byref(c), byref(elems)), what="dsb_plan_sizes")

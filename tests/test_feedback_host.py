@@ -203,6 +203,9 @@ def test_front_end_refusals():
     f, b = torch.zeros(4), torch.zeros(4, 8, dtype=torch.bfloat16)
     with pytest.raises(ValueError):
         ops.token_logprobs(b, b, torch.zeros(4, dtype=torch.int64))  # host tensors
+    for lens in ([1.5, 2.0], [3, -1], [1 << 31], ["3"], [True]):
+        with pytest.raises(ValueError):
+            ops.pack_plan(lens)
     with pytest.raises(ValueError):
         ops.token_logprobs(b.float(), b, torch.zeros(4, dtype=torch.int64))
     with pytest.raises(ValueError):

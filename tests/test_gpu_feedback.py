@@ -552,6 +552,23 @@ def test_losses_at_odd_addresses():
         assert n == plan.n
 
 
+@pytest.mark.parametrize("lens", [LENS["ragged"], LENS["tiles"], LENS["crowd"]], ids=["ragged", "tiles", "crowd"])
+def test_any_byte_but_zero_is_set(lens):
+    ops = _ops()
+    plan, seq, mask, logp, old, ref, A = _packing(lens, 19, 4)
+    n = len(logp)
+    byte = torch.randint(1, 256, (n,), generator=_gen(5), device=DEV).to(torch.uint8)
+    byte[::5], byte[1::5] = 128, 1
+    byte = byte * mask
+    ids = torch.arange(n, device=DEV)
+    for f in (lambda m: ops.preference_loss(logp, ref, plan, mask=m),
+              lambda m: ops.policy_loss(logp, old, A, plan, mask=m, ref_logp=ref, kl_coef=0.1),
+              lambda m: ops.policy_loss(logp, old, A, plan, mask=m, reduction="sequence"),
+              lambda m: ops.next_token_labels(ids, plan, m)):
+        for x, y in zip(f(byte), f(mask)):
+            assert torch.equal(x, y)
+
+
 def test_losses_captured_and_on_a_side_stream():
     ops = _ops()
     for lens in (LENS["ragged"], LENS["long"]):
