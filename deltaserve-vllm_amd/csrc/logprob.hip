@@ -35,7 +35,7 @@ constexpr long kMaxChunk = 1L << 21;
 // rows at 1024 wide (122 µs against 142 for 128 × 128 forward, 229 against 195 backward).
 constexpr int kRun = 128;  // columns of a wave's tile
 // K slices of the dH product, most: 8 tiles (500 rows × 1024) fill the CUs 32 times
-// (349 µs; 16 slices 414, 8 580).
+// (349 µs; 16 slices 414, 8 580; before the probabilities' stores went past the caches).
 constexpr int kMaxSlices = 32;
 
 // An accumulator's value, read from its AGPR here: left to itself the compiler reads all 256
@@ -206,7 +206,10 @@ struct EpiProb {
         const int c = lane + 64 * it, row = c / CG, m = mw + b * 32 + row;
         const int n = nw + (c % CG) * 8;
         const u32x4 v = *reinterpret_cast<const u32x4*>(buf + row * PITCH + (c % CG) * 8);
-        if (m < M && n < Nc8) stg128(P + (long)m * ldp + n, v);
+        // past the caches: the next tiles' panels stay (500 rows × 1024 × 151936: 334 → 322 µs;
+        // the dH product's accumulators, read at once, lose by it: 347)
+        if (m < M && n < Nc8)
+          __builtin_nontemporal_store(v, reinterpret_cast<u32x4*>(P + (long)m * ldp + n));
       }
     }
   }
