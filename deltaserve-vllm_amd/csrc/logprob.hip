@@ -37,6 +37,10 @@ constexpr int kRun = 128;  // columns of a wave's tile
 // K slices of the dH product, most: 8 tiles (500 rows × 1024) fill the CUs 32 times
 // (349 µs; 16 slices 414, 8 580; before the probabilities' stores went past the caches).
 constexpr int kMaxSlices = 32;
+// Up to this many rows each block of the gather counts the scored rows before its own, which
+// saves a launch (1024 × 151936, forward: 504 rows 162 → 158 µs, 1024 226 → 224; 2048, as
+// many rows to count, 424 → 421, its gradient 829 → 833).
+constexpr int kAloneRows = 1024;
 
 // An accumulator's value, read from its AGPR here: left to itself the compiler reads all 256
 // at the start of the epilogue and spills what else is live. (volatile: stays behind the
@@ -306,8 +310,12 @@ LPWork lp_layout(int n, int D, int V, bool backward, void* base, size_t* bytes) 
 
 }  // namespace
 
-// Single block, four rows to a thread: the scored rows' indices in order and their count. A
-// row is scored when 0 <= label < V and, with dlogp, dlogp ≠ 0 and logp < 0 (NaN: scored).
+// A row is scored (0) when 0 <= label < V and, with dlogp, dlogp ≠ 0 and logp < 0 (NaN: scored);
+// −2: its label is past V, −1 otherwise.
+DSB_DEV int lp_state(int64_t lab, int V, float g, float p) {
+  return lab < 0 || g == 0.f ? -1 : lab >= V ? -2 : p >= 0.f ? -1 : 0;
+}
+// Single block, four rows to a thread: the scored rows' indices in order and their count.
 // Without dlogp the other rows' outputs are written here: 0, or NaN for a label past V.
 __global__ __launch_bounds__(1024) void lp_rows_kernel(const int64_t* __restrict__ labels, int n,
                                                        int V, const float* __restrict__ dlogp,
@@ -331,7 +339,7 @@ __global__ __launch_bounds__(1024) void lp_rows_kernel(const int64_t* __restrict
     int state[4], mine = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      state[i] = lab[i] < 0 || g[i] == 0.f ? -1 : lab[i] >= V ? -2 : p[i] >= 0.f ? -1 : 0;
+      state[i] = lp_state(lab[i], V, g[i], p[i]);
       mine += state[i] == 0;
     }
     int before = mine;  // of the wave's lanes up to this one
@@ -366,16 +374,44 @@ __global__ __launch_bounds__(1024) void lp_rows_kernel(const int64_t* __restrict
 }
 
 // One block per scored row: the row copied to its place, its label, and its softmax
-// reference: forward the dot with W[label], backward the forward's `other`.
+// reference: forward the dot with W[label], backward the forward's `other`. ALONE: one
+// per row, with lp_rows_kernel's part for it.
+template <bool ALONE>
 __global__ __launch_bounds__(256) void lp_gather_kernel(const bf16* __restrict__ H, long ldh,
                                                         const bf16* __restrict__ W,
-                                                        const int64_t* __restrict__ labels, int D,
+                                                        const int64_t* __restrict__ labels, int n,
+                                                        int D, int V,
+                                                        const float* __restrict__ dlogp,
+                                                        const float* __restrict__ logp_in,
                                                         const float* __restrict__ other,
-                                                        LPWork w) {
+                                                        float* __restrict__ logp_out,
+                                                        float* __restrict__ other_out, LPWork w) {
   __shared__ float red[4];
-  const int m = blockIdx.x;
-  if (m >= *w.count) return;
-  const int r = w.rows[m], lab = (int)labels[r];
+  int m = blockIdx.x, r = m;
+  if constexpr (ALONE) {
+    auto state = [&](int q) {
+      return lp_state(labels[q], V, dlogp ? dlogp[q] : 1.f, dlogp ? logp_in[q] : -1.f);
+    };
+    const int mine = state(r);
+    float before = 0.f;  // exact
+#pragma unroll
+    for (int i = 0; i < kAloneRows / 256; ++i) {
+      const int q = 256 * i + threadIdx.x;
+      if (q < r) before += state(q) == 0 ? 1.f : 0.f;
+    }
+    m = (int)block_sum<256>(before, red);
+    if (threadIdx.x == 0) {
+      w.place[r] = mine == 0 ? m : mine;
+      if (mine == 0) w.rows[m] = r;
+      if (r == n - 1) *w.count = m + (mine == 0);
+      if (mine < 0 && !dlogp) logp_out[r] = other_out[r] = mine == -2 ? NAN : 0.f;
+    }
+    if (mine < 0) return;
+  } else {
+    if (m >= *w.count) return;
+    r = w.rows[m];
+  }
+  const int lab = (int)labels[r];
   const bf16 *x = H + (long)r * ldh, *wt = W + (long)lab * D;
   bf16* o = w.X + (long)m * D;
   float dot = 0.f;
@@ -510,6 +546,20 @@ int64_t logprob_bytes(int n, int D, int V, bool backward) {
     if (_e != hipSuccess) return _e;     \
   } while (0)
 
+// The scored rows, gathered.
+static hipError_t lp_gather(const bf16* H, long ldh, const bf16* W, const int64_t* labels, int n,
+                            int D, int V, const float* dlogp, const float* logp,
+                            const float* other, float* logp_out, float* other_out,
+                            const LPWork& w, hipStream_t s) {
+  if (n > kAloneRows)
+    hipLaunchKernelGGL(lp_rows_kernel, dim3(1), dim3(1024), 0, s, labels, n, V, dlogp, logp, logp_out,
+                       other_out, w);
+  hipLaunchKernelGGL(n > kAloneRows ? lp_gather_kernel<false> : lp_gather_kernel<true>, dim3(n),
+                     dim3(256), 0, s, H, ldh, W, labels, n, D, V, dlogp, logp, other, logp_out,
+                     other_out, w);
+  return hipGetLastError();
+}
+
 // Over one block of rows (n <= 256) each block of the products reads columns of the head of its
 // own: past the caches (µs, through them → past them: 149 rows × 5120 × 151936 forward 349 → 335,
 // gradient 711 → 690; 113 × 4096 × 128256 219 → 214, 443 → 429).
@@ -517,11 +567,7 @@ hipError_t token_logprobs(const bf16* normed, long ldh, const bf16* W, const int
                           int D, int V, float* logp, float* other, void* work, hipStream_t s) {
   size_t bytes = 0;
   const LPWork w = lp_layout(n, D, V, false, work, &bytes);
-  hipLaunchKernelGGL(lp_rows_kernel, dim3(1), dim3(1024), 0, s, labels, n, V,
-                     (const float*)nullptr, (const float*)nullptr, logp, other, w);
-  hipLaunchKernelGGL(lp_gather_kernel, dim3(n), dim3(256), 0, s, normed, ldh, W, labels, D,
-                     (const float*)nullptr, w);
-  LPCK(hipGetLastError());
+  LPCK(lp_gather(normed, ldh, W, labels, n, D, V, nullptr, nullptr, nullptr, logp, other, w, s));
   const int V1 = V - w.narrow;
   GemmProblem p{w.X, (long)D, W, (long)D, nullptr, 0, nullptr, 0, n, V1, D, 0, w.count};
   if (n > 256) {
@@ -549,10 +595,7 @@ hipError_t token_logprobs_bwd(const bf16* normed, long ldh, const bf16* W, const
                               hipStream_t s) {
   size_t bytes = 0;
   const LPWork w = lp_layout(n, D, V, true, work, &bytes);
-  hipLaunchKernelGGL(lp_rows_kernel, dim3(1), dim3(1024), 0, s, labels, n, V, dlogp, logp,
-                     (float*)nullptr, (float*)nullptr, w);
-  hipLaunchKernelGGL(lp_gather_kernel, dim3(n), dim3(256), 0, s, normed, ldh, W, labels, D, other, w);
-  LPCK(hipGetLastError());
+  LPCK(lp_gather(normed, ldh, W, labels, n, D, V, dlogp, logp, other, nullptr, nullptr, w, s));
   const int vchunk = w.plan.vchunk;
   for (int c0 = 0; c0 < V; c0 += vchunk) {
     const int Vc = std::min(vchunk, V - c0), Nc8 = (Vc + 7) / 8 * 8;

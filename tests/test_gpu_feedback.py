@@ -198,6 +198,34 @@ def test_logprobs_of_labels_past_the_vocabulary():
     assert torch.equal(dh[keep], ops.token_logprobs_backward(H, W, lab, *want, d)[keep])
 
 
+@pytest.mark.parametrize("n", [1023, 1024, 1025])
+def test_logprobs_where_the_rows_are_counted_otherwise(n):
+    """Scored rows, rows left out and labels past the vocabulary are the same on both sides of the size
+    from which a kernel of its own counts the rows."""
+    ops = _ops()
+    V = 500
+    H, W, lab = _head_inputs(n, 64, V, 3, "some")
+    lab[5::11] = V
+    d = torch.randn(n, generator=_gen(4), device=DEV)
+    d[::7] = 0.0
+    logp, other = ops.token_logprobs(H, W, lab)
+    got = ops.token_logprobs_backward(H, W, lab, logp, other, d, F32)
+    e_logp, e_other, _ = _head_exact(H, W, lab.clamp(max=V - 1))
+    _, tol = _head_tol(H, W)
+    past, live = lab >= V, (lab >= 0) & (lab < V)
+    assert logp[past].isnan().all() and other[past].isnan().all()
+    assert (logp[lab < 0] == 0).all() and (other[lab < 0] == 0).all()
+    _within(logp[live], e_logp[live], (tol + 4 * U32 * e_logp.abs())[live])
+    assert got[past & (d != 0)].isnan().all() and (got[(lab < 0) | (d == 0)] == 0).all()
+    k = 300  # a shorter batch of the same rows, each row's gradient the same
+    few = ops.token_logprobs_backward(H[:k], W, lab[:k], logp[:k], other[:k], d[:k], F32)
+    rows = ((live & (d != 0))[:k]).nonzero()[:, 0]
+    assert len(rows) > 50
+    # sums of V terms in another order, of parts of at most |d| and |d|·|W| times 1 − p
+    size = d[:k][rows, None].double().abs() * W.double().abs().max()
+    _within(few[rows], got[:k][rows].double(), 4 * (V + 8) * U32 * size)
+
+
 def test_logprobs_leave_unscored_rows_out():
     """NaN in an unscored row stays there, and a row's results do not depend on which others are
     scored beyond the tiles' sums (compared against a call on the scored rows alone)."""
