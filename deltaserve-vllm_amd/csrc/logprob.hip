@@ -20,9 +20,13 @@ namespace dsb {
 
 namespace {
 
-// Limit on a run's Σ exp(logit − ref), as for the cross-entropy head: above it
-// (a logit more than about 40 over the label's) the run takes its own maximum.
-constexpr float kRunLimit = 0x1p57f;
+// Bounds on a run's Σ exp(logit − ref), ref being about the label's logit: past them (a logit
+// more than about 40 over the label's, or all more than about 44 under it) the run takes its own
+// maximum, the label's left out. Above the lower one what underflows in a run, 128 terms below
+// 2^-126, is less than 2^-55 of its sum.
+constexpr float kRunLimit = 0x1p57f, kRunFloor = 0x1p-64f;
+constexpr float kRefOver = 39.5f, kRefUnder = -44.4f;  // ln of the two
+constexpr float kNoWord = -0x1p126f;  // under every logit
 
 // Probabilities held at a time: 1 GiB of bf16. Fewer chunks have fewer half-filled last
 // rounds of tiles and read and write the dH accumulators less often.
@@ -52,7 +56,7 @@ DSB_DEV float acc_read(const float& a) {
 }
 
 struct LPStat {
-  float ref, sum;  // Σ exp(logit − ref) over a run, the label left out
+  float ref, sum;  // Σ exp(logit − ref) over a run, the label left out; 0: no other word in it
 };
 
 // Per run of TN columns and row: LPStat into stats[run · cap + m] (the 16 rows of
@@ -96,10 +100,13 @@ struct EpiLogProb {
         for (int fn = 0; fn < FN; ++fn)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            float e = __expf(acc_read(acc[fm][fn][i]) - r);
+            float x = acc_read(acc[fm][fn][i]) - r;
+            // the label's own column by a factor of 0 (as tests the masks of 128 columns spill):
+            // it may be any height above r, so its e is bounded (the others' are below the bound;
+            // a NaN stays)
+            if (decltype(skips)::value) x = x > 64.f ? 64.f : x;
+            float e = __expf(x);
             if (!whole) e = nw + fn * 16 + 4 * lq + i < V ? e : 0.f;
-            // the label's own column (whose e is at most about 1, r being its logit or more) by
-            // a factor of 0: as tests the masks of 128 columns spill
             if (decltype(skips)::value) e *= fminf(fabsf((float)(fn * 16 + i) - tl), 1.f);
             part[i] += e;
           }
@@ -109,21 +116,25 @@ struct EpiLogProb {
       };
       const int m = mw + fm * 16 + l16;
       LPStat st = take(ref0, std::false_type{});
-      if (__any(!(st.sum <= kRunLimit) || (unsigned)tc < (unsigned)TN)) {
-        // rare: a row with its label in the run, or past the limit
-        float v = -INFINITY, xt = 0.f;
+      if (__any(!(st.sum <= kRunLimit && st.sum >= kRunFloor) || (unsigned)tc < (unsigned)TN)) {
+        // rare: a row with its label in the run, or past the bounds; v: the most of the others (the
+        // label's column by kNoWord under it, as tests the masks spill)
+        float v = kNoWord, xt = 0.f;
 #pragma unroll
         for (int fn = 0; fn < FN; ++fn)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float x = acc_read(acc[fm][fn][i]);
-            v = whole || nw + fn * 16 + 4 * lq + i < V ? fmaxf(v, x) : v;
-            xt = (float)(fn * 16 + i) == tl ? x : xt;
+            const float at = (float)(fn * 16 + i);
+            const float u = x + fmaf(fminf(fabsf(at - tl), 1.f), -kNoWord, kNoWord);
+            v = whole || nw + fn * 16 + 4 * lq + i < V ? fmaxf(v, u) : v;
+            xt = at == tl ? x : xt;
           }
         if ((unsigned)tc < (unsigned)TN && ((tc >> 2) & 3) == lq && m < M) tgt[m] = xt;
         v = fmaxf(v, __shfl_xor(v, 16, 64));
         v = fmaxf(v, __shfl_xor(v, 32, 64));
-        st = take(st.sum <= kRunLimit ? st.ref : fmaxf(st.ref, v), std::true_type{});
+        const bool moves = v > ref0 + kRefOver || (v < ref0 + kRefUnder && v > 0.5f * kNoWord);
+        st = take(moves ? v : ref0, std::true_type{});
       }
       if (lq == 0 && m < M) out[m] = st;
       // one fragment's values at a time: with several in flight the registers spill
@@ -444,7 +455,7 @@ __global__ __launch_bounds__(1024) void lp_finish_kernel(LPWork w, int cap,
   const int M = *w.count;
   if ((int)blockIdx.x * 16 >= M) return;  // uniform
   const float ref = m < M ? w.ref[m] : 0.f;
-  float mx = ref, L = 0.f;
+  float mx = -INFINITY, L = 0.f;
   if (m < M) {
     bool other_ref = false;
 #pragma unroll 8
@@ -453,10 +464,13 @@ __global__ __launch_bounds__(1024) void lp_finish_kernel(LPWork w, int cap,
       L += s.sum;
       other_ref |= s.ref != ref;
     }
-    if (other_ref) {
+    if (!other_ref) {
+      mx = L == 0.f ? mx : ref;
+    } else {
       L = 0.f;
       for (int t = part; t < w.runs; t += 64) {
         const LPStat s = w.stats[(long)t * cap + m];
+        if (s.sum == 0.f) continue;  // no word but the label: its reference is none
         const float mn = fmaxf(mx, s.ref);
         L = L * __expf(mx - mn) + s.sum * __expf(s.ref - mn);
         mx = mn;
@@ -469,14 +483,16 @@ __global__ __launch_bounds__(1024) void lp_finish_kernel(LPWork w, int cap,
   if (part >= 4) return;  // the first wave: 4 threads to a row, in a fixed order
   for (int k = 0; k < 64; ++k) mx = fmaxf(mx, ms[k][i]);
   L = 0.f;
-  for (int k = part; k < 64; k += 4) L += ls[k][i] * __expf(ms[k][i] - mx);
+  for (int k = part; k < 64; k += 4) L += ls[k][i] == 0.f ? 0.f : ls[k][i] * __expf(ms[k][i] - mx);
   L += __shfl_xor(L, 16, 64);
   L += __shfl_xor(L, 32, 64);
   if (part || m >= M) return;
   const float xt = w.tgt[m], d = xt - mx, et = __expf(d);
   const int r = w.rows[m];
-  // log(1 + L/e_t), exact in L where the sum would round it away
-  logp[r] = -(L < et ? log1pf(L / et) : logf(et + L) - d);
+  // log(1 + L/e_t), exact in L where the sum would round it away; 1/e_t in two factors, as it
+  // underflows before the quotient where the label is far above the rest (e_t infinite)
+  const float h = __expf(-0.5f * d);
+  logp[r] = -(L < et ? log1pf(L * h * h) : logf(et + L) - d);
   other[r] = mx + logf(L);
 }
 

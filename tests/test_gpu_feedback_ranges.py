@@ -1,0 +1,76 @@
+"""The operators for training from feedback at the ends of their ranges: labels far above the
+other words. Against the formulas in 64 bits; U32 and U16 as in test_gpu_feedback."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from test_gpu_feedback import BF16, DEV, F32, U16, U32, _gen, _head_exact, _head_tol, _ops, _within
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _dev():
+    if not torch.cuda.is_available():
+        pytest.skip("no HIP device")
+
+
+# ---------------------------------------------------------------- log probabilities
+
+def _leads(n, V, label, seed, near=None):
+    """Rows whose label lies from 160 logits below to 160 above the other words (about 0 each); near:
+    another word that lies that far below the label where that is above the rest."""
+    D, g = 64, _gen(seed)
+    W = torch.zeros(V, D, device=DEV)
+    W[:, 2:] = torch.randn(V, D - 2, generator=g, device=DEV) * 0.05
+    W[label, 0] = 1
+    H = torch.randn(n, D, generator=g, device=DEV)
+    H[:, 0] = torch.linspace(-160, 160, n, device=DEV)
+    H[:, 1] = 0
+    if near is not None:
+        W[near[0], 1] = 1
+        H[:, 1] = H[:, 0] - near[1]
+    return H.to(BF16), W.to(BF16), torch.full((n,), label, device=DEV)
+
+
+# label in the first, a middle and the last place; alone in the last run of 128 columns (129, 257); past
+# 65536 words a narrower product takes the last ones of up to 256 rows
+LEADS = [(200, 2, 0, None), (200, 2, 1, None), (200, 31, 4, None), (200, 128, 127, None), (200, 129, 128, None),
+         (300, 257, 256, None), (200, 777, 5, (6, 84.0)), (200, 777, 5, (700, 60.0)), (300, 5000, 4321, (17, 92.0)),
+         (130, 70001, 69999, None), (130, 70001, 40000, (41, 84.0)), (300, 70001, 3, (65900, 100.0))]
+
+
+@pytest.mark.parametrize("n,V,label,near", LEADS)
+def test_logprobs_of_labels_far_above_the_rest(n, V, label, near):
+    """other is the plain log-sum-exp however far the label leads, and logp keeps its relative precision
+    down to the smallest normal number."""
+    ops = _ops()
+    H, W, lab = _leads(n, V, label, V + label, near)
+    logp, other = ops.token_logprobs(H, W, lab)
+    e_logp, e_other, q = _head_exact(H, W, lab)
+    ex, tol = _head_tol(H, W)
+    _within(other, e_other, tol + 4 * U32 * e_other.abs())
+    # the exponent other − x_t: both numbers' errors; and its own two halves' (256·U32)
+    rel = ex + tol + (256 + 8) * U32
+    _within(logp, e_logp, rel * e_logp.abs() + 2.0 ** -126)
+    d = torch.ones(n, device=DEV)
+    got = ops.token_logprobs_backward(H, W, lab, logp, other, d, out_dtype=F32)
+    W64 = W.double()
+    want = -e_logp.expm1()[:, None] * (W64[label] - q @ W64)
+    spread = -e_logp.expm1()[:, None] * (q @ W64.abs() + W64[label].abs())
+    _within(got, want, (2 * (U16 + ex + tol + e_other.abs() * U32 + 256 * U32) + 1024 * U32 + rel)[:, None] * spread
+            + 2.0 ** -120)
+
+
+@pytest.mark.parametrize("n", [40, 300])
+@pytest.mark.parametrize("word", [3, 100, 300])
+def test_logprobs_show_words_that_are_not_numbers(n, word):
+    """A NaN among the head's words is seen in every row, whether its run holds the label, leads or
+    neither."""
+    ops = _ops()
+    H, W, lab = _leads(n, 400, 5, 1)
+    W[word] = float("nan")
+    logp, other = ops.token_logprobs(H, W, lab)
+    assert logp.isnan().all() and other.isnan().all()
