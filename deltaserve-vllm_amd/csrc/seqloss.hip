@@ -485,7 +485,9 @@ DSB_DEV RowOut policy_row(const PolicyHyper& h, float lp, float old, float ref, 
   o.grad = o.clipped ? 0.f : -gain;
   o.kl = 0.f;
   if (has_ref) {
+    // with a coefficient of 0 only the KL itself is wanted, and may be infinite
     const float u = (float)((double)ref - (double)lp);
+    float dkl;
     if (h.kl == DSB_KL_K3) {
       float em1, val;
       if (fabsf(u) < 1.f) {
@@ -503,14 +505,15 @@ DSB_DEV RowOut policy_row(const PolicyHyper& h, float lp, float old, float ref, 
         em1 = u + val;
       } else {
         em1 = expf(u) - 1.f;
-        val = em1 - u;
+        val = em1 == INFINITY ? em1 : em1 - u;
       }
       o.kl = val;
-      o.grad -= h.kl_coef * em1;
+      dkl = em1;
     } else {
       o.kl = 0.5f * u * u;
-      o.grad -= h.kl_coef * u;
+      dkl = u;
     }
+    if (h.kl_coef != 0.f) o.grad -= h.kl_coef * dkl;
   }
   return o;
 }
@@ -567,7 +570,7 @@ DSB_DEV void policy_rows4(const PolicyIn& in, const int* starts, const PolicyHyp
 // {loss, policy, kl, clipped share}
 DSB_DEV void policy_out(float* out, const PolicyHyper& h, double pol, double kl, double clipped,
                         double count) {
-  out[0] = (float)(pol + (double)h.kl_coef * kl);
+  out[0] = (float)(h.kl_coef != 0.f ? pol + (double)h.kl_coef * kl : pol);
   out[1] = (float)pol;
   out[2] = (float)kl;
   out[3] = count > 0 ? (float)(clipped / count) : 0.f;

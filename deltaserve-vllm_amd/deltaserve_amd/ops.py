@@ -517,8 +517,8 @@ def policy_loss(logp, old_logp, adv, plan, mask=None, ref_logp=None, clip_low=0.
     (mean over scored rows), "sequence" (mean over the sequences that have some, of their rows'
     mean) or "sum" (sum / divisor). Returns fp32 (loss = policy + kl_coef·kl; stats [3] = policy, kl,
     the share of scored rows whose ratio is clipped; dlogp [n] = grad_scale·dloss/dlogp). Without
-    scored rows all are 0. As the formula has it, an infinite ratio with an advantage of 0 gives
-    NaN."""
+    scored rows all are 0. With kl_coef = 0 ref_logp enters the KL statistic alone, also where its term
+    is infinite. As the formula has it, an infinite ratio with an advantage of 0 gives NaN."""
     what = "policy_loss"
     if kl not in L.KL_KINDS:
         raise ValueError(f"{what}: kl is one of {', '.join(L.KL_KINDS)}")

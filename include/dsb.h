@@ -463,7 +463,8 @@ int dsb_op_preference_loss(const float* logp, const float* ref, const uint8_t* m
  * _SEQUENCE (mean over the sequences with scored rows of their rows' mean) or _SUM
  * (sum / divisor). adv is fp32 [n] (adv_rows) or [nseq]. Writes out[4] = {policy +
  * kl_coef·kl, policy, kl, share of scored rows whose ratio is clipped} and dlogp [n] =
- * grad_scale · d out[0] / dlogp. */
+ * grad_scale · d out[0] / dlogp. With kl_coef = 0 the reference enters out[2] alone, also where
+ * its term is infinite. */
 enum { DSB_KL_K3 = 0, DSB_KL_K2 = 1 };
 enum { DSB_REDUCE_TOKEN = 0, DSB_REDUCE_SEQUENCE = 1, DSB_REDUCE_SUM = 2 };
 int dsb_op_policy_loss(const float* logp, const float* old_logp, const float* ref,

@@ -1,12 +1,13 @@
 """The operators for training from feedback at the ends of their ranges: labels far above the
-other words. Against the formulas in 64 bits; U32 and U16 as in test_gpu_feedback."""
+other words, KL terms of weight 0. Against the formulas in 64 bits; U32 and U16 as in test_gpu_feedback."""
 
 from __future__ import annotations
 
 import pytest
 import torch
 
-from test_gpu_feedback import BF16, DEV, F32, U16, U32, _gen, _head_exact, _head_tol, _ops, _within
+from test_gpu_feedback import BF16, DEV, F32, U16, U32, _gen, _head_exact, _head_tol, _ops, \
+    _packing, _within
 
 pytestmark = pytest.mark.gpu
 
@@ -74,3 +75,33 @@ def test_logprobs_show_words_that_are_not_numbers(n, word):
     W[word] = float("nan")
     logp, other = ops.token_logprobs(H, W, lab)
     assert logp.isnan().all() and other.isnan().all()
+
+
+# ---------------------------------------------------------------- policy loss
+
+@pytest.mark.parametrize("lens", [[40, 3, 61], [5000, 20, 6000]], ids=["small", "large"])
+@pytest.mark.parametrize("reduction", ["token", "sequence", "sum"])
+@pytest.mark.parametrize("kl", ["k3", "k2"])
+def test_policy_loss_watches_a_kl_of_weight_0(lens, reduction, kl):
+    """With kl_coef = 0 the reference enters the second statistic alone, also where its term is
+    infinite."""
+    ops = _ops()
+    plan, seq, mask, logp, old, A = _packing(lens, 3, 3)
+    logp, old = logp - 100, old - 100
+    ref = logp + 0.3
+    rows = mask.nonzero()[:, 0]
+    ref[rows[2]] = logp[rows[2]] + 95
+    kw = dict(mask=mask, reduction=reduction, kl=kl)
+
+    def same(logp):
+        loss, stats, d = ops.policy_loss(logp, old, A, plan, ref_logp=ref, **kw)
+        want = ops.policy_loss(logp, old, A, plan, **kw)
+        assert loss.isfinite() and d.isfinite().all()
+        assert torch.equal(loss, want[0]) and torch.equal(d, want[2])
+        assert torch.equal(stats[[0, 2]], want[1][[0, 2]])
+        return stats[1]
+
+    seen = same(logp)
+    assert seen.isinf() if kl == "k3" else seen.isfinite() and seen > 0
+    logp[rows[5]] = -float("inf")  # of probability 0
+    assert same(logp).isinf()
