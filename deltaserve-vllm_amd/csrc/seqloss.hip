@@ -473,12 +473,19 @@ struct RowOut {
 };
 // One scored row. The border tests take logp − old in 64 bits, where it is exact.
 // e^u − 1 − u cancels for small u: |u| < 1 takes u²·Σ u^k / (k + 2)! (k <= 9, off by
-// 2^-24), which gives e^u − 1 = u + that too.
+// 2^-24), which gives e^u − 1 = u + that too. PAST: as in policy_rows4.
+template <bool PAST>
 DSB_DEV RowOut policy_row(const PolicyHyper& h, float lp, float old, float ref, bool has_ref,
                           float A) {
   RowOut o;
   const double d = (double)lp - (double)old;
-  const float rho = expf((float)d), gain = rho * A;
+  const float rho = expf((float)d);
+  float gain = rho * A;
+  if (PAST && rho == INFINITY && d < INFINITY) {
+    // the product may be 0 or small: e^d = 2^k · 2^f, k last
+    const double t = d * 1.4426950408889634074, k = rint(t);
+    gain = ldexpf(exp2f((float)(t - k)) * A, (int)fmin(k, 1e6));
+  }
   const bool high = d > h.log_high && A > 0.f, low = d < h.log_low && A < 0.f;
   o.clipped = high || low;
   o.pol = -(high ? h.high * A : low ? h.low * A : gain);
@@ -539,8 +546,10 @@ struct PolicyIn {
   }
 };
 // Rows r .. r+k-1 of the batch, in sequences [lo, hi] of `starts`. weight(seq): a scored row's
-// weight in the loss.
-template <class K, class W>
+// weight in the loss. PAST: the ratio may be past fp32. Where one was, the thread's policy sum is not a
+// finite number and its rows are gone over again (tested in each row or group, 16 M rows take
+// 1.2 to 1.4 µs more).
+template <bool PAST, class K, class W>
 DSB_DEV void policy_rows4(const PolicyIn& in, const int* starts, const PolicyHyper& h, int r, K k,
                           const Rows& x, int lo, int hi, bool need_seq, W&& weight, float* dlogp,
                           PolicySums& sums) {
@@ -554,8 +563,8 @@ DSB_DEV void policy_rows4(const PolicyIn& in, const int* starts, const PolicyHyp
     if (need_seq)
       while (r + i >= end) end = starts[++seq + 1];
     if (in.mask ? m >> i & 1 : r + i + 1 < end) {
-      const RowOut o = policy_row(h, x.lp[i], x.old[i], x.ref[i], in.ref != nullptr,
-                                  in.adv_rows ? x.adv[i] : in.adv[seq]);
+      const RowOut o = policy_row<PAST>(h, x.lp[i], x.old[i], x.ref[i], in.ref != nullptr,
+                                        in.adv_rows ? x.adv[i] : in.adv[seq]);
       const float w = weight(seq);
       g[i] = w * o.grad * (float)h.grad_scale;
       sums.pol += (double)w * (double)o.pol;
@@ -640,14 +649,22 @@ __global__ __launch_bounds__(1024) void policy_small_kernel(PolicyIn in, dsb_pac
     return by_seq ? (float)(1.0 / ((double)max(cnt[s], 1) * fmax(nonempty, 1.0))) : all;
   };
   PolicySums sums;
+  auto rows = [&](auto past) {
+    constexpr bool PAST = decltype(past)::value;
+    sums = PolicySums{};
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int r = 4 * (tid + 1024 * j);
-    if (left[j] == 4)
-      policy_rows4(in, starts, h, r, Int<4>{}, x[j], 0, p.nseq - 1, need_seq, weight, dlogp, sums);
-    else if (left[j] > 0)
-      policy_rows4(in, starts, h, r, left[j], x[j], 0, p.nseq - 1, need_seq, weight, dlogp, sums);
-  }
+    for (int j = 0; j < 2; ++j) {
+      const int r = 4 * (tid + 1024 * j);
+      if (left[j] == 4)
+        policy_rows4<PAST>(in, starts, h, r, Int<4>{}, x[j], 0, p.nseq - 1, need_seq, weight, dlogp,
+                           sums);
+      else if (left[j] > 0)
+        policy_rows4<PAST>(in, starts, h, r, left[j], x[j], 0, p.nseq - 1, need_seq, weight, dlogp,
+                           sums);
+    }
+  };
+  rows(std::false_type{});
+  if (!(fabs(sums.pol) < INFINITY)) rows(std::true_type{});
   double v[4] = {sums.pol, sums.kl, (double)sums.clipped, (double)sums.count};
   block_sums<1024>(v, red);
   if (tid == 0) policy_out(out, h, v[0], v[1], v[2], v[3]);
@@ -736,11 +753,17 @@ __global__ __launch_bounds__(256) void policy_kernel(PolicyIn in, dsb_pack_plan 
   const int r0 = blockIdx.x * kChunkRows, r1 = min(p.n - r0, kChunkRows) + r0;
   // rows are read once, past the caches (16 M rows with a reference and advantages by row: 80.9
   // → 70.6 µs; the gradients past them too 72.3)
-  for_rows<256, 2>(
-      r0, r1, threadIdx.x, [&](int r, auto k) { return in.load<true>(r, k); },
-      [&](int r, auto k, const Rows& x) {
-        policy_rows4(in, p.starts, h, r, k, x, lo, hi, need_seq, weight, dlogp, sums);
-      });
+  auto rows = [&](auto past) {
+    sums = PolicySums{};
+    for_rows<256, 2>(
+        r0, r1, threadIdx.x, [&](int r, auto k) { return in.load<true>(r, k); },
+        [&](int r, auto k, const Rows& x) {
+          policy_rows4<decltype(past)::value>(in, p.starts, h, r, k, x, lo, hi, need_seq, weight,
+                                              dlogp, sums);
+        });
+  };
+  rows(std::false_type{});
+  if (!(fabs(sums.pol) < INFINITY)) rows(std::true_type{});
   double v[4] = {sums.pol, sums.kl, (double)sums.clipped, (double)sums.count};
   block_sums<256>(v, red4);
   if (threadIdx.x == 0)

@@ -1,5 +1,6 @@
 """The operators for training from feedback at the ends of their ranges: labels far above the
-other words, KL terms of weight 0. Against the formulas in 64 bits; U32 and U16 as in test_gpu_feedback."""
+other words, KL terms of weight 0, ratios past fp32. Against the formulas in 64 bits; U32 and U16 as
+in test_gpu_feedback."""
 
 from __future__ import annotations
 
@@ -7,7 +8,7 @@ import pytest
 import torch
 
 from test_gpu_feedback import BF16, DEV, F32, U16, U32, _gen, _head_exact, _head_tol, _ops, \
-    _packing, _within
+    _packing, _policy_exact, _within
 
 pytestmark = pytest.mark.gpu
 
@@ -105,3 +106,23 @@ def test_policy_loss_watches_a_kl_of_weight_0(lens, reduction, kl):
     assert seen.isinf() if kl == "k3" else seen.isfinite() and seen > 0
     logp[rows[5]] = -float("inf")  # of probability 0
     assert same(logp).isinf()
+
+
+@pytest.mark.parametrize("lens", [[64], [20000]], ids=["small", "large"])
+def test_policy_loss_of_ratios_past_fp32(lens):
+    """Ratios e^89 to e^120, whose product with the advantage is 0 or within fp32."""
+    ops = _ops()
+    n = sum(lens)
+    plan, seq, mask, A = _packing(lens, 9, 1)
+    logp = -torch.rand(n, generator=_gen(1), device=DEV)
+    old = logp - torch.linspace(60, 120, n, device=DEV)
+    A = A * 1e-20
+    A[::3] = 0.0
+    loss, stats, d = ops.policy_loss(logp, old, A, plan, mask=mask, reduction="sum", divisor=3.0)
+    e_loss, P, K, share, e_d, (size, _), gsize = _policy_exact(
+        logp, old, A, None, seq, mask, 1, 0.2, 0.2, 0.0, "k3", "sum", 3.0)
+    # the ratio's argument is rounded: 2^7·U32 relative in the ratio; the rest as for other rows
+    tol = (2 ** 7 + 24) * U32
+    _within(loss, e_loss, tol * size + 1e-30)
+    _within(d, e_d, tol * gsize + 1e-30)
+    assert abs(stats[2].item() - share) <= U32
