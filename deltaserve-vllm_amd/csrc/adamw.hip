@@ -171,6 +171,21 @@ DSB_DEV float value(Run<E> o, int i, bool bf) {
   const unsigned x = i & 1 ? two & 0xffff0000u : two << 16;
   return __builtin_bit_cast(float, bf ? x : one);
 }
+// A run's elements times a power of two.
+template <int E>
+DSB_DEV void rescale(Run<E>& o, float by, bool bf) {
+#pragma unroll
+  for (int i = 0; i < E; i += 2) {
+    const float a = value(o, i, bf) * by, b = value(o, i + 1, bf) * by;
+    if (bf) {
+      o[i / 2] = (unsigned)__builtin_bit_cast(uint16_t, (bf16)a) |
+                 (unsigned)__builtin_bit_cast(uint16_t, (bf16)b) << 16;
+    } else {
+      o[i] = __builtin_bit_cast(unsigned, a);
+      o[i + 1] = __builtin_bit_cast(unsigned, b);
+    }
+  }
+}
 // A run of E elements from e, past the caches.
 template <int E>
 DSB_DEV void store_run(void* p, int e, int count, bool bf, const float (&v)[E]) {
@@ -323,14 +338,22 @@ DSB_DEV double block_sum64(double s, double* red) {
   for (int i = 0; i < NT / 64; ++i) s += red[i];
   return s;
 }
+// The clip's factor, in two where one would leave fp32's normal range: g·first·second.
+struct Clip {
+  float first, second;
+};
+// With 8 bits a reciprocal and a product in fp32, each rounded (as elementary operations give it),
+// else the quotient in 64 bits. A norm near or past fp32's range, or a factor that small, takes the
+// quotient and leaves 2^-64 of it to a factor of its own.
 template <int BITS>
-DSB_DEV float clip_factor(double norm, double max_norm) {
-  if constexpr (BITS == 8) {
-    const float c = 1.f / ((float)norm + 1e-6f) * (float)max_norm;
-    return c > 1.f ? 1.f : c;  // NaN stays
+DSB_DEV Clip clip_factor(double norm, double max_norm) {
+  if (BITS == 8 && norm <= 0x1p100 && norm <= 0x1p100 * max_norm) {
+    const float f = 1.f / ((float)norm + 1e-6f) * (float)max_norm;
+    return Clip{1.f, f > 1.f ? 1.f : f};
   }
-  const double c = max_norm / (norm + 1e-6);
-  return c > 1.0 ? 1.f : (float)c;
+  const double c = max_norm / (norm + 1e-6);  // (NaN stays)
+  if (c < 0x1p-100) return Clip{0x1p-64f, (float)(c * 0x1p64)};
+  return Clip{1.f, c > 1.0 ? 1.f : (float)c};
 }
 // x / s to nearest, from inv = 1 / s to nearest: what the product leaves over, times inv. (s and
 // the largest x are not near the smallest numbers, so that the rest is exact.)
@@ -358,7 +381,7 @@ template <int BITS>
 __global__ __launch_bounds__(1024) void adam_norm_kernel(const int* __restrict__ group_chunks,
                                                          const double* __restrict__ partial,
                                                          double max_norm, float* __restrict__ norms,
-                                                         float* __restrict__ coef) {
+                                                         Clip* __restrict__ coef) {
   __shared__ double red[16];
   const int c0 = group_chunks[blockIdx.x], c1 = group_chunks[blockIdx.x + 1];
   double s = 0.0;
@@ -376,7 +399,7 @@ __global__ __launch_bounds__(1024) void adam_norm_kernel(const int* __restrict__
 enum { CLIP_NONE, CLIP_GIVEN, CLIP_SUM };
 struct ClipArgs {
   int how;
-  const float* coef;
+  const Clip* coef;
   const int* group_chunks;
   int ngroups;
   const double* partial;
@@ -444,7 +467,7 @@ DSB_DEV void adam_chunk(const AdamKernelArgs& a, const dsb_adam_chunk& t, int ch
       rs = a.r_scale[b];
     }
   }
-  float cf = 1.f;
+  Clip cf{1.f, 1.f};
   if (clip.how == CLIP_GIVEN) {
     cf = clip.coef[t.group];
   } else if (clip.how == CLIP_SUM) {
@@ -456,6 +479,10 @@ DSB_DEV void adam_chunk(const AdamKernelArgs& a, const dsb_adam_chunk& t, int ch
         if (clip.group_chunks[g] == clip.group_chunks[g + 1]) clip.norms[g] = 0.f;
   }
   if (!live) return;
+  if (cf.first != 1.f) {  // rare
+#pragma unroll
+    for (int k = 0; k < G; ++k) rescale(graw[k], cf.first, gbf);
+  }
   Hyper h = a.hv;
   if (a.hp) h = *a.hp;
   unsigned mtop = 0, rtop = 0;
@@ -471,7 +498,7 @@ DSB_DEV void adam_chunk(const AdamKernelArgs& a, const dsb_adam_chunk& t, int ch
     float w[E];
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-      const float gi = value(graw[k], i, gbf) * cf, wi = value(wraw[k], i, wbf);
+      const float gi = value(graw[k], i, gbf) * cf.second, wi = value(wraw[k], i, wbf);
       if constexpr (BITS == 8) {
         const float ro = r[k][i] * rs;
         m[k][i] = blend(h.b1, m[k][i] * ms, h.ob1, gi);
@@ -578,13 +605,14 @@ __global__ __launch_bounds__(kThreads) void adam_kernel(AdamKernelArgs a) {
 }
 
 int64_t adam_bytes(int nchunks, int ngroups) {
-  return 256 + ((int64_t)nchunks * 8 + 255) / 256 * 256 + ((int64_t)ngroups * 4 + 255) / 256 * 256;
+  return 256 + ((int64_t)nchunks * 8 + 255) / 256 * 256 +
+         ((int64_t)ngroups * (int64_t)sizeof(Clip) + 255) / 256 * 256;
 }
 
 hipError_t adam_step(const AdamArgs& a, void* work, hipStream_t s) {
   Hyper* hp = (Hyper*)work;
   double* partial = (double*)((char*)work + 256);
-  float* coef = (float*)((char*)partial + ((int64_t)a.nchunks * 8 + 255) / 256 * 256);
+  Clip* coef = (Clip*)((char*)partial + ((int64_t)a.nchunks * 8 + 255) / 256 * 256);
   const bool dev = a.lr_dev || a.step_dev, clip = a.max_norm >= 0;
   Hyper hv{};
   if (dev)

@@ -1,13 +1,13 @@
 """The operators for training from feedback at the ends of their ranges: labels far above the
-other words, KL terms of weight 0, ratios past fp32. Against the formulas in 64 bits; U32 and U16 as
-in test_gpu_feedback."""
+other words, KL terms of weight 0, ratios and gradient norms past fp32. Against the formulas in 64
+bits; U32 and U16 as in test_gpu_feedback."""
 
 from __future__ import annotations
 
 import pytest
 import torch
 
-from test_gpu_feedback import BF16, DEV, F32, U16, U32, _gen, _head_exact, _head_tol, _ops, \
+from test_gpu_feedback import BF16, DEV, F32, U16, U32, Ref, _gen, _head_exact, _head_tol, _ops, \
     _packing, _policy_exact, _within
 
 pytestmark = pytest.mark.gpu
@@ -126,3 +126,33 @@ def test_policy_loss_of_ratios_past_fp32(lens):
     _within(loss, e_loss, tol * size + 1e-30)
     _within(d, e_d, tol * gsize + 1e-30)
     assert abs(stats[2].item() - share) <= U32
+
+
+# ---------------------------------------------------------------- AdamW
+
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("size", [1000, (1 << 20) + 5000])
+@pytest.mark.parametrize("max_norm", [1.0, 1e20, 1e-3])
+@pytest.mark.parametrize("dtypes", [(F32, F32), (BF16, BF16), (BF16, F32), (F32, BF16)], ids=["ff", "bb", "bf", "fb"])
+def test_adamw_clips_gradients_of_any_finite_size(bits, size, max_norm, dtypes):
+    """Norms from 2^126 on, past fp32's range: the group is clipped to max_norm as any other, and the
+    groups beside it are not touched by it."""
+    ops = _ops()
+    g = [torch.randn(k, generator=_gen(k), device=DEV) for k in (size, 700)]
+    g[0] = (g[0].clamp(-3, 3) * 1e38)
+    g = [x.to(dtypes[1]) for x in g]
+    w = [torch.randn(k, generator=_gen(k + 1), device=DEV).to(dtypes[0]) for k in (size, 700)]
+    w2 = w[1].clone()
+    opt = ops.AdamW(w, g, bits=bits, groups=[0, 1])
+    for step in (1, 2):
+        ref = Ref(opt, w, g, [0, 1])
+        hyper = dict(lr=1e-2, step=step, wd=0.1, max_norm=max_norm, seed=5)
+        norms = opt.step(**hyper)
+        ref.step(**hyper)
+        assert norms[0] > 1e38 and norms[1].isfinite()
+        ref.check(dtypes[0])
+    alone = ops.AdamW([w2], [g[1]], bits=bits)
+    for step in (1, 2):
+        alone.step(lr=1e-2, step=step, wd=0.1, max_norm=max_norm, seed=5)
+    if bits == 32:  # (8 bits: rounded at random by the block's number)
+        assert torch.equal(w[1], w2)
