@@ -28,10 +28,21 @@ const char* check_plan(const dsb_pack_plan* p) {
 
 int64_t plan_part(int64_t elems) { return (elems + 3) / 4 * 4; }
 
+// A launch holds fewer than 2^32 threads: blocks of 256 up to this many.
+constexpr int64_t kMostBlocks = (1 << 24) - 1;
+// Sequences and tiles of a plan, which take a wave each.
+constexpr int64_t kMostSeqs = 4 * kMostBlocks - 8;
+
+const char* check_head(int n, int D, int V) {
+  if (n < 0 || n > kMostBlocks || V < 2 || D < 8 || D % 8 || D > 65536 || V > (1 << 24))
+    return "n below 2^24, D a multiple of 8 up to 65536 and V from 2 to 2^24 are taken";
+  if (((int64_t)n + 255) / 256 * ((V + 255) / 256) > kMostBlocks)
+    return "n / 256 times V / 256 must be below 2^24";
+  return nullptr;
+}
 const char* check_logprob(const void* normed, int64_t ldh, const void* lm_w, const int64_t* labels,
                           int n, int D, int V) {
-  if (n < 0 || n > (1 << 30) || V < 2 || D < 8 || D % 8 || D > 65536 || V > (1 << 24))
-    return "n up to 2^30, D a multiple of 8 up to 65536 and V from 2 to 2^24 are taken";
+  if (const char* e = check_head(n, D, V)) return e;
   if (ldh < D || ldh % 8) return "ldh must be a multiple of 8 and >= D";
   if (n > 0 && (!normed || !lm_w || !labels)) return "null argument";
   if (misaligned(normed, 16) || misaligned(lm_w, 16)) return "normed and lm_w must be 16-byte aligned";
@@ -51,8 +62,7 @@ extern "C" {
 int dsb_op_logprob_workspace(int n, int D, int V, int backward, int64_t* bytes) {
   const char* what = "dsb_op_logprob_workspace";
   if (!bytes) return bad(what, "null argument");
-  if (const char* e = check_logprob(nullptr, D, nullptr, nullptr, 0, D, V)) return bad(what, e);
-  if (n < 0) return bad(what, "n must not be negative");
+  if (const char* e = check_head(n, D, V)) return bad(what, e);
   *bytes = n ? logprob_bytes(n, D, V, backward != 0) : 0;
   return 0;
 }
@@ -99,6 +109,7 @@ int dsb_plan_sizes(const int32_t* seq_lens, int nseq, dsb_pack_plan* plan, int64
     longest = len > longest ? len : longest;
   }
   if (n > 0x7fffffffLL - DSB_CHUNK_ROWS) return bad(what, "the sequences hold too many rows");
+  if (nseq > kMostSeqs || tiles > kMostSeqs) return bad(what, "there are too many sequences");
   plan->ntiles = (int)tiles;
   plan->nseq = nseq;
   plan->n = (int)n;
@@ -220,7 +231,8 @@ int dsb_op_policy_loss(const float* logp, const float* old_logp, const float* re
 }
 
 int dsb_op_adam_workspace(int nchunks, int ngroups, int64_t* bytes) {
-  if (!bytes || nchunks < 0 || ngroups < 0) return bad("dsb_op_adam_workspace", "bad argument");
+  if (!bytes || nchunks < 0 || nchunks > kMostBlocks || ngroups < 0)
+    return bad("dsb_op_adam_workspace", "bad argument");
   *bytes = adam_bytes(nchunks, ngroups);
   return 0;
 }
@@ -232,7 +244,7 @@ int dsb_op_adam_step(const dsb_adam_chunk* chunks, int nchunks, const int32_t* g
                      const float* lr_dev, const int64_t* step_dev, float* norms, void* work,
                      int64_t work_bytes, void* stream) {
   const char* what = "dsb_op_adam_step";
-  if (nchunks < 0 || ngroups < 1 || most_chunks < 0 || most_chunks > nchunks)
+  if (nchunks < 0 || nchunks > kMostBlocks || ngroups < 1 || most_chunks < 0 || most_chunks > nchunks)
     return bad(what, "bad sizes");
   if (bits != 8 && bits != 32) return bad(what, "the moments have 8 or 32 bits");
   if (!(beta1 >= 0 && beta1 < 1) || !(beta2 >= 0 && beta2 < 1))

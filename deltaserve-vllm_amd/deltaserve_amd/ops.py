@@ -445,7 +445,8 @@ def token_logprobs(normed, lm_w, labels):
     stride a multiple of 8), lm_w bf16 [V, D], labels int64 [n], a negative one unscored. Returns
     fp32 (logp [n] = log softmax(normed·lm_wᵀ)[label], other [n] = the log-sum-exp of the other
     words' logits, which :func:`token_logprobs_backward` takes); 0 on unscored rows, NaN where a
-    label is past the vocabulary. Only scored rows cost a product."""
+    label is past the vocabulary. Only scored rows cost a product. n and (n / 256)·(V / 256) are below
+    2^24."""
     what = "token_logprobs"
     n, D, V, ld = _head_args(what, normed, lm_w, labels)
     with _on(what, normed, lm_w, labels):
@@ -588,7 +589,7 @@ class AdamW:
             chunks = -(-numel // L.ADAM_CHUNK)
             block0 = np.cumsum(blocks) - blocks
             self.nblocks, self.nchunks = int(blocks.sum()), int(chunks.sum())
-            if self.nchunks > 0x7fffffff:
+            if self.nchunks >= 1 << 24:  # (a launch's blocks)
                 raise ValueError(f"{what}: too many elements")
             # a record per chunk: one table to read, no second one behind it
             t = np.repeat(np.arange(len(ws)), chunks)

@@ -394,8 +394,9 @@ int dsb_op_clip_adamw(float* const* w, float* const* g, float* const* m, float* 
 /* Log probabilities of labels: row t of normed [n, D] (bf16, row stride ldh)
  * against the LM head lm_w [V, D], labels int64 [n]; a negative label leaves the
  * row unscored, one >= V gives NaN. logp[t] = log softmax(h·Wᵀ)[label] and
- * other[t] = log Σ_{v ≠ label} exp(h·W_v), fp32 [n], 0 on unscored rows. D and
- * ldh multiples of 8, V at least 2. */
+ * other[t] = log Σ_{v ≠ label} exp(h·W_v), fp32 [n], 0 on unscored rows. D (up to
+ * 65536) and ldh multiples of 8, V from 2 to 2^24, n below 2^24 and so is
+ * ceil(n / 256)·ceil(V / 256). */
 int dsb_op_logprob_workspace(int n, int D, int V, int backward, int64_t* bytes);
 int dsb_op_token_logprobs(const void* normed, int64_t ldh, const void* lm_w, const int64_t* labels,
                           int n, int D, int V, float* logp, float* other, void* work,
@@ -425,8 +426,8 @@ typedef struct dsb_pack_plan {
   const int32_t* chunk_seq;
   int32_t ntiles, nseq, n, npred, nonempty, longest;
 } dsb_pack_plan;
-/* Host only. seq_lens int32 [nseq], each >= 0, their sum below 2^31: the counts of
- * the plan (its pointers untouched) and the int32 elements of all four tables. */
+/* Host only. seq_lens int32 [nseq], each >= 0, their sum at most 2^31 − 4097, the
+ * sequences and their tiles below 2^26 − 12: the counts of the plan (its pointers untouched) and the int32 elements of all four tables. */
 int dsb_plan_sizes(const int32_t* seq_lens, int nseq, dsb_pack_plan* plan, int64_t* elems);
 /* Host only. Fills `tables` (host memory of `elems` int32) and the plan's pointers,
  * as offsets from `device_base`, where the caller copies it. */
@@ -492,7 +493,7 @@ typedef struct dsb_adam_chunk {
 /* Clip by group and AdamW over many tensors (the arithmetic of dsb_op_clip_adamw; the
  * gradients are left as they are). chunks, in order of their groups, and group_chunks
  * [ngroups + 1] (first chunk of each group) live on the device; most_chunks: those of the
- * largest group.
+ * largest group. nchunks is below 2^24.
  * bits 32: m and v fp32 by block. bits 8: m holds e4m3 codes of m / m_scale and v those
  * of sqrt(v) / r_scale, scales fp32 by block, the block's largest magnitude / 448; m is
  * rounded to nearest, sqrt(v) up or down at random in proportion (a function of seed, step,
