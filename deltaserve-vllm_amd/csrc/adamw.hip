@@ -8,15 +8,19 @@
 // sqrt(v) = code·r_scale, codes e4m3 (3 mantissa bits, largest 448, smallest 2^-9).
 // The square root halves the exponents that v takes, so a block holds v over 11
 // decades. m moves by a tenth of the gradient a step and is rounded to nearest
-// (half a step, 2^-4 relative). sqrt(v) moves by at most 0.05 % a step, far below
-// half a step of 6 to 12 %: to nearest it would never fall, so it is rounded up or
+// (half a step, 2^-4 relative). sqrt(v) falls by at most 0.05 % a step (β2 = 0.999), far
+// below half a step of 6 to 12 %: to nearest it would never fall, so it is rounded up or
 // down at random in proportion to where it lies, and the mean moves as it should. It
 // is never rounded to 0 from above, where m / (0 + ε) would leap. The step uses m' and
-// v' before they are rounded. Blocks whose largest magnitude is below 2^-100 are held as
-// zeros. The moments take the formula's operations one by one in fp32, each to nearest, so
-// that their codes are those that elementary operations give, bit for bit: a code on the
-// other side of where two meet (one in a million with fused operations) is a step of 6 to
-// 12 % that later updates show.
+// v' before they are rounded. The moments take the formula's operations one by one in fp32,
+// each to nearest, so that their codes are those that elementary operations give, bit for
+// bit: a code on the other side of where two meet (one in a million with fused operations) is
+// a step of 6 to 12 % that later updates show.
+//
+// Range. Blocks whose largest |m| or sqrt(v) is below 2^-100 are held as zeros. The squares
+// are taken in fp32: gradients (after the clip) and sqrt(v) lose bits in v below 2^-63 and
+// count as 0 there below 2^-74.5, and from 2^64 on v is infinite; the root is to nearest for v
+// from 2^-100 on.
 //
 // A workgroup takes a chunk of 4096 elements, a wave 4 blocks, 16 lanes a block:
 // loads of 16 bytes a lane cover whole 256-byte runs, and the block's
@@ -361,8 +365,9 @@ DSB_DEV float divided(float x, float s, float inv) {
   const float q = x * inv;
   return fmaf(fmaf(-q, s, x), inv, q);
 }
-// sqrt(v) to nearest: the instruction is off by at most a step, and a neighbour s' of its s is
-// the nearer one where v − s·s' says so (not with 0, infinity or NaN, where s stays).
+// sqrt(v) to nearest, by Tuckerman's test: the instruction is off by at most a step, and a
+// neighbour s' of its s is the nearer one where v − s·s' says so (not with 0, infinity or NaN,
+// where s stays). Below v = 2^-100 that difference may underflow.
 DSB_DEV float root(float v) {
   const float s = __builtin_amdgcn_sqrtf(v);
   const float down = __builtin_bit_cast(float, __builtin_bit_cast(int, s) - 1);
@@ -583,7 +588,9 @@ DSB_DEV void adam_chunk(const AdamKernelArgs& a, const dsb_adam_chunk& t, int ch
 // A block per chunk. With 8-bit moments the element types are constants of the code (2.3 M fp32
 // elements: 15.3 → 14.8 µs; with 32 bits 258 → 261, where they stay variables), and a lane takes
 // 8 elements at a time of bf16 weights and gradients (252 M: 508 → 494 µs), else 4 (84 M fp32
-// ones with 8: 230 → 265).
+// ones with 8: 230 → 265). 84 M elements, no clip, weights and gradients fp32 / bf16 / bf16 and
+// fp32 / fp32 and bf16: 215 / 147 / 163 / 192 µs with 8 bits (6.3 / 5.8 / 6.2 / 6.2 TB/s), 381 /
+// 301 / 331 / 353 with 32 (6.1 to 6.2).
 template <int BITS>
 __global__ __launch_bounds__(kThreads) void adam_kernel(AdamKernelArgs a) {
   __shared__ double red[kThreads / 64];
@@ -626,7 +633,7 @@ hipError_t adam_step(const AdamArgs& a, void* work, hipStream_t s) {
       hipLaunchKernelGGL(adam_sumsq_kernel, dim3((a.nchunks + 3) / 4), dim3(256), 0, s, a.chunks,
                          a.nchunks, partial);
     // Groups of at most 256 chunks (a million elements) are added up by each of their blocks,
-    // which saves a launch (2.3 M elements in 28 groups: 15.3 µs, 17.2 with it); a thread of a
+    // which saves a launch (2.3 M elements in 28 groups: 14.6 µs, about 2 more with it); a thread of a
     // block reads one sum.
     c.how = a.most_chunks <= kThreads && a.nchunks > 0 ? CLIP_SUM : CLIP_GIVEN;
     if (c.how == CLIP_GIVEN)

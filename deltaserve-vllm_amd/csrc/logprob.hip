@@ -33,10 +33,17 @@ constexpr float kNoWord = -0x1p126f;  // under every logit
 constexpr long kProbElems = 1L << 29;
 // and at most this many columns: 256 rows of them stay within 32-bit byte offsets
 constexpr long kMaxChunk = 1L << 21;
-// Every product takes 256 × 256 tiles, also over few rows, where the head streams once:
-// at 16 to 2428 scored rows of the configured widths no other tile is ahead by more than
-// 2 % (149 rows × 5120 × 151936, forward: 401 µs; 256 × 128 457, 128 × 128 567), but under 40
-// rows at 1024 wide (122 µs against 142 for 128 × 128 forward, 229 against 195 backward).
+// Every product takes 256 × 256 tiles (with lp_narrow's last ones), also over few rows, though a
+// tile multiplies all its rows, scored or not (5120 × 151936: 398 GFLOP, 290 µs at the rate of a large
+// product). µs at 256 × 256 / 256 × 128 / 128 × 128 tiles, forward and gradient:
+//   149 rows × 5120 × 151936   338 / 393 / 498    679 / 717 / 1138
+//   504 × 1024 × 151936        170 / 211 / 255    335 / 365 / 498
+//   113 × 4096 × 128256        211 / 255 / 203    417 / 462 / 424
+//   64 × 5120 × 151936         309 / 373 / 291    620 / 670 / 592
+//   16 × 5120 × 151936         297 / 360 / 269    590 / 641 / 539
+//   16 × 1024 × 151936          79 /  95 /  72    180 / 198 / 131
+// so half as tall ones would be ahead by 4 to 27 % up to 64 scored rows. That number is the
+// device's, and the tile is chosen on the host.
 constexpr int kRun = 128;  // columns of a wave's tile
 // K slices of the dH product, most: 8 tiles (500 rows × 1024) fill the CUs 32 times
 // (349 µs; 16 slices 414, 8 580; before the probabilities' stores went past the caches).
@@ -262,7 +269,8 @@ LPPlan lp_plan(int n, int D, int V) {
 // Columns, the last ones of the vocabulary, that the forward's product takes in 256 × 128
 // tiles: over one block of rows the head is streamed by whole rounds of the device's CUs, and
 // where the last round of 256 × 256 tiles is at most half full, half-wide ones fill it better
-// (149 rows × 5120 × 151936, 82 tiles in the third round: 386 → 355 µs, both through the caches).
+// (5120 × 151936, 82 tiles in the third round: 149 rows 361 → 338 µs, 16 rows 309 → 297; 1024 wide
+// 16 rows 81 → 79).
 int lp_narrow(int n, int V) {
   const int tiles = (V + 255) / 256, last = tiles % kGemmCus;
   return n <= 256 && tiles > kGemmCus && last > 0 && last <= kGemmCus / 2

@@ -461,7 +461,9 @@ def token_logprobs(normed, lm_w, labels):
 
 def token_logprobs_backward(normed, lm_w, labels, logp, other, dlogp, out_dtype=BF16):
     """The rows' gradient [n, D] (bf16 or fp32) of Σ dlogp·logp, from the forward's logp and other;
-    zeros on unscored rows and where dlogp is 0, which cost no product."""
+    zeros on unscored rows and where dlogp is 0, which cost no product. The probabilities that multiply
+    the head are bf16 (2^-9 relative on average, their common part divided out) and the sums fp32, also
+    where the result is fp32."""
     what = "token_logprobs_backward"
     n, D, V, ld = _head_args(what, normed, lm_w, labels)
     for name, t in (("logp", logp), ("other", other), ("dlogp", dlogp)):
@@ -644,7 +646,9 @@ class AdamW:
         rounded at random by ``seed`` and step, the same way for the same two. For a step that is
         captured into a graph, lr (fp32) and step (int64) may be one-element tensors on the device,
         read when it runs; numbers are baked in. A NaN or infinite gradient reaches the weights that
-        it reaches in the formula, and with 8 bits its block's moments."""
+        it reaches in the formula, and with 8 bits its block's moments. A finite one of 2^64 or more
+        (after the clip) has an infinite square in fp32: with 32 bits its weight stays where it is, with
+        8 bits its block's moments are lost."""
         what = "AdamW.step"
         lr_t = lr if isinstance(lr, torch.Tensor) else None
         step_t = step if isinstance(step, torch.Tensor) else None

@@ -404,7 +404,7 @@ int dsb_op_token_logprobs(const void* normed, int64_t ldh, const void* lm_w, con
 /* The gradient of Σ_t dlogp[t]·logp[t] with respect to the rows, given the
  * forward's logp and other: dH [n, D] bf16 or (out_f32) fp32, row stride lddh (a
  * multiple of 8). Unscored rows and rows with dlogp = 0 get zeros and cost no
- * product. */
+ * product. The probabilities are rounded to bf16, with either output type. */
 int dsb_op_token_logprobs_bwd(const void* normed, int64_t ldh, const void* lm_w,
                               const int64_t* labels, int n, int D, int V, const float* logp,
                               const float* other, const float* dlogp, void* dH, int64_t lddh,
@@ -499,7 +499,8 @@ typedef struct dsb_adam_chunk {
  * rounded to nearest, sqrt(v) up or down at random in proportion (a function of seed, step,
  * block and element) and never down to 0 from above it. The step itself uses the moments
  * before they are rounded. max_norm < 0: no clip, norms unused; else norms [ngroups]
- * gets each group's gradient norm. lr_dev / step_dev: when set, the learning rate (fp32)
+ * gets each group's gradient norm, summed in 64 bits (infinite past fp32; the clip is not). The
+ * clip's factor is taken in 64 bits, with bits 8 as a reciprocal times max_norm in fp32. lr_dev / step_dev: when set, the learning rate (fp32)
  * and the step count (int64) are read on the device, for a captured step. */
 int dsb_op_adam_workspace(int nchunks, int ngroups, int64_t* bytes);
 int dsb_op_adam_step(const dsb_adam_chunk* chunks, int nchunks, const int32_t* group_chunks,
