@@ -24,11 +24,13 @@ ROPE_DEFAULT, ROPE_LINEAR, ROPE_LLAMA3 = 0, 1, 2
 PROJS = ("q", "k", "v", "o", "gate", "up", "down")
 PROJ_INDEX = {p: i for i, p in enumerate(PROJS)}
 FLAG_GRAPH, FLAG_NO_CLIP, FLAG_KTIMING, FLAG_SERIAL_LAYERS = 1, 2, 4, 8
-DT_BF16, DT_F16, DT_F32 = 0, 1, 2
+DT_BF16, DT_F16, DT_F32, DT_E4M3, DT_INT8 = 0, 1, 2, 3, 4
 PREF_KINDS = {"sigmoid": 0, "hinge": 1, "ipo": 2}
 KL_KINDS = {"k3": 0, "k2": 1}
 REDUCTIONS = {"token": 0, "sequence": 1, "sum": 2}
 ADAM_BLOCK, ADAM_CHUNK = 256, 4096
+ROWS8_BLOCK = 32
+GATE_NONE, GATE_CHANNEL, GATE_ROW, GATE_FULL = 0, 1, 2, 3
 
 
 class DsbDesc(Structure):
@@ -196,6 +198,29 @@ _SIGS = {
                                  c_void_p, c_void_p, c_void_p, c_int, c_double, c_double, c_double, c_double,
                                  c_double, c_double, c_int64, c_uint32, c_void_p, c_void_p, c_void_p,
                                  c_void_p, c_int64, c_void_p]),
+    "dsb_save_rows8": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int, c_void_p,
+                               c_void_p, c_int, c_int, c_void_p, c_int64, c_void_p, c_int64, c_int,
+                               c_int64, c_void_p]),
+    "dsb_op_restore_rows8": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int, c_int, c_int,
+                                     c_void_p, c_int64, c_int, c_void_p]),
+    "dsb_op_swiglu": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int, c_int, c_int, c_void_p,
+                              c_int64, c_void_p]),
+    "dsb_op_swiglu_bwd": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int, c_int, c_int,
+                                  c_void_p, c_int64, c_int, c_void_p, c_int64, c_void_p, c_int64,
+                                  c_void_p]),
+    "dsb_op_norm_join": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int, c_void_p, c_int64,
+                                 c_void_p, c_void_p, c_void_p, c_int64, c_int, c_double, c_double,
+                                 c_int, c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p]),
+    "dsb_op_norm_join_workspace": (c_int, [c_int, c_int, c_int, POINTER(c_int64)]),
+    "dsb_op_norm_join_bwd": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int, c_void_p, c_int64,
+                                     c_void_p, c_int64, c_int, c_void_p, c_int64, c_int, c_void_p,
+                                     c_int64, c_int, c_void_p, c_void_p, c_void_p, c_int64, c_int,
+                                     c_double, c_double, c_int, c_int, c_void_p, c_int64, c_int,
+                                     c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p,
+                                     c_void_p, c_int64, c_void_p]),
+    "dsb_op_rotary": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int,
+                              c_void_p, c_int, c_void_p, c_double, c_int, c_int, c_int, c_int,
+                              c_int, c_int, c_void_p]),
 }
 
 EXPORTED = tuple(_SIGS)

@@ -33,6 +33,7 @@ from typing import Optional
 import torch
 
 from . import _lib as L
+from .rows8 import Rows8
 
 _DT = {torch.bfloat16: L.DT_BF16, torch.float16: L.DT_F16, torch.float32: L.DT_F32}
 
@@ -74,7 +75,14 @@ def save_rows(x: torch.Tensor, r: Optional[torch.Tensor], buf: torch.Tensor,
     ``buf.index_copy_(0, dst, (x.index_select(0, src) + ...).to(buf.dtype))``
     (ft_save_op.py:84-89), except that slots aimed at the scratch row
     ``buf[-1]`` are not written (nothing reads that row) and slots whose source
-    row lies outside ``x`` are skipped instead of faulting."""
+    row lies outside ``x`` are skipped instead of faulting. ``buf`` may be
+    :class:`Rows8`, which takes the rows in 8 bits (x and r of any row strides
+    and width)."""
+    if isinstance(buf, Rows8):
+        from . import ops
+
+        ops.pack_rows8(x, r, out=buf, src=src, dst=dst)
+        return
     if x.dtype not in _DT:
         raise TypeError(f"save_rows: x must be bf16, fp16 or fp32, got {x.dtype}")
     if buf.dtype != torch.bfloat16:

@@ -17,6 +17,7 @@ import numpy as np
 import torch
 
 from . import _lib as L
+from .rows8 import CODES, Rows8
 
 BF16 = torch.bfloat16
 
@@ -133,7 +134,10 @@ def gemm_glu(A, B, A2=None, B2=None, with_h=True):
 # ---------------------------------------------------------------- norms / rope
 
 def rmsnorm(x, w, eps):
-    """ops.py:84-88 (bf16 in/out, fp32 internals)."""
+    """ops.py:84-88 (bf16 in/out, fp32 internals). x may be :class:`Rows8`; the call then only
+    enqueues."""
+    if isinstance(x, Rows8):
+        return _rmsnorm8(x, w, eps)
     _dev(x, w)
     y = torch.empty(x.shape, dtype=BF16, device=x.device)
     L.check(L.load().dsb_op_rmsnorm(_p(x), _ld(x), _p(w), _p(y), _ld(y), x.shape[0], x.shape[1],
@@ -143,7 +147,10 @@ def rmsnorm(x, w, eps):
 
 def rmsnorm_backward(x, g, w, eps, resid=None):
     """ops.py:91-100 (+ bf16 residual add, llama3.py:205); bf16 out. An fp32 g
-    [parts, n, D] is added up in order first."""
+    [parts, n, D] is added up in order first. x may be :class:`Rows8`, g then a matrix; the call
+    then only enqueues."""
+    if isinstance(x, Rows8):
+        return _rmsnorm8_backward(x, g, w, eps, resid)
     _dev(x, g, w, resid)
     out = torch.empty(x.shape, dtype=BF16, device=x.device)
     if g.dim() == 3:
@@ -668,3 +675,376 @@ class AdamW:
                 seed & 0xffffffff, _at(lr_t), _at(step_t), _at(norms), _at(work), self._bytes, _now()),
                 what="dsb_op_adam_step")
         return norms
+
+
+# ---------------------------------------------------------------- a block's memory-bound operators
+#
+# SwiGLU, the join of a block with the residual stream and the norms around it, and rotary positions,
+# forward and backward, with activations that may be kept in 8 bits. They only enqueue on the current
+# stream of their tensors' device, as the ops for training from feedback do, and can be captured; the
+# reference has no counterpart of them but for the norms' formulas (cited above) and SwiGLU's
+# (ffn.py:29-48). A row's elements are contiguous; rows of bf16 and fp32 start on 16 bytes and lie a
+# multiple of 16 bytes apart, rows of codes on 8.
+
+_FLOATS = (BF16, torch.float32)
+_DT = {BF16: L.DT_BF16, torch.float16: L.DT_F16, torch.float32: L.DT_F32}
+
+
+def _matrix(what, name, t, shape, dtypes):
+    """The row stride of a matrix of this shape (None: any) and one of these types."""
+    if t.dtype not in dtypes or t.dim() != 2 or (shape is not None and t.shape != shape):
+        of = "" if shape is None else f" [{shape[0]}, {shape[1]}]"
+        raise ValueError(f"{what}: {name} must be a matrix{of} of "
+                         f"{' or '.join(str(d) for d in dtypes)}")
+    n, width = t.shape
+    if t.numel() and width > 1 and t.stride(1) != 1:
+        raise ValueError(f"{what}: {name}'s last dimension must be contiguous")
+    # the row stride of a single row is any number: one that is whole
+    return t.stride(0) if n > 1 else -(-width // 8) * 8
+
+
+def _rows(what, name, t, shape, dtypes=_FLOATS):
+    """(address, row stride, scales' address, scales' row stride, type) of rows, 8-bit ones among
+    them."""
+    if isinstance(t, Rows8):
+        if shape is not None and t.shape != shape:
+            raise ValueError(f"{what}: {name} must be [{shape[0]}, {shape[1]}]")
+        c, s = t.codes, t.scales
+        n, width = c.shape
+        return (c.data_ptr(), c.stride(0) if n > 1 else -(-width // 8) * 8, s.data_ptr(),
+                s.stride(0) if n > 1 else s.shape[1], t.type)
+    return t.data_ptr(), _matrix(what, name, t, shape, dtypes), None, 0, _DT[t.dtype]
+
+
+def _where(*ts):
+    """Their tensors, for :func:`_on`."""
+    out = []
+    for t in ts:
+        out += [t.codes, t.scales] if isinstance(t, Rows8) else [t]
+    return out
+
+
+def pack_rows8(x, r=None, code="e4m3", out=None, src=None, dst=None):
+    """x (+ r, added in x's type) as :class:`Rows8`: matrices of bf16, fp16 or fp32, of any width and
+    row stride. ``out`` is written and returned if given. With src and dst (int64 vectors of one
+    length) row src[i] goes into row dst[i] of ``out``, whose last row is a scratch row: slots that
+    name it, or a row outside x or out, are skipped."""
+    what = "pack_rows8"
+    ldx = _matrix(what, "x", x, None, tuple(_DT))
+    n, width = x.shape
+    ldr = 0 if r is None else _matrix(what, "r", r, x.shape, (x.dtype,))
+    if (src is None) != (dst is None) or (src is not None and out is None):
+        raise ValueError(f"{what}: src, dst and out are given together")
+    if src is not None:
+        _vec(what, "src", src, src.numel(), torch.int64)
+        _vec(what, "dst", dst, src.numel(), torch.int64)
+    if out is None:
+        out = Rows8.zeros(n, width, code, x.device)
+    elif not isinstance(out, Rows8) or out.shape[1] != width or (src is None and len(out) != n):
+        raise ValueError(f"{what}: out must be Rows8 of x's width" + (" and rows" if src is None else ""))
+    count = n if src is None else src.numel()
+    c, ldc, s, lds, kind = _rows(what, "out", out, None)
+    with _on(what, *_where(x, r, src, dst, out)):
+        L.check(L.load().dsb_save_rows8(
+            _at(x), ldx, _at(r), ldr, n, _DT[x.dtype], _at(src), _at(dst), count,
+            width, c, ldc, s, lds, kind, len(out), _now()), what="dsb_save_rows8")
+    return out
+
+
+def unpack_rows8(q, dtype=BF16):
+    """The values of :class:`Rows8` as a matrix of bf16 (which holds them exactly, but for values below
+    2^-126) or fp32."""
+    what = "unpack_rows8"
+    if dtype not in _FLOATS:
+        raise ValueError(f"{what}: dtype is bfloat16 or float32")
+    c, ldc, s, lds, kind = _rows(what, "q", q, None)
+    n, width = q.shape
+    with _on(what, *_where(q)):
+        out = torch.empty(n, width, dtype=dtype, device=q.device)
+        L.check(L.load().dsb_op_restore_rows8(c, ldc, s, lds, kind, n, width, _at(out), width,
+                                              dtype == torch.float32, _now()),
+                what="dsb_op_restore_rows8")
+    return out
+
+
+def _rmsnorm8(x, w, eps):
+    what = "rmsnorm"
+    n, D = x.shape
+    args = _rows(what, "x", x, None)
+    _vec(what, "w", w, D, BF16)
+    with _on(what, *_where(x, w)):
+        y = torch.empty(n, D, dtype=BF16, device=x.device)
+        L.check(L.load().dsb_op_norm_join(*args, None, 0, None, _at(w), None, 0, L.GATE_NONE, 1.0, eps,
+                                          n, D, None, 0, _at(y), D, _now()), what="dsb_op_norm_join")
+    return y
+
+
+def _rmsnorm8_backward(x, g, w, eps, resid):
+    what = "rmsnorm_backward"
+    n, D = x.shape
+    args = _rows(what, "x", x, None)
+    ldg = _matrix(what, "g", g, x.shape, _FLOATS)
+    ldr = 0 if resid is None else _matrix(what, "resid", resid, x.shape, (BF16,))
+    _vec(what, "w", w, D, BF16)
+    with _on(what, *_where(x, g, w, resid)):
+        out = torch.empty(n, D, dtype=BF16, device=x.device)
+        L.check(L.load().dsb_op_norm_join_bwd(
+            *args, None, 0, None, 0, 0, _at(g), ldg, g.dtype == torch.float32, _at(resid), ldr, 0, None,
+            _at(w), None, 0, L.GATE_NONE, 1.0, eps, n, D, _at(out), D, 0, None, 0, None, 0, None, None,
+            None, 0, _now()), what="dsb_op_norm_join_bwd")
+    return out
+
+
+def _glu_args(what, gu):
+    args = _rows(what, "gu", gu, None, (BF16,))
+    n, width = gu.shape
+    if width % 16:
+        raise ValueError(f"{what}: gu is [n, 2I] with I a multiple of 8")
+    return args, n, width // 2
+
+
+def swiglu(gu):
+    """bf16(silu(gate)·up) [n, I] of gate‖up rows [n, 2I], bf16 or :class:`Rows8`; I a multiple of 8."""
+    what = "swiglu"
+    args, n, I = _glu_args(what, gu)
+    with _on(what, *_where(gu)):
+        h = torch.empty(n, I, dtype=BF16, device=gu.device)
+        L.check(L.load().dsb_op_swiglu(*args, n, I, _at(h), I, _now()), what="dsb_op_swiglu")
+    return h
+
+
+def swiglu_backward(gu, dh, with_h=False):
+    """The gradient [n, 2I] (bf16) of gate‖up rows, bf16 or :class:`Rows8`, for the gradient dh [n, I]
+    (bf16 or fp32) of :func:`swiglu`'s rows; ``with_h``: (the gradient, those rows)."""
+    what = "swiglu_backward"
+    args, n, I = _glu_args(what, gu)
+    lddh = _matrix(what, "dh", dh, (n, I), _FLOATS)
+    with _on(what, *_where(gu, dh)):
+        dgu = torch.empty(n, 2 * I, dtype=BF16, device=gu.device)
+        h = torch.empty(n, I, dtype=BF16, device=gu.device) if with_h else None
+        L.check(L.load().dsb_op_swiglu_bwd(*args, n, I, _at(dh), lddh, dh.dtype == torch.float32,
+                                           _at(dgu), 2 * I, _at(h), I, _now()),
+                what="dsb_op_swiglu_bwd")
+    return (dgu, h) if with_h else dgu
+
+
+def _join_args(what, n, D, w_in, w_out, gate):
+    """(the gate's row stride, its kind) of a join's weights and gate."""
+    for name, w in (("w_in", w_in), ("w_out", w_out)):
+        if w is not None:
+            _vec(what, name, w, D, BF16)
+    if gate is None:
+        return 0, L.GATE_NONE
+    if gate.dim() == 2 and gate.shape == (n, D):
+        return _matrix(what, "gate", gate, (n, D), (BF16,)), L.GATE_FULL
+    if gate.dim() == 2 and gate.shape == (n, 1):
+        if gate.dtype != BF16:
+            raise ValueError(f"{what}: the gate must be bf16")
+        return max(gate.stride(0), 1) if n > 1 else 1, L.GATE_ROW
+    if gate.dim() == 1 and gate.shape[0] == D:
+        _vec(what, "gate", gate, D, BF16)
+        return 0, L.GATE_CHANNEL
+    _vec(what, "gate", gate, n, BF16)
+    return 1, L.GATE_ROW
+
+
+def residual_norm(x, y, w_in, eps, w_out=None, gate=None, scale=1.0):
+    """A block's output y (bf16 [n, D]) joined to the residual stream x (bf16 or fp32): with z = y, or
+    y / rms(y)·w_out with ``w_out``,
+
+        x_new = x + scale·gate·z,  normed = x_new / rms(x_new)·w_in,  rms(v) = sqrt(mean(v²) + eps).
+
+    Weights bf16 [D]. gate: None (1) or bf16, by channel [D], by row [n] or [n, 1] (n = D: [D] is by
+    channel) or [n, D]. Returns (x_new in x's type, normed bf16, of x_new as it is returned; None
+    where w_in is None). D a multiple of 8 up to 8192."""
+    what = "residual_norm"
+    args = _rows(what, "x", x, None)
+    if isinstance(x, Rows8):
+        raise ValueError(f"{what}: x must be bf16 or fp32")
+    n, D = x.shape
+    ldy = _matrix(what, "y", y, x.shape, (BF16,))
+    ldg, kind = _join_args(what, n, D, w_in, w_out, gate)
+    with _on(what, x, y, w_in, w_out, gate):
+        x_new = torch.empty(n, D, dtype=x.dtype, device=x.device)
+        normed = None if w_in is None else torch.empty(n, D, dtype=BF16, device=x.device)
+        L.check(L.load().dsb_op_norm_join(*args, _at(y), ldy, _at(w_out), _at(w_in), _at(gate), ldg,
+                                          kind, scale, eps, n, D, _at(x_new), D, _at(normed), D, _now()),
+                what="dsb_op_norm_join")
+    return x_new, normed
+
+
+def residual_norm_backward(x_new, y, dnormed, w_in, eps, dx_new=None, w_out=None, gate=None, scale=1.0,
+                           weight_grads=True):
+    """The backward of :func:`residual_norm` from the x_new that it returned (bf16, fp32 or
+    :class:`Rows8`) and y (bf16 or Rows8), for the gradients dnormed (None where w_in is None; x_new
+    is then not used) and dx_new (None: zero) of its results, bf16 or fp32 each. Returns
+
+        dx      of x and of x_new's whole, in dx_new's type, or dnormed's without one
+        dy      bf16
+        dgate   in the gate's shape: fp32 by channel and by row, bf16 [n, D]; None without a gate
+        dw_out, dw_in   fp32 [D]; None without the weight
+
+    ``weight_grads=False`` leaves dw_out, dw_in and a channel gate's dgate out (None)."""
+    what = "residual_norm_backward"
+    n, D = y.shape
+    if (dnormed is None) != (w_in is None) or (dnormed is None and dx_new is None):
+        raise ValueError(f"{what}: dnormed comes with w_in, and one of dnormed and dx_new is given")
+    xargs = (None, 0, None, 0, L.DT_BF16) if w_in is None else _rows(what, "x_new", x_new, (n, D))
+    yargs = _rows(what, "y", y, None, (BF16,))
+    ldn = 0 if dnormed is None else _matrix(what, "dnormed", dnormed, (n, D), _FLOATS)
+    ldx = 0 if dx_new is None else _matrix(what, "dx_new", dx_new, (n, D), _FLOATS)
+    ldg, kind = _join_args(what, n, D, w_in, w_out, gate)
+    f32 = lambda t: t is not None and t.dtype == torch.float32  # noqa: E731
+    with _on(what, *_where(None if w_in is None else x_new, y, dnormed, dx_new, w_in, w_out, gate)):
+        new = lambda dt, *s: torch.empty(*s, dtype=dt, device=y.device)  # noqa: E731
+        dx = new((dnormed if dx_new is None else dx_new).dtype, n, D)
+        dy = new(BF16, n, D)
+        dw_out = new(torch.float32, D) if w_out is not None and weight_grads else None
+        dw_in = new(torch.float32, D) if w_in is not None and weight_grads else None
+        dgate = None
+        if kind == L.GATE_FULL:
+            dgate = new(BF16, n, D)
+        elif kind == L.GATE_ROW:
+            dgate = new(torch.float32, *gate.shape)
+        elif kind == L.GATE_CHANNEL and weight_grads:
+            dgate = new(torch.float32, D)
+        sums = dw_out is not None or dw_in is not None or (kind == L.GATE_CHANNEL and weight_grads)
+        work, nbytes = None, c_int64(0)
+        if sums:
+            L.check(L.load().dsb_op_norm_join_workspace(n, D, 1, byref(nbytes)),
+                    what="dsb_op_norm_join_workspace")
+            work = _work(nbytes.value, y.device)
+        L.check(L.load().dsb_op_norm_join_bwd(
+            *xargs, *yargs, _at(dnormed), ldn, f32(dnormed), _at(dx_new), ldx, f32(dx_new), _at(w_out),
+            _at(w_in), _at(gate), ldg, kind, scale, eps, n, D, _at(dx), D, f32(dx), _at(dy), D,
+            _at(dgate), D, _at(dw_out), _at(dw_in), _at(work), nbytes.value, _now()),
+            what="dsb_op_norm_join_bwd")
+    return dx, dy, dgate, dw_out, dw_in
+
+
+class RotaryPlan:
+    """The frequencies of rotary positions, on the device; made by :func:`rotary_plan`. ``inv_freq``
+    (numpy, 64 bits), ``factor`` (of cosine and sine), ``head_dim``, ``rotary_dim``,
+    ``interleaved``."""
+
+    __slots__ = ("head_dim", "rotary_dim", "interleaved", "inv_freq", "factor", "turns")
+
+    def __init__(self, head_dim, rotary_dim, interleaved, inv_freq, factor, device):
+        self.head_dim, self.rotary_dim = int(head_dim), int(rotary_dim)
+        self.interleaved, self.factor = bool(interleaved), float(factor)
+        self.inv_freq = inv_freq
+        self.turns = torch.from_numpy(inv_freq / (2 * np.pi)).to(device)
+
+
+def _rotary_frequencies(d, theta, scaling, seq_len):
+    """(inv_freq [d / 2], factor) in 64 bits; ``scaling`` as model configurations spell it."""
+    what = "rotary_plan"
+    rs = dict(scaling or {})
+    kind = rs.get("rope_type", rs.get("type", "default")) or "default"
+    if kind not in ("default", "linear", "dynamic", "llama3", "yarn", "longrope"):
+        raise NotImplementedError(f"{what}: rotary scaling {kind!r} is not supported")
+    inv = theta ** (-np.arange(0, d, 2, dtype=np.float64) / d)
+    if kind == "default":
+        return inv, 1.0
+
+    def given(name):
+        if rs.get(name) is None:
+            raise ValueError(f"{what}: {kind!r} scaling needs {name}")
+        v = float(rs[name])
+        if not (np.isfinite(v) and v > 0):
+            raise ValueError(f"{what}: {name} must be positive")
+        return v
+
+    if kind == "longrope":
+        length = given("original_max_position_embeddings")
+        long = seq_len is not None and seq_len > length
+        by = np.asarray(rs.get("long_factor" if long else "short_factor", ()), dtype=np.float64)
+        if by.shape != inv.shape or not (by > 0).all():
+            raise ValueError(f"{what}: long_factor and short_factor hold {d // 2} positive factors")
+        if rs.get("attention_factor") is not None:
+            return inv / by, given("attention_factor")
+        s = given("factor")
+        return inv / by, np.sqrt(1 + np.log(s) / np.log(length)) if s > 1 else 1.0
+    s = given("factor")
+    if kind == "linear":
+        return inv / s, 1.0
+    length = given("original_max_position_embeddings")
+    if kind == "dynamic":
+        if d < 4:
+            raise ValueError(f"{what}: dynamic scaling needs a rotary_dim of 4 or more")
+        now = max(float(seq_len or length), length)
+        base = theta * (s * now / length - (s - 1)) ** (d / (d - 2))
+        return base ** (-np.arange(0, d, 2, dtype=np.float64) / d), 1.0
+    turns = length * inv / (2 * np.pi)  # a pair's turns over the original length
+    if kind == "llama3":
+        low, high = given("low_freq_factor"), given("high_freq_factor")
+        if not high > low:
+            raise ValueError(f"{what}: high_freq_factor must be above low_freq_factor")
+        keep = np.clip((turns - low) / (high - low), 0, 1)
+        return inv * (keep + (1 - keep) / s), 1.0
+    # yarn: the (fractional) pair that makes n turns over the original length
+    at = lambda n: d * np.log(length / (n * 2 * np.pi)) / (2 * np.log(theta))  # noqa: E731
+    fast, slow = (given(k) if rs.get(k) is not None else v for k, v in (("beta_fast", 32.0), ("beta_slow", 1.0)))
+    low, high = max(np.floor(at(fast)), 0.0), min(np.ceil(at(slow)), d - 1.0)
+    ramp = np.clip((np.arange(d // 2) - low) / max(high - low, 0.001), 0, 1)
+    if rs.get("attention_factor") is not None:
+        factor = given("attention_factor")
+    else:
+        factor = 0.1 * np.log(s) + 1 if s > 1 else 1.0
+    return inv * (1 - ramp) + inv / s * ramp, factor
+
+
+def rotary_plan(head_dim, theta, scaling=None, rotary_dim=None, interleaved=False, seq_len=None,
+                device="cuda"):
+    """The :class:`RotaryPlan` of heads of ``head_dim`` elements (even, to 1024), the first
+    ``rotary_dim`` of which (even; default: all) turn, in pairs of neighbours (``interleaved``) or of
+    the halves' (i, i + rotary_dim / 2), at theta^(−2i / rotary_dim) a position.
+
+    ``scaling``: None or a dict with "rope_type" "linear" (factor), "dynamic" (factor,
+    original_max_position_embeddings; theta grows with ``seq_len`` past it), "llama3" (as
+    :func:`rope_inv_freq`), "yarn" (factor, original_max_position_embeddings, beta_fast 32, beta_slow
+    1, attention_factor 0.1·ln(factor) + 1) or "longrope" (short_factor, long_factor from ``seq_len``
+    past original_max_position_embeddings on, factor or attention_factor). Frequencies are computed in
+    64 bits."""
+    what = "rotary_plan"
+    d = int(head_dim if rotary_dim is None else rotary_dim)
+    if not (2 <= d <= head_dim <= 1024) or d % 2:
+        raise ValueError(f"{what}: rotary_dim must be even, from 2 to head_dim, which is at most 1024")
+    if not theta > 1:
+        raise ValueError(f"{what}: theta must be above 1")
+    inv, factor = _rotary_frequencies(d, float(theta), scaling, seq_len)
+    if torch.device(device).type != "cuda":
+        raise ValueError(f"{what}: the plan's device must be CUDA (HIP)")
+    return RotaryPlan(head_dim, d, interleaved, inv, factor, device)
+
+
+def rotary(x, positions, plan, out=None):
+    """Rotary positions: x [n, heads, head_dim] (bf16, fp16 or fp32; any strides, a head's elements
+    contiguous, so a view of fused q/k/v rows will do) turned by ``positions`` (int32 or int64 [n], below 2^53),
+    in x's type. ``out``: written and returned, of x's shape and type; x itself works in place.
+    Angles are reduced in 64 bits, cosine and sine are fp32."""
+    return _rotary("rotary", x, positions, plan, out, False)
+
+
+def rotary_backward(g, positions, plan, out=None):
+    """The gradient of :func:`rotary`'s input for the gradient g of its result, likewise."""
+    return _rotary("rotary_backward", g, positions, plan, out, True)
+
+
+def _rotary(what, x, positions, plan, out, inverse):
+    if x.dtype not in _DT or x.dim() != 3 or x.shape[2] != plan.head_dim:
+        raise ValueError(f"{what}: takes bf16, fp16 or fp32 [n, heads, {plan.head_dim}]")
+    n, heads, hd = x.shape
+    _vec(what, "positions", positions, n, torch.int32, torch.int64)
+    with _on(what, x, positions, plan.turns, out):
+        if out is None:
+            out = torch.empty(n, heads, hd, dtype=x.dtype, device=x.device)
+        elif out.shape != x.shape or out.dtype != x.dtype:
+            raise ValueError(f"{what}: out must have x's shape and type")
+        if x.numel() and (x.stride(2) != 1 or out.stride(2) != 1):
+            raise ValueError(f"{what}: a head's elements must be contiguous")
+        L.check(L.load().dsb_op_rotary(
+            _at(x), x.stride(0), x.stride(1), _at(out), out.stride(0), out.stride(1), _DT[x.dtype],
+            _at(positions), positions.dtype == torch.int64, _at(plan.turns), plan.factor, n, heads, hd,
+            plan.rotary_dim, plan.interleaved, inverse, _now()), what="dsb_op_rotary")
+    return out

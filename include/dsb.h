@@ -30,8 +30,8 @@ enum {
   DSB_PROJ_Q = 0, DSB_PROJ_K = 1, DSB_PROJ_V = 2, DSB_PROJ_O = 3,
   DSB_PROJ_GATE = 4, DSB_PROJ_UP = 5, DSB_PROJ_DOWN = 6, DSB_NUM_PROJ = 7
 };
-/* element types of the capture entry points */
-enum { DSB_DT_BF16 = 0, DSB_DT_F16 = 1, DSB_DT_F32 = 2 };
+/* element types of the capture entry points and of rows (the last two: 8-bit rows, below) */
+enum { DSB_DT_BF16 = 0, DSB_DT_F16 = 1, DSB_DT_F32 = 2, DSB_DT_E4M3 = 3, DSB_DT_INT8 = 4 };
 /* dsb_desc.flags */
 /* DSB_FLAG_SERIAL_LAYERS: run each layer's recompute right before its
    backward on the cycle's stream, instead of beside the previous layer's
@@ -509,6 +509,76 @@ int dsb_op_adam_step(const dsb_adam_chunk* chunks, int nchunks, const int32_t* g
                      double weight_decay, double max_norm, int64_t step, uint32_t seed,
                      const float* lr_dev, const int64_t* step_dev, float* norms, void* work,
                      int64_t work_bytes, void* stream);
+
+/* ---- a decoder block's memory-bound operators, with its activations kept in 8 bits
+ *
+ * No counterpart in the reference, which keeps activations in bf16 and knows the pre-norm block with
+ * rotate-half positions alone. Stream-ordered like the ops above: they allocate nothing and do
+ * not synchronise, `work` is scratch of at least the bytes that the *_workspace call gives. The
+ * stream's device has to be the current one. Row counts are below 2^24; strides count elements. Outputs
+ * overlap neither each other nor an input, but where a call says so.
+ *
+ * 8-bit rows (types DSB_DT_E4M3 and DSB_DT_INT8): codes of one byte, and a byte per
+ * DSB_ROWS8_BLOCK columns of a row, from the row's first, the exponent of their scale + 127. A value is
+ * code·2^(byte − 127); byte 255 makes NaN of a code of 0. Saving takes the least exponent, at least −126, that brings the
+ * block's largest magnitude to at most 448 (e4m3) or 127 (int8) and rounds to the nearest code, ties to
+ * even; a block that holds an infinity or a NaN is kept as NaN whole. */
+enum { DSB_ROWS8_BLOCK = 32 };
+/* dsb_save_rows into 8-bit rows: codes (row stride ldc) and scales (ldsc) of buf_rows rows, the last of
+ * them the scratch row. src and dst null: rows 0 to count − 1 of x into those of the buffer, the last one
+ * included. Any width, strides and alignment; whole 16-byte accesses where they allow them. */
+int dsb_save_rows8(const void* x, int64_t ldx, const void* r, int64_t ldr, int64_t x_rows, int x_dtype,
+                   const int64_t* src, const int64_t* dst, int count, int width, void* codes,
+                   int64_t ldc, uint8_t* scales, int64_t ldsc, int code, int64_t buf_rows, void* stream);
+/* The values of 8-bit rows [rows, width], bf16 (exact, but for subnormals) or fp32. */
+int dsb_op_restore_rows8(const void* codes, int64_t ldc, const uint8_t* scales, int64_t ldsc, int code,
+                         int rows, int width, void* out, int64_t ldo, int out_f32, void* stream);
+/* h [rows, I] = bf16(silu(gate)·up) of gate‖up rows [rows, 2I], bf16 or 8-bit (gu_type; scales null for
+ * bf16); and their gradient dgu [rows, 2I] (bf16) for dh (bf16 or fp32), with h too unless it is null.
+ * I a multiple of 8; bf16 and fp32 rows 16-byte aligned with strides of whole 16 bytes, codes 8-byte aligned
+ * with strides of a multiple of 8. */
+int dsb_op_swiglu(const void* gu, int64_t ldgu, const uint8_t* gu_scales, int64_t ldsc, int gu_type,
+                  int rows, int I, void* h, int64_t ldh, void* stream);
+int dsb_op_swiglu_bwd(const void* gu, int64_t ldgu, const uint8_t* gu_scales, int64_t ldsc, int gu_type,
+                      int rows, int I, const void* dh, int64_t lddh, int dh_f32, void* dgu,
+                      int64_t lddgu, void* h, int64_t ldh, void* stream);
+/* The join of a block's output y with the residual stream x and the norms around it, by row:
+ *   z = y / rms(y)·w_out (y where w_out is null),  x_new = x + scale·gate·z,
+ *   normed = x_new / rms(x_new)·w_in,  rms(v) = sqrt(mean(v²) + eps)
+ * x and x_new bf16 or fp32 (x_type), y, normed and the weights [D] bf16, the gate bf16 [D] (DSB_GATE_CHANNEL),
+ * a value a row, ldg apart (_ROW), or rows of stride ldg (_FULL). w_in and normed null: no norm after. y null: a
+ * norm alone of x, which may then be 8-bit rows; x_new, w_out and the gate are null. D a multiple
+ * of 8 up to 8192, alignment as for SwiGLU. normed is of x_new as it is kept. */
+enum { DSB_GATE_NONE = 0, DSB_GATE_CHANNEL = 1, DSB_GATE_ROW = 2, DSB_GATE_FULL = 3 };
+int dsb_op_norm_join(const void* x, int64_t ldx, const uint8_t* x_scales, int64_t ldxs, int x_type,
+                     const void* y, int64_t ldy, const void* w_out, const void* w_in, const void* gate,
+                     int64_t ldg, int gate_kind, double scale, double eps, int rows, int D, void* x_new,
+                     int64_t ldxn, void* normed, int64_t ldn, void* stream);
+/* Its backward from x_new (bf16, fp32 or 8-bit rows) and y (bf16 or 8-bit rows), given the gradients dn of
+ * normed and dxn of x_new (bf16 or fp32 each; null: zeros; dn null: w_in and x_new are not used):
+ *   dx (bf16 or fp32, of x and of x_new's whole), dy (bf16), dw_out and dw_in fp32 [D] (null: not wanted),
+ *   dgate: null (not wanted), fp32 [D], fp32 [rows] or bf16 rows of stride lddg, as the gate's kind is.
+ * y null: the gradient of a norm alone. `sums`: whether any of dw_out, dw_in and a channel
+ * gate's dgate is wanted; they are added over rows in fp32 in a fixed order. */
+int dsb_op_norm_join_workspace(int rows, int D, int sums, int64_t* bytes);
+int dsb_op_norm_join_bwd(const void* x_new, int64_t ldx, const uint8_t* x_scales, int64_t ldxs,
+                         int x_type, const void* y, int64_t ldy, const uint8_t* y_scales, int64_t ldys,
+                         int y_type, const void* dn, int64_t lddn, int dn_f32, const void* dxn,
+                         int64_t lddxn, int dxn_f32, const void* w_out, const void* w_in,
+                         const void* gate, int64_t ldg, int gate_kind, double scale, double eps,
+                         int rows, int D, void* dx, int64_t lddx, int dx_f32, void* dy, int64_t lddy,
+                         void* dgate, int64_t lddg, float* dw_out, float* dw_in, void* work,
+                         int64_t work_bytes, void* stream);
+/* Rotary positions: element h·hx + i of row t of x (head h, row stride ldx, of x_dtype) into y likewise,
+ * the pairs (2i, 2i + 1) (interleaved) or (i, i + rot / 2) of the first `rot` elements of a head
+ * turned by pos[t]·2π·turns[i] and scaled by `factor`, the others as they are. turns: fp64 [rot / 2];
+ * pos: int32, or int64 below 2^53 in size (pos64). inverse: turned back, which with the same factor is
+ * the gradient. y may be x; they do not overlap otherwise. rot is even, at most DSB_ROTARY_MOST; n·heads
+ * below 2^26, heads·head_dim up to 2^20. */
+enum { DSB_ROTARY_MOST = 1024 };
+int dsb_op_rotary(const void* x, int64_t ldx, int64_t hx, void* y, int64_t ldy, int64_t hy, int dtype,
+                  const void* pos, int pos64, const double* turns, double factor, int n, int heads,
+                  int head_dim, int rot, int interleaved, int inverse, void* stream);
 
 #ifdef __cplusplus
 }
