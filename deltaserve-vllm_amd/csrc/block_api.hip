@@ -225,16 +225,18 @@ int dsb_op_norm_join_bwd(const void* x_new, int64_t ldx, const uint8_t* x_scales
   if (gate_kind == kGateFull) a.dgate_full = (bf16*)dgate;
   a.lddg = lddg;
   if (dgate && gate_kind == kGateNone) return bad(what, "dgate without a gate");
+  if (dgate == nullptr && gate_kind == kGateFull && rows > 0) return bad(what, "null argument");
+  if (rows > 0 && !has_y && dw_in) return bad(what, "dw_in comes with a block");
   if ((dw_in && !w_in) || (dw_out && !w_out)) return bad(what, "a weight's gradient without the weight");
   if (misaligned(dw_in, 16) || misaligned(dw_out, 16) || misaligned(a.dgate, 16) || misaligned(a.dgate_row, 4))
     return bad(what, "gradients of vectors must be 16-byte aligned");
   if (rows > 0) {
     if (!dn != !w_in) return bad(what, "dn and w_in are given together or not at all");
     if (!dn && !dxn) return bad(what, "there is no gradient to start from");
+    if (!has_y && !dn) return bad(what, "there is neither a block nor a norm");
     if (y && !has_y) return bad(what, "dy is null");
     if (dn)
       if (const char* e = check_rows(a.x, rows, D, kFloats | kCodes)) return bad(what, e);
-    if (!dn) a.x.type = DSB_DT_BF16;
     if (has_y)
       if (const char* e = check_rows(a.y, rows, D, kHalf | kCodes)) return bad(what, e);
     if (dn)

@@ -15,8 +15,9 @@
 // so that one pass over a row takes six sums at once and one barrier a row does. All of it is fp32,
 // rounded once where it is stored; the kernels are bound by their bytes.
 //
-// A block of threads takes row after row, two runs of 8 columns a thread; the weights stay in its
-// registers and so do its sums over rows, which a second launch adds up over the blocks, in order.
+// A block of threads takes row after row, the next one's loads on their way while it computes; the weights
+// stay in its registers and so do its sums over rows, which a second launch adds up over the
+// blocks, in order.
 #include <algorithm>
 #include <type_traits>
 
@@ -26,46 +27,52 @@ namespace dsb {
 
 namespace {
 
-constexpr int kRuns = 2;                       // of 8 columns a thread
-constexpr int kMostThreads = 8192 / 8 / kRuns;  // D <= 8192
+constexpr int kMostThreads = 1024;  // 8 columns each: D <= 8192
 constexpr int kMostWaves = kMostThreads / 64;
 
-// The sum over a wave, the same for all: within rows of 16 lanes, then over them.
-DSB_DEV float wave_total(float v) {
-  auto dpp = [](float x, auto ctrl, auto rows) {
-    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(
-        0, __builtin_bit_cast(int, x), decltype(ctrl)::value, decltype(rows)::value, 0xf, false));
-  };
-  using std::integral_constant;
-  v += dpp(v, integral_constant<int, 0x128>{}, integral_constant<int, 0xf>{});  // row_ror:8
-  v += dpp(v, integral_constant<int, 0x124>{}, integral_constant<int, 0xf>{});
-  v += dpp(v, integral_constant<int, 0x122>{}, integral_constant<int, 0xf>{});
-  v += dpp(v, integral_constant<int, 0x121>{}, integral_constant<int, 0xf>{});
-  v += dpp(v, integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{});  // row_bcast:15
-  v += dpp(v, integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});  // row_bcast:31
-  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+template <int CTRL, int ROWS>
+DSB_DEV float dpp_add(float v) {
+  return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(
+                 0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, false));
+}
+// The sum over each 16 lanes, in all of them.
+DSB_DEV float row_total(float v) {
+  v = dpp_add<0x128, 0xf>(v);  // row_ror:8, 4, 2, 1
+  v = dpp_add<0x124, 0xf>(v);
+  v = dpp_add<0x122, 0xf>(v);
+  return dpp_add<0x121, 0xf>(v);
 }
 
 // K sums over the block, the same for all. red holds two sets of them, taken in turn: a set is
 // written again only after the barrier of the call between, which every wave reaches after it has
-// read the set, so one barrier a call is enough.
+// read the set, so one barrier a call is enough. (It orders LDS alone: a fence would wait for the next
+// row's loads.)
 template <int K>
 DSB_DEV void block_totals(float (&v)[K], float (&red)[2][kMostWaves][8], int& turn) {
 #pragma unroll
-  for (int k = 0; k < K; ++k) v[k] = wave_total(v[k]);
-  const int waves = blockDim.x >> 6;
-  if (waves == 1) return;
-  if ((threadIdx.x & 63) == 0) {
+  for (int k = 0; k < K; ++k) {
+    v[k] = row_total(v[k]);
+    v[k] = dpp_add<0x142, 0xa>(v[k]);  // row_bcast:15 into rows 1 and 3
+    v[k] = dpp_add<0x143, 0xc>(v[k]);  // row_bcast:31 into rows 2 and 3: lane 63 has all
+  }
+  const int waves = blockDim.x >> 6, lane = threadIdx.x & 63;
+  if (waves == 1) {
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+      v[k] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v[k]), 63));
+    return;
+  }
+  if (lane == 63) {
 #pragma unroll
     for (int k = 0; k < K; ++k) red[turn][threadIdx.x >> 6][k] = v[k];
   }
-  __syncthreads();
+  wait_lgkm0();
+  lds_barrier();
+  const int w = lane & 15;
 #pragma unroll
-  for (int k = 0; k < K; ++k) v[k] = 0.f;
-  for (int w = 0; w < waves; ++w) {
+  for (int k = 0; k < K; ++k) v[k] = w < waves ? red[turn][w][k] : 0.f;
 #pragma unroll
-    for (int k = 0; k < K; ++k) v[k] += red[turn][w][k];
-  }
+  for (int k = 0; k < K; ++k) v[k] = row_total(v[k]);
   turn ^= 1;
 }
 
@@ -76,15 +83,16 @@ DSB_DEV void weights8(u32x4 raw, bool have, float v[8]) {
   for (int e = 0; e < 8; ++e) v[e] = have ? v[e] : 1.f;
 }
 
-template <int XK, int YK>
-__global__ __launch_bounds__(kMostThreads) void join_fwd_kernel(JoinArgs a) {
+// R runs of 8 columns a thread; XK, YK: the types of x and y.
+template <int XK, int YK, int P, int R>
+__global__ __launch_bounds__(kMostThreads / 2) void join_fwd_kernel(JoinArgs a) {
   __shared__ float red[2][kMostWaves][8];
   int turn = 0;
   const int nch = a.D >> 3;
   const float rD = 1.f / (float)a.D;
-  u32x4 wo[kRuns] = {}, wi[kRuns] = {}, gc[kRuns] = {};
+  u32x4 wo[R] = {}, wi[R] = {}, gc[R] = {};
 #pragma unroll
-  for (int i = 0; i < kRuns; ++i) {
+  for (int i = 0; i < R; ++i) {
     const int c = threadIdx.x + i * blockDim.x;
     if (c < nch) {
       if (YK != kRowsNone && a.w_out) wo[i] = ldg128(a.w_out + 8 * c);
@@ -93,15 +101,16 @@ __global__ __launch_bounds__(kMostThreads) void join_fwd_kernel(JoinArgs a) {
     }
   }
   for (long row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    Raw8<XK> x[kRuns];
-    Raw8<YK> y[kRuns];
+    Raw8<XK> x[R];
+    Raw8<YK> y[R];
 #pragma unroll
-    for (int i = 0; i < kRuns; ++i) {
+    for (int i = 0; i < R; ++i) {
       const int c = threadIdx.x + i * blockDim.x;
       if (c < nch) {
-        x[i].load(a.x, row, c);
-        y[i].load(a.y, row, c);
-        if (YK != kRowsNone && a.gate_kind == kGateFull) gc[i] = ldg128_nt(a.gate + row * a.ldg + 8 * c);
+        x[i].template load<P>(a.x, row, c);
+        y[i].template load<P>(a.y, row, c);
+        if (YK != kRowsNone && a.gate_kind == kGateFull)
+          gc[i] = load_as<P, u32x4>(a.gate + row * a.ldg + 8 * c);
       }
     }
     const float gr = YK != kRowsNone && a.gate_kind == kGateRow ? (float)a.gate[row * a.ldg] : 1.f;
@@ -110,10 +119,10 @@ __global__ __launch_bounds__(kMostThreads) void join_fwd_kernel(JoinArgs a) {
     if (YK != kRowsNone && a.w_out) {
       float ss[1] = {0.f};
 #pragma unroll
-      for (int i = 0; i < kRuns; ++i) {
+      for (int i = 0; i < R; ++i) {
         if (threadIdx.x + i * blockDim.x < nch) {
           float yv[8];
-          y[i].get(a.y, yv);
+          y[i].get(yv);
 #pragma unroll
           for (int e = 0; e < 8; ++e) ss[0] += yv[e] * yv[e];
         }
@@ -121,23 +130,23 @@ __global__ __launch_bounds__(kMostThreads) void join_fwd_kernel(JoinArgs a) {
       block_totals(ss, red, turn);
       j = rsqrtf(ss[0] * rD + a.eps);
     }
-    float xv[kRuns][8], ss[1] = {0.f};
+    float xv[R][8], ss[1] = {0.f};
 #pragma unroll
-    for (int i = 0; i < kRuns; ++i) {
+    for (int i = 0; i < R; ++i) {
       const int c = threadIdx.x + i * blockDim.x;
       if (c < nch) {
-        x[i].get(a.x, xv[i]);
+        x[i].get(xv[i]);
         if (YK != kRowsNone) {
           float yv[8], w[8], g[8];
-          y[i].get(a.y, yv);
+          y[i].get(yv);
           weights8(wo[i], a.w_out, w);
           weights8(gc[i], each, g);
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             xv[i][e] += a.scale * (g[e] * gr) * (yv[e] * j * w[e]);
-            if (XK == kRowsBF16) xv[i][e] = (float)(bf16)xv[i][e];  // the norm is of the rows as they are kept
+            if (XK == DSB_DT_BF16) xv[i][e] = (float)(bf16)xv[i][e];  // the norm is of the rows as they are kept
           }
-          put8(a.x_new, row * a.ldxn + 8 * c, XK == kRowsF32, xv[i]);
+          put8<P>(a.x_new, row * a.ldxn + 8 * c, XK == DSB_DT_F32, xv[i]);
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) ss[0] += xv[i][e] * xv[i][e];
@@ -147,84 +156,82 @@ __global__ __launch_bounds__(kMostThreads) void join_fwd_kernel(JoinArgs a) {
     block_totals(ss, red, turn);
     const float inv = rsqrtf(ss[0] * rD + a.eps);
 #pragma unroll
-    for (int i = 0; i < kRuns; ++i) {
+    for (int i = 0; i < R; ++i) {
       const int c = threadIdx.x + i * blockDim.x;
       if (c < nch) {
         float w[8], o[8];
         unpack8(wi[i], w);
 #pragma unroll
         for (int e = 0; e < 8; ++e) o[e] = (xv[i][e] * inv) * w[e];
-        put8(a.normed, row * a.ldn + 8 * c, false, o);
+        put8<P>(a.normed, row * a.ldn + 8 * c, false, o);
       }
     }
   }
 }
 
-// SUMS: sums over rows too, by block into part [3][gridDim.x][D] (w_in, w_out, gate).
-template <int XK, int YK, int GK, bool SUMS>
-__global__ __launch_bounds__(kMostThreads) void join_bwd_kernel(JoinArgs a, float* part) {
-  constexpr bool Y = YK != kRowsNone;
+// R runs of 8 columns a thread; XT, YT, GT: the types of x', y and dn, FULL: a gate of rows. With a block
+// its sums over rows go into part [2][gridDim.x][D]: Σ dn·x̂, and Σ t·ŷ with a gate that differs by row,
+// of which dw_out and a channel gate's dgate are multiples (join_sums_kernel).
+template <int XT, int YT, int GT, bool FULL, int P, int R>
+__global__ __launch_bounds__(R == 1 ? kMostThreads : kMostThreads / 2) void join_bwd_kernel(JoinArgs a, float* part) {
+  constexpr bool Y = YT != kRowsNone, N = GT != kRowsNone;
   __shared__ float red[2][kMostWaves][8];
   int turn = 0;
   const int nch = a.D >> 3;
   const float rD = 1.f / (float)a.D;
-  u32x4 wo[kRuns] = {}, wi[kRuns] = {}, gc[kRuns] = {};
-  float s_in[kRuns][8] = {}, s_out[kRuns][8] = {}, s_gate[kRuns][8] = {};
+  float cw[Y ? R : 1][8];  // w_out·a gate by channel
+  u32x4 wi[R] = {};
 #pragma unroll
-  for (int i = 0; i < kRuns; ++i) {
+  for (int i = 0; i < R; ++i) {
     const int c = threadIdx.x + i * blockDim.x;
     if (c < nch) {
-      if (Y && a.w_out) wo[i] = ldg128(a.w_out + 8 * c);
-      if (a.w_in) wi[i] = ldg128(a.w_in + 8 * c);
-      if (Y && a.gate_kind == kGateChannel) gc[i] = ldg128(a.gate + 8 * c);
+      if (N) wi[i] = ldg128(a.w_in + 8 * c);
+      if constexpr (Y) {
+        float g[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) cw[i][e] = g[e] = 1.f;
+        if (a.w_out) unpack8(ldg128(a.w_out + 8 * c), cw[i]);
+        if (a.gate_kind == kGateChannel) unpack8(ldg128(a.gate + 8 * c), g);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) cw[i][e] *= g[e];
+      }
     }
   }
-  const bool each = a.gate_kind == kGateChannel || a.gate_kind == kGateFull;
+  float s_in[Y ? R : 1][8] = {}, s_out[Y ? R : 1][8] = {};
   for (long row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    Raw8<XK> x[kRuns];
-    Raw8<YK> y[kRuns];
-    Raw8<GK> dn[kRuns];
-    u32x4 ta[kRuns] = {}, tb[kRuns] = {};  // dx', bf16 or fp32
+    Raw8<XT> x[R];
+    Raw8<YT> y[R];
+    Raw8<GT> dn[R];
+    u32x4 ta[R] = {}, tb[R] = {}, gf[R];  // dx' (bf16 or fp32), a gate of rows
 #pragma unroll
-    for (int i = 0; i < kRuns; ++i) {
+    for (int i = 0; i < R; ++i) {
       const int c = threadIdx.x + i * blockDim.x;
       if (c < nch) {
-        if (GK != kRowsNone) x[i].load(a.x, row, c);
-        y[i].load(a.y, row, c);
-        dn[i].load(a.dn, row, c);
+        if (N) x[i].template load<P>(a.x, row, c);
+        y[i].template load<P>(a.y, row, c);
+        dn[i].template load<P>(a.dn, row, c);
         if (a.dxn.p) {
           if (a.dxn.type == DSB_DT_F32) {
             const float* p = (const float*)a.dxn.p + row * a.dxn.ld + 8 * c;
-            ta[i] = ldg128_nt(p);
-            tb[i] = ldg128_nt(p + 4);
+            ta[i] = load_as<P, u32x4>(p);
+            tb[i] = load_as<P, u32x4>(p + 4);
           } else {
-            ta[i] = ldg128_nt((const bf16*)a.dxn.p + row * a.dxn.ld + 8 * c);
+            ta[i] = load_as<P, u32x4>((const bf16*)a.dxn.p + row * a.dxn.ld + 8 * c);
           }
         }
-        if (Y && a.gate_kind == kGateFull) gc[i] = ldg128_nt(a.gate + row * a.ldg + 8 * c);
+        if (FULL) gf[i] = load_as<P, u32x4>(a.gate + row * a.ldg + 8 * c);
       }
     }
     const float gr = Y && a.gate_kind == kGateRow ? (float)a.gate[row * a.ldg] : 1.f;
-    auto carried = [&](int i, float v[8]) {
-      if (a.dxn.type == DSB_DT_F32) {  // the same for all
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const unsigned p = ta[i][e], q = tb[i][e];
-          v[e] = __builtin_bit_cast(float, p);
-          v[4 + e] = __builtin_bit_cast(float, q);
-        }
-      } else {
-        unpack8(ta[i], v);
-      }
-    };
     // Σ x'², Σ dn·w_in·x', Σ y², Σ c·y·dx', Σ c·y·dn·w_in, Σ c·y·x'; c without a row's gate
     float s[Y ? 6 : 2] = {};
 #pragma unroll
-    for (int i = 0; i < kRuns; ++i) {
-      if (threadIdx.x + i * blockDim.x < nch) {
-        float xv[8] = {}, dv[8], w[8];
-        if (GK != kRowsNone) x[i].get(a.x, xv);
-        dn[i].get(a.dn, dv);
+    for (int i = 0; i < R; ++i) {
+      if (threadIdx.x + i * blockDim.x >= nch) continue;
+      float xv[8], dv[8], yv[8], t[8], w[8], g[8];
+      if (N) {
+        x[i].get(xv);
+        dn[i].get(dv);
         unpack8(wi[i], w);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -232,17 +239,20 @@ __global__ __launch_bounds__(kMostThreads) void join_bwd_kernel(JoinArgs a, floa
           s[0] += xv[e] * xv[e];
           s[1] += dv[e] * xv[e];
         }
-        if constexpr (Y) {
-          float yv[8], tv[8], wv[8], gv[8];
-          y[i].get(a.y, yv);
-          carried(i, tv);
-          weights8(wo[i], a.w_out, wv);
-          weights8(gc[i], each, gv);
+      }
+      if constexpr (Y) {
+        y[i].get(yv);
+        if (a.dxn.type == DSB_DT_F32)
+          floats8(ta[i], tb[i], t);
+        else
+          unpack8(ta[i], t);
+        if (FULL) unpack8(gf[i], g);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float cy = gv[e] * wv[e] * yv[e];
-            s[2] += yv[e] * yv[e];
-            s[3] += cy * tv[e];
+        for (int e = 0; e < 8; ++e) {
+          const float cy = (FULL ? cw[i][e] * g[e] : cw[i][e]) * yv[e];
+          s[2] += yv[e] * yv[e];
+          s[3] += cy * t[e];
+          if (N) {
             s[4] += cy * dv[e];
             s[5] += cy * xv[e];
           }
@@ -255,153 +265,219 @@ __global__ __launch_bounds__(kMostThreads) void join_bwd_kernel(JoinArgs a, floa
     float j = 1.f, m = 0.f;           // 1 / rms(y), mean(α·gate·t·w_out·ŷ)
     if constexpr (Y) {
       float p = s[3];
-      if (GK != kRowsNone) p += inv * (s[4] - k * (inv * s[5]));
+      if (N) p += inv * (s[4] - k * (inv * s[5]));
       if (a.w_out) {
         j = rsqrtf(s[2] * rD + a.eps);
         m = a.scale * gr * p * j * rD;
       }
       if (a.dgate_row && threadIdx.x == 0) a.dgate_row[row] = a.scale * p * j;
     }
+    const float to_y = a.scale * gr * j, back = m * j;
 #pragma unroll
-    for (int i = 0; i < kRuns; ++i) {
+    for (int i = 0; i < R; ++i) {
       const int c = threadIdx.x + i * blockDim.x;
-      if (c < nch) {
-        float t[8];
-        carried(i, t);
-        if (GK != kRowsNone) {
-          float xv[8], dv[8], w[8];
-          x[i].get(a.x, xv);
-          dn[i].get(a.dn, dv);
-          unpack8(wi[i], w);
+      if (c >= nch) continue;
+      float t[8];
+      if (a.dxn.type == DSB_DT_F32)
+        floats8(ta[i], tb[i], t);
+      else
+        unpack8(ta[i], t);
+      if (N) {
+        float xv[8], dv[8], w[8];
+        x[i].get(xv);
+        dn[i].get(dv);
+        unpack8(wi[i], w);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float hat = xv[e] * inv;
+          t[e] += (dv[e] * w[e] - hat * k) * inv;
+          if (Y) s_in[i][e] += dv[e] * hat;
+        }
+      }
+      put8<P>(a.dx, row * a.lddx + 8 * c, a.dx_f32, t);
+      if constexpr (Y) {
+        float yv[8], g[8], o[8];
+        y[i].get(yv);
+        if (FULL) unpack8(gf[i], g);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          yv[e] *= j;
+          o[e] = (FULL ? cw[i][e] * g[e] : cw[i][e]) * t[e] * to_y;
+        }
+        if (a.w_out) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) o[e] -= yv[e] * back;
+        }
+        put8<P>(a.dy, row * a.lddy + 8 * c, false, o);
+        if (FULL) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            const float hat = xv[e] * inv;
-            t[e] += (dv[e] * w[e] - hat * k) * inv;
-            if (SUMS) s_in[i][e] += dv[e] * hat;
+            o[e] = a.scale * (t[e] * yv[e]) * cw[i][e];
+            yv[e] *= g[e];
           }
-        }
-        put8(a.dx, row * a.lddx + 8 * c, a.dx_f32, t);
-        if constexpr (Y) {
-          float yv[8], wv[8], gv[8], o[8], q[8];
-          y[i].get(a.y, yv);
-          weights8(wo[i], a.w_out, wv);
-          weights8(gc[i], each, gv);
+          put8<P>(a.dgate_full, row * a.lddg + 8 * c, false, o);
+        } else if (a.gate_kind == kGateRow) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float hat = yv[e] * j, at = a.scale * t[e], dz = gv[e] * gr * at;
-            o[e] = a.w_out ? (dz * wv[e] - hat * m) * j : dz;
-            q[e] = at * hat * wv[e];
-            if (SUMS) {
-              s_out[i][e] += dz * hat;
-              s_gate[i][e] += q[e];
-            }
-          }
-          put8(a.dy, row * a.lddy + 8 * c, false, o);
-          if (a.dgate_full) put8(a.dgate_full, row * a.lddg + 8 * c, false, q);
+          for (int e = 0; e < 8; ++e) yv[e] *= gr;
         }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s_out[i][e] += t[e] * yv[e];
       }
     }
   }
-  if (SUMS) {
+  if constexpr (Y) {
+    if (!part) return;
     const long plane = (long)gridDim.x * a.D;
 #pragma unroll
-    for (int i = 0; i < kRuns; ++i) {
+    for (int i = 0; i < R; ++i) {
       const int c = threadIdx.x + i * blockDim.x;
-      if (c < nch) {
-        float* p = part + (long)blockIdx.x * a.D + 8 * c;
-        auto put = [&](float* o, const float* v) {
-          *reinterpret_cast<f32x4*>(o) = f32x4{v[0], v[1], v[2], v[3]};
-          *reinterpret_cast<f32x4*>(o + 4) = f32x4{v[4], v[5], v[6], v[7]};
-        };
-        if (a.dw_in) put(p, s_in[i]);
-        if (a.dw_out) put(p + plane, s_out[i]);
-        if (a.dgate) put(p + 2 * plane, s_gate[i]);
-      }
+      if (c >= nch) continue;
+      auto put = [&](float* o, const float* v) {
+        *reinterpret_cast<f32x4*>(o) = f32x4{v[0], v[1], v[2], v[3]};
+        *reinterpret_cast<f32x4*>(o + 4) = f32x4{v[4], v[5], v[6], v[7]};
+      };
+      float* p = part + (long)blockIdx.x * a.D + 8 * c;
+      if (a.dw_in) put(p, s_in[i]);
+      put(p + plane, s_out[i]);
     }
   }
 }
 
-// out[k][c] = Σ_b part[k][b][c]: 32 columns a block, 32 threads to each group of 4 of them.
-__global__ __launch_bounds__(256) void join_sums_kernel(const float* __restrict__ part, int blocks,
-                                                        int D, float* o0, float* o1, float* o2) {
-  float* out = blockIdx.y == 0 ? o0 : blockIdx.y == 1 ? o1 : o2;
-  if (!out) return;
-  __shared__ f32x4 red[256];
-  const int c = blockIdx.x * 32 + (threadIdx.x & 7) * 4, g = threadIdx.x >> 3;
+// The sums over the blocks, kSumLanes threads to a row of 4 columns each and as many rows at once as a
+// workgroup has threads for: dw_in from plane 0; dw_out (times α·a channel gate) and dgate (times
+// α·w_out) from plane 1.
+constexpr int kSumLanes = 8, kSumThreads = 512;
+__global__ __launch_bounds__(kSumThreads) void join_sums_kernel(JoinArgs a, const float* __restrict__ part,
+                                                                int blocks) {
+  const bool first = blockIdx.y == 0;
+  if (first ? !a.dw_in : !a.dw_out && !a.dgate) return;
+  __shared__ f32x4 red[kSumThreads];
+  const int t = threadIdx.x, c = (blockIdx.x * kSumLanes + t % kSumLanes) * 4;
   f32x4 s = {0.f, 0.f, 0.f, 0.f};
-  if (c < D) {
-    const float* p = part + (long)blockIdx.y * blocks * D + c;
+  if (c < a.D) {
+    const float* p = part + (long)blockIdx.y * blocks * a.D + c;
 #pragma unroll 8
-    for (int b = g; b < blocks; b += 32) s += *reinterpret_cast<const f32x4*>(p + (long)b * D);
+    for (int b = t / kSumLanes; b < blocks; b += kSumThreads / kSumLanes)
+      s += *reinterpret_cast<const f32x4*>(p + (long)b * a.D);
   }
-  red[threadIdx.x] = s;
+  red[t] = s;
   __syncthreads();
-  if (threadIdx.x < 8 && c < D) {
-    for (int i = 1; i < 32; ++i) s += red[threadIdx.x + 8 * i];
-    *reinterpret_cast<f32x4*>(out + c) = s;
+  if (t < 64) {
+    for (int i = 64; i < kSumThreads; i += 64) s += red[t + i];
+    red[t] = s;
   }
+  __syncthreads();
+  if (t >= kSumLanes || c >= a.D) return;
+  for (int i = kSumLanes; i < 64; i += kSumLanes) s += red[t + i];
+  if (first) {
+    *reinterpret_cast<f32x4*>(a.dw_in + c) = s;
+    return;
+  }
+  s *= a.scale;
+  auto times = [&](const bf16* v) {
+    f32x4 r = s;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) r[e] *= v ? (float)v[c + e] : 1.f;
+    return r;
+  };
+  if (a.dw_out) *reinterpret_cast<f32x4*>(a.dw_out + c) = times(a.gate_kind == kGateChannel ? a.gate : nullptr);
+  if (a.dgate) *reinterpret_cast<f32x4*>(a.dgate + c) = times(a.w_out);
 }
 
-int threads_of(int D) { return std::max(64, (D / 8 + kRuns * 64 - 1) / (kRuns * 64) * 64); }
-constexpr int kFwdBlocks = 2048, kBwdBlocks = 512;
+int waves_of(int D, int runs) { return (D / 8 + 64 * runs - 1) / (64 * runs); }
+constexpr int kCUs = 256;
+// Threads of a kernel that keeps no sums: the chip's.
+constexpr int kThreads = 1 << 19;
+int blocks_of(int rows, int D, int runs) { return std::min(rows, kThreads / (64 * waves_of(D, runs))); }
+// With sums a thread needs 170 to 250 registers, so that a CU holds 8 waves: whole blocks of them. Two
+// runs a thread, or three where more blocks fit that way (640 columns' runs: one block of 5 waves, or two of 4).
+constexpr int kSumWaves = 8;
+int best_runs(int D) {
+  return kSumWaves / waves_of(D, 3) > kSumWaves / waves_of(D, 2) ? 3 : 2;
+}
+int sum_blocks(int rows, int D) {
+  const int most = kCUs * std::max(1, kSumWaves / waves_of(D, best_runs(D)));
+  // a CU has a block before a block has a second row, whose sums cost nothing more to write out
+  return rows <= kCUs ? rows : std::min(std::max(kCUs, (rows + 1) / 2), most);
+}
 
 }  // namespace
 
 hipError_t join_fwd(const JoinArgs& a, hipStream_t s) {
   if (a.rows <= 0) return hipSuccess;
+  const double in = row_bytes(a.x) + row_bytes(a.y) + (a.gate_kind == kGateFull ? 2 : 0);
+  const double out = (a.x_new ? row_bytes(a.x) : 0) + (a.normed ? 2 : 0);
+  const bool near = cache_of(in * a.rows * a.D, out * a.rows * a.D) == kNear;
+  const int runs = best_runs(a.D);
   auto go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(std::min(a.rows, kFwdBlocks)), dim3(threads_of(a.D)), 0, s, a);
+    hipLaunchKernelGGL(kernel, dim3(blocks_of(a.rows, a.D, runs)), dim3(64 * waves_of(a.D, runs)), 0, s, a);
     return hipGetLastError();
   };
-  auto by_x = [&](auto k) {
-    constexpr int K = decltype(k)::value;
-    return a.y.p ? go(join_fwd_kernel<K, kRowsBF16>) : go(join_fwd_kernel<K, kRowsNone>);
+  auto by_cache = [&](auto x, auto y) {
+    constexpr int X = decltype(x)::value, Y = decltype(y)::value;
+    if (runs == 2) return near ? go(join_fwd_kernel<X, Y, kNear, 2>) : go(join_fwd_kernel<X, Y, kFar, 2>);
+    return near ? go(join_fwd_kernel<X, Y, kNear, 3>) : go(join_fwd_kernel<X, Y, kFar, 3>);
   };
-  switch (rows_kind(a.x.type)) {
-    case kRowsBF16: return by_x(std::integral_constant<int, kRowsBF16>{});
-    case kRowsF32: return by_x(std::integral_constant<int, kRowsF32>{});
-    default: return a.y.p ? hipErrorInvalidValue : go(join_fwd_kernel<kRows8, kRowsNone>);
-  }
+  return by_type(a.x, [&](auto x) {
+    constexpr int X = decltype(x)::value;
+    if constexpr (X == DSB_DT_BF16 || X == DSB_DT_F32)
+      if (a.y.p) return by_cache(x, Int<DSB_DT_BF16>{});
+    return by_cache(x, Int<kRowsNone>{});
+  });
 }
 
 int64_t join_bwd_bytes(int rows, int D, int sums) {
-  return sums ? 12ll * std::min(rows, kBwdBlocks) * D : 0;
+  return sums ? 8ll * sum_blocks(rows, D) * D : 0;
 }
 
 hipError_t join_bwd(const JoinArgs& a, void* work, hipStream_t s) {
-  const bool sums = a.dw_in || a.dw_out || a.dgate;
-  const int blocks = sums ? std::min(a.rows, kBwdBlocks) : std::min(a.rows, kFwdBlocks);
-  float* part = (float*)work;
+  const bool sums = a.dw_in || a.dw_out || a.dgate, full = a.gate_kind == kGateFull;
+  const int runs = a.y.p ? best_runs(a.D) : 1;
+  const int blocks = a.y.p ? sum_blocks(a.rows, a.D) : blocks_of(a.rows, a.D, runs);
+  float* part = sums ? (float*)work : nullptr;
+  const double in = (a.dn.p ? row_bytes(a.x) : 0) + row_bytes(a.y) + row_bytes(a.dn) + row_bytes(a.dxn) +
+                    (full ? 2 : 0);
+  const double out = (a.dx_f32 ? 4 : 2) + (a.y.p ? 2 : 0) + (full ? 2 : 0);
+  const bool near = cache_of(in * a.rows * a.D, out * a.rows * a.D) == kNear;
   auto go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(threads_of(a.D)), 0, s, a, part);
+    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(64 * waves_of(a.D, runs)), 0, s, a, part);
     return hipGetLastError();
   };
-  auto by_sums = [&](auto x, auto y, auto g) {
+  auto by_cache = [&](auto x, auto y, auto g, auto f) {
     constexpr int X = decltype(x)::value, Y = decltype(y)::value, G = decltype(g)::value;
-    return sums ? go(join_bwd_kernel<X, Y, G, true>) : go(join_bwd_kernel<X, Y, G, false>);
+    constexpr bool F = decltype(f)::value;
+    if constexpr (Y == kRowsNone)
+      return near ? go(join_bwd_kernel<X, Y, G, F, kNear, 1>) : go(join_bwd_kernel<X, Y, G, F, kFar, 1>);
+    else if (runs == 2)
+      return near ? go(join_bwd_kernel<X, Y, G, F, kNear, 2>) : go(join_bwd_kernel<X, Y, G, F, kFar, 2>);
+    else
+      return near ? go(join_bwd_kernel<X, Y, G, F, kNear, 3>) : go(join_bwd_kernel<X, Y, G, F, kFar, 3>);
   };
-  auto by_g = [&](auto x, auto y) {
-    if (!a.dn.p) return by_sums(x, y, std::integral_constant<int, kRowsNone>{});
-    return a.dn.type == DSB_DT_F32 ? by_sums(x, y, std::integral_constant<int, kRowsF32>{})
-                                   : by_sums(x, y, std::integral_constant<int, kRowsBF16>{});
+  auto by_gate = [&](auto x, auto y, auto g) {
+    return full ? by_cache(x, y, g, std::true_type{}) : by_cache(x, y, g, std::false_type{});
   };
-  auto by_y = [&](auto x) {
-    if (!a.y.p) return by_g(x, std::integral_constant<int, kRowsNone>{});
-    return a.y.type == DSB_DT_BF16 ? by_g(x, std::integral_constant<int, kRowsBF16>{})
-                                   : by_g(x, std::integral_constant<int, kRows8>{});
+  auto by_y = [&](auto x, auto g) {
+    switch (a.y.type) {
+      case DSB_DT_BF16: return by_gate(x, Int<DSB_DT_BF16>{}, g);
+      case DSB_DT_E4M3: return by_gate(x, Int<DSB_DT_E4M3>{}, g);
+      default: return by_gate(x, Int<DSB_DT_INT8>{}, g);
+    }
   };
+  auto by_g = [&](auto x, auto f) { return a.dn.type == DSB_DT_F32 ? f(x, Int<DSB_DT_F32>{}) : f(x, Int<DSB_DT_BF16>{}); };
   if (a.rows > 0) {
     hipError_t e;
-    switch (rows_kind(a.x.type)) {
-      case kRowsBF16: e = by_y(std::integral_constant<int, kRowsBF16>{}); break;
-      case kRowsF32: e = by_y(std::integral_constant<int, kRowsF32>{}); break;
-      default: e = by_y(std::integral_constant<int, kRows8>{});
-    }
+    if (!a.dn.p)  // no norm after: x' is not read
+      e = by_y(Int<kRowsNone>{}, Int<kRowsNone>{});
+    else if (a.y.p)
+      e = by_type(a.x, [&](auto x) { return by_g(x, by_y); });
+    else
+      e = by_type(a.x, [&](auto x) {
+        return by_g(x, [&](auto x1, auto g) { return by_cache(x1, Int<kRowsNone>{}, g, std::false_type{}); });
+      });
     if (e != hipSuccess) return e;
   }
   if (sums)
-    hipLaunchKernelGGL(join_sums_kernel, dim3((a.D + 31) / 32, 3), dim3(256), 0, s, part,
-                       std::max(blocks, 0), a.D, a.dw_in, a.dw_out, a.dgate);
+    hipLaunchKernelGGL(join_sums_kernel, dim3((a.D + 4 * kSumLanes - 1) / (4 * kSumLanes), 2), dim3(kSumThreads), 0, s, a, part, blocks);
   return hipGetLastError();
 }
 

@@ -9,8 +9,11 @@
 //
 // A wave takes a token, or a part of its heads where there are few tokens. It computes the token's
 // cosines and sines once, a pair of them a lane, and keeps them in LDS, where all of its heads read
-// them; then it moves 8 elements of either member of 8 pairs (or 4 pairs of neighbours) a lane. Bound
-// by its bytes.
+// them; then a lane moves 8 elements of either member of 8 pairs (halves), of 4 pairs (neighbours) or of what
+// stays. Accesses of 16 bytes need their elements' alignment only, so all strides and widths go
+// the same way: the last run of a region that is no multiple of 8 starts earlier and overlaps the
+// one before. Both compute the same values there; in place, where the first may have written
+// already, the second leaves them out. Bound by its bytes.
 #include <algorithm>
 #include <type_traits>
 
@@ -20,7 +23,8 @@ namespace dsb {
 
 namespace {
 
-constexpr int kWaves = 4, kMostPairs = DSB_ROTARY_MOST / 2;
+constexpr int kWaves = 4, kMostPairs = DSB_ROTARY_MOST / 2 + 8;  // (a run may read past the last pair)
+constexpr int kSlots = 2;  // runs that a lane has in flight
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
@@ -37,18 +41,22 @@ struct Elem<DSB_DT_F32> {
   using type = float;
 };
 
-// 8 elements as they lie.
+typedef float f32x4e __attribute__((ext_vector_type(4), aligned(4)));
+
+// 8 elements as they lie, wherever they start.
 template <int T>
 struct Vec8 {
   u32x4 a, b;
   using E = typename Elem<T>::type;
+  template <int P>
   DSB_DEV void load(const E* p) {
-    a = ldg128_nt(p);
-    if constexpr (T == DSB_DT_F32) b = ldg128_nt(p + 4);
+    a = load_as<P, u32x4h>(p);
+    if constexpr (T == DSB_DT_F32) b = load_as<P, u32x4h>(p + 4);
   }
+  template <int P>
   DSB_DEV void store(E* p) const {
-    __builtin_nontemporal_store(a, reinterpret_cast<u32x4*>(p));
-    if constexpr (T == DSB_DT_F32) __builtin_nontemporal_store(b, reinterpret_cast<u32x4*>(p + 4));
+    store_as<P, u32x4h>(p, a);
+    if constexpr (T == DSB_DT_F32) store_as<P, u32x4h>(p + 4, b);
   }
   DSB_DEV void get(float v[8]) const {
     if constexpr (T == DSB_DT_BF16) {
@@ -58,12 +66,7 @@ struct Vec8 {
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = (float)h[i];
     } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const unsigned x = a[i], y = b[i];
-        v[i] = __builtin_bit_cast(float, x);
-        v[4 + i] = __builtin_bit_cast(float, y);
-      }
+      floats8(a, b, v);
     }
   }
   DSB_DEV void set(const float v[8]) {
@@ -84,11 +87,11 @@ struct Vec8 {
   }
 };
 
-// VEC: 16-byte accesses, `slots` a head: with halves rot / 16 slots of 8 pairs, then 8 elements that
-// stay; with neighbours 8 elements each, the first rot / 8 of them turned. Else one pair or element
-// a slot.
-template <int T, bool NEXT, bool VEC>
-__global__ __launch_bounds__(64 * kWaves) void rotary_kernel(RotaryArgs a, int parts, int per,
+// EVEN: the regions are multiples of 8 elements.
+// Runs of 8 elements (of all there are, in a region with fewer) of a head: `turned` of them over the
+// pairs' first members or, with neighbours (NEXT), over both, and the rest over what stays.
+template <int T, bool NEXT, bool EVEN, int P>
+__global__ __launch_bounds__(64 * kWaves) void rotary_kernel(RotaryArgs a, int parts, int per, int turned,
                                                              int slots, unsigned magic) {
   using E = typename Elem<T>::type;
   __shared__ __align__(16) float table[kWaves][2][kMostPairs];
@@ -115,86 +118,90 @@ __global__ __launch_bounds__(64 * kWaves) void rotary_kernel(RotaryArgs a, int p
   const E* x = (const E*)a.x + t * a.ldx + h0 * a.hx;
   E* y = (E*)a.y + t * a.ldy + h0 * a.hy;
   const int total = heads * slots;
-  if constexpr (VEC) {
-    const int turned = NEXT ? a.rot >> 3 : a.rot >> 4;
-    const bool keep = a.x == a.y;  // what stays is there
-    constexpr int U = 2;
-    for (int k0 = lane; k0 < total; k0 += 64 * U) {
-      Vec8<T> p[U], q[U];
-      const E* xi[U];
-      E* yi[U];
-      int s[U];
+  const bool place = a.x == a.y;
+  // elements of a run in the two regions
+  const int count1 = EVEN ? 8 : min(8, NEXT ? a.rot : half);
+  const int count2 = EVEN ? 8 : min(8, a.hd - a.rot);
+  for (int k0 = lane; k0 < total; k0 += 64 * kSlots) {
+    Vec8<T> p[kSlots], q[kSlots];
+    float pe[8], qe[8];  // of runs of less than 8 elements, which are the whole region
+    int slot[kSlots], at[kSlots], from[kSlots];
+    const E* xi[kSlots];
+    E* yi[kSlots];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int k = k0 + 64 * u;
-        const int h = magic ? (int)__umulhi((unsigned)k, magic) : k;
-        s[u] = k < total ? k - h * slots : -1;
-        const int at = NEXT ? 8 * s[u] : s[u] < turned ? 8 * s[u] : a.rot + 8 * (s[u] - turned);
-        xi[u] = x + h * a.hx + at;
-        yi[u] = y + h * a.hy + at;
-        if (s[u] >= 0 && (s[u] < turned || !keep)) {
-          p[u].load(xi[u]);
-          if (!NEXT && s[u] < turned) q[u].load(xi[u] + half);
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (s[u] < 0) continue;
-        if (s[u] >= turned) {
-          if (!keep) p[u].store(yi[u]);
-          continue;
-        }
-        float pv[8], qv[8];
-        p[u].get(pv);
-        if constexpr (NEXT) {
-          const f32x4 c = *reinterpret_cast<const f32x4*>(cosv + 4 * s[u]);
-          const f32x4 sn = *reinterpret_cast<const f32x4*>(sinv + 4 * s[u]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float f = pv[2 * e], g = pv[2 * e + 1];
-            pv[2 * e] = f * c[e] - g * sn[e];
-            pv[2 * e + 1] = g * c[e] + f * sn[e];
-          }
-          p[u].set(pv);
-          p[u].store(yi[u]);
-        } else {
-          q[u].get(qv);
-#pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            const f32x4 c = *reinterpret_cast<const f32x4*>(cosv + 8 * s[u] + 4 * b);
-            const f32x4 sn = *reinterpret_cast<const f32x4*>(sinv + 8 * s[u] + 4 * b);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float f = pv[4 * b + e], g = qv[4 * b + e];
-              pv[4 * b + e] = f * c[e] - g * sn[e];
-              qv[4 * b + e] = g * c[e] + f * sn[e];
-            }
-          }
-          p[u].set(pv);
-          q[u].set(qv);
-          p[u].store(yi[u]);
-          q[u].store(yi[u] + half);
-        }
+    for (int u = 0; u < kSlots; ++u) {
+      const int k = k0 + 64 * u;
+      const int h = magic ? (int)__umulhi((unsigned)k, magic) : k;
+      const int s = k - h * slots;
+      slot[u] = k < total ? s : slots;  // (slots: none)
+      const bool turns = s < turned;
+      const int length = turns ? (NEXT ? a.rot : half) : a.hd - a.rot;
+      const int want = 8 * (turns ? s : s - turned);
+      at[u] = EVEN ? want : max(0, min(want, length - 8));
+      from[u] = want - at[u];
+      xi[u] = x + h * a.hx + at[u] + (turns ? 0 : a.rot);
+      yi[u] = y + h * a.hy + at[u] + (turns ? 0 : a.rot);
+      if (k < total && (turns || !place) && (turns ? count1 : count2) == 8) {
+        p[u].template load<P>(xi[u]);
+        if (!NEXT && turns) q[u].template load<P>(xi[u] + half);
       }
     }
-  } else {
-    for (int k = lane; k < total; k += 64) {
-      const int h = magic ? (int)__umulhi((unsigned)k, magic) : k, s = k - h * slots;
-      const E* xi = x + h * a.hx;
-      E* yi = y + h * a.hy;
-      if (s >= half) {
-        yi[half + s] = xi[half + s];
+#pragma unroll
+    for (int u = 0; u < kSlots; ++u) {
+      if (slot[u] >= slots) continue;
+      if (slot[u] >= turned) {
+        if (place) continue;
+        if (count2 == 8) {
+          p[u].template store<P>(yi[u]);
+        } else {
+          for (int e = 0; e < count2; ++e) yi[u][e] = xi[u][e];
+        }
+        continue;
+      }
+      if (count1 == 8) {
+        p[u].get(pe);
+        if (!NEXT) q[u].get(qe);
       } else {
-        const int i0 = NEXT ? 2 * s : s, i1 = NEXT ? 2 * s + 1 : s + half;
-        const float p = (float)xi[i0], q = (float)xi[i1], c = cosv[s], sn = sinv[s];
-        yi[i0] = (E)(p * c - q * sn);
-        yi[i1] = (E)(q * c + p * sn);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          pe[e] = e < count1 ? (float)xi[u][e] : 0.f;
+          if (!NEXT) qe[e] = e < count1 ? (float)xi[u][half + e] : 0.f;
+        }
+      }
+      const int pair = NEXT ? at[u] >> 1 : at[u];
+#pragma unroll
+      for (int b = 0; b < (NEXT ? 1 : 2); ++b) {
+        using Four = typename std::conditional<EVEN, f32x4, f32x4e>::type;
+        const f32x4 c = *reinterpret_cast<const Four*>(cosv + pair + 4 * b);
+        const f32x4 sn = *reinterpret_cast<const Four*>(sinv + pair + 4 * b);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float &f = NEXT ? pe[2 * e] : pe[4 * b + e], &g = NEXT ? pe[2 * e + 1] : qe[4 * b + e];
+          const float f0 = f, g0 = g;
+          f = f0 * c[e] - g0 * sn[e];
+          g = g0 * c[e] + f0 * sn[e];
+        }
+      }
+      const int skip = place ? from[u] : 0;
+      if (count1 == 8 && skip == 0) {
+        p[u].set(pe);
+        p[u].template store<P>(yi[u]);
+        if (!NEXT) {
+          q[u].set(qe);
+          q[u].template store<P>(yi[u] + half);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if (e >= skip && e < count1) {
+            yi[u][e] = (E)pe[e];
+            if (!NEXT) yi[u][half + e] = (E)qe[e];
+          }
+        }
       }
     }
   }
 }
-
-bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 // Waves wanted before a token's heads stay with one of them.
 constexpr long kMostSplit = 4096;
@@ -203,11 +210,9 @@ constexpr long kMostSplit = 4096;
 
 hipError_t rotary(const RotaryArgs& a, hipStream_t s) {
   if (a.n <= 0 || a.heads <= 0) return hipSuccess;
-  const int es = a.dtype == DSB_DT_F32 ? 4 : 2;
-  auto whole = [&](long v) { return v * es % 16 == 0; };
-  const bool vec = a.hd % 8 == 0 && a.rot % (a.interleaved ? 8 : 16) == 0 && aligned16(a.x) &&
-                   aligned16(a.y) && whole(a.ldx) && whole(a.hx) && whole(a.ldy) && whole(a.hy);
-  const int slots = !vec ? a.hd - a.rot / 2 : a.interleaved ? a.hd / 8 : a.rot / 16 + (a.hd - a.rot) / 8;
+  const int turned = ((a.interleaved ? a.rot : a.rot / 2) + 7) / 8;
+  const bool even = a.rot % (a.interleaved ? 8 : 16) == 0 && (a.hd - a.rot) % 8 == 0;
+  const int slots = turned + (a.hd - a.rot + 7) / 8;
   // at least a wave's worth of slots to a part
   const int least = (64 + slots - 1) / slots;
   const long want = std::max(1l, kMostSplit / a.n);
@@ -216,20 +221,29 @@ hipError_t rotary(const RotaryArgs& a, hipStream_t s) {
   // k / slots for k below per·slots and a wave's step past it: exact while k·slots < 2^32 (0: one slot)
   const unsigned magic = slots == 1 ? 0u : (unsigned)(((1ull << 32) + slots - 1) / slots);
   const unsigned blocks = (unsigned)(((long)a.n * parts + kWaves - 1) / kWaves);
+  const double bytes = (double)a.n * a.heads * a.hd * (a.dtype == DSB_DT_F32 ? 4 : 2);
+  const int cache = cache_of(bytes, bytes);
   auto go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(64 * kWaves), 0, s, a, parts, per, slots, magic);
+    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(64 * kWaves), 0, s, a, parts, per, turned, slots, magic);
     return hipGetLastError();
   };
-  auto by_type = [&](auto t) {
+  auto by_cache = [&](auto t, auto next, auto ev) {
     constexpr int T = decltype(t)::value;
-    if (a.interleaved) return vec ? go(rotary_kernel<T, true, true>) : go(rotary_kernel<T, true, false>);
-    return vec ? go(rotary_kernel<T, false, true>) : go(rotary_kernel<T, false, false>);
+    constexpr bool N = decltype(next)::value, E = decltype(ev)::value;
+    return cache == kNear  ? go(rotary_kernel<T, N, E, kNear>)
+           : cache == kFar ? go(rotary_kernel<T, N, E, kFar>)
+                           : go(rotary_kernel<T, N, E, kPast>);
+  };
+  using std::false_type;
+  using std::true_type;
+  auto by_type = [&](auto t) {
+    if (even) return a.interleaved ? by_cache(t, true_type{}, true_type{}) : by_cache(t, false_type{}, true_type{});
+    return a.interleaved ? by_cache(t, true_type{}, false_type{}) : by_cache(t, false_type{}, false_type{});
   };
   switch (a.dtype) {
     case DSB_DT_BF16: return by_type(std::integral_constant<int, DSB_DT_BF16>{});
     case DSB_DT_F16: return by_type(std::integral_constant<int, DSB_DT_F16>{});
-    case DSB_DT_F32: return by_type(std::integral_constant<int, DSB_DT_F32>{});
-    default: return hipErrorInvalidValue;
+    default: return by_type(std::integral_constant<int, DSB_DT_F32>{});
   }
 }
 

@@ -10,6 +10,8 @@
 // the byte's 2^128 (infinity) is NaN again.
 #pragma once
 
+#include <type_traits>
+
 #include "kernels.h"
 
 namespace dsb {
@@ -83,6 +85,38 @@ DSB_DEV unsigned quad_max(unsigned v) {
 }
 DSB_DEV unsigned abs_bits(float v) { return __builtin_bit_cast(unsigned, v) & 0x7fffffffu; }
 
+// ---- memory
+// What a kernel leaves in the caches (the last level, 256 MB, keeps data from one kernel to the next):
+//   kNear  loads through them, stores past the L2: calls of up to 256 MB, whose inputs the kernel
+//          before may have left there; stores that stay in the L2 are written back at the kernel's end
+//   kFar   loads past them, stores into them: larger calls whose outputs the next kernel finds there
+//   kPast  both past them: outputs of more than 256 MB
+// µs, near / far / past (bytes of the call): RMSNorm of 2048 × 4096 8-bit rows (25 MB) 4.9 / 8.2 / 7.1, of
+// 8192 × 4096 (102 MB) 21 / 29 / 29; SwiGLU of 8192 × 14336 (477 MB) 91 / 73 / 86, its backward (1.2 GB, 705
+// MB of them out) 229 / 237 / 222; rows of 8192 × 28672 restored (712 MB, 470 out) 129 / 141 / 127.
+enum { kNear, kFar, kPast };
+inline int cache_of(double in, double out) {
+  constexpr double kLast = 256 << 20;
+  return in + out <= kLast ? kNear : out <= kLast ? kFar : kPast;
+}
+template <int P, class V>
+DSB_DEV V load_as(const void* p) {
+  const V* q = reinterpret_cast<const V*>(p);
+  if constexpr (P == kNear) return *q;
+  return __builtin_nontemporal_load(q);
+}
+template <int P, class V>
+DSB_DEV void store_as(void* p, V v) {
+  V* q = reinterpret_cast<V*>(p);
+  if constexpr (P == kFar)
+    *q = v;
+  else
+    __builtin_nontemporal_store(v, q);
+}
+// Accesses of 16 and 8 bytes that need their elements' alignment only.
+typedef unsigned u32x4h __attribute__((ext_vector_type(4), aligned(2)));
+typedef unsigned u32x2b __attribute__((ext_vector_type(2), aligned(1)));
+
 // ---- rows of any of the types, 8 columns at a time
 struct RowsArg {
   const void* p;
@@ -91,69 +125,82 @@ struct RowsArg {
   long lds;
   int type;  // DSB_DT_*
 };
-enum { kRowsBF16 = 0, kRowsF32 = 1, kRows8 = 2, kRowsNone = 3 };
-inline int rows_kind(int type) {
-  return type == DSB_DT_BF16 ? kRowsBF16 : type == DSB_DT_F32 ? kRowsF32 : kRows8;
+constexpr int kRowsNone = -1;
+// Bytes of a column of such rows.
+inline double row_bytes(const RowsArg& r) {
+  return !r.p ? 0 : r.type == DSB_DT_BF16 ? 2 : r.type == DSB_DT_F32 ? 4 : 1 + 1.0 / kBlock8;
 }
 
-template <int KIND>
-struct Raw8 {
-  u32x4 a;
-  DSB_DEV void load(const RowsArg& r, long row, int c) {
-    a = ldg128_nt((const bf16*)r.p + row * r.ld + 8 * c);
-  }
-  DSB_DEV void get(const RowsArg&, float v[8]) const { unpack8(a, v); }
-};
-template <>
-struct Raw8<kRowsF32> {
-  u32x4 a, b;
-  DSB_DEV void load(const RowsArg& r, long row, int c) {
-    const float* p = (const float*)r.p + row * r.ld + 8 * c;
-    a = ldg128_nt(p);
-    b = ldg128_nt(p + 4);
-  }
-  DSB_DEV void get(const RowsArg&, float v[8]) const {
+DSB_DEV void floats8(u32x4 a, u32x4 b, float v[8]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const unsigned x = a[i], y = b[i];
-      v[i] = __builtin_bit_cast(float, x);
-      v[4 + i] = __builtin_bit_cast(float, y);
-    }
+  for (int i = 0; i < 4; ++i) {
+    const unsigned x = a[i], y = b[i];
+    v[i] = __builtin_bit_cast(float, x);
+    v[4 + i] = __builtin_bit_cast(float, y);
   }
-};
-template <>
-struct Raw8<kRows8> {
+}
+// As they lie, of type T.
+template <int T>
+struct Raw8 {  // 8-bit rows
   u32x2 c;
   unsigned byte;
+  template <int P>
   DSB_DEV void load(const RowsArg& r, long row, int ch) {
-    c = __builtin_nontemporal_load(
-        reinterpret_cast<const u32x2*>((const uint8_t*)r.p + row * r.ld + 8 * ch));
+    c = load_as<P, u32x2>((const uint8_t*)r.p + row * r.ld + 8 * ch);
     byte = r.s[row * r.lds + (ch >> 2)];
   }
-  DSB_DEV void get(const RowsArg& r, float v[8]) const {
-    if (r.type == DSB_DT_E4M3)  // the same for all lanes
-      decode8<DSB_DT_E4M3>(c, byte, v);
-    else
-      decode8<DSB_DT_INT8>(c, byte, v);
+  DSB_DEV void get(float v[8]) const { decode8<T>(c, byte, v); }
+};
+template <>
+struct Raw8<DSB_DT_BF16> {
+  u32x4 a;
+  template <int P>
+  DSB_DEV void load(const RowsArg& r, long row, int c) {
+    a = load_as<P, u32x4>((const bf16*)r.p + row * r.ld + 8 * c);
   }
+  DSB_DEV void get(float v[8]) const { unpack8(a, v); }
+};
+template <>
+struct Raw8<DSB_DT_F32> {
+  u32x4 a, b;
+  template <int P>
+  DSB_DEV void load(const RowsArg& r, long row, int c) {
+    const float* p = (const float*)r.p + row * r.ld + 8 * c;
+    a = load_as<P, u32x4>(p);
+    b = load_as<P, u32x4>(p + 4);
+  }
+  DSB_DEV void get(float v[8]) const { floats8(a, b, v); }
 };
 template <>
 struct Raw8<kRowsNone> {
+  template <int P>
   DSB_DEV void load(const RowsArg&, long, int) {}
-  DSB_DEV void get(const RowsArg&, float v[8]) const {
+  DSB_DEV void get(float v[8]) const {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = 0.f;
   }
 };
+template <int K>
+using Int = std::integral_constant<int, K>;
+// f with the type of rows as a constant.
+template <class F>
+hipError_t by_type(const RowsArg& r, F f) {
+  switch (r.type) {
+    case DSB_DT_BF16: return f(Int<DSB_DT_BF16>{});
+    case DSB_DT_F32: return f(Int<DSB_DT_F32>{});
+    case DSB_DT_E4M3: return f(Int<DSB_DT_E4M3>{});
+    default: return f(Int<DSB_DT_INT8>{});
+  }
+}
 
-// 8 columns out, past the caches.
+// 8 columns out.
+template <int P>
 DSB_DEV void put8(void* p, long at, bool f32, const float v[8]) {
   if (f32) {
-    f32x4* o = reinterpret_cast<f32x4*>((float*)p + at);
-    __builtin_nontemporal_store(f32x4{v[0], v[1], v[2], v[3]}, o);
-    __builtin_nontemporal_store(f32x4{v[4], v[5], v[6], v[7]}, o + 1);
+    store_as<P>((float*)p + at, f32x4{v[0], v[1], v[2], v[3]});
+    store_as<P>((float*)p + at + 4, f32x4{v[4], v[5], v[6], v[7]});
   } else {
-    __builtin_nontemporal_store(pack8(v), reinterpret_cast<u32x4*>((bf16*)p + at));
+    store_as<P>((bf16*)p + at, pack8(v));
   }
 }
 

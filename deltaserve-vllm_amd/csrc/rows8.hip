@@ -2,7 +2,8 @@
 // either kind. All of it is bound by its bytes.
 //
 // A lane holds 8 columns: its loads of 16 bytes (8 of codes) cover whole lines over a wave, and a
-// block of 32 columns is four neighbouring lanes, whose maximum takes two DPP steps.
+// block of 32 columns is four neighbouring lanes, whose maximum takes two DPP steps. Rows may start
+// anywhere; the last columns of a width that is no multiple of 8 are moved one by one.
 #include "block.h"
 
 namespace dsb {
@@ -25,22 +26,18 @@ DSB_DEV float narrow(float v) {
 template <int T>
 struct In8 {
   u32x4 a, b;
+  template <int P>
   DSB_DEV void load(const void* p, long i) {
     if constexpr (T == DSB_DT_F32) {
-      a = ldg128_nt((const float*)p + i);
-      b = ldg128_nt((const float*)p + i + 4);
+      a = load_as<P, u32x4h>((const float*)p + i);
+      b = load_as<P, u32x4h>((const float*)p + i + 4);
     } else {
-      a = ldg128_nt((const bf16*)p + i);
+      a = load_as<P, u32x4h>((const bf16*)p + i);
     }
   }
   DSB_DEV void get(float v[8]) const {
     if constexpr (T == DSB_DT_F32) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const unsigned x = a[i], y = b[i];
-        v[i] = __builtin_bit_cast(float, x);
-        v[4 + i] = __builtin_bit_cast(float, y);
-      }
+      floats8(a, b, v);
     } else if constexpr (T == DSB_DT_F16) {
       typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
       const f16x8 h = __builtin_bit_cast(f16x8, a);
@@ -51,6 +48,11 @@ struct In8 {
     }
   }
 };
+template <int T>
+DSB_DEV void few(const void* p, long i, int count, float v[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = e < count ? widen<T>(p, i + e) : 0.f;
+}
 
 // The rows that slot i moves; false: none.
 DSB_DEV bool slot_rows(const Save8Args& a, int i, long& s, long& d) {
@@ -60,7 +62,7 @@ DSB_DEV bool slot_rows(const Save8Args& a, int i, long& s, long& d) {
 }
 
 constexpr int kSaveVec = 2, kSaveRun = 256 * 8 * kSaveVec;
-template <int T, int CODE, bool RES>
+template <int T, int CODE, bool RES, int P>
 __global__ __launch_bounds__(256) void save_rows8_kernel(Save8Args a) {
   long s, d;
   if (!slot_rows(a, blockIdx.x, s, d)) return;
@@ -69,21 +71,25 @@ __global__ __launch_bounds__(256) void save_rows8_kernel(Save8Args a) {
 #pragma unroll
   for (int i = 0; i < kSaveVec; ++i) {
     const int c = c0 + 2048 * i;
-    if (c < a.width) {
-      x[i].load(a.x, s * a.ldx + c);
-      if (RES) r[i].load(a.r, s * a.ldr + c);
+    if (c + 8 <= a.width) {
+      x[i].template load<P>(a.x, s * a.ldx + c);
+      if (RES) r[i].template load<P>(a.r, s * a.ldr + c);
     }
   }
 #pragma unroll
   for (int i = 0; i < kSaveVec; ++i) {
-    const int c = c0 + 2048 * i;
-    float v[8] = {};
+    const int c = c0 + 2048 * i, left = a.width - c;
+    float v[8] = {}, w[8];
     unsigned top = 0;
-    if (c < a.width) {
-      x[i].get(v);
+    if (left > 0) {
+      if (left >= 8) {
+        x[i].get(v);
+        if (RES) r[i].get(w);
+      } else {
+        few<T>(a.x, s * a.ldx + c, left, v);
+        if (RES) few<T>(a.r, s * a.ldr + c, left, w);
+      }
       if (RES) {
-        float w[8];
-        r[i].get(w);
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = narrow<T>(v[e] + w[e]);
       }
@@ -91,91 +97,78 @@ __global__ __launch_bounds__(256) void save_rows8_kernel(Save8Args a) {
       for (int e = 0; e < 8; ++e) top = max(top, abs_bits(v[e]));
     }
     const unsigned byte = scale_byte<CODE>(quad_max(top));
-    if (c < a.width) {
-      __builtin_nontemporal_store(encode8<CODE>(v, byte),
-                                  reinterpret_cast<u32x2*>(a.codes + d * a.ldc + c));
+    if (left > 0) {
+      const u32x2 code = encode8<CODE>(v, byte);
+      uint8_t* o = a.codes + d * a.ldc + c;
+      if (left >= 8) {
+        store_as<P, u32x2b>(o, code);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 7; ++e)
+          if (e < left) o[e] = (uint8_t)(code[e >> 2] >> (8 * (e & 3)));
+      }
       if ((threadIdx.x & 3) == 0) a.scales[d * a.lds + c / kBlock8] = (uint8_t)byte;
     }
   }
 }
 
-// Any width, strides and alignment: 32 lanes to a block, a column each.
-template <int T, int CODE>
-__global__ __launch_bounds__(256) void save_rows8_any_kernel(Save8Args a) {
-  long s, d;
-  if (!slot_rows(a, blockIdx.x, s, d)) return;
-  const int lane = threadIdx.x & 31;
-  const int nb = (a.width + kBlock8 - 1) / kBlock8;
-  for (int b = blockIdx.y * 8 + (threadIdx.x >> 5); b < nb; b += gridDim.y * 8) {
-    const int c = b * kBlock8 + lane;
-    float v = 0.f;
-    if (c < a.width) {
-      v = widen<T>(a.x, s * a.ldx + c);
-      if (a.r) v = narrow<T>(v + widen<T>(a.r, s * a.ldr + c));
-    }
-    unsigned top = abs_bits(v);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, o, 64));
-    const unsigned byte = scale_byte<CODE>(top);
-    if (c < a.width) {
-      const float four[4] = {v, 0.f, 0.f, 0.f};
-      a.codes[d * a.ldc + c] =
-          byte == 255u ? 0 : (uint8_t)encode4<CODE>(four, inverse_scale_of(byte));
-      if (lane == 0) a.scales[d * a.lds + b] = (uint8_t)byte;
-    }
-  }
-}
-
 constexpr int kRestoreVec = 4, kRestoreRun = 256 * 8 * kRestoreVec;
-template <int CODE, bool F32>
+template <int CODE, bool F32, int P>
 __global__ __launch_bounds__(256) void restore_rows8_kernel(RowsArg q, int width, void* out, long ldo) {
   const long row = blockIdx.x;
   const int c0 = blockIdx.y * kRestoreRun + threadIdx.x * 8;
-  Raw8<kRows8> x[kRestoreVec];
-#pragma unroll
-  for (int i = 0; i < kRestoreVec; ++i)
-    if (c0 + 2048 * i < width) x[i].load(q, row, (c0 + 2048 * i) / 8);
+  const uint8_t* in = (const uint8_t*)q.p + row * q.ld;
+  u32x2 x[kRestoreVec];
+  unsigned byte[kRestoreVec];
 #pragma unroll
   for (int i = 0; i < kRestoreVec; ++i) {
     const int c = c0 + 2048 * i;
-    if (c < width) {
-      float v[8];
-      decode8<CODE>(x[i].c, x[i].byte, v);
-      put8(out, row * ldo + c, F32, v);
-    }
+    if (c + 8 <= width) x[i] = load_as<P, u32x2b>(in + c);
+    if (c < width) byte[i] = q.s[row * q.lds + c / kBlock8];
   }
-}
-template <int CODE, bool F32>
-__global__ __launch_bounds__(256) void restore_rows8_any_kernel(RowsArg q, int width, void* out,
-                                                                long ldo) {
-  const long row = blockIdx.x;
-  const uint8_t* p = (const uint8_t*)q.p + row * q.ld;
-  for (int c = blockIdx.y * 256 + threadIdx.x; c < width; c += gridDim.y * 256) {
-    float v[4];
-    decode4<CODE>(p[c], scale_of(q.s[row * q.lds + c / kBlock8]), v);
-    if (F32)
-      ((float*)out)[row * ldo + c] = v[0];
-    else
-      ((bf16*)out)[row * ldo + c] = (bf16)v[0];
+#pragma unroll
+  for (int i = 0; i < kRestoreVec; ++i) {
+    const int c = c0 + 2048 * i, left = width - c;
+    float v[8];
+    if (left >= 8) {
+      decode8<CODE>(x[i], byte[i], v);
+      if (F32) {
+        store_as<P, u32x4h>((float*)out + row * ldo + c, __builtin_bit_cast(u32x4, f32x4{v[0], v[1], v[2], v[3]}));
+        store_as<P, u32x4h>((float*)out + row * ldo + c + 4, __builtin_bit_cast(u32x4, f32x4{v[4], v[5], v[6], v[7]}));
+      } else {
+        store_as<P, u32x4h>((bf16*)out + row * ldo + c, pack8(v));
+      }
+    } else if (left > 0) {
+      u32x2 few = {0u, 0u};
+#pragma unroll
+      for (int e = 0; e < 7; ++e)
+        if (e < left) few[e >> 2] |= (unsigned)in[c + e] << (8 * (e & 3));
+      decode8<CODE>(few, byte[i], v);
+#pragma unroll
+      for (int e = 0; e < 7; ++e) {
+        if (e < left && F32) ((float*)out)[row * ldo + c + e] = v[e];
+        if (e < left && !F32) ((bf16*)out)[row * ldo + c + e] = (bf16)v[e];
+      }
+    }
   }
 }
 
 // A lane takes 8 gate and 8 up columns of a row. BWD with σ = σ(gate):
 //   dgate = dh·up·σ·(1 + gate·(1 − σ)), dup = dh·gate·σ
 constexpr int kGluVec = 2, kGluRun = 256 * 8 * kGluVec;
-template <int KIND, int DH>
+template <int T, int DH, int P>
 __global__ __launch_bounds__(256) void swiglu_kernel(SwigluArgs a) {
   const long row = blockIdx.x;
   const int c0 = blockIdx.y * kGluRun + threadIdx.x * 8;
-  Raw8<KIND> g[kGluVec], u[kGluVec];
+  Raw8<T> g[kGluVec], u[kGluVec];
   Raw8<DH> dh[kGluVec];
 #pragma unroll
   for (int i = 0; i < kGluVec; ++i) {
     const int c = c0 + 2048 * i;
     if (c < a.I) {
-      g[i].load(a.gu, row, c / 8);
-      u[i].load(a.gu, row, (a.I + c) / 8);
-      dh[i].load(a.dh, row, c / 8);
+      g[i].template load<P>(a.gu, row, c / 8);
+      u[i].template load<P>(a.gu, row, (a.I + c) / 8);
+      dh[i].template load<P>(a.dh, row, c / 8);
     }
   }
 #pragma unroll
@@ -183,9 +176,9 @@ __global__ __launch_bounds__(256) void swiglu_kernel(SwigluArgs a) {
     const int c = c0 + 2048 * i;
     if (c >= a.I) continue;
     float gv[8], uv[8], dv[8], og[8], ou[8], h[8];
-    g[i].get(a.gu, gv);
-    u[i].get(a.gu, uv);
-    dh[i].get(a.dh, dv);
+    g[i].get(gv);
+    u[i].get(uv);
+    dh[i].get(dv);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const float sg = sigmoid(gv[e]), silu = gv[e] * sg;
@@ -194,85 +187,90 @@ __global__ __launch_bounds__(256) void swiglu_kernel(SwigluArgs a) {
       ou[e] = dv[e] * silu;
     }
     if (DH != kRowsNone) {
-      put8(a.dgu, row * a.lddgu + c, false, og);
-      put8(a.dgu, row * a.lddgu + a.I + c, false, ou);
+      put8<P>(a.dgu, row * a.lddgu + c, false, og);
+      put8<P>(a.dgu, row * a.lddgu + a.I + c, false, ou);
     }
-    if (a.h) put8(a.h, row * a.ldh + c, false, h);
+    if (a.h) put8<P>(a.h, row * a.ldh + c, false, h);
   }
 }
 
-bool aligned(const void* p, unsigned to) { return ((uintptr_t)p & (to - 1)) == 0; }
 unsigned runs(int width, int run) { return (unsigned)((width + run - 1) / run); }
+template <class F>
+hipError_t by_cache(double in, double out, F f) {
+  switch (cache_of(in, out)) {
+    case kNear: return f(Int<kNear>{});
+    case kFar: return f(Int<kFar>{});
+    default: return f(Int<kPast>{});
+  }
+}
 
 }  // namespace
 
 hipError_t save_rows8(const Save8Args& a, hipStream_t s) {
   if (a.count <= 0 || a.width <= 0) return hipSuccess;
-  const long es = a.dtype == DSB_DT_F32 ? 4 : 2;
-  const bool vec = a.width % 8 == 0 && a.ldx * es % 16 == 0 && (!a.r || a.ldr * es % 16 == 0) &&
-                   a.ldc % 8 == 0 && aligned(a.x, 16) && aligned(a.r, 16) && aligned(a.codes, 8);
-  const bool e4 = a.code == DSB_DT_E4M3;
-  auto go = [&](auto kernel, unsigned gy) {
-    hipLaunchKernelGGL(kernel, dim3(a.count, gy), dim3(256), 0, s, a);
-    return hipGetLastError();
-  };
-  auto by_type = [&](auto t) {
-    constexpr int T = decltype(t)::value;
-    if (!vec) {
-      const unsigned gy = runs(a.width, 8 * kBlock8 * 4);
-      return e4 ? go(save_rows8_any_kernel<T, DSB_DT_E4M3>, gy)
-                : go(save_rows8_any_kernel<T, DSB_DT_INT8>, gy);
+  const double n = (double)a.count * a.width, es = a.dtype == DSB_DT_F32 ? 4 : 2;
+  // (never kFar: 139 µs in place of 124 for 8192 × 28672)
+  return by_cache((a.r ? 2 : 1) * es * n, (a.r ? 2 : 1) * es * n, [&](auto p) {
+    constexpr int P = decltype(p)::value;
+    auto go = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3(a.count, runs(a.width, kSaveRun)), dim3(256), 0, s, a);
+      return hipGetLastError();
+    };
+    auto by_code = [&](auto t, auto c) {
+      constexpr int T = decltype(t)::value, C = decltype(c)::value;
+      return a.r ? go(save_rows8_kernel<T, C, true, P>) : go(save_rows8_kernel<T, C, false, P>);
+    };
+    auto by_type = [&](auto t) {
+      return a.code == DSB_DT_E4M3 ? by_code(t, Int<DSB_DT_E4M3>{}) : by_code(t, Int<DSB_DT_INT8>{});
+    };
+    switch (a.dtype) {
+      case DSB_DT_BF16: return by_type(Int<DSB_DT_BF16>{});
+      case DSB_DT_F16: return by_type(Int<DSB_DT_F16>{});
+      default: return by_type(Int<DSB_DT_F32>{});
     }
-    const unsigned gy = runs(a.width, kSaveRun);
-    if (a.r)
-      return e4 ? go(save_rows8_kernel<T, DSB_DT_E4M3, true>, gy)
-                : go(save_rows8_kernel<T, DSB_DT_INT8, true>, gy);
-    return e4 ? go(save_rows8_kernel<T, DSB_DT_E4M3, false>, gy)
-              : go(save_rows8_kernel<T, DSB_DT_INT8, false>, gy);
-  };
-  switch (a.dtype) {
-    case DSB_DT_BF16: return by_type(std::integral_constant<int, DSB_DT_BF16>{});
-    case DSB_DT_F16: return by_type(std::integral_constant<int, DSB_DT_F16>{});
-    case DSB_DT_F32: return by_type(std::integral_constant<int, DSB_DT_F32>{});
-    default: return hipErrorInvalidValue;
-  }
+  });
 }
 
 hipError_t restore_rows8(const RowsArg& q, int rows, int width, void* out, long ldo, bool f32,
                          hipStream_t s) {
   if (rows <= 0 || width <= 0) return hipSuccess;
-  const bool vec = width % 8 == 0 && q.ld % 8 == 0 && aligned(q.p, 8) &&
-                   ldo * (f32 ? 4 : 2) % 16 == 0 && aligned(out, 16);
-  auto go = [&](auto kernel, unsigned gy) {
-    hipLaunchKernelGGL(kernel, dim3(rows, gy), dim3(256), 0, s, q, width, out, ldo);
-    return hipGetLastError();
-  };
-  auto by_code = [&](auto c) {
-    constexpr int C = decltype(c)::value;
-    if (!vec) {
-      const unsigned gy = runs(width, 2048);
-      return f32 ? go(restore_rows8_any_kernel<C, true>, gy) : go(restore_rows8_any_kernel<C, false>, gy);
-    }
-    const unsigned gy = runs(width, kRestoreRun);
-    return f32 ? go(restore_rows8_kernel<C, true>, gy) : go(restore_rows8_kernel<C, false>, gy);
-  };
-  return q.type == DSB_DT_E4M3 ? by_code(std::integral_constant<int, DSB_DT_E4M3>{})
-                               : by_code(std::integral_constant<int, DSB_DT_INT8>{});
+  const double n = (double)rows * width;
+  return by_cache(n, (f32 ? 4 : 2) * n, [&](auto p) {
+    constexpr int P = decltype(p)::value;
+    auto go = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3(rows, runs(width, kRestoreRun)), dim3(256), 0, s, q, width, out, ldo);
+      return hipGetLastError();
+    };
+    auto by_code = [&](auto c) {
+      constexpr int C = decltype(c)::value;
+      return f32 ? go(restore_rows8_kernel<C, true, P>) : go(restore_rows8_kernel<C, false, P>);
+    };
+    return q.type == DSB_DT_E4M3 ? by_code(Int<DSB_DT_E4M3>{}) : by_code(Int<DSB_DT_INT8>{});
+  });
 }
 
 hipError_t swiglu(const SwigluArgs& a, hipStream_t s) {
   if (a.rows <= 0 || a.I <= 0) return hipSuccess;
-  auto go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(a.rows, runs(a.I, kGluRun)), dim3(256), 0, s, a);
-    return hipGetLastError();
-  };
-  auto by_kind = [&](auto k) {
-    constexpr int K = decltype(k)::value;
-    if (!a.dh.p) return go(swiglu_kernel<K, kRowsNone>);
-    return a.dh.type == DSB_DT_F32 ? go(swiglu_kernel<K, kRowsF32>) : go(swiglu_kernel<K, kRowsBF16>);
-  };
-  return a.gu.type == DSB_DT_BF16 ? by_kind(std::integral_constant<int, kRowsBF16>{})
-                                  : by_kind(std::integral_constant<int, kRows8>{});
+  const double n = (double)a.rows * a.I;
+  return by_cache(n * (2 * row_bytes(a.gu) + row_bytes(a.dh)), n * ((a.dh.p ? 4 : 0) + (a.h ? 2 : 0)),
+                  [&](auto p) {
+    constexpr int P = decltype(p)::value;
+    auto go = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3(a.rows, runs(a.I, kGluRun)), dim3(256), 0, s, a);
+      return hipGetLastError();
+    };
+    auto by_dh = [&](auto t) {
+      constexpr int T = decltype(t)::value;
+      if (!a.dh.p) return go(swiglu_kernel<T, kRowsNone, P>);
+      return a.dh.type == DSB_DT_F32 ? go(swiglu_kernel<T, DSB_DT_F32, P>)
+                                     : go(swiglu_kernel<T, DSB_DT_BF16, P>);
+    };
+    switch (a.gu.type) {
+      case DSB_DT_BF16: return by_dh(Int<DSB_DT_BF16>{});
+      case DSB_DT_E4M3: return by_dh(Int<DSB_DT_E4M3>{});
+      default: return by_dh(Int<DSB_DT_INT8>{});
+    }
+  });
 }
 
 }  // namespace dsb
