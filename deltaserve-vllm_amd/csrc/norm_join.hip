@@ -169,96 +169,82 @@ __global__ __launch_bounds__(kMostThreads / 2) void join_fwd_kernel(JoinArgs a) 
   }
 }
 
-// R runs of 8 columns a thread; XT, YT, GT: the types of x', y and dn, FULL: a gate of rows. With a block
-// its sums over rows go into part [2][gridDim.x][D]: Σ dn·x̂, and Σ t·ŷ with a gate that differs by row,
-// of which dw_out and a channel gate's dgate are multiples (join_sums_kernel).
-template <int XT, int YT, int GT, bool FULL, int P, int R>
-__global__ __launch_bounds__(R == 1 ? kMostThreads : kMostThreads / 2) void join_bwd_kernel(JoinArgs a, float* part) {
+// 8 columns a thread; XT, YT, GT: the types of x', y and dn, FULL: a gate of rows. With a block its
+// sums over rows go into part [2][gridDim.x][D]: Σ dn·x̂, and Σ t·ŷ times a gate that differs by row, of
+// which dw_out and a channel gate's dgate are multiples (join_sums_kernel).
+template <int XT, int YT, int GT, bool FULL, int P>
+__global__ __launch_bounds__(kMostThreads) void join_bwd_kernel(JoinArgs a, float* part) {
   constexpr bool Y = YT != kRowsNone, N = GT != kRowsNone;
   __shared__ float red[2][kMostWaves][8];
   int turn = 0;
-  const int nch = a.D >> 3;
+  // threads past the row take its last columns too, and leave them out of sums and results
+  const int c = min((int)threadIdx.x, (a.D >> 3) - 1);
+  const bool live = threadIdx.x == c;
   const float rD = 1.f / (float)a.D;
-  float cw[Y ? R : 1][8];  // w_out·a gate by channel
-  u32x4 wi[R] = {};
+  float cw[8];  // w_out·a gate by channel
+  u32x4 wi = {};
+  if (N) wi = ldg128(a.w_in + 8 * c);
+  if constexpr (Y) {
+    float g[8];
 #pragma unroll
-  for (int i = 0; i < R; ++i) {
-    const int c = threadIdx.x + i * blockDim.x;
-    if (c < nch) {
-      if (N) wi[i] = ldg128(a.w_in + 8 * c);
-      if constexpr (Y) {
-        float g[8];
+    for (int e = 0; e < 8; ++e) cw[e] = g[e] = 1.f;
+    if (a.w_out) unpack8(ldg128(a.w_out + 8 * c), cw);
+    if (a.gate_kind == kGateChannel) unpack8(ldg128(a.gate + 8 * c), g);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) cw[i][e] = g[e] = 1.f;
-        if (a.w_out) unpack8(ldg128(a.w_out + 8 * c), cw[i]);
-        if (a.gate_kind == kGateChannel) unpack8(ldg128(a.gate + 8 * c), g);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) cw[i][e] *= g[e];
-      }
-    }
+    for (int e = 0; e < 8; ++e) cw[e] *= g[e];
   }
-  float s_in[Y ? R : 1][8] = {}, s_out[Y ? R : 1][8] = {};
+  float s_in[8] = {}, s_out[8] = {};
   for (long row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    Raw8<XT> x[R];
-    Raw8<YT> y[R];
-    Raw8<GT> dn[R];
-    u32x4 ta[R] = {}, tb[R] = {}, gf[R];  // dx' (bf16 or fp32), a gate of rows
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-      const int c = threadIdx.x + i * blockDim.x;
-      if (c < nch) {
-        if (N) x[i].template load<P>(a.x, row, c);
-        y[i].template load<P>(a.y, row, c);
-        dn[i].template load<P>(a.dn, row, c);
-        if (a.dxn.p) {
-          if (a.dxn.type == DSB_DT_F32) {
-            const float* p = (const float*)a.dxn.p + row * a.dxn.ld + 8 * c;
-            ta[i] = load_as<P, u32x4>(p);
-            tb[i] = load_as<P, u32x4>(p + 4);
-          } else {
-            ta[i] = load_as<P, u32x4>((const bf16*)a.dxn.p + row * a.dxn.ld + 8 * c);
-          }
-        }
-        if (FULL) gf[i] = load_as<P, u32x4>(a.gate + row * a.ldg + 8 * c);
+    Raw8<XT> x;
+    Raw8<YT> y;
+    Raw8<GT> dn;
+    u32x4 ta = {}, tb = {}, gf;  // dx' (bf16 or fp32), a gate of rows
+    if (N) x.template load<P>(a.x, row, c);
+    y.template load<P>(a.y, row, c);
+    dn.template load<P>(a.dn, row, c);
+    if (a.dxn.p) {
+      if (a.dxn.type == DSB_DT_F32) {
+        const float* p = (const float*)a.dxn.p + row * a.dxn.ld + 8 * c;
+        ta = load_as<P, u32x4>(p);
+        tb = load_as<P, u32x4>(p + 4);
+      } else {
+        ta = load_as<P, u32x4>((const bf16*)a.dxn.p + row * a.dxn.ld + 8 * c);
       }
     }
+    if (FULL) gf = load_as<P, u32x4>(a.gate + row * a.ldg + 8 * c);
     const float gr = Y && a.gate_kind == kGateRow ? (float)a.gate[row * a.ldg] : 1.f;
+    float xv[8], dv[8], yv[8], t[8], w[8], g[8];
+    if (N) {
+      x.get(xv);
+      dn.get(dv);
+      unpack8(wi, w);
+    }
+    if (Y) y.get(yv);
+    if (FULL) unpack8(gf, g);
+    if (a.dxn.type == DSB_DT_F32)
+      floats8(ta, tb, t);
+    else
+      unpack8(ta, t);
     // Σ x'², Σ dn·w_in·x', Σ y², Σ c·y·dx', Σ c·y·dn·w_in, Σ c·y·x'; c without a row's gate
     float s[Y ? 6 : 2] = {};
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-      if (threadIdx.x + i * blockDim.x >= nch) continue;
-      float xv[8], dv[8], yv[8], t[8], w[8], g[8];
+    for (int e = 0; e < 8; ++e) {
       if (N) {
-        x[i].get(xv);
-        dn[i].get(dv);
-        unpack8(wi[i], w);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          dv[e] *= w[e];
-          s[0] += xv[e] * xv[e];
-          s[1] += dv[e] * xv[e];
-        }
+        s[0] += xv[e] * xv[e];
+        s[1] += dv[e] * w[e] * xv[e];
       }
       if constexpr (Y) {
-        y[i].get(yv);
-        if (a.dxn.type == DSB_DT_F32)
-          floats8(ta[i], tb[i], t);
-        else
-          unpack8(ta[i], t);
-        if (FULL) unpack8(gf[i], g);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float cy = (FULL ? cw[i][e] * g[e] : cw[i][e]) * yv[e];
-          s[2] += yv[e] * yv[e];
-          s[3] += cy * t[e];
-          if (N) {
-            s[4] += cy * dv[e];
-            s[5] += cy * xv[e];
-          }
+        const float cy = (FULL ? cw[e] * g[e] : cw[e]) * yv[e];
+        s[2] += yv[e] * yv[e];
+        s[3] += cy * t[e];
+        if (N) {
+          s[4] += cy * (dv[e] * w[e]);
+          s[5] += cy * xv[e];
         }
       }
     }
+#pragma unroll
+    for (int i = 0; i < (Y ? 6 : 2); ++i) s[i] = live ? s[i] : 0.f;
     block_totals(s, red, turn);
     const float inv = rsqrtf(s[0] * rD + a.eps);
     const float k = s[1] * inv * rD;  // mean(dn·w_in·x̂)
@@ -272,74 +258,52 @@ __global__ __launch_bounds__(R == 1 ? kMostThreads : kMostThreads / 2) void join
       }
       if (a.dgate_row && threadIdx.x == 0) a.dgate_row[row] = a.scale * p * j;
     }
-    const float to_y = a.scale * gr * j, back = m * j;
+    if (N) {
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-      const int c = threadIdx.x + i * blockDim.x;
-      if (c >= nch) continue;
-      float t[8];
-      if (a.dxn.type == DSB_DT_F32)
-        floats8(ta[i], tb[i], t);
-      else
-        unpack8(ta[i], t);
-      if (N) {
-        float xv[8], dv[8], w[8];
-        x[i].get(xv);
-        dn[i].get(dv);
-        unpack8(wi[i], w);
+      for (int e = 0; e < 8; ++e) {
+        const float hat = xv[e] * inv;
+        t[e] += (dv[e] * w[e] - hat * k) * inv;
+        if (Y) s_in[e] += dv[e] * hat;
+      }
+    }
+    if (live) put8<P>(a.dx, row * a.lddx + 8 * c, a.dx_f32, t);
+    if constexpr (Y) {
+      const float to_y = a.scale * gr * j, back = m * j;
+      float o[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        yv[e] *= j;
+        o[e] = (FULL ? cw[e] * g[e] : cw[e]) * t[e] * to_y;
+      }
+      if (a.w_out) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] -= yv[e] * back;
+      }
+      if (live) put8<P>(a.dy, row * a.lddy + 8 * c, false, o);
+      if (FULL) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float hat = xv[e] * inv;
-          t[e] += (dv[e] * w[e] - hat * k) * inv;
-          if (Y) s_in[i][e] += dv[e] * hat;
+          o[e] = a.scale * (t[e] * yv[e]) * cw[e];
+          yv[e] *= g[e];
         }
+        if (live) put8<P>(a.dgate_full, row * a.lddg + 8 * c, false, o);
+      } else if (a.gate_kind == kGateRow) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) yv[e] *= gr;
       }
-      put8<P>(a.dx, row * a.lddx + 8 * c, a.dx_f32, t);
-      if constexpr (Y) {
-        float yv[8], g[8], o[8];
-        y[i].get(yv);
-        if (FULL) unpack8(gf[i], g);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          yv[e] *= j;
-          o[e] = (FULL ? cw[i][e] * g[e] : cw[i][e]) * t[e] * to_y;
-        }
-        if (a.w_out) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) o[e] -= yv[e] * back;
-        }
-        put8<P>(a.dy, row * a.lddy + 8 * c, false, o);
-        if (FULL) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            o[e] = a.scale * (t[e] * yv[e]) * cw[i][e];
-            yv[e] *= g[e];
-          }
-          put8<P>(a.dgate_full, row * a.lddg + 8 * c, false, o);
-        } else if (a.gate_kind == kGateRow) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) yv[e] *= gr;
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) s_out[i][e] += t[e] * yv[e];
-      }
+      for (int e = 0; e < 8; ++e) s_out[e] += t[e] * yv[e];
     }
   }
   if constexpr (Y) {
-    if (!part) return;
-    const long plane = (long)gridDim.x * a.D;
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-      const int c = threadIdx.x + i * blockDim.x;
-      if (c >= nch) continue;
-      auto put = [&](float* o, const float* v) {
-        *reinterpret_cast<f32x4*>(o) = f32x4{v[0], v[1], v[2], v[3]};
-        *reinterpret_cast<f32x4*>(o + 4) = f32x4{v[4], v[5], v[6], v[7]};
-      };
-      float* p = part + (long)blockIdx.x * a.D + 8 * c;
-      if (a.dw_in) put(p, s_in[i]);
-      put(p + plane, s_out[i]);
-    }
+    if (!part || !live) return;
+    auto put = [&](float* o, const float* v) {
+      *reinterpret_cast<f32x4*>(o) = f32x4{v[0], v[1], v[2], v[3]};
+      *reinterpret_cast<f32x4*>(o + 4) = f32x4{v[4], v[5], v[6], v[7]};
+    };
+    float* p = part + (long)blockIdx.x * a.D + 8 * c;
+    if (a.dw_in) put(p, s_in);
+    if (a.dw_out || a.dgate) put(p + (long)gridDim.x * a.D, s_out);
   }
 }
 
@@ -386,17 +350,17 @@ __global__ __launch_bounds__(kSumThreads) void join_sums_kernel(JoinArgs a, cons
 
 int waves_of(int D, int runs) { return (D / 8 + 64 * runs - 1) / (64 * runs); }
 constexpr int kCUs = 256;
-// Threads of a kernel that keeps no sums: the chip's.
-constexpr int kThreads = 1 << 19;
-int blocks_of(int rows, int D, int runs) { return std::min(rows, kThreads / (64 * waves_of(D, runs))); }
-// With sums a thread needs 170 to 250 registers, so that a CU holds 8 waves: whole blocks of them. Two
-// runs a thread, or three where more blocks fit that way (640 columns' runs: one block of 5 waves, or two of 4).
-constexpr int kSumWaves = 8;
-int best_runs(int D) {
-  return kSumWaves / waves_of(D, 3) > kSumWaves / waves_of(D, 2) ? 3 : 2;
-}
+// Blocks of a kernel that keeps no sums: of the chip's threads.
+int blocks_of(int rows, int waves) { return std::min(rows, (1 << 13) / waves); }
+// The forward's runs a thread: two, or three where more of its blocks fit 8 waves that way (8191 × 5120, 5
+// waves or 4: 76 or 62 µs; 8192 wide, 8 or 6: 88 or 128; one run each 74 and 101).
+int fwd_runs(int D) { return 8 / waves_of(D, 3) > 8 / waves_of(D, 2) ? 3 : 2; }
+// With sums, 8 waves a CU, which leave the fewest sums to write out, or two blocks where 16 waves, all
+// that fit its registers, hold them: a lone block waits at its barriers. 8192 × 4096, one / two blocks of 8
+// waves a CU: 104 / 92 µs; 32768 × 1024, eight / sixteen of one wave: 88 / 94.
 int sum_blocks(int rows, int D) {
-  const int most = kCUs * std::max(1, kSumWaves / waves_of(D, best_runs(D)));
+  const int w = waves_of(D, 1);
+  const int most = kCUs * std::max(1, std::max(8 / w, std::min(2, 16 / w)));
   // a CU has a block before a block has a second row, whose sums cost nothing more to write out
   return rows <= kCUs ? rows : std::min(std::max(kCUs, (rows + 1) / 2), most);
 }
@@ -408,9 +372,9 @@ hipError_t join_fwd(const JoinArgs& a, hipStream_t s) {
   const double in = row_bytes(a.x) + row_bytes(a.y) + (a.gate_kind == kGateFull ? 2 : 0);
   const double out = (a.x_new ? row_bytes(a.x) : 0) + (a.normed ? 2 : 0);
   const bool near = cache_of(in * a.rows * a.D, out * a.rows * a.D) == kNear;
-  const int runs = best_runs(a.D);
+  const int runs = fwd_runs(a.D), waves = waves_of(a.D, runs);
   auto go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(blocks_of(a.rows, a.D, runs)), dim3(64 * waves_of(a.D, runs)), 0, s, a);
+    hipLaunchKernelGGL(kernel, dim3(blocks_of(a.rows, waves)), dim3(64 * waves), 0, s, a);
     return hipGetLastError();
   };
   auto by_cache = [&](auto x, auto y) {
@@ -432,26 +396,21 @@ int64_t join_bwd_bytes(int rows, int D, int sums) {
 
 hipError_t join_bwd(const JoinArgs& a, void* work, hipStream_t s) {
   const bool sums = a.dw_in || a.dw_out || a.dgate, full = a.gate_kind == kGateFull;
-  const int runs = a.y.p ? best_runs(a.D) : 1;
-  const int blocks = a.y.p ? sum_blocks(a.rows, a.D) : blocks_of(a.rows, a.D, runs);
+  const int waves = waves_of(a.D, 1);
+  const int blocks = a.y.p ? sum_blocks(a.rows, a.D) : blocks_of(a.rows, waves);
   float* part = sums ? (float*)work : nullptr;
   const double in = (a.dn.p ? row_bytes(a.x) : 0) + row_bytes(a.y) + row_bytes(a.dn) + row_bytes(a.dxn) +
                     (full ? 2 : 0);
   const double out = (a.dx_f32 ? 4 : 2) + (a.y.p ? 2 : 0) + (full ? 2 : 0);
   const bool near = cache_of(in * a.rows * a.D, out * a.rows * a.D) == kNear;
   auto go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(64 * waves_of(a.D, runs)), 0, s, a, part);
+    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(64 * waves), 0, s, a, part);
     return hipGetLastError();
   };
   auto by_cache = [&](auto x, auto y, auto g, auto f) {
     constexpr int X = decltype(x)::value, Y = decltype(y)::value, G = decltype(g)::value;
     constexpr bool F = decltype(f)::value;
-    if constexpr (Y == kRowsNone)
-      return near ? go(join_bwd_kernel<X, Y, G, F, kNear, 1>) : go(join_bwd_kernel<X, Y, G, F, kFar, 1>);
-    else if (runs == 2)
-      return near ? go(join_bwd_kernel<X, Y, G, F, kNear, 2>) : go(join_bwd_kernel<X, Y, G, F, kFar, 2>);
-    else
-      return near ? go(join_bwd_kernel<X, Y, G, F, kNear, 3>) : go(join_bwd_kernel<X, Y, G, F, kFar, 3>);
+    return near ? go(join_bwd_kernel<X, Y, G, F, kNear>) : go(join_bwd_kernel<X, Y, G, F, kFar>);
   };
   auto by_gate = [&](auto x, auto y, auto g) {
     return full ? by_cache(x, y, g, std::true_type{}) : by_cache(x, y, g, std::false_type{});

@@ -3,7 +3,8 @@
 //
 // A lane holds 8 columns: its loads of 16 bytes (8 of codes) cover whole lines over a wave, and a
 // block of 32 columns is four neighbouring lanes, whose maximum takes two DPP steps. Rows may start
-// anywhere; the last columns of a width that is no multiple of 8 are moved one by one.
+// anywhere; the last columns of a width that is no multiple of 8 are moved one by one. A workgroup takes
+// several narrow rows, or a part of a wide one (Span).
 #include "block.h"
 
 namespace dsb {
@@ -54,6 +55,30 @@ DSB_DEV void few(const void* p, long i, int count, float v[8]) {
   for (int e = 0; e < 8; ++e) v[e] = e < count ? widen<T>(p, i + e) : 0.f;
 }
 
+// How 256 threads lie over rows: 2^lanes_log (4 to 256) of them to a row, V runs of 8 columns each.
+struct Span {
+  int rows, lanes_log;
+};
+template <int V>
+struct Spot {
+  long row;
+  int column, step;  // of the thread's first run, and between its runs
+  DSB_DEV Spot(Span p) {
+    row = (long)blockIdx.x * (256 >> p.lanes_log) + (threadIdx.x >> p.lanes_log);
+    step = 8 << p.lanes_log;
+    column = blockIdx.y * V * step + (threadIdx.x & ((1 << p.lanes_log) - 1)) * 8;
+  }
+};
+template <int V>
+Span span_of(int rows, int width, dim3& grid) {
+  Span p{rows, 2};
+  while (p.lanes_log < 8 && (8l * V << p.lanes_log) < width) ++p.lanes_log;
+  const int each = 256 >> p.lanes_log;
+  const long run = 8l * V << p.lanes_log;
+  grid = dim3((unsigned)((rows + each - 1) / each), (unsigned)((width + run - 1) / run));
+  return p;
+}
+
 // The rows that slot i moves; false: none.
 DSB_DEV bool slot_rows(const Save8Args& a, int i, long& s, long& d) {
   s = a.src ? a.src[i] : i;
@@ -61,16 +86,16 @@ DSB_DEV bool slot_rows(const Save8Args& a, int i, long& s, long& d) {
   return d >= 0 && d < a.out_rows && s >= 0 && s < a.x_rows;
 }
 
-constexpr int kSaveVec = 2, kSaveRun = 256 * 8 * kSaveVec;
+constexpr int kSaveVec = 2;
 template <int T, int CODE, bool RES, int P>
-__global__ __launch_bounds__(256) void save_rows8_kernel(Save8Args a) {
+__global__ __launch_bounds__(256) void save_rows8_kernel(Save8Args a, Span span) {
+  const Spot<kSaveVec> at(span);
   long s, d;
-  if (!slot_rows(a, blockIdx.x, s, d)) return;
-  const int c0 = blockIdx.y * kSaveRun + threadIdx.x * 8;
+  if (at.row >= span.rows || !slot_rows(a, (int)at.row, s, d)) return;  // (a block's lanes are of one row)
   In8<T> x[kSaveVec], r[kSaveVec];
 #pragma unroll
   for (int i = 0; i < kSaveVec; ++i) {
-    const int c = c0 + 2048 * i;
+    const int c = at.column + at.step * i;
     if (c + 8 <= a.width) {
       x[i].template load<P>(a.x, s * a.ldx + c);
       if (RES) r[i].template load<P>(a.r, s * a.ldr + c);
@@ -78,7 +103,7 @@ __global__ __launch_bounds__(256) void save_rows8_kernel(Save8Args a) {
   }
 #pragma unroll
   for (int i = 0; i < kSaveVec; ++i) {
-    const int c = c0 + 2048 * i, left = a.width - c;
+    const int c = at.column + at.step * i, left = a.width - c;
     float v[8] = {}, w[8];
     unsigned top = 0;
     if (left > 0) {
@@ -112,23 +137,25 @@ __global__ __launch_bounds__(256) void save_rows8_kernel(Save8Args a) {
   }
 }
 
-constexpr int kRestoreVec = 4, kRestoreRun = 256 * 8 * kRestoreVec;
+constexpr int kRestoreVec = 4;
 template <int CODE, bool F32, int P>
-__global__ __launch_bounds__(256) void restore_rows8_kernel(RowsArg q, int width, void* out, long ldo) {
-  const long row = blockIdx.x;
-  const int c0 = blockIdx.y * kRestoreRun + threadIdx.x * 8;
+__global__ __launch_bounds__(256) void restore_rows8_kernel(RowsArg q, int width, void* out, long ldo,
+                                                            Span span) {
+  const Spot<kRestoreVec> at(span);
+  const long row = at.row;
+  if (row >= span.rows) return;
   const uint8_t* in = (const uint8_t*)q.p + row * q.ld;
   u32x2 x[kRestoreVec];
   unsigned byte[kRestoreVec];
 #pragma unroll
   for (int i = 0; i < kRestoreVec; ++i) {
-    const int c = c0 + 2048 * i;
+    const int c = at.column + at.step * i;
     if (c + 8 <= width) x[i] = load_as<P, u32x2b>(in + c);
     if (c < width) byte[i] = q.s[row * q.lds + c / kBlock8];
   }
 #pragma unroll
   for (int i = 0; i < kRestoreVec; ++i) {
-    const int c = c0 + 2048 * i, left = width - c;
+    const int c = at.column + at.step * i, left = width - c;
     float v[8];
     if (left >= 8) {
       decode8<CODE>(x[i], byte[i], v);
@@ -155,16 +182,17 @@ __global__ __launch_bounds__(256) void restore_rows8_kernel(RowsArg q, int width
 
 // A lane takes 8 gate and 8 up columns of a row. BWD with σ = σ(gate):
 //   dgate = dh·up·σ·(1 + gate·(1 − σ)), dup = dh·gate·σ
-constexpr int kGluVec = 2, kGluRun = 256 * 8 * kGluVec;
+constexpr int kGluVec = 2;
 template <int T, int DH, int P>
-__global__ __launch_bounds__(256) void swiglu_kernel(SwigluArgs a) {
-  const long row = blockIdx.x;
-  const int c0 = blockIdx.y * kGluRun + threadIdx.x * 8;
+__global__ __launch_bounds__(256) void swiglu_kernel(SwigluArgs a, Span span) {
+  const Spot<kGluVec> at(span);
+  const long row = at.row;
+  if (row >= span.rows) return;
   Raw8<T> g[kGluVec], u[kGluVec];
   Raw8<DH> dh[kGluVec];
 #pragma unroll
   for (int i = 0; i < kGluVec; ++i) {
-    const int c = c0 + 2048 * i;
+    const int c = at.column + at.step * i;
     if (c < a.I) {
       g[i].template load<P>(a.gu, row, c / 8);
       u[i].template load<P>(a.gu, row, (a.I + c) / 8);
@@ -173,7 +201,7 @@ __global__ __launch_bounds__(256) void swiglu_kernel(SwigluArgs a) {
   }
 #pragma unroll
   for (int i = 0; i < kGluVec; ++i) {
-    const int c = c0 + 2048 * i;
+    const int c = at.column + at.step * i;
     if (c >= a.I) continue;
     float gv[8], uv[8], dv[8], og[8], ou[8], h[8];
     g[i].get(gv);
@@ -194,7 +222,6 @@ __global__ __launch_bounds__(256) void swiglu_kernel(SwigluArgs a) {
   }
 }
 
-unsigned runs(int width, int run) { return (unsigned)((width + run - 1) / run); }
 template <class F>
 hipError_t by_cache(double in, double out, F f) {
   switch (cache_of(in, out)) {
@@ -213,7 +240,9 @@ hipError_t save_rows8(const Save8Args& a, hipStream_t s) {
   return by_cache((a.r ? 2 : 1) * es * n, (a.r ? 2 : 1) * es * n, [&](auto p) {
     constexpr int P = decltype(p)::value;
     auto go = [&](auto kernel) {
-      hipLaunchKernelGGL(kernel, dim3(a.count, runs(a.width, kSaveRun)), dim3(256), 0, s, a);
+      dim3 grid;
+      const Span span = span_of<kSaveVec>(a.count, a.width, grid);
+      hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, a, span);
       return hipGetLastError();
     };
     auto by_code = [&](auto t, auto c) {
@@ -238,7 +267,9 @@ hipError_t restore_rows8(const RowsArg& q, int rows, int width, void* out, long 
   return by_cache(n, (f32 ? 4 : 2) * n, [&](auto p) {
     constexpr int P = decltype(p)::value;
     auto go = [&](auto kernel) {
-      hipLaunchKernelGGL(kernel, dim3(rows, runs(width, kRestoreRun)), dim3(256), 0, s, q, width, out, ldo);
+      dim3 grid;
+      const Span span = span_of<kRestoreVec>(rows, width, grid);
+      hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, q, width, out, ldo, span);
       return hipGetLastError();
     };
     auto by_code = [&](auto c) {
@@ -256,7 +287,9 @@ hipError_t swiglu(const SwigluArgs& a, hipStream_t s) {
                   [&](auto p) {
     constexpr int P = decltype(p)::value;
     auto go = [&](auto kernel) {
-      hipLaunchKernelGGL(kernel, dim3(a.rows, runs(a.I, kGluRun)), dim3(256), 0, s, a);
+      dim3 grid;
+      const Span span = span_of<kGluVec>(a.rows, a.I, grid);
+      hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, a, span);
       return hipGetLastError();
     };
     auto by_dh = [&](auto t) {
