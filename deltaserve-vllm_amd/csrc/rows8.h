@@ -91,10 +91,11 @@ DSB_DEV unsigned abs_bits(float v) { return __builtin_bit_cast(unsigned, v) & 0x
 //          before may have left there; stores that stay in the L2 are written back at the kernel's end
 //   kFar   loads past them, stores into them: larger calls whose outputs the next kernel finds there
 //   kPast  both past them: outputs of more than 256 MB
+//   kIn    both through them: for stores that cover lines in parts
 // µs, near / far / past (bytes of the call): RMSNorm of 2048 × 4096 8-bit rows (25 MB) 4.9 / 8.2 / 7.1, of
 // 8192 × 4096 (102 MB) 21 / 29 / 29; SwiGLU of 8192 × 14336 (477 MB) 91 / 73 / 86, its backward (1.2 GB, 705
 // MB of them out) 229 / 237 / 222; rows of 8192 × 28672 restored (712 MB, 470 out) 129 / 141 / 127.
-enum { kNear, kFar, kPast };
+enum { kNear, kFar, kPast, kIn };
 inline int cache_of(double in, double out) {
   constexpr double kLast = 256 << 20;
   return in + out <= kLast ? kNear : out <= kLast ? kFar : kPast;
@@ -102,13 +103,13 @@ inline int cache_of(double in, double out) {
 template <int P, class V>
 DSB_DEV V load_as(const void* p) {
   const V* q = reinterpret_cast<const V*>(p);
-  if constexpr (P == kNear) return *q;
+  if constexpr (P == kNear || P == kIn) return *q;
   return __builtin_nontemporal_load(q);
 }
 template <int P, class V>
 DSB_DEV void store_as(void* p, V v) {
   V* q = reinterpret_cast<V*>(p);
-  if constexpr (P == kFar)
+  if constexpr (P == kFar || P == kIn)
     *q = v;
   else
     __builtin_nontemporal_store(v, q);

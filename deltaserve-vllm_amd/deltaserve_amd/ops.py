@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 from ctypes import byref, c_float, c_int, c_int32, c_int64, c_void_p
 
 import numpy as np
@@ -136,7 +137,7 @@ def gemm_glu(A, B, A2=None, B2=None, with_h=True):
 def rmsnorm(x, w, eps):
     """ops.py:84-88 (bf16 in/out, fp32 internals). x may be :class:`Rows8`; the call then only
     enqueues."""
-    if isinstance(x, Rows8):
+    if type(x) is Rows8:
         return _rmsnorm8(x, w, eps)
     _dev(x, w)
     y = torch.empty(x.shape, dtype=BF16, device=x.device)
@@ -149,7 +150,7 @@ def rmsnorm_backward(x, g, w, eps, resid=None):
     """ops.py:91-100 (+ bf16 residual add, llama3.py:205); bf16 out. An fp32 g
     [parts, n, D] is added up in order first. x may be :class:`Rows8`, g then a matrix; the call
     then only enqueues."""
-    if isinstance(x, Rows8):
+    if type(x) is Rows8:
         return _rmsnorm8_backward(x, g, w, eps, resid)
     _dev(x, g, w, resid)
     out = torch.empty(x.shape, dtype=BF16, device=x.device)
@@ -692,36 +693,32 @@ _DT = {BF16: L.DT_BF16, torch.float16: L.DT_F16, torch.float32: L.DT_F32}
 
 def _matrix(what, name, t, shape, dtypes):
     """The row stride of a matrix of this shape (None: any) and one of these types."""
-    if t.dtype not in dtypes or t.dim() != 2 or (shape is not None and t.shape != shape):
+    size = t.shape
+    if t.dtype not in dtypes or len(size) != 2 or (shape is not None and size != shape):
         of = "" if shape is None else f" [{shape[0]}, {shape[1]}]"
         raise ValueError(f"{what}: {name} must be a matrix{of} of "
                          f"{' or '.join(str(d) for d in dtypes)}")
-    n, width = t.shape
-    if t.numel() and width > 1 and t.stride(1) != 1:
+    n, width = size
+    step, unit = t.stride()
+    if unit != 1 and width > 1 and n:
         raise ValueError(f"{what}: {name}'s last dimension must be contiguous")
     # the row stride of a single row is any number: one that is whole
-    return t.stride(0) if n > 1 else -(-width // 8) * 8
+    return step if n > 1 else -(-width // 8) * 8
 
 
 def _rows(what, name, t, shape, dtypes=_FLOATS):
     """(address, row stride, scales' address, scales' row stride, type) of rows, 8-bit ones among
     them."""
-    if isinstance(t, Rows8):
-        if shape is not None and t.shape != shape:
+    if type(t) is Rows8:
+        if shape is not None and t.codes.shape != shape:
             raise ValueError(f"{what}: {name} must be [{shape[0]}, {shape[1]}]")
-        c, s = t.codes, t.scales
-        n, width = c.shape
-        return (c.data_ptr(), c.stride(0) if n > 1 else -(-width // 8) * 8, s.data_ptr(),
-                s.stride(0) if n > 1 else s.shape[1], t.type)
+        return t.codes.data_ptr(), t.ld, t.scales.data_ptr(), t.ld_scales, t.type
     return t.data_ptr(), _matrix(what, name, t, shape, dtypes), None, 0, _DT[t.dtype]
 
 
-def _where(*ts):
-    """Their tensors, for :func:`_on`."""
-    out = []
-    for t in ts:
-        out += [t.codes, t.scales] if isinstance(t, Rows8) else [t]
-    return out
+def _held(t):
+    """A tensor of rows, for :func:`_on`."""
+    return t.codes if type(t) is Rows8 else t
 
 
 def pack_rows8(x, r=None, code="e4m3", out=None, src=None, dst=None):
@@ -744,7 +741,7 @@ def pack_rows8(x, r=None, code="e4m3", out=None, src=None, dst=None):
         raise ValueError(f"{what}: out must be Rows8 of x's width" + (" and rows" if src is None else ""))
     count = n if src is None else src.numel()
     c, ldc, s, lds, kind = _rows(what, "out", out, None)
-    with _on(what, *_where(x, r, src, dst, out)):
+    with _on(what, x, r, src, dst, out.codes):
         L.check(L.load().dsb_save_rows8(
             _at(x), ldx, _at(r), ldr, n, _DT[x.dtype], _at(src), _at(dst), count,
             width, c, ldc, s, lds, kind, len(out), _now()), what="dsb_save_rows8")
@@ -759,7 +756,7 @@ def unpack_rows8(q, dtype=BF16):
         raise ValueError(f"{what}: dtype is bfloat16 or float32")
     c, ldc, s, lds, kind = _rows(what, "q", q, None)
     n, width = q.shape
-    with _on(what, *_where(q)):
+    with _on(what, q.codes):
         out = torch.empty(n, width, dtype=dtype, device=q.device)
         L.check(L.load().dsb_op_restore_rows8(c, ldc, s, lds, kind, n, width, _at(out), width,
                                               dtype == torch.float32, _now()),
@@ -772,7 +769,7 @@ def _rmsnorm8(x, w, eps):
     n, D = x.shape
     args = _rows(what, "x", x, None)
     _vec(what, "w", w, D, BF16)
-    with _on(what, *_where(x, w)):
+    with _on(what, x.codes, w):
         y = torch.empty(n, D, dtype=BF16, device=x.device)
         L.check(L.load().dsb_op_norm_join(*args, None, 0, None, _at(w), None, 0, L.GATE_NONE, 1.0, eps,
                                           n, D, None, 0, _at(y), D, _now()), what="dsb_op_norm_join")
@@ -786,7 +783,7 @@ def _rmsnorm8_backward(x, g, w, eps, resid):
     ldg = _matrix(what, "g", g, x.shape, _FLOATS)
     ldr = 0 if resid is None else _matrix(what, "resid", resid, x.shape, (BF16,))
     _vec(what, "w", w, D, BF16)
-    with _on(what, *_where(x, g, w, resid)):
+    with _on(what, x.codes, g, w, resid):
         out = torch.empty(n, D, dtype=BF16, device=x.device)
         L.check(L.load().dsb_op_norm_join_bwd(
             *args, None, 0, None, 0, 0, _at(g), ldg, g.dtype == torch.float32, _at(resid), ldr, 0, None,
@@ -807,7 +804,7 @@ def swiglu(gu):
     """bf16(silu(gate)·up) [n, I] of gate‖up rows [n, 2I], bf16 or :class:`Rows8`; I a multiple of 8."""
     what = "swiglu"
     args, n, I = _glu_args(what, gu)
-    with _on(what, *_where(gu)):
+    with _on(what, _held(gu)):
         h = torch.empty(n, I, dtype=BF16, device=gu.device)
         L.check(L.load().dsb_op_swiglu(*args, n, I, _at(h), I, _now()), what="dsb_op_swiglu")
     return h
@@ -819,7 +816,7 @@ def swiglu_backward(gu, dh, with_h=False):
     what = "swiglu_backward"
     args, n, I = _glu_args(what, gu)
     lddh = _matrix(what, "dh", dh, (n, I), _FLOATS)
-    with _on(what, *_where(gu, dh)):
+    with _on(what, _held(gu), dh):
         dgu = torch.empty(n, 2 * I, dtype=BF16, device=gu.device)
         h = torch.empty(n, I, dtype=BF16, device=gu.device) if with_h else None
         L.check(L.load().dsb_op_swiglu_bwd(*args, n, I, _at(dh), lddh, dh.dtype == torch.float32,
@@ -848,6 +845,14 @@ def _join_args(what, n, D, w_in, w_out, gate):
     return 1, L.GATE_ROW
 
 
+@functools.lru_cache(maxsize=1024)
+def _join_bytes(n, D):
+    """The workspace of a join's backward with sums."""
+    nbytes = c_int64()
+    L.check(L.load().dsb_op_norm_join_workspace(n, D, 1, byref(nbytes)), what="dsb_op_norm_join_workspace")
+    return nbytes.value
+
+
 def residual_norm(x, y, w_in, eps, w_out=None, gate=None, scale=1.0):
     """A block's output y (bf16 [n, D]) joined to the residual stream x (bf16 or fp32): with z = y, or
     y / rms(y)·w_out with ``w_out``,
@@ -859,7 +864,7 @@ def residual_norm(x, y, w_in, eps, w_out=None, gate=None, scale=1.0):
     where w_in is None). D a multiple of 8 up to 8192."""
     what = "residual_norm"
     args = _rows(what, "x", x, None)
-    if isinstance(x, Rows8):
+    if args[2] is not None:
         raise ValueError(f"{what}: x must be bf16 or fp32")
     n, D = x.shape
     ldy = _matrix(what, "y", y, x.shape, (BF16,))
@@ -894,30 +899,30 @@ def residual_norm_backward(x_new, y, dnormed, w_in, eps, dx_new=None, w_out=None
     ldn = 0 if dnormed is None else _matrix(what, "dnormed", dnormed, (n, D), _FLOATS)
     ldx = 0 if dx_new is None else _matrix(what, "dx_new", dx_new, (n, D), _FLOATS)
     ldg, kind = _join_args(what, n, D, w_in, w_out, gate)
-    f32 = lambda t: t is not None and t.dtype == torch.float32  # noqa: E731
-    with _on(what, *_where(None if w_in is None else x_new, y, dnormed, dx_new, w_in, w_out, gate)):
-        new = lambda dt, *s: torch.empty(*s, dtype=dt, device=y.device)  # noqa: E731
-        dx = new((dnormed if dx_new is None else dx_new).dtype, n, D)
-        dy = new(BF16, n, D)
-        dw_out = new(torch.float32, D) if w_out is not None and weight_grads else None
-        dw_in = new(torch.float32, D) if w_in is not None and weight_grads else None
-        dgate = None
+    with _on(what, None if w_in is None else _held(x_new), _held(y), dnormed, dx_new, w_in, w_out, gate):
+        dev = y.device
+        f32 = torch.float32
+        dx = torch.empty(n, D, dtype=(dnormed if dx_new is None else dx_new).dtype, device=dev)
+        dy = torch.empty(n, D, dtype=BF16, device=dev)
+        dw_out = dw_in = dgate = work = None
+        nbytes = 0
+        if weight_grads and (w_out is not None or w_in is not None or kind == L.GATE_CHANNEL):
+            sums = list(torch.empty((w_out is not None) + (w_in is not None) + (kind == L.GATE_CHANNEL), D,
+                                    dtype=f32, device=dev).unbind(0))
+            dw_out = None if w_out is None else sums.pop()
+            dw_in = None if w_in is None else sums.pop()
+            dgate = sums.pop() if sums else None
+            nbytes = _join_bytes(n, D)
+            work = _work(nbytes, dev)
         if kind == L.GATE_FULL:
-            dgate = new(BF16, n, D)
+            dgate = torch.empty(n, D, dtype=BF16, device=dev)
         elif kind == L.GATE_ROW:
-            dgate = new(torch.float32, *gate.shape)
-        elif kind == L.GATE_CHANNEL and weight_grads:
-            dgate = new(torch.float32, D)
-        sums = dw_out is not None or dw_in is not None or (kind == L.GATE_CHANNEL and weight_grads)
-        work, nbytes = None, c_int64(0)
-        if sums:
-            L.check(L.load().dsb_op_norm_join_workspace(n, D, 1, byref(nbytes)),
-                    what="dsb_op_norm_join_workspace")
-            work = _work(nbytes.value, y.device)
+            dgate = torch.empty(gate.shape, dtype=f32, device=dev)
         L.check(L.load().dsb_op_norm_join_bwd(
-            *xargs, *yargs, _at(dnormed), ldn, f32(dnormed), _at(dx_new), ldx, f32(dx_new), _at(w_out),
-            _at(w_in), _at(gate), ldg, kind, scale, eps, n, D, _at(dx), D, f32(dx), _at(dy), D,
-            _at(dgate), D, _at(dw_out), _at(dw_in), _at(work), nbytes.value, _now()),
+            *xargs, *yargs, _at(dnormed), ldn, dnormed is not None and dnormed.dtype == f32, _at(dx_new),
+            ldx, dx_new is not None and dx_new.dtype == f32, _at(w_out), _at(w_in), _at(gate), ldg, kind,
+            scale, eps, n, D, _at(dx), D, dx.dtype == f32, _at(dy), D, _at(dgate), D, _at(dw_out),
+            _at(dw_in), _at(work), nbytes, _now()),
             what="dsb_op_norm_join_bwd")
     return dx, dy, dgate, dw_out, dw_in
 

@@ -25,7 +25,7 @@ class Rows8:
     """codes [rows, width] (``torch.float8_e4m3fn`` or ``torch.int8``) and scales uint8 [rows,
     ceil(width / 32)], on one device, each row contiguous. Slices of rows share their memory."""
 
-    __slots__ = ("codes", "scales", "type")
+    __slots__ = ("codes", "scales", "type", "ld", "ld_scales")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
         if codes.dtype not in _TYPE or codes.dim() != 2:
@@ -39,6 +39,9 @@ class Rows8:
             if t.numel() and t.shape[1] > 1 and t.stride(1) != 1:
                 raise ValueError("Rows8: rows must be contiguous")
         self.codes, self.scales, self.type = codes, scales, _TYPE[codes.dtype]
+        # (the row stride of a single row is any number)
+        self.ld = codes.stride(0) if n > 1 else -(-w // 8) * 8
+        self.ld_scales = scales.stride(0) if n > 1 else scales.shape[1]
 
     @classmethod
     def zeros(cls, rows: int, width: int, code: str = "e4m3", device="cuda") -> "Rows8":

@@ -558,7 +558,7 @@ int dsb_op_norm_join(const void* x, int64_t ldx, const uint8_t* x_scales, int64_
  * normed and dxn of x_new (bf16 or fp32 each; null: zeros; dn null: w_in and x_new are not used):
  *   dx (bf16 or fp32, of x and of x_new's whole), dy (bf16), dw_out and dw_in fp32 [D] (null: not wanted),
  *   dgate: null (not wanted), fp32 [D], fp32 [rows] or bf16 rows of stride lddg, as the gate's kind is.
- * y null: the gradient of a norm alone. `sums`: whether any of dw_out, dw_in and a channel
+ * y null: the gradient of a norm alone, without dw_in. `sums`: whether any of dw_out, dw_in and a channel
  * gate's dgate is wanted; they are added over rows in fp32 in a fixed order. */
 int dsb_op_norm_join_workspace(int rows, int D, int sums, int64_t* bytes);
 int dsb_op_norm_join_bwd(const void* x_new, int64_t ldx, const uint8_t* x_scales, int64_t ldxs,

@@ -186,7 +186,11 @@ def test_norm_join_backward_refusals():
     bad("without the weight", w_in=None)
     bad("without a gate", gate=None, kind=0)
     bad("block's", dy=None)
-    bad("dy is null", dy=None, w_out=None, dw_out=None, gate=None, kind=0, dgate=None)
+    alone = dict(dy=None, w_out=None, dw_out=None, gate=None, kind=0, dgate=None)
+    bad("dy is null", **alone, dw_in=None)
+    bad("comes with a block", **alone)
+    bad("neither a block nor a norm", **alone, y=None, dn=None, w_in=None, dw_in=None)
+    bad("null", kind=3, ldg=64, dgate=None)
     bad("null", dx=None)
     bad("null", y=None)
     bad("stride", lddx=56)
@@ -194,7 +198,7 @@ def test_norm_join_backward_refusals():
     bad("16-byte", kind=3, ldg=64, lddg=68)
     bad("vectors", dw_in=A + 4)
     bad("vectors", dgate=A + 4)
-    bad("too small", bytes=12 * 4 * 64 - 1)
+    bad("too small", bytes=8 * 4 * 64 - 1)
     bad("too small", work=None)
     bad("workspace must", work=A + 4)
 
@@ -202,7 +206,7 @@ def test_norm_join_backward_refusals():
 def test_norm_join_workspace():
     L, lib = _lib()
     b = ctypes.c_int64(-1)
-    for rows, D, sums, want in ((0, 64, 1, 0), (4, 64, 1, 12 * 4 * 64), (4, 64, 0, 0)):
+    for rows, D, sums, want in ((0, 64, 1, 0), (4, 64, 1, 8 * 4 * 64), (4, 64, 0, 0)):
         assert lib.dsb_op_norm_join_workspace(rows, D, sums, ctypes.byref(b)) == 0 and b.value == want
     for args in ((-1, 64, 1, ctypes.byref(b)), (1, 65, 1, ctypes.byref(b)), (1, 64, 1, None)):
         _refused("dsb_op_norm_join_workspace", args, "bad argument")
