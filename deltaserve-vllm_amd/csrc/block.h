@@ -21,8 +21,9 @@ struct Save8Args {
   long out_rows;               // rows that may be written
 };
 hipError_t save_rows8(const Save8Args& a, hipStream_t s);
+// rows_dev (or null): rows past *rows_dev are left as they are.
 hipError_t restore_rows8(const RowsArg& q, int rows, int width, void* out, long ldo, bool f32,
-                         hipStream_t s);
+                         hipStream_t s, const int* rows_dev = nullptr);
 // h = silu(gate)·up of gate‖up rows, and with dh (bf16 or fp32) its gradient dgu; h or dgu null: not
 // wanted.
 struct SwigluArgs {

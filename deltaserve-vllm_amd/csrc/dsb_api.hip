@@ -24,6 +24,7 @@
 #include <vector>
 
 #include "../../include/dsb.h"
+#include "block.h"
 #include "gemm_nt.h"
 #include "kernels.h"
 #include "workspace.h"
@@ -218,6 +219,10 @@ struct dsb_handle {
   const bf16* lm_w = nullptr;
   const bf16* norm_w = nullptr;
   std::vector<const bf16*> layer_in;
+  // layer inputs and gate‖up kept in 8 bits (empty: bf16), and where a layer's
+  // input is restored for its recompute and backward (one by recompute set)
+  std::vector<RowsArg> layer_in8, gate_up_in8;
+  bf16* xr[2] = {};
   std::vector<const bf16*> gate_up_in;  // saved gate‖up per layer (empty: recompute)
   long ld_gate_up = 0;
   // the other optional save points per layer (empty: recomputed)
@@ -964,15 +969,16 @@ int enqueue_layer(dsb_handle* h, int li, int lo, hipStream_t st, bool rec, bool 
     const double au = (double)Hq * h->hd;
     const double arow = 2.0 * (q + 2.0 * kv);
     LayerState& ls = h->layers[li];
-    const bf16* x = h->layer_in[li];
-    const long ldx = h->act_ld;
+    const bool x8 = !h->layer_in8.empty(), gu8 = !h->gate_up_in8.empty();
+    const bf16* x = x8 ? h->xr[li & 1] : h->layer_in[li];
+    const long ldx = x8 ? (long)D : h->act_ld;
     const bool hq = has_qkv(ls), ho = ls.has[DSB_PROJ_O], hg = has_gu(ls),
                hd = ls.has[DSB_PROJ_DOWN];
     // gate‖up: the saved forward activations when the store carries them
     // (ffn.py:18-26, llama3.py:63-72), else recomputed into h->gu
-    const bool saved_gu = !h->gate_up_in.empty();
-    const bf16* gu = saved_gu ? h->gate_up_in[li] : h->gu;
-    const long ldgu = saved_gu ? h->ld_gate_up : 2L * I;
+    const bool saved_gu = gu8 || !h->gate_up_in.empty();
+    const bf16* gu = saved_gu && !gu8 ? h->gate_up_in[li] : h->gu;
+    const long ldgu = saved_gu && !gu8 ? h->ld_gate_up : 2L * I;
     const bf16* wqkv = (const bf16*)ls.w.qkv;
     const bf16* wo = (const bf16*)ls.w.o;
     const bf16* wgu = (const bf16*)ls.w.gate_up;
@@ -1001,6 +1007,14 @@ int enqueue_layer(dsb_handle* h, int li, int lo, hipStream_t st, bool rec, bool 
 
     // ================= forward recompute (llama3.py:62-146, qwen3.py:68-130)
     if (rec) {
+    if (x8) {
+      KScope ks(h, st, "restore8", 0, 0, 0, 3.0 * D, 0, 0);
+      LK(restore_rows8(h->layer_in8[li], N, D, h->xr[li & 1], D, false, st, nd));
+    }
+    if (gu8) {
+      KScope ks(h, st, "restore8", 0, 0, 0, 6.0 * I, 0, 0);
+      LK(restore_rows8(h->gate_up_in8[li], N, 2 * I, h->gu, 2L * I, false, st, nd));
+    }
     {
       KScope ks(h, st, "rmsnorm_fwd", 0, 0, 0, 4.0 * D, 0, 2.0 * D);
       LK(rmsnorm_fwd(x, ldx, (const bf16*)ls.w.in_ln, h->xn1, D, N, nd, D, eps, st));
@@ -1788,15 +1802,31 @@ int dsb_bind_lora(dsb_handle* h, int layer, int proj, const dsb_lora_tensors* t)
   return 0;
 }
 
-int dsb_bind_activations(dsb_handle* h, const dsb_activations* a) {
-  if (!h || !a || !a->layer_in || !a->final_in || !a->input_ids)
+int dsb_bind_activations8(dsb_handle* h, const dsb_activations* a, const dsb_rows8* layer_in8,
+                          const dsb_rows8* gate_up8) {
+  if (!h || !a || !a->final_in || !a->input_ids || (!a->layer_in && !layer_in8))
     return fail(h, "dsb_bind_activations: null argument");
+  if ((a->layer_in && layer_in8) || (a->mlp_gate_up && gate_up8))
+    return fail(h, "dsb_bind_activations: a save point is bound in bf16 or in 8 bits");
   std::lock_guard<std::mutex> lk(h->mu);
   if (h->in_step) return fail(h, "dsb_bind_activations: a segmented cycle is in progress");
   if (a->ld < h->D || a->ld % 8) return fail(h, "dsb_bind_activations: bad row stride");
   if (a->mlp_gate_up && (a->ld_gate_up < 2L * h->I || a->ld_gate_up % 8))
     return fail(h, "dsb_bind_activations: mlp_gate_up row stride must be a multiple of 8 and "
                    ">= 2*intermediate");
+  std::vector<RowsArg> li8, gu8;
+  auto rows8 = [&](const dsb_rows8* r, int width, std::vector<RowsArg>& out) -> int {
+    for (int i = 0; r && i < h->L; ++i) {
+      const dsb_rows8& q = r[i];
+      if ((q.type != DSB_DT_E4M3 && q.type != DSB_DT_INT8) || !q.codes || !q.scales || q.ld < width ||
+          q.ld_scales < (width + DSB_ROWS8_BLOCK - 1) / DSB_ROWS8_BLOCK)
+        return fail(h, "dsb_bind_activations: bad 8-bit rows");
+      out.push_back(RowsArg{q.codes, (long)q.ld, q.scales, (long)q.ld_scales, q.type});
+    }
+    return 0;
+  };
+  CKR(rows8(layer_in8, h->D, li8));
+  CKR(rows8(gate_up8, 2 * h->I, gu8));
   std::vector<const bf16*> gu;
   if (a->mlp_gate_up) {
     for (int i = 0; i < h->L; ++i) {
@@ -1837,11 +1867,18 @@ int dsb_bind_activations(dsb_handle* h, const dsb_activations* a) {
   CKR(saved(a->attn_v, a->ld_v, h->kv, "attn_v", vv));
   CKR(saved(a->attn_ctx, a->ld_ctx, h->q, "attn_ctx", cv));
   CKR(saved(a->resid_mid, a->ld_resid_mid, h->D, "resid_mid", rv));
+  if (!li8.empty() && !h->xr[0]) {
+    CKR(dalloc(h, &h->xr[0], (h->N + 1L) * h->D));
+    h->xr[1] = h->xr[0];
+    if (h->overlap) CKR(dalloc(h, &h->xr[1], (h->N + 1L) * h->D));
+  }
   h->layer_in.assign(h->L, nullptr);
-  for (int i = 0; i < h->L; ++i) {
+  for (int i = 0; a->layer_in && i < h->L; ++i) {
     if (!a->layer_in[i]) return fail(h, "dsb_bind_activations: null layer_in");
     h->layer_in[i] = (const bf16*)a->layer_in[i];
   }
+  h->layer_in8 = li8;
+  h->gate_up_in8 = gu8;
   h->gate_up_in = gu;
   h->ld_gate_up = a->mlp_gate_up ? (long)a->ld_gate_up : 0;
   h->q_in = qv; h->k_in = kv_; h->v_in = vv; h->ctx_in = cv; h->rm_in = rv;
@@ -1853,6 +1890,10 @@ int dsb_bind_activations(dsb_handle* h, const dsb_activations* a) {
   // Rebinding activations after capture changes baked pointers: drop the graphs.
   drop_graphs(h);
   return 0;
+}
+
+int dsb_bind_activations(dsb_handle* h, const dsb_activations* a) {
+  return dsb_bind_activations8(h, a, nullptr, nullptr);
 }
 
 int dsb_reset_optimizer(dsb_handle* h, float weight_decay) {

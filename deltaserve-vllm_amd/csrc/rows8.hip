@@ -142,10 +142,10 @@ __global__ __launch_bounds__(256) void save_rows8_kernel(Save8Args a, Span span)
 constexpr int kRestoreVec = 4;
 template <int CODE, bool F32, int P>
 __global__ __launch_bounds__(256) void restore_rows8_kernel(RowsArg q, int width, void* out, long ldo,
-                                                            Span span) {
+                                                            Span span, const int* rows_dev) {
   const Spot<kRestoreVec> at(span);
   const long row = at.row;
-  if (row >= span.rows) return;
+  if (row >= (rows_dev ? min(span.rows, *rows_dev) : span.rows)) return;
   const uint8_t* in = (const uint8_t*)q.p + row * q.ld;
   u32x2 x[kRestoreVec];
   unsigned byte[kRestoreVec];
@@ -263,7 +263,7 @@ hipError_t save_rows8(const Save8Args& a, hipStream_t s) {
 }
 
 hipError_t restore_rows8(const RowsArg& q, int rows, int width, void* out, long ldo, bool f32,
-                         hipStream_t s) {
+                         hipStream_t s, const int* rows_dev) {
   if (rows <= 0 || width <= 0) return hipSuccess;
   const double n = (double)rows * width;
   return by_cache(n, (f32 ? 4 : 2) * n, [&](auto p) {
@@ -271,7 +271,7 @@ hipError_t restore_rows8(const RowsArg& q, int rows, int width, void* out, long 
     auto go = [&](auto kernel) {
       dim3 grid;
       const Span span = span_of<kRestoreVec>(rows, width, 2, grid);
-      hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, q, width, out, ldo, span);
+      hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, q, width, out, ldo, span, rows_dev);
       return hipGetLastError();
     };
     auto by_code = [&](auto c) {

@@ -92,6 +92,11 @@ class DsbAdamChunk(Structure):
                 ("pad", c_int32)]
 
 
+class DsbRows8(Structure):
+    _fields_ = [("codes", c_void_p), ("scales", c_void_p), ("ld", c_int64), ("ld_scales", c_int64),
+                ("type", c_int32), ("pad", c_int32)]
+
+
 # name -> (restype, argtypes)
 _SIGS = {
     "dsb_create": (c_int, [POINTER(DsbDesc), POINTER(c_void_p)]),
@@ -101,6 +106,8 @@ _SIGS = {
     "dsb_bind_head": (c_int, [c_void_p, c_void_p, c_void_p]),
     "dsb_bind_lora": (c_int, [c_void_p, c_int, c_int, POINTER(DsbLoraTensors)]),
     "dsb_bind_activations": (c_int, [c_void_p, POINTER(DsbActivations)]),
+    "dsb_bind_activations8": (c_int, [c_void_p, POINTER(DsbActivations), POINTER(DsbRows8),
+                                      POINTER(DsbRows8)]),
     "dsb_step": (c_int, [c_void_p, POINTER(c_int32), c_int, c_int, c_float, c_int64,
                          c_void_p, POINTER(c_float), POINTER(c_int),
                          POINTER(DsbCycleInfo)]),

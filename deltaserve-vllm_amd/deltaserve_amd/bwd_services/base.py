@@ -56,6 +56,7 @@ import torch
 
 from deltaserve_amd import dprint, handover, integrity, mark_backward_process
 from deltaserve_amd.pause import PauseGate
+from deltaserve_amd.rows8 import Rows8
 
 # Environment the child inherits from the parent's MPS wrapping; echoed in
 # ``ready`` so the parent can log what the child got.
@@ -470,7 +471,7 @@ class BackwardService:
     def _wipe_activations(self) -> None:
         for value in (self.activations or {}).values():
             for t in (value if isinstance(value, (list, tuple)) else [value]):
-                if torch.is_tensor(t):
+                if torch.is_tensor(t) or isinstance(t, Rows8):
                     t.zero_()
 
     def _report(self, cyc: Cycle, gpu_ms: float | None) -> None:

@@ -30,6 +30,7 @@ from deltaserve_amd.bwd_services.base import BackwardService
 from deltaserve_amd.bwd_services.common.family import LORA_PROJS, Family
 from deltaserve_amd.checkpoint import AdapterCheckpointer, write_save_error
 from deltaserve_amd.ops import rope_inv_freq  # noqa: F401  (re-exported for callers)
+from deltaserve_amd.rows8 import Rows8
 
 # PEFT adapter keys turned into fp32 masters (trainer.py:46-47, extended to the
 # MLP projections).
@@ -245,6 +246,10 @@ class LoraSftTrainerService(BackwardService):
                 continue
             if len(bufs) != self.L:
                 raise ValueError(f"{name} carries {len(bufs)} layers, the model has {self.L}")
+            if name == "mlp_gate_up" and any(isinstance(t, Rows8) for t in bufs):
+                self._check_rows8(name, bufs, width)
+                out[name] = (bufs, 0)
+                continue
             ld = bufs[0].stride(0)
             for t in bufs:
                 if (t.dtype != torch.bfloat16 or not t.is_cuda or t.stride(0) != ld
@@ -254,6 +259,14 @@ class LoraSftTrainerService(BackwardService):
             out[name] = (bufs, ld)
         return out
 
+    def _check_rows8(self, name, bufs, width) -> None:
+        """8-bit rows, all of a save point's (``ActivationStore(code=...)``)."""
+        for t in bufs:
+            if not isinstance(t, Rows8) or not t.codes.is_cuda or t.shape[1] != width:
+                raise TypeError(f"{name} buffers must be Rows8 [rows, {width}] on the device, all of them")
+            if len(t) <= self._s_max:
+                raise ValueError(f"{name} buffers hold fewer rows than a cycle may have")
+
     def _bind_activations(self, activations) -> None:
         li = activations["layer_in"]
         fi = activations["final_in"]
@@ -261,13 +274,18 @@ class LoraSftTrainerService(BackwardService):
         if len(li) != self.L:
             raise ValueError(f"activations carry {len(li)} layer inputs, the model has {self.L}")
         ld = fi.stride(0)
-        for t in list(li) + [fi]:
+        li8 = any(isinstance(t, Rows8) for t in li)
+        if li8:
+            self._check_rows8("layer_in", li, self.D)
+        for t in ([] if li8 else list(li)) + [fi]:
             if t.dtype != torch.bfloat16 or not t.is_cuda or t.stride(0) != ld or t.stride(1) != 1:
                 raise TypeError("activation buffers must be bf16 CUDA [rows, D] with one row stride")
         if ids.dtype != torch.int64 or not ids.is_cuda:
             raise TypeError("concat_input_ids must be an int64 CUDA tensor")
         saved = self._saved_points(activations)
-        key = (tuple(t.data_ptr() for t in li), fi.data_ptr(), ids.data_ptr(), ld,
+        scales = [t.scales.data_ptr() for bufs in (li, saved.get("mlp_gate_up", ((),))[0]) for t in bufs
+                  if isinstance(t, Rows8)]
+        key = (tuple(t.data_ptr() for t in li), tuple(scales), fi.data_ptr(), ids.data_ptr(), ld,
                tuple((name, tuple(t.data_ptr() for t in bufs), sld)
                      for name, (bufs, sld) in sorted(saved.items())))
         if key == self._act_key:
@@ -279,16 +297,31 @@ class LoraSftTrainerService(BackwardService):
             keep.append(arr)
             return ctypes.cast(arr, ctypes.POINTER(c_void_p))
 
+        def rows8(bufs):
+            return (L.DsbRows8 * self.L)(*[L.DsbRows8(t.codes.data_ptr(), t.scales.data_ptr(), t.ld,
+                                                      t.ld_scales, t.type) for t in bufs])
+
         a = L.DsbActivations()
-        a.layer_in, a.final_in, a.input_ids, a.ld = ptrs(li), fi.data_ptr(), ids.data_ptr(), ld
+        a.final_in, a.input_ids, a.ld = fi.data_ptr(), ids.data_ptr(), ld
+        if not li8:
+            a.layer_in = ptrs(li)
+        gu8 = None
+        if "mlp_gate_up" in saved and isinstance(saved["mlp_gate_up"][0][0], Rows8):
+            gu8 = rows8(saved["mlp_gate_up"][0])
         fields = {"mlp_gate_up": ("mlp_gate_up", "ld_gate_up"), "attn_qh": ("attn_q", "ld_q"),
                   "attn_kh": ("attn_k", "ld_k"), "attn_vh": ("attn_v", "ld_v"),
                   "attn_ctx": ("attn_ctx", "ld_ctx"), "resid_mid": ("resid_mid", "ld_resid_mid")}
         for name, (bufs, sld) in saved.items():
+            if name == "mlp_gate_up" and gu8 is not None:
+                continue
             f_ptr, f_ld = fields[name]
             setattr(a, f_ptr, ptrs(bufs))
             setattr(a, f_ld, sld)
-        L.check(L.load().dsb_bind_activations(self._h, byref(a)), self._h, "dsb_bind_activations")
+        if li8 or gu8 is not None:
+            L.check(L.load().dsb_bind_activations8(self._h, byref(a), rows8(li) if li8 else None, gu8),
+                    self._h, "dsb_bind_activations8")
+        else:
+            L.check(L.load().dsb_bind_activations(self._h, byref(a)), self._h, "dsb_bind_activations")
         self._act_ptrs = keep
         self._act_key = key
         self.saved_points = sorted(saved)
@@ -380,10 +413,10 @@ class LoraSftTrainerService(BackwardService):
         base = {k.replace(".base_layer.", "."): v for k, v in (self.shared.get("base") or {}).items()}
         out = []
 
-        def judge(name, got, want):
+        def judge(name, got, want, tol=self.VERIFY_TOL):
             err = float((got.float() - want.float()).abs().max())
             rel = err / (float(want.float().abs().max()) + 1e-6)
-            ok = rel < self.VERIFY_TOL
+            ok = rel < tol
             dprint(f"[verify] {name}: max|d|={err:.3e} rel={rel:.3e} {'OK' if ok else 'FAIL'}")
             out.append((name, rel, ok))
 
@@ -391,7 +424,12 @@ class LoraSftTrainerService(BackwardService):
         layer_in = activations.get("layer_in") or []
         embed = base.get(meta.get("embed_weight_key") or "model.embed_tokens.weight")
         if layer_in and embed is not None:
-            judge("layer_in[0] vs embed[ids]", layer_in[0][:n], embed[ids])
+            got, tol = layer_in[0][:n], self.VERIFY_TOL
+            if isinstance(got, Rows8):  # a code is off by half a step, 2^-4 of the value, at most
+                from deltaserve_amd import ops
+
+                got, tol = ops.unpack_rows8(got), tol + 2.0 ** -4
+            judge("layer_in[0] vs embed[ids]", got, embed[ids], tol)
         final_in, final_hidden = activations.get("final_in"), activations.get("final_hidden")
         norm_w = base.get(meta.get("norm_weight_key") or "model.norm.weight")
         if final_in is not None and final_hidden is not None and norm_w is not None and n > 0:

@@ -177,6 +177,10 @@ class ActivationStore:
     output), ``save_resid_mid`` → ``resid_mid`` ``[max_saved + 1, hidden]``
     (the post-attention residual), and ``save_final_hidden`` →
     ``final_hidden`` (the final norm's output, for the debug capture check).
+    ``code`` ("e4m3" or "int8") keeps ``layer_in`` and ``mlp_gate_up``, nearly all of the
+    store, in 8 bits (:class:`Rows8`, 1.03 bytes a value in place of 2): the save calls round
+    to it and a backward cycle restores a layer's rows when it recomputes the layer. The other
+    points stay bf16. The reference's store is bf16 alone.
     The slot table has the reference's 7 slots per layer plus the final
     norm's; the slots of save points that are off hold no buffer, so their
     save calls are no-ops, as in the reference.
@@ -187,7 +191,8 @@ class ActivationStore:
     def __init__(self, num_layers: int, hidden_size: int, max_saved: int, device="cuda",
                  intermediate_size: int = 0, q_size: int = 0, kv_size: int = 0,
                  save_attn_qkv: bool = False, save_attn_ctx: bool = False,
-                 save_resid_mid: bool = False, save_final_hidden: bool = False):
+                 save_resid_mid: bool = False, save_final_hidden: bool = False,
+                 code: Optional[str] = None):
         if max_saved <= 0 or num_layers <= 0 or hidden_size <= 0 or intermediate_size < 0:
             raise ValueError("ActivationStore: sizes must be positive")
         if (save_attn_qkv and (q_size <= 0 or kv_size <= 0)) or (save_attn_ctx and q_size <= 0):
@@ -200,8 +205,11 @@ class ActivationStore:
         def buf(width=hidden_size):
             return torch.zeros(max_saved + 1, width, dtype=torch.bfloat16, device=self.device)
 
-        self.layer_in = [buf() for _ in range(num_layers)]
-        self.mlp_gate_up = ([buf(2 * intermediate_size) for _ in range(num_layers)]
+        def point(width=hidden_size):
+            return buf(width) if code is None else Rows8.zeros(max_saved + 1, width, code, self.device)
+
+        self.layer_in = [point() for _ in range(num_layers)]
+        self.mlp_gate_up = ([point(2 * intermediate_size) for _ in range(num_layers)]
                             if intermediate_size > 0 else [])
         per_layer = lambda on, width: [buf(width) for _ in range(num_layers)] if on else []  # noqa: E731
         self.attn_qh = per_layer(save_attn_qkv, q_size)

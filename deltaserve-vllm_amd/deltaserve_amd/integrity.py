@@ -18,6 +18,7 @@ import re
 import torch
 
 from deltaserve_amd import dprint
+from deltaserve_amd.rows8 import Rows8
 
 _LAYER_NO = re.compile(r"layers?\.(\d+)\.")
 
@@ -25,6 +26,9 @@ _LAYER_NO = re.compile(r"layers?\.(\d+)\.")
 def tensor_digest(t: torch.Tensor) -> str:
     """16-hex-digit SHA-1 of the tensor's values as fp32, whatever its dtype
     (backward_process.py:44-47)."""
+    if isinstance(t, Rows8):  # the bytes of the codes, then of the scales
+        data = [x.contiguous().view(torch.uint8).cpu().numpy().tobytes() for x in (t.codes, t.scales)]
+        return hashlib.sha1(b"".join(data)).hexdigest()[:16]
     data = t.detach().to("cpu", torch.float32).contiguous().numpy()
     return hashlib.sha1(data.tobytes()).hexdigest()[:16]
 

@@ -69,6 +69,9 @@ class Rows8:
     def nbytes(self) -> int:
         return self.codes.nbytes + self.scales.nbytes
 
+    def data_ptr(self) -> int:
+        return self.codes.data_ptr()
+
     def __len__(self) -> int:
         return self.codes.shape[0]
 

@@ -156,6 +156,19 @@ int dsb_bind_head(dsb_handle* h, const void* lm_head, const void* final_norm);
 int dsb_bind_lora(dsb_handle* h, int layer, int proj, const dsb_lora_tensors* t);
 /* Binds the shared activation buffers (base.py:438-461 share_activations). */
 int dsb_bind_activations(dsb_handle* h, const dsb_activations* a);
+/* The same with a layer's inputs, or its inputs and gate‖up, in 8 bits (the formats are described
+ * with dsb_save_rows8): n_layers descriptors each, or NULL; `a` then holds NULL in their place. The cycle restores a
+ * layer's rows to bf16, exactly, when it recomputes the layer, and is that of a bf16 store of these
+ * values bit for bit. No counterpart in the reference, whose store is bf16. */
+typedef struct dsb_rows8 {
+  const void* codes;
+  const uint8_t* scales;
+  int64_t ld, ld_scales;
+  int32_t type; /* DSB_DT_E4M3 or DSB_DT_INT8 */
+  int32_t pad;
+} dsb_rows8;
+int dsb_bind_activations8(dsb_handle* h, const dsb_activations* a, const dsb_rows8* layer_in,
+                          const dsb_rows8* mlp_gate_up);
 
 /* One backward cycle + AdamW step (+ the served-slot publish when slots are
  * bound, dsb_bind_served): trainer.py:503-678.

@@ -333,3 +333,62 @@ def test_rotary_refusals():
                  lambda: ops.rotary(x, p.float(), plan)):
         with pytest.raises(ValueError):
             call()
+
+
+# ---------------------------------------------------------------- the store in 8 bits, around the cycle
+
+def test_rows8_go_between_processes_and_are_fingerprinted_and_wiped():
+    import pickle
+
+    from deltaserve_amd import integrity
+    from deltaserve_amd.bwd_services.base import BackwardService
+    from deltaserve_amd.rows8 import Rows8
+
+    q = Rows8.zeros(5, 40, "int8", "cpu")
+    q.codes.copy_(torch.arange(200, dtype=torch.int8).view(5, 40))
+    q.scales.fill_(120)
+    p = pickle.loads(pickle.dumps(q))
+    assert type(p) is Rows8 and torch.equal(p.codes, q.codes) and torch.equal(p.scales, q.scales)
+    assert (p.type, p.shape, p.ld_scales) == (q.type, q.shape, q.ld_scales)
+    acts = {"layer_in": [q, p], "concat_input_ids": torch.arange(5)}
+    rep = integrity.activation_hash_report(acts, 4)
+    assert rep["layer_in_first"] == rep["layer_in_last"] != integrity.tensor_digest(q[:3])
+    p.scales[0, 0] = 121
+    assert integrity.activation_hash_report(acts, 4)["layer_in_last"] != rep["layer_in_last"]
+    svc = BackwardService.__new__(BackwardService)
+    svc.activations = acts
+    svc._wipe_activations()
+    assert (q.codes == 0).all() and (q.scales == 1).all() and (acts["concat_input_ids"] == 0).all()
+
+
+def test_a_store_in_8_bits_on_the_host():
+    from deltaserve_amd.capture import ActivationStore
+    from deltaserve_amd.rows8 import Rows8
+
+    s = ActivationStore(2, 64, 10, device="cpu", intermediate_size=96, code="e4m3")
+    assert all(isinstance(b, Rows8) and b.shape == (11, 64) for b in s.layer_in)
+    assert all(b.shape == (11, 192) for b in s.mlp_gate_up) and torch.is_tensor(s.final_in)
+    s.layer_in[0].codes.view(torch.uint8).fill_(9)
+    s.zero_offset_range(3, 4)
+    rows = s.layer_in[0].codes.view(torch.uint8)[:, 0]
+    assert rows.tolist() == [9] * 3 + [0] * 4 + [9] * 4
+    with pytest.raises(ValueError):
+        ActivationStore(2, 64, 10, device="cpu", code="int4")
+
+
+def test_rows8_struct_matches_header(tmp_path):
+    import os
+    import subprocess
+
+    from harness import ROOT
+
+    L, _ = _lib()
+    src = tmp_path / "p.c"
+    names = [f for f, _ in L.DsbRows8._fields_]
+    src.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "dsb.h"\nint main(void) {\n'
+                   + "".join(f'printf("%zu ", offsetof(dsb_rows8, {f}));\n' for f in names)
+                   + 'printf("%zu", sizeof(dsb_rows8)); return 0; }\n')
+    subprocess.run(["gcc", "-std=c99", "-Wall", "-Werror", "-I", os.path.join(ROOT, "include"), str(src),
+                    "-o", str(tmp_path / "p")], check=True)
+    got = subprocess.run([str(tmp_path / "p")], check=True, capture_output=True, text=True).stdout.split()
+    assert [int(v) for v in got] == [*(getattr(L.DsbRows8, f).offset for f in names), ctypes.sizeof(L.DsbRows8)]
