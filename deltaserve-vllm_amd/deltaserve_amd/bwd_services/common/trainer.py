@@ -283,9 +283,10 @@ class LoraSftTrainerService(BackwardService):
         if ids.dtype != torch.int64 or not ids.is_cuda:
             raise TypeError("concat_input_ids must be an int64 CUDA tensor")
         saved = self._saved_points(activations)
-        scales = [t.scales.data_ptr() for bufs in (li, saved.get("mlp_gate_up", ((),))[0]) for t in bufs
-                  if isinstance(t, Rows8)]
-        key = (tuple(t.data_ptr() for t in li), tuple(scales), fi.data_ptr(), ids.data_ptr(), ld,
+        # (what a code means is not in its address: memory may come back with another)
+        small = [(t.scales.data_ptr(), t.ld, t.ld_scales, t.type)
+                 for bufs in (li, saved.get("mlp_gate_up", ((),))[0]) for t in bufs if isinstance(t, Rows8)]
+        key = (tuple(t.data_ptr() for t in li), tuple(small), fi.data_ptr(), ids.data_ptr(), ld,
                tuple((name, tuple(t.data_ptr() for t in bufs), sld)
                      for name, (bufs, sld) in sorted(saved.items())))
         if key == self._act_key:

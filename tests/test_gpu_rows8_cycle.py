@@ -74,6 +74,32 @@ def test_cycle_on_8_bits_equals_the_cycle_on_their_values(family, code, points):
         b.close()
 
 
+def test_the_same_memory_with_another_code():
+    """Buffers that come back at the same addresses with another code or stride are bound again."""
+    from deltaserve_amd import ops
+
+    _, model, acts = _setup()
+    rows, D = acts["layer_in"][0].shape
+    codes = [torch.zeros(rows, D + 32, dtype=torch.uint8, device="cuda") for _ in range(3)]
+    scales = [torch.zeros(rows, D // 32 + 1, dtype=torch.uint8, device="cuda") for _ in range(3)]
+    a, b = build_service(model, "llama3"), build_service(model, "llama3")
+    try:
+        for epoch, (code, ld, lds) in enumerate([("e4m3", D, D // 32), ("int8", D, D // 32), ("int8", D + 32, D // 32),
+                                                 ("int8", D + 32, D // 32 + 1), ("e4m3", D + 32, D // 32 + 1)]):
+            kind = torch.float8_e4m3fn if code == "e4m3" else torch.int8
+            small, plain = dict(acts), dict(acts)
+            small["layer_in"] = [
+                ops.pack_rows8(t, out=ops.Rows8(c.flatten()[:rows * ld].view(rows, ld)[:, :D].view(kind),
+                                                s.flatten()[:rows * lds].view(rows, lds)[:, :D // 32]))
+                for t, c, s in zip(acts["layer_in"], codes, scales)]
+            plain["layer_in"] = [ops.unpack_rows8(q) for q in small["layer_in"]]
+            assert a.process_backward(small, SEQ, N, epoch) == b.process_backward(plain, SEQ, N, epoch)
+            _same(a, b, (code, ld, lds))
+    finally:
+        a.close()
+        b.close()
+
+
 @pytest.mark.parametrize("meta", [dict(backward_serial_layers=True), dict(backward_hip_graph=False),
                                   dict(backward_pause_boundaries=True, backward_run_ahead_boundaries=1)])
 def test_cycle_orders_agree_on_8_bits(meta):
