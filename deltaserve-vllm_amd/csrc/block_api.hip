@@ -261,10 +261,10 @@ int dsb_op_rotary(const void* x, int64_t ldx, int64_t hx, void* y, int64_t ldy, 
   const char* what = "dsb_op_rotary";
   if (dtype != DSB_DT_BF16 && dtype != DSB_DT_F16 && dtype != DSB_DT_F32)
     return bad(what, "x must be bf16, fp16 or fp32");
-  if (rot < 2 || rot % 2 || rot > head_dim || rot > DSB_ROTARY_MOST)
-    return bad(what, "rot must be even, from 2 to the head's width and at most 1024");
-  if (n < 0 || heads < 0 || (int64_t)n * heads >= (1 << 26) || (int64_t)heads * head_dim > (1 << 20))
-    return bad(what, "n times heads must be below 2^26, heads times head_dim at most 2^20");
+  if (rot < 2 || rot % 2 || rot > head_dim || head_dim > DSB_ROTARY_MOST)
+    return bad(what, "rot must be even, from 2 to the head's width, which is at most 1024");
+  if (n < 0 || n > kMostRows || heads < 0 || (int64_t)heads * head_dim > (1 << 20))
+    return bad(what, "n must be below 2^24, heads times head_dim at most 2^20");
   if (!std::isfinite(factor)) return bad(what, "the factor must be finite");
   if (n == 0 || heads == 0) return 0;
   if (!x || !y || !pos || !turns) return bad(what, "null argument");
@@ -272,6 +272,8 @@ int dsb_op_rotary(const void* x, int64_t ldx, int64_t hx, void* y, int64_t ldy, 
   if (misaligned(x, es) || misaligned(y, es) || misaligned(pos, pos64 ? 8 : 4) || misaligned(turns, 8))
     return bad(what, "a pointer is not aligned to its type");
   if (x == y && (ldx != ldy || hx != hy)) return bad(what, "in place the strides are the same");
+  if ((n > 1 && ldy < head_dim) || (heads > 1 && hy < head_dim))
+    return bad(what, "the heads of y overlap");
   RotaryArgs a{};
   a.x = x;
   a.ldx = ldx;

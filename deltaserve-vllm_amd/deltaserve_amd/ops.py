@@ -725,7 +725,7 @@ def pack_rows8(x, r=None, code="e4m3", out=None, src=None, dst=None):
     """x (+ r, added in x's type) as :class:`Rows8`: matrices of bf16, fp16 or fp32, of any width and
     row stride. ``out`` is written and returned if given. With src and dst (int64 vectors of one
     length) row src[i] goes into row dst[i] of ``out``, whose last row is a scratch row: slots that
-    name it, or a row outside x or out, are skipped."""
+    name it, or a row outside x or out, are skipped; dst names no other row twice."""
     what = "pack_rows8"
     ldx = _matrix(what, "x", x, None, tuple(_DT))
     n, width = x.shape
@@ -837,7 +837,7 @@ def _join_args(what, n, D, w_in, w_out, gate):
     if gate.dim() == 2 and gate.shape == (n, 1):
         if gate.dtype != BF16:
             raise ValueError(f"{what}: the gate must be bf16")
-        return max(gate.stride(0), 1) if n > 1 else 1, L.GATE_ROW
+        return gate.stride(0) if n > 1 else 1, L.GATE_ROW
     if gate.dim() == 1 and gate.shape[0] == D:
         _vec(what, "gate", gate, D, BF16)
         return 0, L.GATE_CHANNEL
@@ -1025,9 +1025,10 @@ def rotary_plan(head_dim, theta, scaling=None, rotary_dim=None, interleaved=Fals
 
 def rotary(x, positions, plan, out=None):
     """Rotary positions: x [n, heads, head_dim] (bf16, fp16 or fp32; any strides, a head's elements
-    contiguous, so a view of fused q/k/v rows will do) turned by ``positions`` (int32 or int64 [n], below 2^53),
-    in x's type. ``out``: written and returned, of x's shape and type; x itself works in place.
-    Angles are reduced in 64 bits, cosine and sine are fp32."""
+    contiguous, so a view of fused q/k/v rows will do) turned by ``positions`` (int32 or int64 [n]), in
+    x's type. ``out``: written and returned, of x's shape and type; x itself works in place.
+    Angles are reduced in 64 bits, cosine and sine are fp32 and as good as that for positions below
+    2^31."""
     return _rotary("rotary", x, positions, plan, out, False)
 
 

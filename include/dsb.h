@@ -539,7 +539,8 @@ int dsb_op_adam_step(const dsb_adam_chunk* chunks, int nchunks, const int32_t* g
 enum { DSB_ROWS8_BLOCK = 32 };
 /* dsb_save_rows into 8-bit rows: codes (row stride ldc) and scales (ldsc) of buf_rows rows, the last of
  * them the scratch row. src and dst null: rows 0 to count − 1 of x into those of the buffer, the last one
- * included. Any width, strides and alignment; whole 16-byte accesses where they allow them. */
+ * included. Any width, strides and alignment. A row that dst names twice (but the scratch row) is
+ * undefined: its codes and scales may be of either source. */
 int dsb_save_rows8(const void* x, int64_t ldx, const void* r, int64_t ldr, int64_t x_rows, int x_dtype,
                    const int64_t* src, const int64_t* dst, int count, int width, void* codes,
                    int64_t ldc, uint8_t* scales, int64_t ldsc, int code, int64_t buf_rows, void* stream);
@@ -585,9 +586,9 @@ int dsb_op_norm_join_bwd(const void* x_new, int64_t ldx, const uint8_t* x_scales
 /* Rotary positions: element h·hx + i of row t of x (head h, row stride ldx, of x_dtype) into y likewise,
  * the pairs (2i, 2i + 1) (interleaved) or (i, i + rot / 2) of the first `rot` elements of a head
  * turned by pos[t]·2π·turns[i] and scaled by `factor`, the others as they are. turns: fp64 [rot / 2];
- * pos: int32, or int64 below 2^53 in size (pos64). inverse: turned back, which with the same factor is
- * the gradient. y may be x; they do not overlap otherwise. rot is even, at most DSB_ROTARY_MOST; n·heads
- * below 2^26, heads·head_dim up to 2^20. */
+ * pos: int32, or int64 (pos64). inverse: turned back, which with the same factor is
+ * the gradient. y may be x; they do not overlap otherwise. rot is even, head_dim at most DSB_ROTARY_MOST, n
+ * below 2^24, heads·head_dim up to 2^20. Angles are exact to fp32 for positions below 2^31 in size. */
 enum { DSB_ROTARY_MOST = 1024 };
 int dsb_op_rotary(const void* x, int64_t ldx, int64_t hx, void* y, int64_t ldy, int64_t hy, int dtype,
                   const void* pos, int pos64, const double* turns, double factor, int n, int heads,

@@ -312,10 +312,12 @@ def test_rotary_refusals():
     bad("even", rot=63)
     bad("even", rot=0)
     bad("even", rot=66)
-    bad("1024", hd=2048, rot=1026)
-    bad("2^26", n=1 << 24)
+    bad("1024", hd=1026, rot=64)
+    bad("2^24", n=1 << 24)
     bad("2^20", heads=1 << 15)
-    bad("2^26", n=-1)
+    bad("2^24", n=-1)
+    bad("overlap", hy=63)
+    bad("overlap", ldy=0)
     bad("factor", factor=math.nan)
     bad("null", x=None)
     bad("null", turns=None)

@@ -498,6 +498,33 @@ def test_residual_norm_backward_sums_over_rows(n, D):
     assert torch.equal(less["dx"], got["dx"]) and torch.equal(less["dy"], got["dy"])
 
 
+def test_broadcast_operands_are_refused_or_read_as_they_are():
+    """A gate of one value for all rows, broadcast, has no rows of its own; rotary reads broadcast heads."""
+    ops = _ops()
+    x, w = _rand(_gen(1), 5, 64, dtype=BF16), torch.ones(64, dtype=BF16, device=DEV)
+    from deltaserve_amd._lib import DsbError
+
+    for kw in (dict(gate=w[:1].view(1, 1).expand(5, 1)), dict(gate=w.expand(5, 64))):
+        with pytest.raises(DsbError):
+            ops.residual_norm(x, x, w, 1e-5, **kw)
+        with pytest.raises(DsbError):
+            ops.residual_norm_backward(x, x, x, w, 1e-5, **kw)
+    for bad in (w.expand(5, 64), x[:, :64].as_strided((5, 64), (32, 1))):
+        with pytest.raises(DsbError):
+            ops.residual_norm(bad, x, w, 1e-5)
+        with pytest.raises(DsbError):
+            ops.pack_rows8(bad)
+    two = _rand(_gen(2), 5, 2, dtype=BF16)  # a column of a matrix is a gate by row
+    got = ops.residual_norm(x, x, w, 1e-5, gate=two[:, 1:])
+    for a, b in zip(got, ops.residual_norm(x, x, w, 1e-5, gate=two[:, 1].contiguous())):
+        assert torch.equal(a, b)
+    plan, pos = ops.rotary_plan(64, 1e4), torch.arange(5, device=DEV)
+    heads = x[:, None].expand(5, 3, 64)
+    assert torch.equal(ops.rotary(heads, pos, plan), ops.rotary(heads.contiguous(), pos, plan))
+    with pytest.raises(DsbError):
+        ops.rotary(heads, pos, plan, out=heads)
+
+
 def test_residual_norm_of_no_rows():
     ops = _ops()
     x = torch.empty(0, 64, dtype=BF16, device=DEV)
