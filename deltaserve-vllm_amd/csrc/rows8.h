@@ -87,18 +87,19 @@ DSB_DEV unsigned abs_bits(float v) { return __builtin_bit_cast(unsigned, v) & 0x
 
 // ---- memory
 // What a kernel leaves in the caches (the last level, 256 MB, keeps data from one kernel to the next):
-//   kNear  loads through them, stores past the L2: calls of up to 256 MB, whose inputs the kernel
-//          before may have left there; stores that stay in the L2 are written back at the kernel's end
-//   kFar   loads past them, stores into them: larger calls whose outputs the next kernel finds there
+//   kNear  loads through them, stores past the L2: inputs of up to a third of the last level, which the
+//          kernel before may have left there; stores that stay in the L2 are written back at the kernel's end
+//   kFar   loads past them, stores into them: larger inputs, and outputs that the next kernel finds there
 //   kPast  both past them: outputs of more than 256 MB
 //   kIn    both through them: for stores that cover lines in parts
-// µs, near / far / past (bytes of the call): RMSNorm of 2048 × 4096 8-bit rows (25 MB) 4.9 / 8.2 / 7.1, of
-// 8192 × 4096 (102 MB) 21 / 29 / 29; SwiGLU of 8192 × 14336 (477 MB) 91 / 73 / 86, its backward (1.2 GB, 705
-// MB of them out) 229 / 237 / 222; rows of 8192 × 28672 restored (712 MB, 470 out) 129 / 141 / 127.
+// µs, near / far / past (MB in, out): RMSNorm of 2048 × 4096 8-bit rows (8, 17) 4.9 / 8.2 / 7.1; rotary
+// positions, 40 heads of 8192 rows (84, 84) 28 / 31 / 34, of 10240 41 / 38 / 42; SwiGLU of 8192 × 14336
+// (242, 235) 91 / 73 / 86, its backward (477, 705) 229 / 237 / 222; 8192 × 28672 rows restored (242, 470)
+// 129 / 141 / 127. (Measured with inputs and outputs that come back every third call.)
 enum { kNear, kFar, kPast, kIn };
 inline int cache_of(double in, double out) {
   constexpr double kLast = 256 << 20;
-  return in + out <= kLast ? kNear : out <= kLast ? kFar : kPast;
+  return in <= kLast / 3 ? kNear : out <= kLast ? kFar : kPast;
 }
 template <int P, class V>
 DSB_DEV V load_as(const void* p) {
