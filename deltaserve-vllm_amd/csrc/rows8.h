@@ -89,17 +89,17 @@ DSB_DEV unsigned abs_bits(float v) { return __builtin_bit_cast(unsigned, v) & 0x
 // What a kernel leaves in the caches (the last level, 256 MB, keeps data from one kernel to the next):
 //   kNear  loads through them, stores past the L2: inputs of up to a third of the last level, which the
 //          kernel before may have left there; stores that stay in the L2 are written back at the kernel's end
-//   kFar   loads past them, stores into them: larger inputs, and outputs that the next kernel finds there
-//   kPast  both past them: outputs of more than 256 MB
+//   kFar   loads past them, stores into them: larger inputs, and outputs that fit beside others
+//   kPast  both past them: larger outputs
 //   kIn    both through them: for stores that cover lines in parts
-// µs, near / far / past (MB in, out): RMSNorm of 2048 × 4096 8-bit rows (8, 17) 4.9 / 8.2 / 7.1; rotary
-// positions, 40 heads of 8192 rows (84, 84) 28 / 31 / 34, of 10240 41 / 38 / 42; SwiGLU of 8192 × 14336
-// (242, 235) 91 / 73 / 86, its backward (477, 705) 229 / 237 / 222; 8192 × 28672 rows restored (242, 470)
-// 129 / 141 / 127. (Measured with inputs and outputs that come back every third call.)
+// µs, near / far / past (MB in, out): RMSNorm of 2048 × 4096 8-bit rows (8, 17) 5.0 / 8 / 8; rotary positions, 40
+// heads of 8192 rows (84, 84) 29 / 31 / 34, of 10240 41 / 38 / 42, of 16384 67 / 68 / 65; SwiGLU of 2048 ×
+// 14336 (61, 59) 18 / 21 / 23, of 4000 43 / 38 / 42, of 6500 71 / 78 / 68; 4096 × 28672 rows restored (121, 235)
+// 70 / 73 / 69. (Three sets of inputs in turn, two of outputs.)
 enum { kNear, kFar, kPast, kIn };
 inline int cache_of(double in, double out) {
   constexpr double kLast = 256 << 20;
-  return in <= kLast / 3 ? kNear : out <= kLast ? kFar : kPast;
+  return in <= kLast / 3 ? kNear : out <= 0.6 * kLast ? kFar : kPast;
 }
 template <int P, class V>
 DSB_DEV V load_as(const void* p) {
