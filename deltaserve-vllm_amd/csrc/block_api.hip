@@ -265,7 +265,7 @@ int dsb_op_rotary(const void* x, int64_t ldx, int64_t hx, void* y, int64_t ldy, 
     return bad(what, "rot must be even, from 2 to the head's width, which is at most 1024");
   if (n < 0 || n > kMostRows || heads < 0 || (int64_t)heads * head_dim > (1 << 20))
     return bad(what, "n must be below 2^24, heads times head_dim at most 2^20");
-  if (!std::isfinite(factor)) return bad(what, "the factor must be finite");
+  if (!std::isfinite((float)factor)) return bad(what, "the factor must be finite");
   if (n == 0 || heads == 0) return 0;
   if (!x || !y || !pos || !turns) return bad(what, "null argument");
   const unsigned es = dtype == DSB_DT_F32 ? 4 : 2;

@@ -13,7 +13,8 @@
 // stays. Accesses of 16 bytes need their elements' alignment only, so all strides and widths go
 // the same way: the last run of a region that is no multiple of 8 starts earlier and overlaps the
 // one before. Both compute the same values there; in place, where the first may have written
-// already, the second leaves them out. Bound by its bytes.
+// already, the second leaves them out. Bound by its bytes: 16384 rows of 40 heads of 128 64 µs, 5.3 TB/s (31 pairs
+// of such a head 88 µs; one element at a time it took 212), 256 rows 3.6 µs.
 #include <algorithm>
 #include <type_traits>
 
@@ -203,7 +204,9 @@ __global__ __launch_bounds__(64 * kWaves) void rotary_kernel(RotaryArgs a, int p
   }
 }
 
-// Waves wanted before a token's heads stay with one of them.
+// Waves wanted before a token's heads stay with one of them, enough to fill the chip's 256 CUs with 16 each. µs with
+// 1024 / 2048 / 4096 / 8192: 256 rows of 48 heads of 128, 32 turned, 4.1 / 3.7 / 3.6 / 3.7; 504 rows of 40 heads 4.3 / 4.0
+// / 3.9 / 3.9; from 4096 rows on no difference.
 constexpr long kMostSplit = 4096;
 
 }  // namespace

@@ -990,12 +990,19 @@ def _rotary_frequencies(d, theta, scaling, seq_len):
     # yarn: the (fractional) pair that makes n turns over the original length
     at = lambda n: d * np.log(length / (n * 2 * np.pi)) / (2 * np.log(theta))  # noqa: E731
     fast, slow = (given(k) if rs.get(k) is not None else v for k, v in (("beta_fast", 32.0), ("beta_slow", 1.0)))
-    low, high = max(np.floor(at(fast)), 0.0), min(np.ceil(at(slow)), d - 1.0)
+    low, high = at(fast), at(slow)
+    if rs.get("truncate", True):  # to whole pairs
+        low, high = np.floor(low), np.ceil(high)
+    low, high = max(low, 0.0), min(high, d - 1.0)
     ramp = np.clip((np.arange(d // 2) - low) / max(high - low, 0.001), 0, 1)
     if rs.get("attention_factor") is not None:
         factor = given("attention_factor")
     else:
-        factor = 0.1 * np.log(s) + 1 if s > 1 else 1.0
+        above, below = (float(v if rs.get(k) is None else rs[k]) for k, v in (("mscale", 1.0), ("mscale_all_dim", 0.0)))
+        if not (0 <= above < np.inf and 0 <= below < np.inf):
+            raise ValueError(f"{what}: mscale and mscale_all_dim must not be negative")
+        grow = 0.1 * np.log(max(s, 1.0))
+        factor = (above * grow + 1) / (below * grow + 1)
     return inv * (1 - ramp) + inv / s * ramp, factor
 
 
@@ -1008,15 +1015,16 @@ def rotary_plan(head_dim, theta, scaling=None, rotary_dim=None, interleaved=Fals
     ``scaling``: None or a dict with "rope_type" "linear" (factor), "dynamic" (factor,
     original_max_position_embeddings; theta grows with ``seq_len`` past it), "llama3" (as
     :func:`rope_inv_freq`), "yarn" (factor, original_max_position_embeddings, beta_fast 32, beta_slow
-    1, attention_factor 0.1·ln(factor) + 1) or "longrope" (short_factor, long_factor from ``seq_len``
+    1, truncate True; attention_factor, else (0.1·mscale·ln(factor) + 1) / (0.1·mscale_all_dim·ln(factor) + 1)
+    with mscale 1 and mscale_all_dim 0 where they are not given) or "longrope" (short_factor, long_factor from ``seq_len``
     past original_max_position_embeddings on, factor or attention_factor). Frequencies are computed in
     64 bits."""
     what = "rotary_plan"
     d = int(head_dim if rotary_dim is None else rotary_dim)
     if not (2 <= d <= head_dim <= 1024) or d % 2:
         raise ValueError(f"{what}: rotary_dim must be even, from 2 to head_dim, which is at most 1024")
-    if not theta > 1:
-        raise ValueError(f"{what}: theta must be above 1")
+    if not 1 < theta < np.inf:
+        raise ValueError(f"{what}: theta must be above 1 and finite")
     inv, factor = _rotary_frequencies(d, float(theta), scaling, seq_len)
     if torch.device(device).type != "cuda":
         raise ValueError(f"{what}: the plan's device must be CUDA (HIP)")
@@ -1026,7 +1034,8 @@ def rotary_plan(head_dim, theta, scaling=None, rotary_dim=None, interleaved=Fals
 def rotary(x, positions, plan, out=None):
     """Rotary positions: x [n, heads, head_dim] (bf16, fp16 or fp32; any strides, a head's elements
     contiguous, so a view of fused q/k/v rows will do) turned by ``positions`` (int32 or int64 [n]), in
-    x's type. ``out``: written and returned, of x's shape and type; x itself works in place.
+    x's type. ``out``: written and returned, of x's shape and type; it is x itself (in place) or shares no
+    element with it.
     Angles are reduced in 64 bits, cosine and sine are fp32 and as good as that for positions below
     2^31."""
     return _rotary("rotary", x, positions, plan, out, False)

@@ -276,6 +276,16 @@ def test_rotary_frequencies():
     assert np.allclose(y[turns < 1e4 ** (-2 / 64)], inv[turns < 1e4 ** (-2 / 64)] / 16)
     assert (np.diff(y) < 0).all() and (y <= inv).all() and (y >= inv / 16).all()
     assert _freq(64, 1e4, {**yarn, "attention_factor": 1.5})[1] == 1.5
+    for above, below in ((1.0, 0.0), (0.707, 0.707), (1.0, 0.5), (0.0, 0.5), (2.0, None)):
+        f = _freq(64, 1e4, {**yarn, "mscale": above, "mscale_all_dim": below})[1]
+        grow = 0.1 * math.log(16)
+        assert f == pytest.approx((above * grow + 1) / ((below or 0) * grow + 1), rel=1e-14)
+    assert _freq(64, 1e4, {**yarn, "factor": 0.5, "mscale": 2.0})[1] == 1
+    # borders between pairs: the share that is divided is the pair's place between them, exactly
+    cut = _freq(64, 1e4, {**yarn, "truncate": False})[0]
+    at = [64 * math.log(4096 / (b * 2 * math.pi)) / (2 * math.log(1e4)) for b in (32, 1)]
+    share = np.clip((i - at[0]) / (at[1] - at[0]), 0, 1)
+    assert np.allclose(cut, inv * (1 - share * (1 - 1 / 16)), rtol=1e-12) and not np.allclose(cut, y, rtol=1e-3)
     lr = {"rope_type": "longrope", "factor": 4.0, "original_max_position_embeddings": 4096,
           "short_factor": [1.0] * 32, "long_factor": list(range(1, 33))}
     assert np.allclose(_freq(64, 1e4, lr, 4096)[0], inv)
@@ -289,7 +299,9 @@ def test_rotary_plans_are_checked():
     for args, kw in (((64, 1e4), dict(rotary_dim=63)), ((64, 1e4), dict(rotary_dim=66)), ((64, 1e4), dict(rotary_dim=0)),
                      ((2048, 1e4), {}), ((63, 1e4), {}), ((64, 1.0), {}), ((64, math.nan), {}),
                      ((64, 1e4, {"rope_type": "linear"}), {}), ((64, 1e4, {"rope_type": "linear", "factor": 0}), {}),
-                     ((64, 1e4, {"rope_type": "yarn", "factor": 2}), {}),
+                     ((64, math.inf), {}), ((64, 1e4, {"rope_type": "yarn", "factor": 2}), {}),
+                     ((64, 1e4, {"rope_type": "yarn", "factor": 2, "original_max_position_embeddings": 64,
+                                 "mscale": -1.0}), {}),
                      ((64, 1e4, {"rope_type": "llama3", "factor": 2, "original_max_position_embeddings": 64,
                                  "low_freq_factor": 4, "high_freq_factor": 4}), {}),
                      ((64, 1e4, {"rope_type": "longrope", "factor": 2, "original_max_position_embeddings": 64,
