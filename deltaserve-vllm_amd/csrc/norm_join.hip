@@ -15,9 +15,13 @@
 // so that one pass over a row takes six sums at once and one barrier a row does. All of it is fp32,
 // rounded once where it is stored; the kernels are bound by their bytes.
 //
-// A block of threads takes row after row, the next one's loads on their way while it computes; the weights
-// stay in its registers and so do its sums over rows, which a second launch adds up over the
-// blocks, in order.
+// A block of threads takes row after row, a lane 8 columns (16 or 24 in the forward, which needs few
+// registers); the weights stay in its registers and so do its two sums over rows, which a second
+// launch adds up over the blocks, in order. In the backward 16 waves a CU cover each other's loads and barriers:
+// two rows' loads ahead of one another in fewer waves (16 columns a lane) took 117 to 124 µs
+// for 8192 × 4096 8-bit rows with everything on, without them 95, this 91 (95 where results live on, and 6 the
+// sums' launch; the bytes take 98 at a copy's rate). Kernel times at that size: forward 47 µs, 5.7 TB/s (fp32
+// 70); a norm alone of 8-bit rows 21 µs, its backward with an fp32 gradient 51 µs, 5.9 TB/s.
 #include <algorithm>
 #include <type_traits>
 
@@ -45,8 +49,8 @@ DSB_DEV float row_total(float v) {
 
 // K sums over the block, the same for all. red holds two sets of them, taken in turn: a set is
 // written again only after the barrier of the call between, which every wave reaches after it has
-// read the set, so one barrier a call is enough. (It orders LDS alone: a fence would wait for the next
-// row's loads.)
+// read the set, so one barrier a call is enough. (It orders LDS alone: a fence would wait for the row
+// before's stores too.)
 template <int K>
 DSB_DEV void block_totals(float (&v)[K], float (&red)[2][kMostWaves][8], int& turn) {
 #pragma unroll
@@ -169,11 +173,12 @@ __global__ __launch_bounds__(kMostThreads / 2) void join_fwd_kernel(JoinArgs a) 
   }
 }
 
-// 8 columns a thread; XT, YT, GT: the types of x', y and dn, FULL: a gate of rows. With a block its
+// 8 columns a thread; XT, YT, GT: the types of x', y and dn, FULL: a gate of rows; through: dx is fp32 and
+// goes into the caches. With a block its
 // sums over rows go into part [2][gridDim.x][D]: Σ dn·x̂, and Σ t·ŷ times a gate that differs by row, of
 // which dw_out and a channel gate's dgate are multiples (join_sums_kernel).
 template <int XT, int YT, int GT, bool FULL, int P>
-__global__ __launch_bounds__(kMostThreads) void join_bwd_kernel(JoinArgs a, float* part) {
+__global__ __launch_bounds__(kMostThreads) void join_bwd_kernel(JoinArgs a, float* part, bool through) {
   constexpr bool Y = YT != kRowsNone, N = GT != kRowsNone;
   __shared__ float red[2][kMostWaves][8];
   int turn = 0;
@@ -266,7 +271,12 @@ __global__ __launch_bounds__(kMostThreads) void join_bwd_kernel(JoinArgs a, floa
         if (Y) s_in[e] += dv[e] * hat;
       }
     }
-    if (live) put8<P>(a.dx, row * a.lddx + 8 * c, a.dx_f32, t);
+    if (live) {
+      if (through)
+        put8<kIn>(a.dx, row * a.lddx + 8 * c, true, t);
+      else
+        put8<P>(a.dx, row * a.lddx + 8 * c, a.dx_f32, t);
+    }
     if constexpr (Y) {
       const float to_y = a.scale * gr * j, back = m * j;
       float o[8];
@@ -402,9 +412,11 @@ hipError_t join_bwd(const JoinArgs& a, void* work, hipStream_t s) {
   const double in = row_bytes(a.x) + row_bytes(a.dn) + row_bytes(a.dxn);
   // (a norm alone; kFar is near kPast: 8192 × 4096 8-bit rows, fp32 gradient, kNear / kFar / kPast 55 / 53 / 52 µs;
   // with a block kNear is as good or better at all sizes: 8192 × 5120 121 / 136 / 132)
-  const bool near = a.y.p || cache_of(in * a.rows * a.D, 0) == kNear;
+  const bool small = cache_of(in * a.rows * a.D, 0) == kNear, near = a.y.p || small;
+  // (see put8: 2048 × 4096 8-bit rows 30 µs past the caches, 33 into them; 4096 58.4, 57.4; 12000 146, 141)
+  const bool through = a.dx_f32 && !small;
   auto go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(64 * waves), 0, s, a, part);
+    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(64 * waves), 0, s, a, part, through);
     return hipGetLastError();
   };
   auto by_cache = [&](auto x, auto y, auto g, auto f) {
