@@ -5,7 +5,8 @@
 //
 // and the rest of the head stays as it is. The backward turns by the opposite angle with the same
 // factor. Angles are taken in turns, position·(inv_freq / 2π) in 64 bits less its nearest whole
-// number, and from there in fp32: at position 2^20 an fp32 angle is off by up to 2^-5 radians.
+// number, and from there in fp32 with what that rounded off put back: at position 2^20 an fp32 angle is off by up
+// to 2^-5 radians, and fp32 results without the last are off by 5.8e-8 (root mean square, relative), with it 4.1e-8.
 //
 // A wave takes a token, or a part of its heads where there are few tokens. It computes the token's
 // cosines and sines once, a pair of them a lane, and keeps them in LDS, where all of its heads read
@@ -107,10 +108,14 @@ __global__ __launch_bounds__(64 * kWaves) void rotary_kernel(RotaryArgs a, int p
     const double pos = a.pos64 ? (double)((const int64_t*)a.pos)[t] : (double)((const int*)a.pos)[t];
     for (int i = lane; i < half; i += 64) {
       const double turn = pos * a.turns[i];
+      const double u = 2 * (turn - __builtin_rint(turn));
       float s, c;
-      sincospif(2.f * (float)(turn - __builtin_rint(turn)), &s, &c);
-      cosv[i] = a.factor * c;
-      sinv[i] = a.inverse ? -a.factor * s : a.factor * s;
+      sincospif((float)u, &s, &c);
+      // what the angle lost to fp32, up to 2^-25 half turns, to the first order
+      const float d = (float)(u - (double)(float)u) * 3.14159265f;
+      const float c1 = a.factor * (c - s * d), s1 = a.factor * (s + c * d);
+      cosv[i] = c1;
+      sinv[i] = a.inverse ? -s1 : s1;
     }
   }
   __syncthreads();
