@@ -269,8 +269,7 @@ hipError_t save_rows8(const Save8Args& a, hipStream_t s) {
 hipError_t restore_rows8(const RowsArg& q, int rows, int width, void* out, long ldo, bool f32,
                          hipStream_t s, const int* rows_dev) {
   if (rows <= 0 || width <= 0) return hipSuccess;
-  const double n = (double)rows * width;
-  return by_cache(n, (f32 ? 4 : 2) * n, [&](auto p) {
+  auto run = [&](auto p) {
     constexpr int P = decltype(p)::value;
     auto go = [&](auto kernel) {
       dim3 grid;
@@ -283,7 +282,9 @@ hipError_t restore_rows8(const RowsArg& q, int rows, int width, void* out, long 
       return f32 ? go(restore_rows8_kernel<C, true, P>) : go(restore_rows8_kernel<C, false, P>);
     };
     return q.type == DSB_DT_E4M3 ? by_code(Int<DSB_DT_E4M3>{}) : by_code(Int<DSB_DT_INT8>{});
-  });
+  };
+  // (results of larger inputs, twice or four times their bytes, fit no cache)
+  return cache_of((double)rows * width, 0) == kNear ? run(Int<kNear>{}) : run(Int<kPast>{});
 }
 
 hipError_t swiglu(const SwigluArgs& a, hipStream_t s) {
