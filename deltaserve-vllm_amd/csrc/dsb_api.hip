@@ -1868,9 +1868,13 @@ int dsb_bind_activations8(dsb_handle* h, const dsb_activations* a, const dsb_row
   CKR(saved(a->attn_ctx, a->ld_ctx, h->q, "attn_ctx", cv));
   CKR(saved(a->resid_mid, a->ld_resid_mid, h->D, "resid_mid", rv));
   if (!li8.empty() && !h->xr[0]) {
-    CKR(dalloc(h, &h->xr[0], (h->N + 1L) * h->D));
-    h->xr[1] = h->xr[0];
-    if (h->overlap) CKR(dalloc(h, &h->xr[1], (h->N + 1L) * h->D));
+    // one allocation, both or none: with the overlap a layer's restore must
+    // never write the rows that the layer after it still reads
+    const long one = ((h->N + 1L) * h->D + 127) / 128 * 128;
+    bf16* both = nullptr;
+    CKR(dalloc(h, &both, (h->overlap ? 2 : 1) * one));
+    h->xr[0] = both;
+    h->xr[1] = h->overlap ? both + one : both;
   }
   h->layer_in.assign(h->L, nullptr);
   for (int i = 0; a->layer_in && i < h->L; ++i) {
