@@ -56,7 +56,10 @@ class BlockPool {
     if (alloc(&b.p, need) != hipSuccess) {
       (void)hipGetLastError();
       trim(0);
-      if (alloc(&b.p, need) != hipSuccess) b = Block{};
+      if (alloc(&b.p, need) != hipSuccess) {
+        (void)hipGetLastError();
+        b = Block{};
+      }
     }
     return b;
   }
@@ -134,14 +137,18 @@ inline BlockPool& pinned_pool() {
 }
 
 // hipMalloc on the current device for memory that is not the pool's; what the
-// pool keeps there makes room if it fails.
+// pool keeps there makes room if it fails. A failure is returned and not left
+// behind for the check of the next launch, ours or torch's, to find.
 inline hipError_t device_malloc(void** p, size_t bytes) {
-  const hipError_t e = hipMalloc(p, bytes);
+  hipError_t e = hipMalloc(p, bytes);
   int dev = 0;
-  if (e == hipSuccess || hipGetDevice(&dev) != hipSuccess || dev >= kPoolDevices) return e;
+  if (e == hipSuccess) return e;
   (void)hipGetLastError();
+  if (hipGetDevice(&dev) != hipSuccess || dev >= kPoolDevices) return e;
   device_pool(dev).trim(0);
-  return hipMalloc(p, bytes);
+  e = hipMalloc(p, bytes);
+  if (e != hipSuccess) (void)hipGetLastError();
+  return e;
 }
 
 // One call's scratch memory on stream s.
