@@ -1827,7 +1827,11 @@ int dsb_bind_activations8(dsb_handle* h, const dsb_activations* a, const dsb_row
   };
   CKR(rows8(layer_in8, h->D, li8));
   CKR(rows8(gate_up8, 2 * h->I, gu8));
-  std::vector<const bf16*> gu;
+  std::vector<const bf16*> li(h->L, nullptr), gu;
+  for (int i = 0; a->layer_in && i < h->L; ++i) {
+    if (!a->layer_in[i]) return fail(h, "dsb_bind_activations: null layer_in");
+    li[i] = (const bf16*)a->layer_in[i];
+  }
   if (a->mlp_gate_up) {
     for (int i = 0; i < h->L; ++i) {
       if (!a->mlp_gate_up[i] || ((uintptr_t)a->mlp_gate_up[i] & 15))
@@ -1867,6 +1871,7 @@ int dsb_bind_activations8(dsb_handle* h, const dsb_activations* a, const dsb_row
   CKR(saved(a->attn_v, a->ld_v, h->kv, "attn_v", vv));
   CKR(saved(a->attn_ctx, a->ld_ctx, h->q, "attn_ctx", cv));
   CKR(saved(a->resid_mid, a->ld_resid_mid, h->D, "resid_mid", rv));
+  // (a bind that fails, here or above, leaves the one before it as it was)
   if (!li8.empty() && !h->xr[0]) {
     // one allocation, both or none: with the overlap a layer's restore must
     // never write the rows that the layer after it still reads
@@ -1876,11 +1881,7 @@ int dsb_bind_activations8(dsb_handle* h, const dsb_activations* a, const dsb_row
     h->xr[0] = both;
     h->xr[1] = h->overlap ? both + one : both;
   }
-  h->layer_in.assign(h->L, nullptr);
-  for (int i = 0; a->layer_in && i < h->L; ++i) {
-    if (!a->layer_in[i]) return fail(h, "dsb_bind_activations: null layer_in");
-    h->layer_in[i] = (const bf16*)a->layer_in[i];
-  }
+  h->layer_in = li;
   h->layer_in8 = li8;
   h->gate_up_in8 = gu8;
   h->gate_up_in = gu;
