@@ -2,7 +2,7 @@
 // columns.
 //
 //   e = the least with max|block| <= M·2^e, M = 448 (e4m3) or 127 (int8), at least −126
-//   code = round(v·2^−e) to nearest even; value = code·2^e
+//   code = round(v·2^−e) to nearest even, or the code below where that makes 2^128; value = code·2^e
 //
 // Every step but the one rounding is exact: the scale is a shift of the exponent, so codes are the same
 // however they are computed, and a value has at most 8 significant bits, so that bf16 holds it. The
@@ -51,10 +51,18 @@ DSB_DEV unsigned encode4(const float* v, float inv) {
     return lo | hi;
   }
 }
+// A block's values are at most M·2^e, so only with the last exponent (which M·2^e takes past fp32) may one round
+// to 2^128: there the code below stands for it, 240 (e4m3) or 63 (int8) times the scale. (8192 × 1024 rows 7.25 µs, 7.2
+// without; in a branch no less.)
 template <int CODE>
 DSB_DEV u32x2 encode8(const float v[8], unsigned byte) {
-  const float inv = inverse_scale_of(byte);
-  const u32x2 c = {encode4<CODE>(v, inv), encode4<CODE>(v + 4, inv)};
+  constexpr unsigned kLastByte = CODE == DSB_DT_E4M3 ? 127 + 120 : 127 + 122;
+  constexpr float kLast = CODE == DSB_DT_E4M3 ? 0x1.ep127f : 0x1.f8p127f;
+  const float inv = inverse_scale_of(byte), most = byte >= kLastByte ? kLast : __builtin_inff();
+  float w[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] = __builtin_amdgcn_fmed3f(v[i], -most, most);
+  const u32x2 c = {encode4<CODE>(w, inv), encode4<CODE>(w + 4, inv)};
   return byte == 255u ? u32x2{0u, 0u} : c;
 }
 template <int CODE>

@@ -535,7 +535,8 @@ int dsb_op_adam_step(const dsb_adam_chunk* chunks, int nchunks, const int32_t* g
  * DSB_ROWS8_BLOCK columns of a row, from the row's first, the exponent of their scale + 127. A value is
  * code·2^(byte − 127); byte 255 makes NaN of a code of 0. Saving takes the least exponent, at least −126, that brings the
  * block's largest magnitude to at most 448 (e4m3) or 127 (int8) and rounds to the nearest code, ties to
- * even; a block that holds an infinity or a NaN is kept as NaN whole. */
+ * even, but to the code below where the nearest one's value is 2^128: finite values stay finite. A block that holds an
+ * infinity or a NaN is kept as NaN whole. */
 enum { DSB_ROWS8_BLOCK = 32 };
 /* dsb_save_rows into 8-bit rows: codes (row stride ldc) and scales (ldsc) of buf_rows rows, the last of
  * them the scratch row. src and dst null: rows 0 to count − 1 of x into those of the buffer, the last one
