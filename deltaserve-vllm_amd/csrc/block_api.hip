@@ -272,7 +272,11 @@ int dsb_op_rotary(const void* x, int64_t ldx, int64_t hx, void* y, int64_t ldy, 
   if (misaligned(x, es) || misaligned(y, es) || misaligned(pos, pos64 ? 8 : 4) || misaligned(turns, 8))
     return bad(what, "a pointer is not aligned to its type");
   if (x == y && (ldx != ldy || hx != hy)) return bad(what, "in place the strides are the same");
-  if ((n > 1 && ldy < head_dim) || (heads > 1 && hy < head_dim))
+  // rows of heads or heads of rows: the outer stride spans all of the inner one
+  const bool rows_out = ldy >= (__int128)(heads - 1) * hy + head_dim,
+             heads_out = hy >= (__int128)(n - 1) * ldy + head_dim;
+  if ((n > 1 && ldy < head_dim) || (heads > 1 && hy < head_dim) ||
+      (n > 1 && heads > 1 && !rows_out && !heads_out))
     return bad(what, "the heads of y overlap");
   RotaryArgs a{};
   a.x = x;

@@ -67,3 +67,21 @@ def test_finite_values_come_back_finite(w, dtype, code):
     r = torch.zeros_like(x)
     same = ops.pack_rows8(x, r, code=code)
     assert torch.equal(same.codes.view(torch.uint8), q.codes.view(torch.uint8)) and torch.equal(same.scales, q.scales)
+
+
+# ---------------------------------------------------------------- rotary positions
+
+@pytest.mark.parametrize("n,heads,hd,ldy,hy", [(5, 4, 64, 256, 64), (5, 4, 64, 64, 320), (3, 3, 64, 212, 74),
+                                               (3, 3, 64, 74, 212), (1, 4, 64, 64, 64), (5, 1, 64, 64, 64)])
+def test_rotary_outputs_as_close_as_they_may_be(n, heads, hd, ldy, hy):
+    ops = _ops()
+    plan = ops.rotary_plan(hd, 1e4)
+    x = torch.randn(n, heads, hd, generator=torch.Generator(device=DEV).manual_seed(1), device=DEV).to(BF16)
+    pos = torch.arange(n, device=DEV) + 3
+    mem = torch.full(((n - 1) * ldy + (heads - 1) * hy + hd + 8,), 7.0, device=DEV, dtype=BF16)
+    out = mem.as_strided((n, heads, hd), (ldy, hy, 1))
+    want = ops.rotary(x, pos, plan)
+    assert torch.equal(ops.rotary(x, pos, plan, out=out), want)
+    at = torch.arange(mem.numel(), device=DEV).as_strided((n, heads, hd), (ldy, hy, 1)).flatten()
+    assert at.unique().numel() == at.numel() == want.numel()
+    assert (mem.index_fill(0, at, 7.0) == 7).all()
