@@ -1036,8 +1036,9 @@ def rotary(x, positions, plan, out=None):
     contiguous, so a view of fused q/k/v rows will do) turned by ``positions`` (int32 or int64 [n]), in
     x's type. ``out``: written and returned, of x's shape and type; it is x itself (in place) or shares no
     element with it.
-    Angles are reduced in 64 bits, cosine and sine are fp32 and as good as that for positions below
-    2^31."""
+    Angles are reduced in 64 bits from the plan's table, which holds a frequency to 2^-52 of itself: off by at
+    most 2^-52·position·inv_freq radians, half a step of fp32 at π where that is 2^29 positions. Cosine and sine
+    are fp32; positions below 2^31."""
     return _rotary("rotary", x, positions, plan, out, False)
 
 

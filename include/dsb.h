@@ -589,7 +589,8 @@ int dsb_op_norm_join_bwd(const void* x_new, int64_t ldx, const uint8_t* x_scales
  * turned by pos[t]·2π·turns[i] and scaled by `factor`, the others as they are. turns: fp64 [rot / 2];
  * pos: int32, or int64 (pos64). inverse: turned back, which with the same factor is
  * the gradient. y may be x; they do not overlap otherwise. rot is even, head_dim at most DSB_ROTARY_MOST, n
- * below 2^24, heads·head_dim up to 2^20. Angles are exact to fp32 for positions below 2^31 in size. */
+ * below 2^24, heads·head_dim up to 2^20. pos·turns is reduced with one rounding, in 64 bits:
+ * angles are exact to fp32 for positions below 2^31 in size. */
 enum { DSB_ROTARY_MOST = 1024 };
 int dsb_op_rotary(const void* x, int64_t ldx, int64_t hx, void* y, int64_t ldy, int64_t hy, int dtype,
                   const void* pos, int pos64, const double* turns, double factor, int n, int heads,

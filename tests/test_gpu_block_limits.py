@@ -4,7 +4,9 @@ value, rotary angles of far positions against exact arithmetic."""
 from __future__ import annotations
 
 import math
+from fractions import Fraction
 
+import numpy as np
 import pytest
 import torch
 
@@ -85,3 +87,65 @@ def test_rotary_outputs_as_close_as_they_may_be(n, heads, hd, ldy, hy):
     at = torch.arange(mem.numel(), device=DEV).as_strided((n, heads, hd), (ldy, hy, 1)).flatten()
     assert at.unique().numel() == at.numel() == want.numel()
     assert (mem.index_fill(0, at, 7.0) == 7).all()
+
+
+PI = Fraction("3.14159265358979323846264338327950288419716939937510582097494459")
+
+
+def _exact_cos_sin(pos, turns, rounded=False):
+    """cos and sin (64 bits) of 2π·pos·turns, the product and its reduction without any rounding; rounded: the
+    reduced half turns as fp32 has them."""
+    ang = []
+    for p in pos.tolist():
+        for t in turns:
+            u = p * t
+            half = 2 * (u - round(u))
+            ang.append(float((Fraction(float(np.float32(float(half)))) if rounded else half) * PI))
+    ang = torch.tensor(ang, dtype=F64).view(len(pos), 1, len(turns)).to(DEV)
+    return ang.cos(), ang.sin()
+
+
+def _far(lo, hi, n=128, heads=64):
+    """A plan of 8 pairs, all of them fast, positions in [lo, hi), and heads of 8 pairs."""
+    g = torch.Generator().manual_seed(9)
+    inv = 0.5 + 0.5 * torch.rand(8, generator=g, dtype=F64)
+    inv[0] = 1.0
+    plan = _ops().RotaryPlan(16, 16, False, inv.numpy(), 1.0, DEV)
+    pos = torch.randint(lo, hi, (n,), generator=g).to(DEV)
+    return plan, pos, torch.randn(n, heads, 16, generator=g).to(DEV)
+
+
+@pytest.mark.parametrize("back", [False, True])
+@pytest.mark.parametrize("lo,hi", [(1, 1 << 12), (1 << 20, 1 << 21), (1 << 30, (1 << 31) - 1)])
+def test_rotary_angles_are_exact_to_fp32(lo, hi, back):
+    """The root mean square error of fp32 results against the angles that the plan's table stands for. In units of
+    2^-24 and of the result's root mean square: a cosine or sine 0.5 (its rounding and its correction's, 0.25 each in
+    root mean square, times √2 as two of them meet), a product 0.3, the sum 0.42: 0.7, 4.2e-8. An angle rounded to
+    fp32 adds 4.1e-8 (2^-25 half turns in the upper half of the range, half of that in the quarter below, ...), one
+    whose product with the position is rounded to 64 bits up to 1.1e-7 at 2^31: 5.8e-8 and more."""
+    ops = _ops()
+    plan, pos, x = _far(lo, hi)
+    got = (ops.rotary_backward if back else ops.rotary)(x, pos, plan).double()
+    p, q = x[..., :8].double(), x[..., 8:].double()
+    for rounded in (False, True):  # (the second: what the bound does not let through)
+        c, s = _exact_cos_sin(pos, [Fraction(t) for t in plan.turns.tolist()], rounded)
+        s = -s if back else s
+        want = torch.cat([p * c - q * s, q * c + p * s], 2)
+        rms = float(((got - want) ** 2).mean().sqrt() / (want ** 2).mean().sqrt())
+        assert (rms > 5e-8) if rounded else (rms < 5e-8), rms
+
+
+@pytest.mark.parametrize("lo,hi", [(1 << 28, 1 << 29), (1 << 30, (1 << 31) - 1)])
+def test_rotary_angles_of_far_positions(lo, hi):
+    """Against the plan's frequencies: a table entry, the frequency over 2π in 64 bits, is off by 2^-52 of itself at
+    most. Cosine and sine are off by 2 units of 2^-24 and their correction's rounding by 1, the products and their
+    sum by 1 each of |p| + |q|."""
+    ops = _ops()
+    plan, pos, x = _far(lo, hi)
+    c, s = _exact_cos_sin(pos, [Fraction(float(f)) / (2 * PI) for f in plan.inv_freq])
+    p, q = x[..., :8].double(), x[..., 8:].double()
+    off = 2.0 ** -52 * pos.double()[:, None, None] * torch.from_numpy(plan.inv_freq).to(DEV) + 5 * 2.0 ** -24
+    tol = off * (p.abs() + q.abs())
+    got = ops.rotary(x, pos, plan).double()
+    assert ((got[..., :8] - (p * c - q * s)).abs() <= tol).all()
+    assert ((got[..., 8:] - (q * c + p * s)).abs() <= tol).all()
