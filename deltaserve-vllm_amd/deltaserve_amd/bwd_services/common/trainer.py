@@ -250,10 +250,11 @@ class LoraSftTrainerService(BackwardService):
                 self._check_rows8(name, bufs, width)
                 out[name] = (bufs, 0)
                 continue
-            ld = bufs[0].stride(0)
+            # (Rows8, which layer_in and mlp_gate_up may be, are no tensors)
+            ld = bufs[0].stride(0) if torch.is_tensor(bufs[0]) else 0
             for t in bufs:
-                if (t.dtype != torch.bfloat16 or not t.is_cuda or t.stride(0) != ld
-                        or t.stride(1) != 1 or t.shape[1] != width):
+                if (not torch.is_tensor(t) or t.dtype != torch.bfloat16 or not t.is_cuda
+                        or t.stride(0) != ld or t.stride(1) != 1 or t.shape[1] != width):
                     raise TypeError(f"{name} buffers must be bf16 CUDA [rows, {width}] with one "
                                     "row stride")
             out[name] = (bufs, ld)
@@ -273,14 +274,15 @@ class LoraSftTrainerService(BackwardService):
         ids = activations["concat_input_ids"]
         if len(li) != self.L:
             raise ValueError(f"activations carry {len(li)} layer inputs, the model has {self.L}")
-        ld = fi.stride(0)
+        ld = fi.stride(0) if torch.is_tensor(fi) else 0
         li8 = any(isinstance(t, Rows8) for t in li)
         if li8:
             self._check_rows8("layer_in", li, self.D)
         for t in ([] if li8 else list(li)) + [fi]:
-            if t.dtype != torch.bfloat16 or not t.is_cuda or t.stride(0) != ld or t.stride(1) != 1:
+            if (not torch.is_tensor(t) or t.dtype != torch.bfloat16 or not t.is_cuda
+                    or t.stride(0) != ld or t.stride(1) != 1):
                 raise TypeError("activation buffers must be bf16 CUDA [rows, D] with one row stride")
-        if ids.dtype != torch.int64 or not ids.is_cuda:
+        if not torch.is_tensor(ids) or ids.dtype != torch.int64 or not ids.is_cuda:
             raise TypeError("concat_input_ids must be an int64 CUDA tensor")
         saved = self._saved_points(activations)
         # (what a code means is not in its address: memory may come back with another)

@@ -7,6 +7,9 @@ import os
 import subprocess
 import sys
 
+import pytest
+import torch
+
 from harness import ROOT
 
 HIP = r"""
@@ -101,3 +104,38 @@ def test_restored_rows_of_overlapped_layers_are_two_buffers_after_a_failed_alloc
     r = subprocess.run([sys.executable, str(tmp_path / "main.py"), str(tmp_path / "hip.so"),
                         os.path.join(ROOT, "deltaserve-vllm_amd")], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and r.stdout.strip() == "ok", r.stdout + r.stderr
+
+
+# ---------------------------------------------------------------- the trainer's checks
+
+def _trainer():
+    from types import SimpleNamespace
+
+    from deltaserve_amd.bwd_services.common.trainer import LoraSftTrainerService
+
+    svc = LoraSftTrainerService.__new__(LoraSftTrainerService)
+    svc.L, svc.D, svc.inter, svc.q_size, svc.kv_size, svc._s_max = 2, 64, 96, 64, 32, 4
+    svc.shared = {"meta": {"save_attn_qkv": True, "save_resid_mid": True}}
+    svc.family = SimpleNamespace(supports_saved_qkv=True)
+    return svc
+
+
+@pytest.mark.parametrize("name,width", [("final_in", 64), ("concat_input_ids", 64), ("attn_ctx", 64), ("attn_qh", 64),
+                                        ("attn_kh", 32), ("attn_vh", 32), ("resid_mid", 64)])
+def test_8_bit_rows_where_the_cycle_takes_bf16_are_a_type_error(name, width, monkeypatch):
+    from deltaserve_amd.rows8 import Rows8
+
+    # (the checks ask of a tensor only whether it is on the device)
+    monkeypatch.setattr(torch.Tensor, "is_cuda", property(lambda t: True))
+
+    def rows(w):
+        return torch.zeros(5, w, dtype=torch.bfloat16)
+
+    acts = {"layer_in": [rows(64)] * 2, "final_in": rows(64), "concat_input_ids": torch.zeros(4, dtype=torch.int64),
+            "attn_ctx": [rows(64)] * 2, "attn_qh": [rows(64)] * 2, "attn_kh": [rows(32)] * 2,
+            "attn_vh": [rows(32)] * 2, "resid_mid": [rows(64)] * 2}
+    small = Rows8.zeros(5, width, device="cpu")
+    for bad in ([small, small], [rows(width), small], [small, rows(width)]):
+        acts[name] = bad if isinstance(acts[name], list) else small
+        with pytest.raises(TypeError):
+            _trainer()._bind_activations(acts)
