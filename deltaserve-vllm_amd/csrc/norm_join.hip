@@ -367,7 +367,7 @@ int blocks_of(int rows, int waves) { return std::min(rows, (1 << 13) / waves); }
 int fwd_runs(int D) { return 8 / waves_of(D, 3) > 8 / waves_of(D, 2) ? 3 : 2; }
 // With sums, 8 waves a CU, which leave the fewest sums to write out, or two blocks where 16 waves, all
 // that fit its registers, hold them: a lone block waits at its barriers. 8192 × 4096, one / two blocks of 8
-// waves a CU: 104 / 92 µs; 32768 × 1024, eight / sixteen of one wave: 88 / 94.
+// waves a CU: 104 / 92 µs; 32768 × 1024, four / eight of two waves, the sums' launch too: 95 / 103.
 int sum_blocks(int rows, int D) {
   const int w = waves_of(D, 1);
   const int most = kCUs * std::max(1, std::max(8 / w, std::min(2, 16 / w)));

@@ -242,7 +242,8 @@ hipError_t save_rows8(const Save8Args& a, hipStream_t s) {
   if (a.count <= 0 || a.width <= 0) return hipSuccess;
   const double n = (double)a.count * a.width, es = a.dtype == DSB_DT_F32 ? 4 : 2;
   const double in = (a.r ? 2 : 1) * es * n;
-  // (kPast where the inputs are past the last level: kFar / kPast 39 / 41 µs at 2600 × 28672, 60 / 54 at 3500)
+  // (where a call ends up past both goes by what it reads, at least twice what it writes: kFar / kPast 39 / 41 µs
+  // at 149 MB, 2600 × 28672, 60 / 54 at 201 MB, 3500)
   return by_cache(in, in, [&](auto p) {
     constexpr int P = decltype(p)::value;
     auto go = [&](auto kernel) {

@@ -18,7 +18,7 @@ import numpy as np
 import torch
 
 from . import _lib as L
-from .rows8 import CODES, Rows8
+from .rows8 import Rows8
 
 BF16 = torch.bfloat16
 
@@ -682,8 +682,9 @@ class AdamW:
 #
 # SwiGLU, the join of a block with the residual stream and the norms around it, and rotary positions,
 # forward and backward, with activations that may be kept in 8 bits. They only enqueue on the current
-# stream of their tensors' device, as the ops for training from feedback do, and can be captured; the
-# reference has no counterpart of them but for the norms' formulas (cited above) and SwiGLU's
+# stream of their tensors' device, as the ops for training from feedback do, and can be captured. The
+# backward cycle calls none of them: on a store in 8 bits it restores rows to bf16 and goes on with the kernels
+# it always had. The reference has no counterpart of them but for the norms' formulas (cited above) and SwiGLU's
 # (ffn.py:29-48). A row's elements are contiguous; rows of bf16 and fp32 start on 16 bytes and lie a
 # multiple of 16 bytes apart, rows of codes on 8.
 
@@ -723,7 +724,7 @@ def _held(t):
 
 def pack_rows8(x, r=None, code="e4m3", out=None, src=None, dst=None):
     """x (+ r, added in x's type) as :class:`Rows8`: matrices of bf16, fp16 or fp32, of any width and
-    row stride. ``out`` is written and returned if given. With src and dst (int64 vectors of one
+    row stride. ``out`` is written, in its own code, and returned if given. With src and dst (int64 vectors of one
     length) row src[i] goes into row dst[i] of ``out``, whose last row is a scratch row: slots that
     name it, or a row outside x or out, are skipped; dst names no other row twice."""
     what = "pack_rows8"

@@ -156,7 +156,7 @@ int dsb_bind_head(dsb_handle* h, const void* lm_head, const void* final_norm);
 int dsb_bind_lora(dsb_handle* h, int layer, int proj, const dsb_lora_tensors* t);
 /* Binds the shared activation buffers (base.py:438-461 share_activations). */
 int dsb_bind_activations(dsb_handle* h, const dsb_activations* a);
-/* The same with a layer's inputs, or its inputs and gate‖up, in 8 bits (the formats are described
+/* The same with the layers' inputs, their gate‖up, or both in 8 bits (the formats are described
  * with dsb_save_rows8): n_layers descriptors each, or NULL; `a` then holds NULL in their place. The cycle restores a
  * layer's rows to bf16, exactly, when it recomputes the layer, and is that of a bf16 store of these
  * values bit for bit. No counterpart in the reference, whose store is bf16. */
@@ -533,7 +533,7 @@ int dsb_op_adam_step(const dsb_adam_chunk* chunks, int nchunks, const int32_t* g
  *
  * 8-bit rows (types DSB_DT_E4M3 and DSB_DT_INT8): codes of one byte, and a byte per
  * DSB_ROWS8_BLOCK columns of a row, from the row's first, the exponent of their scale + 127. A value is
- * code·2^(byte − 127); byte 255 makes NaN of a code of 0. Saving takes the least exponent, at least −126, that brings the
+ * code·2^(byte − 127); byte 255 makes NaN of a code of 0, and byte 0, which saving never writes, 0. Saving takes the least exponent, at least −126, that brings the
  * block's largest magnitude to at most 448 (e4m3) or 127 (int8) and rounds to the nearest code, ties to
  * even, but to the code below where the nearest one's value is 2^128: finite values stay finite. A block that holds an
  * infinity or a NaN is kept as NaN whole. */
@@ -572,7 +572,8 @@ int dsb_op_norm_join(const void* x, int64_t ldx, const uint8_t* x_scales, int64_
 /* Its backward from x_new (bf16, fp32 or 8-bit rows) and y (bf16 or 8-bit rows), given the gradients dn of
  * normed and dxn of x_new (bf16 or fp32 each; null: zeros; dn null: w_in and x_new are not used):
  *   dx (bf16 or fp32, of x and of x_new's whole), dy (bf16), dw_out and dw_in fp32 [D] (null: not wanted),
- *   dgate: null (not wanted), fp32 [D], fp32 [rows] or bf16 rows of stride lddg, as the gate's kind is.
+ *   dgate: fp32 [D], fp32 [rows] or bf16 rows of stride lddg, as the gate's kind is; null (not wanted) for the
+ *   first two, a gate of rows always gets its own.
  * y null: the gradient of a norm alone, without dw_in. `sums`: whether any of dw_out, dw_in and a channel
  * gate's dgate is wanted; they are added over rows in fp32 in a fixed order. */
 int dsb_op_norm_join_workspace(int rows, int D, int sums, int64_t* bytes);
