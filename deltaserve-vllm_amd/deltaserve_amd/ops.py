@@ -1038,8 +1038,8 @@ def rotary(x, positions, plan, out=None):
     x's type. ``out``: written and returned, of x's shape and type; it is x itself (in place) or shares no
     element with it.
     Angles are reduced in 64 bits from the plan's table, which holds a frequency to 2^-52 of itself: off by at
-    most 2^-52·position·inv_freq radians, half a step of fp32 at π where that is 2^29 positions. Cosine and sine
-    are fp32; positions below 2^31."""
+    most 2^-52·position·inv_freq radians (half a step of fp32 at π where position·inv_freq is 2^29). Cosine and
+    sine are fp32. Positions are below 2^31 in size."""
     return _rotary("rotary", x, positions, plan, out, False)
 
 

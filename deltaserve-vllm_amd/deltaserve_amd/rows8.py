@@ -2,9 +2,9 @@
 
 ``Rows8`` holds codes (e4m3 or int8) and a byte per 32 columns of a row, the exponent of their scale
 + 127: a value is code·2^(byte − 127); byte 0 makes 0, byte 255 (codes 0: a lost block) NaN.
-``capture.save_rows`` fills one from the serving step's rows, ``ops.pack_rows8`` from a matrix; ``ops.rmsnorm``, ``rmsnorm_backward``, ``swiglu``,
-``swiglu_backward`` and ``residual_norm_backward`` read it in place of bf16 rows, ``ops.unpack_rows8``
-gives bf16 or fp32 ones. The reference keeps activations in bf16 and has no counterpart.
+``capture.save_rows`` fills one from the serving step's rows, ``ops.pack_rows8`` from a matrix;
+``ops.rmsnorm``, ``rmsnorm_backward``, ``swiglu``, ``swiglu_backward`` and ``residual_norm_backward``
+read it in place of bf16 rows, ``ops.unpack_rows8`` gives bf16 or fp32 ones. The reference keeps activations in bf16 and has no counterpart.
 
 Which code: int8 is off by at most 1/254 to 1/127 of its block's largest magnitude, whatever the value;
 e4m3 by 2^-4 of the value itself down to 2^-14 of the largest. The values of a Gaussian block come back

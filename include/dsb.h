@@ -533,8 +533,8 @@ int dsb_op_adam_step(const dsb_adam_chunk* chunks, int nchunks, const int32_t* g
  *
  * 8-bit rows (types DSB_DT_E4M3 and DSB_DT_INT8): codes of one byte, and a byte per
  * DSB_ROWS8_BLOCK columns of a row, from the row's first, the exponent of their scale + 127. A value is
- * code·2^(byte − 127); byte 255 makes NaN of a code of 0, and byte 0, which saving never writes, 0. Saving takes the least exponent, at least −126, that brings the
- * block's largest magnitude to at most 448 (e4m3) or 127 (int8) and rounds to the nearest code, ties to
+ * code·2^(byte − 127); byte 255 makes NaN of a code of 0, and byte 0, which saving never writes, 0. Saving
+ * takes the least exponent, at least −126, that brings the block's largest magnitude to at most 448 (e4m3) or 127 (int8) and rounds to the nearest code, ties to
  * even, but to the code below where the nearest one's value is 2^128: finite values stay finite. A block that holds an
  * infinity or a NaN is kept as NaN whole. */
 enum { DSB_ROWS8_BLOCK = 32 };
